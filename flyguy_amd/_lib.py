@@ -70,6 +70,14 @@ _SIGS = {
     "ft_scan_order": (ci, [ctypes.c_char_p, ci, ctypes.c_char_p, ci]),
     "fd_gather16": (None, [vp, vp, vp, ci, vp, ci, ci, ci, vp, vp, vp]),
     "fd_unpack16": (None, [vp, ci, ci, ci, vp, vp, vp]),
+    # include/flyguy_memory.h (argument structures are packed by memory_hip.py)
+    "fm_turn": (ci, [ctypes.c_char_p, vp]),
+    "fm_turn_bwd": (ci, [ctypes.c_char_p, vp]),
+    "fm_turn_partial": (cll, [ctypes.c_char_p]),
+    "fm_attention": (ci, [ctypes.c_char_p, vp]),
+    "fm_attention_bwd": (ci, [ctypes.c_char_p, vp]),
+    "fm_attention_workspace": (cll, [ctypes.c_char_p, ci]),
+    "fm_step": (ci, [ctypes.c_char_p, vp]),
     "fc_layers": (ci, [vp, ctypes.POINTER(ci), ci]),
     "fc_survey": (ci, [vp, vp, vp, ci, ci, cf, ci]),
     "fc_survey_read": (cll, [vp, vp, vp, ctypes.POINTER(ctypes.c_double)]),

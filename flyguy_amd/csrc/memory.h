@@ -1,0 +1,51 @@
+// What the kernels of the memory over decisions share (include/flyguy_memory.h): value types, views, wave sums.
+#pragma once
+#include "../../include/flyguy_memory.h"
+#include "common.h"
+
+namespace fg {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+template <class T>
+__device__ __forceinline__ float widen(T v) { return (float)v; }
+// to the nearest, ties to even: the one rounding of an output
+template <class T>
+__device__ __forceinline__ T narrow(float v) { return (T)v; }
+
+// x exp(g) with the factor kept to more than 24 bits near 1: a state is multiplied by it once a moment (or a chunk) for as
+// long as it remembers, and a rounded factor's errors would all point the same way (g = -1e-5 over 20,000 moments: 3e-4).
+struct Keep {
+    float one, f;                        // exp(g) = one + f
+    __device__ __forceinline__ explicit Keep(float g) : one(g > -0.5f ? 1.f : 0.f), f(g > -0.5f ? expm1f(g) : expf(g)) {}
+    __device__ __forceinline__ float operator()(float x) const { return fmaf(f, x, one * x); }
+};
+
+// values of a 16-byte load
+template <class T>
+struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));
+};
+
+__device__ __forceinline__ float wave_sum(float v, int width) {
+    for (int m = 1; m < width; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+// an entry of an index array of either width
+__device__ __forceinline__ long long index_at(const void* p, long long i, bool wide) {
+    return wide ? reinterpret_cast<const long long*>(p)[i] : reinterpret_cast<const int*>(p)[i];
+}
+
+inline bool aligned16(const fm_view& v, int size) {
+    return !(((uintptr_t)v.data | (uintptr_t)(v.seq * size) | (uintptr_t)(v.moment * size) | (uintptr_t)(v.head * size)) & 15);
+}
+
+inline int fail(const char* what) {
+    set_error(what);
+    return -1;
+}
+
+}  // namespace fg

@@ -1,0 +1,490 @@
+"""The memory over decisions (flyguy_amd.memory_hip: rotary, norm_rotary, decay_attention, decay_step) against 64-bit
+restatements, at the sizes, layouts and values where such kernels go wrong."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import memory_helpers as ref
+from gpu_helpers import say
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def draw(gen, *shape, dtype=F32):
+    return torch.randn(*shape, generator=gen).to(dtype).cuda()
+
+
+def laid_out(x, how):
+    """x [N, T, H, D] with the same values: dense, part of a wider projection (16-byte rows kept or not), or heads first."""
+    N, T, H, D = x.shape
+    if how == "dense":
+        return x
+    if how == "packed" or how == "odd":
+        pad = 8 if how == "packed" else 3
+        wide = torch.zeros(N, T, H * D + 2 * pad, dtype=x.dtype, device=x.device)
+        part = wide[..., pad:pad + H * D].unflatten(-1, (H, D))
+        part.copy_(x)
+        return part
+    if how == "heads first":
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    if how == "values first":
+        return x.movedim(3, 0).contiguous().movedim(0, 3)
+    raise ValueError(how)
+
+
+# ------------------------------------------------------------------------------------------------ rotation and norm
+TURNS = [  # N, T, Hq, Hk, D, R, interleaved, type, layout
+    (1, 1, 1, 0, 2, 2, False, F32, "dense"),
+    (1, 1, 8, 8, 64, 64, False, F32, "dense"),
+    (2, 5, 3, 1, 64, 64, True, BF16, "packed"),
+    (3, 17, 4, 2, 128, 128, False, BF16, "packed"),
+    (2, 33, 16, 4, 128, 64, True, BF16, "packed"),
+    (2, 9, 5, 5, 80, 32, False, F32, "packed"),
+    (2, 9, 5, 5, 80, 32, False, BF16, "odd"),
+    (1, 70, 2, 2, 96, 96, False, F16, "heads first"),
+    (1, 7, 3, 3, 100, 50, False, F32, "dense"),
+    (1, 7, 3, 3, 100, 50, True, F16, "dense"),
+    (2, 3, 2, 1, 33, 6, True, BF16, "values first"),
+    (1, 3, 9, 4, 512, 512, False, F32, "dense"),
+    (1, 40, 7, 2, 256, 192, False, BF16, "dense"),
+    (2, 300, 1, 1, 8, 8, False, BF16, "dense"),
+    (4, 100, 4, 4, 16, 16, True, F16, "dense"),
+    (1, 4, 300, 1, 64, 16, False, BF16, "dense"),
+    (1, 1, 1, 1, 1, 0, False, F32, "dense"),
+    (1, 65, 2, 2, 24, 8, True, BF16, "packed"),
+    (1, 65, 2, 2, 40, 16, False, BF16, "packed"),
+]
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("case", TURNS, ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+def test_turns_and_their_gradients(gpu_lib, case, norm):
+    from flyguy_amd.memory_hip import norm_rotary, rotary, rotary_table
+    N, T, Hq, Hk, D, R, il, dt, how = case
+    say(f"turn {case} norm {norm}")
+    if not norm and not R:
+        pytest.skip("nothing to turn")
+    gen = torch.Generator().manual_seed(N + T + D + R)
+    q = laid_out(draw(gen, N, T, Hq, D, dtype=dt), how).requires_grad_()
+    k = laid_out(draw(gen, N, T, Hk, D, dtype=dt), how).requires_grad_() if Hk else None
+    table = rotary_table(2 * T + 3, R, scaling="linear", factor=2.0).cuda() if R else None
+    pos = torch.randint(0, 2 * T + 3, (N, T), generator=gen, dtype=torch.int64 if D % 3 else torch.int32)
+    ws = [(1 + 0.3 * draw(gen, D)).requires_grad_() for _ in range(2 if k is not None else 1)] if norm else []
+    gs = [laid_out(draw(gen, *x.shape, dtype=dt), how) for x in (q, k) if x is not None]
+    eps = 1e-5
+    if norm:
+        out = norm_rotary(q, k, ws[0], ws[1] if k is not None else None, table, pos.cuda(), interleaved=il, eps=eps)
+    else:
+        out = rotary(q, k, table, pos.cuda(), interleaved=il)
+    out = [y for y in out if y is not None]
+    xs = [x for x in (q, k) if x is not None]
+    grads = torch.autograd.grad(out, xs + ws, gs)
+    cs = table.cpu().double()[pos][:, :, None] if R else torch.zeros(N, T, 1, 0, 2, dtype=torch.float64)
+    for i, (x, g, y, gx) in enumerate(zip(xs, gs, out, grads)):
+        x, g = x.detach().cpu().double(), g.cpu().double()
+        w = ws[i].detach().cpu().double() if norm else torch.ones(D, dtype=torch.float64)
+        r = (x.square().mean(-1, keepdim=True) + eps).rsqrt() if norm else torch.ones(1, dtype=torch.float64)
+        z = x * r * w
+        n = D if norm else 0                       # the norm's sum of D squares, then a few roundings
+        ref.within(y, ref.turned(z, cs, il), ref.turned_magnitude(z, cs, il), n + 12, "value")
+        gz, gm = ref.turned(g, cs, il, back=True), ref.turned_magnitude(g, cs, il)
+        if not norm:
+            ref.within(gx, gz, gm, 12, "gradient")
+            continue
+        xh, u, um = x * r, gz * w, gm * w.abs()
+        want = r * (u - xh * (u * xh).mean(-1, keepdim=True))
+        mag = r * (um + xh.abs() * (um * xh.abs()).mean(-1, keepdim=True))
+        ref.within(gx, want, mag, 3 * D + 40, "gradient")
+        rows = x.shape[0] * x.shape[1] * x.shape[2]
+        ref.within(grads[len(xs) + i], (gz * xh).sum((0, 1, 2)), (gm * xh.abs()).sum((0, 1, 2)), rows + D + 20, "weight's")
+
+
+def test_norm_gradient_against_differences(gpu_lib):
+    """The loss <g, y> along a direction d: (L(x + h d) - L(x - h d)) / 2h is the gradient's <gx, d> up to h^2 / 6 of the
+    third derivative (of the order of the terms' magnitudes: values of order 1) and 2^-24 of L's terms / h."""
+    from flyguy_amd.memory_hip import norm_rotary, rotary_table
+    gen = torch.Generator().manual_seed(5)
+    q, k, d = draw(gen, 2, 9, 3, 64), draw(gen, 2, 9, 2, 64), draw(gen, 2, 9, 3, 64)
+    wq, wk, g = 1 + 0.2 * draw(gen, 64), 1 + 0.2 * draw(gen, 64), draw(gen, 2, 9, 3, 64)
+    dw = draw(gen, 64)
+    table = rotary_table(9, 32).cuda()
+    loss = lambda x, w: (norm_rotary(x, k, w, wk, table)[0].double() * g.double()).sum()          # noqa: E731
+    x, w = q.clone().requires_grad_(), wq.clone().requires_grad_()
+    gx, gw = torch.autograd.grad(loss(x, w), [x, w])
+    h = 2.0 ** -7
+    for grad, way, fore, back in ((gx, d, (q + h * d, wq), (q - h * d, wq)), (gw, dw, (q, wq + h * dw), (q, wq - h * dw))):
+        want = (loss(*fore) - loss(*back)) / (2 * h)
+        terms = float((grad.double() * way.double()).abs().sum())
+        noise = 24 * 2.0 ** -24 * float(g.abs().double().sum() * 4) / h
+        assert abs(float((grad.double() * way.double()).sum()) - float(want)) <= 8 * h * h * terms + noise
+
+
+def test_positions(gpu_lib):
+    """None, an int, one row for all, int32, int64, and strided positions name the same turns; outside the table: NaN."""
+    from flyguy_amd.memory_hip import rotary, rotary_table
+    gen = torch.Generator().manual_seed(1)
+    q = draw(gen, 2, 6, 3, 16)
+    table = rotary_table(20, 8).cuda()
+    at = torch.arange(6, device="cuda")
+    first = rotary(q, None, table)[0]
+    for pos in (0, at, at.int(), at.expand(2, 6), torch.stack([at, at], 1).int().t(), torch.stack([at, at + 1], 1)[:, 0]):
+        assert torch.equal(rotary(q, None, table, pos)[0], first)
+    assert torch.equal(rotary(q, None, table, 3)[0], rotary(q, None, table, at + 3)[0])
+    out = rotary(q, None, table, torch.tensor([[0, -1, 19, 20, 5, 2 ** 40]], device="cuda"))[0]
+    bad = torch.tensor([False, True, False, True, False, True], device="cuda")
+    assert torch.isnan(out[:, bad][..., :8]).all() and torch.equal(out[..., 8:], q[..., 8:])
+    assert torch.isfinite(out[:, ~bad]).all()
+    assert torch.isnan(rotary(q, None, table, 18)[0][:, 2:, :, :8]).all()
+
+
+def test_a_norm_keeps_rows_apart(gpu_lib):
+    """A row of zeros, one of infinity and one of NaN: the others are what they are without them, the row of zeros is zeros."""
+    from flyguy_amd.memory_hip import norm_rotary, rotary_table
+    gen = torch.Generator().manual_seed(2)
+    for dt in (F32, BF16):
+        q = draw(gen, 2, 8, 4, 64, dtype=dt)
+        w, table = torch.ones(64, device="cuda"), rotary_table(8, 64).cuda()
+        clean = norm_rotary(q, None, w, None, table)[0]
+        bad = q.clone()
+        bad[0, 1, 2], bad[0, 3, 1, 5], bad[1, 7, 0, 63] = 0, float("inf"), float("nan")
+        got = norm_rotary(bad, None, w, None, table)[0]
+        touched = torch.zeros(2, 8, 4, dtype=torch.bool)
+        touched[0, 1, 2] = touched[0, 3, 1] = touched[1, 7, 0] = True
+        assert torch.equal(got[~touched], clean[~touched])
+        assert (got[0, 1, 2] == 0).all() and torch.isnan(got[1, 7, 0]).all() and torch.isnan(got[0, 3, 1]).any()
+
+
+# ------------------------------------------------------------------------------------------------ linear attention
+ATTENTION = [  # N, T, Hq, Hk, K, V, type, layout, start state
+    (1, 1, 1, 1, 1, 1, F32, "dense", True),
+    (1, 1, 2, 1, 64, 64, BF16, "dense", True),
+    (2, 15, 2, 2, 16, 16, BF16, "packed", False),
+    (1, 16, 1, 1, 128, 128, BF16, "dense", True),
+    (2, 17, 3, 3, 40, 56, F16, "packed", True),
+    (1, 63, 2, 2, 64, 64, F32, "packed", True),
+    (2, 64, 2, 1, 64, 128, BF16, "packed", True),
+    (1, 65, 4, 2, 128, 64, BF16, "dense", True),
+    (1, 130, 2, 2, 128, 128, F32, "heads first", True),
+    (1, 200, 1, 1, 5, 7, BF16, "odd", True),
+    (1, 150, 2, 1, 72, 100, BF16, "odd", False),
+    (1, 150, 2, 1, 72, 104, F32, "values first", False),
+    (1, 300, 3, 1, 24, 8, F16, "dense", True),
+    (2, 700, 1, 1, 32, 32, BF16, "dense", True),
+    (1, 1100, 1, 1, 64, 16, F32, "dense", True),
+    (1, 2500, 1, 1, 16, 64, BF16, "dense", True),
+]
+
+
+def decays(H):
+    """From none to all at once: heads remember everything, about 1,000 / 20 / 1 moments, or nothing."""
+    return torch.tensor([0.0, -1e-3, -0.05, -1.0, -30.0, -math.inf])[torch.arange(H) * 5 % 6].cuda()
+
+
+def inputs(gen, N, T, Hq, Hk, K, V, dt, how, state):
+    q, k, v = (laid_out(draw(gen, N, T, h, d, dtype=dt), how) for h, d in ((Hq, K), (Hk, K), (Hk, V)))
+    return q, k, v, draw(gen, N, Hq, K, V) if state else None
+
+
+def check_attention(q, k, v, g, s, starts=None, scale=None):
+    """Values and gradients against the restatement; the bounds count a sum over K or V values inside a sum over moments,
+    the powers of the decay (a rounding a chunk, and 2^-24 of an exponent of at most 88 where the power still counts), and in
+    bfloat16 two terms of 8 bits each for what a product rounds (2^-16 with both operands)."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(9)
+    K, V = q.shape[-1], v.shape[-1]
+    c = K ** -0.5 if scale is None else scale
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)] + ([s.clone().requires_grad_()] if s is not None else [])
+    st = None if starts is None else torch.tensor(starts, dtype=torch.int32, device="cuda")
+    o, end = decay_attention(*leaves[:3], g, leaves[3] if s is not None else None, st, scale=scale)
+    go, ge = draw(gen, *o.shape, dtype=o.dtype), draw(gen, *end.shape)
+    grads = torch.autograd.grad([o, end], leaves, [go, ge])
+    f = [x.detach().cpu().double() if x is not None else None for x in (q, k, v, s, go, ge)]
+    args = dict(log_decay=g.cpu(), starts=starts)
+    want = ref.attention(*f[:3], state=f[3], scale=c, go=f[4], gs=f[5], **args)
+    m = [x.abs() if x is not None else None for x in f]
+    mag = ref.attention(*m[:3], state=m[3], scale=abs(c), go=m[4], gs=m[5], **args)
+    T = max(e - b for b, e in zip(starts[:-1], starts[1:])) if starts else q.shape[1]
+    count, extra = K + V + T + 200, 2.0 ** -16 if q.dtype == BF16 else 0.0
+    for i, what in enumerate(("o", "end state", "gradient of q", "of k", "of v", "of the state")):
+        got = (o, end, *grads)[i] if i < 5 or s is not None else None
+        if got is not None:
+            ref.within(got, want[i], mag[i], count, what, extra)
+    return o, end
+
+
+@pytest.mark.parametrize("case", ATTENTION, ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+def test_attention_and_its_gradients(gpu_lib, case):
+    say(f"attention {case}")
+    N, T, Hq, Hk, K, V, dt, how, state = case
+    gen = torch.Generator().manual_seed(T + K)
+    check_attention(*inputs(gen, N, T, Hq, Hk, K, V, dt, how, state)[:3], decays(Hq),
+                    draw(gen, N, Hq, K, V) if state else None)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("lengths", [[0], [1], [0, 3, 0, 64, 1, 129, 0], [65, 63, 2, 700, 17, 16], [1200, 5]])
+def test_packed_stretches(gpu_lib, dt, lengths):
+    say(f"packed {lengths} {dt}")
+    gen = torch.Generator().manual_seed(len(lengths))
+    starts = [0]
+    for n in lengths:
+        starts.append(starts[-1] + n)
+    H, Hk, K, V = 4, 2, 48, 40
+    q, k, v = (draw(gen, starts[-1], h, d, dtype=dt) for h, d in ((H, K), (Hk, K), (Hk, V)))
+    check_attention(q, k, v, decays(H), draw(gen, len(lengths), H, K, V), starts)
+
+
+def test_starts_of_another_kind(gpu_lib):
+    """int64 starts give the int32 ones' results; moments of no stretch give zeros, and take no gradient; starts beyond the
+    moments, or falling, read nothing outside."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (draw(gen, 200, 2, 32) .requires_grad_() for _ in range(3))
+    g = decays(2)
+    starts = torch.tensor([10, 70, 70, 190], dtype=torch.int32, device="cuda")
+    o, s = decay_attention(q, k, v, g, None, starts)
+    o64, s64 = decay_attention(q, k, v, g, None, starts.long())
+    assert torch.equal(o, o64) and torch.equal(s, s64)
+    assert (o[:10] == 0).all() and (o[190:] == 0).all() and (o[10:190].abs().sum((1, 2)) > 0).all()
+    for x in torch.autograd.grad([o, s], [q, k, v], [torch.ones_like(o), torch.ones_like(s)]):
+        assert (x[:10] == 0).all() and (x[190:] == 0).all() and torch.isfinite(x).all()
+    o2, s2 = decay_attention(q, k, v, g, None, torch.tensor([-5, 100, 500], dtype=torch.int32, device="cuda"))
+    w, sw = decay_attention(q, k, v, g, None, torch.tensor([0, 100, 200], dtype=torch.int32, device="cuda"))
+    assert torch.equal(o2, w) and torch.equal(s2, sw)
+    decay_attention(q, k, v, g, None, torch.tensor([150, 20, 400, -3], dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_no_moments(gpu_lib, dt):
+    """No moments pass the state on, both ways; no stretches give nothing."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(4)
+    s = draw(gen, 3, 2, 16, 24).requires_grad_()
+    q, k, v = (torch.empty(3, 0, 2, d, dtype=dt, device="cuda") for d in (16, 16, 24))
+    o, e = decay_attention(q, k, v, decays(2), s)
+    assert o.shape == (3, 0, 2, 24) and torch.equal(e, s)
+    assert torch.equal(torch.autograd.grad(e, s, 2 * torch.ones_like(e))[0], 2 * torch.ones_like(e))
+    o, e = decay_attention(q[:0], k[:0], v[:0], decays(2))
+    assert o.shape == (0, 0, 2, 24) and e.shape == (0, 2, 16, 24)
+
+
+@pytest.mark.parametrize("dt,K,V", [(F32, 64, 64), (BF16, 64, 128), (BF16, 128, 48), (F16, 40, 40)])
+def test_a_later_moment_does_not_reach_an_earlier_one(gpu_lib, dt, K, V):
+    """NaN and infinities at a moment leave the outputs before it, and the gradients after it, as they were, bit for bit;
+    another stretch's leave a stretch alone."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(6)
+    q, k, v, _ = inputs(gen, 2, 200, 2, 2, K, V, dt, "dense", False)
+    go = draw(gen, 2, 200, 2, V, dtype=dt)
+    g = torch.tensor([-0.02, -1.0], device="cuda")
+
+    def both(q, k, v, go):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        o, _ = decay_attention(*leaves, g)
+        return (o.detach(), *torch.autograd.grad(o, leaves, go))
+    clean = both(q, k, v, go)
+    for t, bad in ((5, math.nan), (77, math.inf), (100, -math.inf), (64, math.nan), (199, math.inf), (120, math.nan)):
+        for which in range(4):
+            x = [y.clone() for y in (q, k, v, go)]
+            x[which][0, t, 1, 3] = bad
+            got = both(*x)
+            # o at moments before t; the gradients of q before t (of k, v there t is among the later moments)
+            for i in (0, 1):
+                if which != 3 or i == 1:
+                    assert torch.equal(got[i][0, :t], clean[i][0, :t]), (t, bad, which, i)
+            for i in (2, 3):                       # the gradients of k and v at moments after t
+                assert torch.equal(got[i][0, t + 1:], clean[i][0, t + 1:]), (t, bad, which, i)
+            for i in range(4):
+                assert torch.equal(got[i][1], clean[i][1]) and torch.equal(got[i][0, :, 0], clean[i][0, :, 0])
+            if which < 3:
+                assert not torch.isfinite(got[0][0, t, 1]).all()
+
+
+def test_gradients_against_differences(gpu_lib):
+    """The loss <go, o> + <ge, end> is linear in q, in k, in v and in the state, so its whole difference along any d is <gx,
+    d>, up to the roundings of both sides: T + K + V + 200 of the terms' magnitudes (f32)."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(8)
+    q, k, v, s = inputs(gen, 2, 150, 4, 2, 32, 24, F32, "dense", True)
+    go, ge = draw(gen, 2, 150, 4, 24), draw(gen, 2, 4, 32, 24)
+    g = decays(4)
+
+    def loss(*x):
+        o, e = decay_attention(*x[:3], g, x[3])
+        return (o.double() * go.double()).sum() + (e.double() * ge.double()).sum()
+    base = [q, k, v, s]
+    leaves = [x.clone().requires_grad_() for x in base]
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    for i in range(4):
+        d = draw(gen, *base[i].shape)
+        moved = [x + d if j == i else x for j, x in enumerate(base)]
+        mags = [x.abs().cpu().double() for x in (moved[i].abs() + base[i].abs() if j == i else base[j] for j in range(4))]
+        o, e = ref.attention(mags[0], mags[1], mags[2], g.cpu(), mags[3], 32 ** -0.5)
+        terms = float((o * go.abs().cpu().double()).sum() + (e * ge.abs().cpu().double()).sum())
+        diff = float(loss(*moved) - loss(*base))
+        assert abs(diff - float((grads[i].double() * d.double()).sum())) <= 406 * ref.U * terms
+
+
+def test_parts_of_the_gradient(gpu_lib):
+    """Any subset of inputs with gradients, and either output's gradient missing, gives the whole call's values."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(10)
+    for Hk in (2, 1):
+        base = inputs(gen, 1, 90, 2, Hk, 16, 24, F32, "dense", True)
+        go, ge = draw(gen, 1, 90, 2, 24), draw(gen, 1, 2, 16, 24)
+
+        def grads(wanted, outs):
+            x = [b.clone().requires_grad_(i in wanted) for i, b in enumerate(base)]
+            res = decay_attention(*x[:3], decays(2), x[3])
+            gs = torch.autograd.grad([res[j] for j in outs], [x[i] for i in wanted], [(go, ge)[j] for j in outs])
+            return dict(zip(wanted, gs))
+        for outs in ((0, 1), (0,), (1,)):
+            whole = grads((0, 1, 2, 3), outs) if 0 in outs else {**grads((1, 2, 3), outs)}
+            for wanted in ((0,), (1,), (2,), (3,), (1, 3), (0, 2)):
+                if outs == (1,) and 0 in wanted:
+                    continue                      # (the end state does not depend on q)
+                for i, x in grads(wanted, outs).items():
+                    assert torch.equal(x, whole[i]), (Hk, outs, wanted, i)
+
+
+def test_pieces_of_a_stretch_and_single_moments(gpu_lib):
+    """A stretch read in two pieces, or moment by moment with decay_step, is the stretch read at once, up to rounding."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step
+    gen = torch.Generator().manual_seed(11)
+    for dt in (F32, BF16):
+        q, k, v, s = inputs(gen, 3, 150, 4, 2, 64, 32, dt, "packed", True)
+        g = decays(4)
+        o, e = decay_attention(q, k, v, g, s)
+        f = [x.cpu().double() for x in (q, k, v)]
+        want = ref.attention(*f, g.cpu(), s.cpu().double(), 0.125)
+        mag = ref.attention(*[x.abs() for x in f], g.cpu(), s.abs().cpu().double(), 0.125)
+        o1, e1 = decay_attention(q[:, :37], k[:, :37], v[:, :37], g, s)
+        o2, e2 = decay_attention(q[:, 37:], k[:, 37:], v[:, 37:], g, e1)
+        live, outs = s.clone(), []
+        for t in range(150):
+            outs.append(decay_step(q[:, t], k[:, t], v[:, t], g, live))
+        extra = 2.0 ** -16 if dt == BF16 else 0.0
+        for a, b in ((o, e), (torch.cat([o1, o2], 1), e2), (torch.stack(outs, 1), live)):
+            ref.within(a, want[0], mag[0], 64 + 32 + 150 + 200, "o", extra)
+            ref.within(b, want[1], mag[1], 64 + 32 + 150 + 200, "state", extra)
+
+
+def test_far_strides(gpu_lib):
+    """Heads and moments more than 2^31 values apart (views of one 6 GB buffer)."""
+    from flyguy_amd.memory_hip import decay_attention, rotary, rotary_table
+    gen = torch.Generator().manual_seed(13)
+    big = torch.empty(3 * 2 ** 30 + 65536, dtype=BF16, device="cuda")
+    far = big.as_strided((1, 2, 2, 64), (0, 2 ** 30, 2 ** 31, 1))
+    x = draw(gen, 1, 2, 2, 64, dtype=BF16)
+    far.copy_(x)
+    table = rotary_table(2, 64).cuda()
+    assert torch.equal(rotary(far, None, table)[0], rotary(x, None, table)[0])
+    g = decays(2)
+    a, b = decay_attention(far, far, far, g), decay_attention(x, x, x, g)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+# ------------------------------------------------------------------------------------------------ single moments
+@pytest.mark.parametrize("n,Hq,Hk,K,V,dt", [(1, 1, 1, 1, 1, F32), (1, 8, 8, 64, 64, F32), (3, 4, 2, 128, 128, BF16),
+                                            (5, 6, 2, 40, 56, F16), (2, 3, 3, 7, 33, BF16), (70, 2, 1, 96, 20, BF16),
+                                            (2, 2, 2, 128, 6, F32)])
+def test_step(gpu_lib, n, Hq, Hk, K, V, dt):
+    from flyguy_amd.memory_hip import decay_step
+    say(f"step {n} {Hq} {Hk} {K} {V} {dt}")
+    gen = torch.Generator().manual_seed(n + K)
+    wide = draw(gen, n, Hq * K + Hk * (K + V) + 5, dtype=dt)
+    q = wide[:, :Hq * K].unflatten(1, (Hq, K))
+    k, v = wide[:, Hq * K:Hq * K + Hk * K].unflatten(1, (Hk, K)), wide[:, -Hk * V:].unflatten(1, (Hk, V))
+    s = draw(gen, n, Hq, K, V)
+    g = decays(Hq)
+    f = [x.cpu().double()[:, None] for x in (q, k, v)]
+    want = ref.attention(*f, g.cpu(), s.cpu().double(), K ** -0.5)
+    mag = ref.attention(*[x.abs() for x in f], g.cpu(), s.abs().cpu().double(), K ** -0.5)
+    into = torch.full_like(s, 7.0)
+    o1 = decay_step(q, k, v, g, s, into=into)
+    kept = s.clone()
+    o2 = decay_step(q, k, v, g, s)
+    assert torch.equal(o1, o2) and torch.equal(into, s) and not torch.equal(kept, s)
+    ref.within(o1[:, None], want[0], mag[0], K + 10, "o")
+    ref.within(s, want[1], mag[1], 10, "state")
+
+
+def test_slots(gpu_lib):
+    """Rows go on from their slots' states, idle rows touch none, a slot past the states gives NaN and touches none."""
+    from flyguy_amd.memory_hip import decay_step
+    gen = torch.Generator().manual_seed(15)
+    q, k, v = draw(gen, 5, 2, 32), draw(gen, 5, 2, 32), draw(gen, 5, 2, 48)
+    s, g = draw(gen, 7, 2, 32, 48), decays(2)
+    slots = torch.tensor([6, -1, 0, 7, 3], dtype=torch.int32, device="cuda")
+    was = s.clone()
+    o = decay_step(q, k, v, g, s, slots)
+    for row, slot in ((0, 6), (2, 0), (4, 3)):
+        one = was[slot:slot + 1].clone()
+        assert torch.equal(decay_step(q[row:row + 1], k[row:row + 1], v[row:row + 1], g, one)[0], o[row])
+        assert torch.equal(one[0], s[slot])
+    assert (o[1] == 0).all() and torch.isnan(o[3]).all()
+    for slot in (1, 2, 4, 5):
+        assert torch.equal(s[slot], was[slot])
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs
+def test_other_streams(gpu_lib):
+    """Calls go to the current stream, and their gradients to it too."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step, norm_rotary, rotary_table
+    gen = torch.Generator().manual_seed(16)
+    q, k, v, s = inputs(gen, 2, 500, 4, 2, 64, 64, BF16, "packed", True)
+    w, table, g = torch.ones(64, device="cuda"), rotary_table(500, 64).cuda(), decays(4)
+    go = draw(gen, 2, 500, 4, 64, dtype=BF16)
+
+    def all_of_it():
+        x = [y.detach().requires_grad_() for y in (q, k, v)]
+        a, b = norm_rotary(x[0], x[1], w, w, table)
+        o, e = decay_attention(a, b, x[2], g, s)
+        return (o.detach(), e.detach(), *torch.autograd.grad(o, x, go), decay_step(q[:, 0], k[:, 0], v[:, 0], g, s.clone()))
+    want = all_of_it()
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        burn = torch.randn(4096, 4096, device="cuda")
+        for _ in range(4):
+            burn = burn @ burn * 1e-3             # (the stream is busy: work on another would overtake it)
+        got = all_of_it()
+    torch.cuda.current_stream().wait_stream(other)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_in_a_graph(gpu_lib):
+    """A decision's calls recorded once and replayed, with eager work between the replays, give the eager results."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step, norm_rotary, rotary_table
+    gen = torch.Generator().manual_seed(17)
+    w, table, g = torch.ones(64, device="cuda"), rotary_table(64, 64).cuda(), decays(4)
+    q, k, v = draw(gen, 3, 1, 4, 64), draw(gen, 3, 1, 2, 64), draw(gen, 3, 1, 2, 64)
+    long = [draw(gen, 1, 700, 2, 32, dtype=BF16) for _ in range(3)]
+    pos = torch.zeros(3, 1, dtype=torch.int32, device="cuda")
+    s = draw(gen, 3, 4, 64, 64)
+    start = s.clone()
+
+    def decide(s):
+        a, b = norm_rotary(q, k, w, w, table, pos)
+        return decay_step(a[:, 0], b[:, 0], v[:, 0], g, s), decay_attention(*long, g[:2])[0]
+    decide(s)                                     # (the first calls load the kernels)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = decide(s)
+    s.copy_(start)
+    eager = start.clone()
+    for i in range(5):
+        pos.fill_(i)
+        q.normal_()
+        long[0].normal_()
+        graph.replay()
+        want = decide(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]) and torch.equal(s, eager)
