@@ -7,6 +7,8 @@
 // the last moment's term does not decay; the second one's end state, decayed once more, is the start state's gradient.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "memory.h"
 
 namespace fg {
@@ -19,16 +21,17 @@ struct Scan {
     void* out;                           // dense [moments][heads][N]; 0: no output
     const float* init;                   // start state [n_seq][heads][K][N] (transposed: [N][K]); 0: zeros
     float* fin;                          // end state [n_seq][heads][K][N]; 0: not wanted
+    float* seg;                          // [slots][heads][K][N]: segments' own states, then their start states
     int K, N, transposed, backwards;
-    float co, cz;
+    float c;
 };
 
 struct Scans {
     Scan s[3];
     const float* log_decay;
     const void* starts;
-    long long n_moments;
-    int wide, heads;
+    long long n_moments, L;              // L: moments per segment (a multiple of CHUNK)
+    int wide, heads, n_seq, nseg, slots; // slots of segments: n_seq x nseg, or an upper bound for packed stretches
 };
 
 // the moments of stretch n: [first, first + count) of the views
@@ -43,6 +46,388 @@ __device__ __forceinline__ void stretch_of(const Scans& a, int n, long long& fir
     e = e < b ? b : e > a.n_moments ? a.n_moments : e;
     first = b;
     count = e - b;
+}
+
+// The slot of a packed stretch's first segment: its segments and the next stretch's never share one, as floor(b / L) + 1 +
+// floor((b + c) / L) - floor(b / L) >= ceil(c / L), and 1 for a stretch without moments.
+__device__ __forceinline__ int first_slot(const Scans& a, int n) {
+    if (!a.starts || a.nseg == 1) return n * a.nseg;
+    long long b = index_at(a.starts, n, a.wide);
+    b = b < 0 ? 0 : b > a.n_moments ? a.n_moments : b;
+    return (int)(b / a.L) + n;
+}
+// (stretch, segment) of a slot; false: the slot is empty
+__device__ __forceinline__ bool segment_of(const Scans& a, int slot, int& n, int& seg, long long& first, long long& count) {
+    if (!a.starts || a.nseg == 1) {
+        n = slot / a.nseg;
+        seg = slot % a.nseg;
+    } else {
+        int lo = 0, hi = a.n_seq - 1;    // the last stretch whose first slot is not past this one
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first_slot(a, mid) <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        n = lo;
+        seg = slot - first_slot(a, n);
+    }
+    stretch_of(a, n, first, count);
+    return seg == 0 || (seg > 0 && seg * a.L < count);
+}
+
+// A state's value at (k, c) of the start state of stretch n, decayed once where the scan goes forwards (Z = l S).
+__device__ __forceinline__ float start_value(const Scan& s, size_t at, int k, int c, const Keep& keep) {
+    if (!s.init || k >= s.K || c >= s.N) return 0.f;
+    const float z = s.init[at + (s.transposed ? (size_t)c * s.K + k : (size_t)k * s.N + c)];
+    return s.backwards ? z : keep(z);
+}
+
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// v = hi + lo (+ what 16 bits do not hold), 8 values
+__device__ __forceinline__ void split2(const float (&v)[8], bf16x8& hi, bf16x8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = (bf16)v[i];
+        lo[i] = (bf16)(v[i] - (float)hi[i]);
+    }
+}
+__device__ __forceinline__ void split3(const float (&v)[8], bf16x8& hi, bf16x8& mid, bf16x8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = (bf16)v[i];
+        const float r = v[i] - (float)hi[i];
+        mid[i] = (bf16)r;
+        lo[i] = (bf16)(r - (float)mid[i]);
+    }
+}
+
+// A 4 x 16 block of 16-bit values in LDS, transposed: lane c of the 16 gets the block's column c, 4 rows.  p: this lane's
+// share of the block, 4 values of row c / 4.
+__device__ __forceinline__ bf16x4 columns4(const bf16* p) {
+    return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// 8 values of a row from column c, zeros past the row's end or width
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const bf16* row, int c, int width, bool there) {
+    uint4 r = make_uint4(0, 0, 0, 0);
+    if (!there || c >= width) return r;
+    if (VEC) return *reinterpret_cast<const uint4*>(row + c);
+    unsigned short v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < width ? reinterpret_cast<const unsigned short*>(row)[c + i] : 0;
+    r.x = v[0] | v[1] << 16;
+    r.y = v[2] | v[3] << 16;
+    r.z = v[4] | v[5] << 16;
+    r.w = v[6] | v[7] << 16;
+    return r;
+}
+
+// The scan in chunks of 64 moments, bfloat16 values, on the matrix cores (v_mfma_f32_16x16x32_bf16).  With i, j the moments
+// inside a chunk of n and Z the state before it, decayed once (Z = l S),
+//   out_i = c sum_{j <= i} l^(i-j) (x_i . y_j) v_j + c' l^i x_i Z,   Z' = l^n Z + sum_j c'' l^(n-j) y_j v_j^T
+// (forwards c' = c, c'' = 1; backwards c' = 1, c'' = c, so that the end state's gradient comes in and the start state's goes
+// out unscaled).
+// A workgroup of WAVES waves walks one segment of one head; wave w owns the state's columns 16 w .., in accumulators all
+// along: a 16 x 16 accumulator block holds, in lane (column c, group g), rows 4g .. 4g + 3, which is also how a product's
+// operand wants it with the rows as the summed index.  So the state passes from product to product in registers, and the
+// order of the summed index (any, if both operands have it) is chosen so: state blocks 2b, 2b + 1 are the rows 32 b + 8g +
+// (0 .. 3), (4 .. 7), and a lane's 8 values of x or y are then side by side.  y^T and v^T come out of LDS by transposing
+// reads.  Outputs are formed transposed, so that a lane stores a row's values side by side.  The weights (x . y) l^(i-j) of
+// the chunk's six 16 x 32 pieces on and below the diagonal are formed by a wave each and shared through LDS.
+// Roundings: x, y, v are exact; weights and Z go into their products as two bfloat16 terms (2^-16), v times its decay as
+// three (2^-24: the state is a float32 result).
+// A value of v that is not finite reaches only the outputs from its moment on (there: NaN), though 0 weights meet it in the
+// products: such a chunk's products run with zeros in its place.
+constexpr int CHUNK = 64;
+template <int KT, int WAVES, bool VEC, bool OUT, class TO>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_scan16(Scans a) {
+    constexpr int KW = 32 * KT, NW = 16 * WAVES, KP = KW + 8, NP = NW + 8;   // widths, and rows in LDS (no bank conflicts)
+    constexpr int XV = 4 * KT / WAVES, VV = 2;                               // a thread's 16-byte shares of x (y), of v
+    __shared__ __align__(16) bf16 sx[OUT ? CHUNK * KP : 8], sy[CHUNK * KP], sv[CHUNK * NP];
+    __shared__ __align__(16) bf16x8 sp[OUT ? 12 : 1][64];                    // the weights' pieces, two terms each
+    const Scan& s = a.s[blockIdx.z];
+    const int nblk = (s.N + NW - 1) / NW;
+    const int slot = blockIdx.x / nblk, blk = blockIdx.x % nblk, h = blockIdx.y;
+    if (slot >= a.slots) return;
+    int n, seg;
+    long long first, count;
+    if (!segment_of(a, slot, n, seg, first, count)) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int n0 = blk * NW, w0 = 16 * wave;              // this workgroup's columns, this wave's from there
+    const long long from = seg * a.L, left = count - from < a.L ? count - from : a.L;
+    const bool last = from + left == count;
+    if (!OUT && last) return;                             // (the last segment's own state is needed by none)
+    const float ld = fmaxf(a.log_decay[h], -1e30f);       // (-inf: 0 times it would not be 0)
+    const size_t at = ((size_t)n * a.heads + h) * s.K * s.N;
+    const float e2 = ld * 1.44269504f;
+    auto power = [&](int i) { return exp2f(e2 * (float)i); };
+
+    f32x4 z[2 * KT];                                      // the state
+    auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    const int col = n0 + w0 + c;
+    {
+        const Keep once(ld);
+        const float* from_seg = s.seg ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : nullptr;
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = row_of(b, r);
+                z[b][r] = !OUT ? 0.f : from_seg ? (k < s.K && col < s.N ? from_seg[(size_t)k * s.N + col] : 0.f)
+                                                : start_value(s, at, k, col, once);
+            }
+    }
+
+    // this thread's shares of a chunk's rows
+    constexpr int XR = 64 * WAVES / (4 * KT), VR = CHUNK / VV;               // rows between a thread's shares
+    const int xrow = tid / (4 * KT), xcol = tid % (4 * KT) * 8, vrow = tid / (2 * WAVES), vcol = tid % (2 * WAVES) * 8;
+    const long long dir = s.backwards ? -1 : 1;
+    const long long t0 = (a.starts ? first : 0) + (s.backwards ? count - 1 - from : from);
+    auto base = [&](const fm_view& v, int share) {
+        return (const bf16*)v.data + (a.starts ? 0 : n * v.seq) + (h / share) * v.head + t0 * v.moment;
+    };
+    const long long dx = dir * s.x.moment, dy = dir * s.y.moment, dv = dir * s.v.moment;
+    const bf16* px = OUT ? base(s.x, s.xs) + xrow * dx : nullptr;
+    const bf16* py = base(s.y, s.ys) + xrow * dy;
+    const bf16* pv = base(s.v, s.vs) + vrow * dv;
+    uint4 rx[XV], ry[XV], rv[VV];
+    auto fetch = [&](long long i0) {                      // the chunk from the segment's moment i0, where the pointers stand
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+            const bool there = i0 + xrow + i * XR < left;
+            if (OUT) rx[i] = load8<VEC>(px + i * XR * dx, xcol, s.K, there);
+            ry[i] = load8<VEC>(py + i * XR * dy, xcol, s.K, there);
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) rv[i] = load8<VEC>(pv + i * VR * dv + n0, vcol, s.N - n0, i0 + vrow + i * VR < left);
+        if (OUT) px += CHUNK * dx;
+        py += CHUNK * dy;
+        pv += CHUNK * dv;
+    };
+    fetch(0);
+
+    float rest[4];                                        // l^(16 - row in its block), times what backwards scales v with
+    const float cv = s.backwards ? s.c : 1.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r);
+    const float row16 = (s.backwards ? 1.f : s.c) * power(c);
+    const float p16 = power(16), p32 = power(32), p48 = power(48);
+    const Keep chunk(ld * CHUNK);
+    TO* out = OUT ? (TO*)s.out : nullptr;
+    const long long out_row = (a.starts ? 0 : n * a.n_moments) + t0;
+
+    for (long long i0 = 0; i0 < left; i0 += CHUNK) {
+        const int rows = (int)(left - i0 < CHUNK ? left - i0 : CHUNK);
+        __syncthreads();                                  // (the chunk before is read)
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+            if (OUT) *reinterpret_cast<uint4*>(&sx[(xrow + i * XR) * KP + xcol]) = rx[i];
+            *reinterpret_cast<uint4*>(&sy[(xrow + i * XR) * KP + xcol]) = ry[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) *reinterpret_cast<uint4*>(&sv[(vrow + i * VR) * NP + vcol]) = rv[i];
+        __syncthreads();
+        if (i0 + CHUNK < left) fetch(i0 + CHUNK);
+
+        f32x4 o[4];
+        if (OUT && out) {
+            // pieces of weights: rows 32 jj .., columns 16 i .. of (0,0) (1,0) (2,0) (3,0) (2,1) (3,1)
+            for (int piece = wave; piece < 6; piece += WAVES) {
+                const int jj = piece >> 2, i = jj ? piece - 2 : piece;
+                f32x4 p0{0.f, 0.f, 0.f, 0.f}, p1{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int b = 0; b < KT; ++b) {
+                    const bf16x8 xf = *reinterpret_cast<const bf16x8*>(&sx[(16 * i + c) * KP + 32 * b + 8 * g]);
+                    const bf16* y = &sy[(32 * jj + c) * KP + 32 * b + 8 * g];
+                    p0 = mfma(*reinterpret_cast<const bf16x8*>(y), xf, p0);
+                    p1 = mfma(*reinterpret_cast<const bf16x8*>(y + 16 * KP), xf, p1);
+                }
+                float v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int d = 16 * i + c - (32 * jj + 16 * (r >> 2) + 4 * g + (r & 3));
+                    v[r] = d >= 0 ? s.c * power(d) * (r < 4 ? p0[r] : p1[r - 4]) : 0.f;      // (whatever x . y is there)
+                }
+                bf16x8 ph, pl;
+                split2(v, ph, pl);
+                sp[2 * piece][lane] = ph;
+                sp[2 * piece + 1][lane] = pl;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < KT; ++b) {
+                bf16x8 zh, zl;
+                float v[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] = z[2 * b + (r >> 2)][r & 3];
+                split2(v, zh, zl);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bf16x8 xf = *reinterpret_cast<const bf16x8*>(&sx[(16 * i + c) * KP + 32 * b + 8 * g]);
+                    o[i] = mfma(zl, xf, o[i]);
+                    o[i] = mfma(zh, xf, o[i]);
+                }
+            }
+            __syncthreads();                              // (the pieces are there)
+        }
+
+        // v^T: block j's rows 4g .. of this wave's columns
+        bf16x4 vt[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vt[j] = columns4(&sv[(16 * j + 4 * g + (c >> 2)) * NP + w0 + 4 * (c & 3)]);
+        if (OUT && out) {
+            unsigned odd = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint2 u = __builtin_bit_cast(uint2, vt[j]);
+                odd |= ((u.x & 0x7f807f80u) + 0x00800080u) | ((u.y & 0x7f807f80u) + 0x00800080u);
+            }
+            const bool poisoned = __ballot((odd & 0x80008000u) != 0) != 0;
+            float since = 1e9f;                           // poisoned: the first row of column c that is not finite
+            bf16x4 vc[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) vc[j] = vt[j];
+            if (poisoned) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!(fabsf((float)vt[j][r]) < INFINITY)) {
+                            vc[j][r] = (bf16)0.f;
+                            since = fminf(since, (float)(16 * j + 4 * g + r));
+                        }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[i] *= row16 * (i == 0 ? 1.f : i == 1 ? p16 : i == 2 ? p32 : p48);
+#pragma unroll
+                for (int jj = 0; jj <= i / 2; ++jj) {
+                    const int piece = jj ? i + 2 : i;
+                    const bf16x8 vf = join(vc[2 * jj], vc[2 * jj + 1]);
+                    o[i] = mfma(vf, sp[2 * piece + 1][lane], o[i]);
+                    o[i] = mfma(vf, sp[2 * piece][lane], o[i]);
+                }
+            }
+            if (poisoned) {
+                since = fminf(since, __shfl_xor(since, 16));
+                since = fminf(since, __shfl_xor(since, 32));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float f = __shfl(since, 4 * g + r);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if ((float)(16 * i + c) >= f) o[i][r] = NAN;
+                }
+            }
+            const int oc = n0 + w0 + 4 * g;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * i + c;
+                if (row >= rows) continue;
+                TO* to = out + ((out_row + dir * (i0 + row)) * a.heads + h) * s.N + oc;
+                if (VEC && oc + 4 <= s.N) {
+                    typedef TO vec __attribute__((ext_vector_type(4)));
+                    vec v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = narrow<TO>(o[i][r]);
+                    *reinterpret_cast<vec*>(to) = v;
+                } else
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (oc + r < s.N) to[r] = narrow<TO>(o[i][r]);
+            }
+        }
+
+        // the state after the chunk; of the stretch's last one forwards, S rather than l S
+        const bool ends = last && i0 + CHUNK >= left;
+        if (ends && !s.fin) break;
+        const int n1 = ends && !s.backwards ? rows - 1 : rows;
+        const bool whole = n1 == CHUNK;
+        const Keep keep = whole ? chunk : Keep(ld * (float)n1);
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[b][r] = keep(z[b][r]);
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            bf16x8 wh, wm, wl;
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const int jb = j + (r >> 2), row = 16 * jb + 4 * g + (r & 3);
+                float w = rest[r & 3] * (jb == 0 ? p48 : jb == 1 ? p32 : jb == 2 ? p16 : 1.f);
+                if (!whole) w = cv * power(n1 - row > 0 ? n1 - row : 0);
+                v[r] = w * (float)vt[jb][r & 3];
+            }
+            split3(v, wh, wm, wl);
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) {
+                const bf16* p = &sy[(16 * j + 4 * g + (c >> 2)) * KP + 32 * (b >> 1) + 8 * (c & 3) + 4 * (b & 1)];
+                const bf16x8 yt = join(columns4(p), columns4(p + 16 * KP));
+                z[b] = mfma(yt, wl, z[b]);
+                z[b] = mfma(yt, wm, z[b]);
+                z[b] = mfma(yt, wh, z[b]);
+            }
+        }
+    }
+
+    float* to = !OUT ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : last ? s.fin : nullptr;
+    if (OUT && to) to += at;
+    if (to) {
+        const Keep none(0.f);
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = row_of(b, r);
+                if (k < s.K && col < s.N)             // (no moments: the start state as it came)
+                    to[(size_t)k * s.N + col] = OUT && count == 0 ? start_value(s, at, k, col, none) : z[b][r];
+            }
+    }
+    if (OUT && a.starts && out && seg == 0 && (n == 0 || n == a.n_seq - 1)) {
+        // moments of no stretch, before the first one and after the last, give zeros
+        for (int e = tid; e < NW; e += 64 * WAVES) {
+            if (n0 + e >= s.N) break;
+            TO* all = out + (size_t)h * s.N + n0 + e;
+            if (n == 0)
+                for (long long t = 0; t < first; ++t) all[t * a.heads * s.N] = narrow<TO>(0.f);
+            if (n == a.n_seq - 1)
+                for (long long t = first + count; t < a.n_moments; ++t) all[t * a.heads * s.N] = narrow<TO>(0.f);
+        }
+    }
+}
+
+// Segments' start states from their own: Z_0 = the stretch's, Z_{s+1} = l^L Z_s + own_s, in place.
+// grid (blocks of values x heads, stretches, scans)
+__global__ __launch_bounds__(256) void k_scan_join(Scans a) {
+    const Scan& s = a.s[blockIdx.z];
+    const int h = blockIdx.x % a.heads, n = blockIdx.y, i = blockIdx.x / a.heads * 256 + threadIdx.x;
+    if (i >= s.K * s.N) return;
+    long long first, count;
+    stretch_of(a, n, first, count);
+    const float ld = fmaxf(a.log_decay[h], -1e30f);
+    const Keep once(ld), keep(ld * (float)a.L);
+    float z = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, i / s.N, i % s.N, once);
+    float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
+    const size_t step = (size_t)a.heads * s.K * s.N;
+    for (long long from = 0;; from += a.L, p += step) {
+        const bool more = from + a.L < count;
+        const float own = more ? *p : 0.f;
+        *p = z;
+        if (!more) break;
+        z = keep(z) + own;
+    }
 }
 
 // Moment by moment: a workgroup holds 32 columns of a head's state, 4 columns and every 32nd row a lane.
@@ -79,7 +464,7 @@ __global__ __launch_bounds__(256) void k_scan_simple(Scans a, int n_seq) {
         __syncthreads();
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
         float vv[4];
-        for (int j = 0; j < 4; ++j) vv[j] = c0 + j < N ? s.cz * widen(v[(first + t) * s.v.moment + c0 + j]) : 0.f;
+        for (int j = 0; j < 4; ++j) vv[j] = c0 + j < N ? (s.backwards ? s.c : 1.f) * widen(v[(first + t) * s.v.moment + c0 + j]) : 0.f;
         const bool first_back = s.backwards && i == 0;
         for (int r = 0; r < 4; ++r) {
             const int k = rg + 32 * r;
@@ -97,7 +482,7 @@ __global__ __launch_bounds__(256) void k_scan_simple(Scans a, int n_seq) {
         __syncthreads();
         if (s.out && tid < 32 && blockIdx.x * 32 + tid < N)
             out[t * a.heads * N + blockIdx.x * 32 + tid] =
-                narrow<TO>(s.co * (part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
+                narrow<TO>((s.backwards ? 1.f : s.c) * (part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
     }
     if (a.starts && s.out) {             // moments of no stretch: those before the first one and after the last
         TO* all = (TO*)s.out + (size_t)h * N + blockIdx.x * 32 + (tid & 31);
@@ -172,10 +557,11 @@ const char* heads_wrong(long long dtype, long long qh, long long kh, long long k
     return nullptr;
 }
 
-const char* attention_wrong(const fm_attention_args& a, bool bwd) {
+const char* attention_wrong(const fm_attention_args& a, bool bwd, bool sizes_only = false) {
     if (const char* e = heads_wrong(a.dtype, a.q_heads, a.k_heads, a.k_dim, a.v_dim)) return e;
     if (a.n_seq < 0 || a.n_seq > 16384) return "other than 0 to 16384 stretches";
     if (a.n_moments < 0 || a.n_moments > 1LL << 31) return "other than 0 to 2^31 moments";
+    if (sizes_only) return nullptr;
     if (!a.log_decay) return "no decays";
     const bool any = a.n_seq && a.n_moments;
     if (any && (!a.q.data || !a.k.data || !a.v.data)) return "a null tensor";
@@ -191,52 +577,132 @@ long long shared_floats(const fm_attention_args& a, bool of_v) {
     return a.q_heads > a.k_heads ? moments * a.q_heads * (of_v ? a.v_dim : a.k_dim) : 0;
 }
 
-template <class T, class TO>
-void launch_scans(const Scans& a, int count, int n_seq, hipStream_t st) {
-    if (!n_seq || !count) return;
-    int widest = 0;
-    for (int i = 0; i < count; ++i) widest = a.s[i].N > widest ? a.s[i].N : widest;
-    k_scan_simple<T, TO><<<dim3((widest + 31) / 32, a.heads, n_seq * count), 256, 0, st>>>(a, n_seq);
+// How a launch's scans are cut into segments: one segment a stretch where the stretches' heads alone fill the chip, else so
+// that about SEG_GROUPS workgroups run, of at least SEG_MIN moments.
+constexpr int SEG_GROUPS = 768, SEG_MIN = 256;
+struct Cut {
+    int nseg, slots;
+    long long L;
+};
+Cut cut_of(const fm_attention_args& p, int scans) {
+    Cut c;
+    const long long moments = p.n_moments * (p.starts ? 1 : p.n_seq);
+    const long long groups = p.n_seq * p.q_heads * scans;
+    c.nseg = 1;
+    c.slots = (int)p.n_seq;
+    c.L = (p.n_moments + CHUNK - 1) / CHUNK * CHUNK;
+    if (groups >= SEG_GROUPS / 2 || !groups) return c;
+    long long L = (moments * p.q_heads * scans / SEG_GROUPS + CHUNK - 1) / CHUNK * CHUNK;
+    if (L < SEG_MIN) L = SEG_MIN;
+    if (L >= p.n_moments) return c;
+    c.L = L;
+    c.nseg = (int)((p.n_moments + L - 1) / L);
+    c.slots = p.starts ? (int)(p.n_moments / L + p.n_seq) : (int)p.n_seq * c.nseg;
+    return c;
+}
+// floats of segments' states of one scan
+long long segment_floats(const fm_attention_args& p, const Cut& c) {
+    return c.nseg == 1 || p.dtype != FM_BF16 ? 0 : (long long)c.slots * p.q_heads * p.k_dim * p.v_dim;
 }
 
-template <class T>
-void attention_fwd(const fm_attention_args& p, hipStream_t st) {
-    const int share = (int)(p.q_heads / p.k_heads);
+template <int KT, int WAVES, bool VEC, class TO>
+void launch16(Scans& a, int count, hipStream_t st) {
+    int nblk = 1, most = 1;
+    for (int i = 0; i < count; ++i) {
+        const int b = (a.s[i].N + 16 * WAVES - 1) / (16 * WAVES), kn = a.s[i].K * a.s[i].N;
+        nblk = b > nblk ? b : nblk;
+        most = kn > most ? kn : most;
+    }
+    const dim3 grid(a.slots * nblk, a.heads, count);
+    if (a.nseg > 1) {
+        k_scan16<KT, WAVES, VEC, false, TO><<<grid, 64 * WAVES, 0, st>>>(a);
+        k_scan_join<<<dim3((most + 255) / 256 * a.heads, a.n_seq, count), 256, 0, st>>>(a);
+    }
+    k_scan16<KT, WAVES, VEC, true, TO><<<grid, 64 * WAVES, 0, st>>>(a);
+}
+template <class TO>
+void launch16_of(Scans& a, int count, bool vec, hipStream_t st) {
+    int widest = 0, n = 0;
+    for (int i = 0; i < count; ++i) {
+        widest = a.s[i].K > widest ? a.s[i].K : widest;
+        n = a.s[i].N > n ? a.s[i].N : n;
+    }
+    if (widest <= 64 && n <= 64) vec ? launch16<2, 4, true, TO>(a, count, st) : launch16<2, 4, false, TO>(a, count, st);
+    else if (widest <= 64) vec ? launch16<2, 8, true, TO>(a, count, st) : launch16<2, 8, false, TO>(a, count, st);
+    else if (n <= 64) vec ? launch16<4, 4, true, TO>(a, count, st) : launch16<4, 4, false, TO>(a, count, st);
+    else vec ? launch16<4, 8, true, TO>(a, count, st) : launch16<4, 8, false, TO>(a, count, st);
+}
+
+template <class T, class TO>
+void launch_scans(Scans& a, int count, const Cut& cut, bool vec, hipStream_t st) {
+    if (!a.n_seq || !count) return;
+    if constexpr (sizeof(T) == 2 && !std::is_same<T, f16>::value) {
+        a.L = cut.L > 0 ? cut.L : CHUNK;
+        a.nseg = cut.nseg;
+        a.slots = cut.slots;
+        launch16_of<TO>(a, count, vec, st);
+    } else {
+        int widest = 0;
+        for (int i = 0; i < count; ++i) widest = a.s[i].N > widest ? a.s[i].N : widest;
+        k_scan_simple<T, TO><<<dim3((widest + 31) / 32, a.heads, a.n_seq * count), 256, 0, st>>>(a, a.n_seq);
+    }
+}
+
+Scans scans_of(const fm_attention_args& p) {
     Scans a{};
     a.log_decay = p.log_decay;
     a.starts = p.starts;
     a.n_moments = p.n_moments;
     a.wide = (int)p.wide;
     a.heads = (int)p.q_heads;
-    a.s[0] = Scan{p.q, p.k, p.v, 1, share, share, p.o, p.state, p.state_out, (int)p.k_dim, (int)p.v_dim, 0, 0,
-                  (float)p.scale, 1.f};
-    launch_scans<T, T>(a, 1, (int)p.n_seq, st);
+    a.n_seq = (int)p.n_seq;
+    return a;
+}
+
+// 16-byte loads and stores: heads of a multiple of 8 values, everything aligned
+bool wide_rows(const fm_attention_args& p, bool bwd) {
+    const int size = p.dtype == FM_F32 ? 4 : 2;
+    if (p.k_dim % 8 || p.v_dim % 8 || !aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
+    if (bwd) return aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv | (uintptr_t)p.workspace) & 15);
+    return !((uintptr_t)p.o & 15);
+}
+
+template <class T>
+void attention_fwd(const fm_attention_args& p, hipStream_t st) {
+    const int share = (int)(p.q_heads / p.k_heads);
+    Scans a = scans_of(p);
+    const Cut cut = cut_of(p, 1);
+    float* seg = segment_floats(p, cut) ? (float*)p.workspace : nullptr;
+    a.s[0] = Scan{p.q, p.k, p.v, 1, share, share, p.o, p.state, p.state_out, seg, (int)p.k_dim, (int)p.v_dim, 0, 0,
+                  (float)p.scale};
+    launch_scans<T, T>(a, 1, cut, wide_rows(p, false), st);
 }
 
 template <class T>
 void attention_bwd(const fm_attention_args& p, hipStream_t st) {
     const int share = (int)(p.q_heads / p.k_heads), K = (int)p.k_dim, V = (int)p.v_dim;
     const float c = (float)p.scale;
-    float* part_k = (float*)p.workspace;
+    const Cut cut = cut_of(p, 3);
+    const bool vec = wide_rows(p, true);
+    const long long floats = segment_floats(p, cut);
+    float* seg[3];
+    for (int i = 0; i < 3; ++i) seg[i] = floats ? (float*)p.workspace + i * floats : nullptr;
+    float* part_k = (float*)p.workspace + 3 * floats;
     float* part_v = part_k + shared_floats(p, false);
-    Scans a{};
-    a.log_decay = p.log_decay;
-    a.starts = p.starts;
-    a.n_moments = p.n_moments;
-    a.wide = (int)p.wide;
-    a.heads = (int)p.q_heads;
-    int n = 0;
-    if (p.gq) a.s[n++] = Scan{p.go, p.v, p.k, 1, share, share, p.gq, p.state, nullptr, V, K, 1, 0, c, 1.f};
     const int own = share == 1;
-    if (own && p.gk) a.s[n++] = Scan{p.v, p.go, p.q, share, 1, 1, p.gk, p.gstate_out, nullptr, V, K, 1, 1, 1.f, c};
-    if (own && (p.gv || p.gstate)) a.s[n++] = Scan{p.k, p.q, p.go, share, 1, 1, p.gv, p.gstate_out, p.gstate, K, V, 0, 1, 1.f, c};
-    launch_scans<T, T>(a, n, (int)p.n_seq, st);
+    Scans a = scans_of(p);
+    int n = 0;
+    if (p.gq) a.s[n++] = Scan{p.go, p.v, p.k, 1, share, share, p.gq, p.state, nullptr, seg[0], V, K, 1, 0, c};
+    const Scan of_k{p.v, p.go, p.q, share, 1, 1, own ? p.gk : part_k, p.gstate_out, nullptr, seg[1], V, K, 1, 1, c};
+    const Scan of_v{p.k, p.q, p.go, share, 1, 1, !p.gv ? nullptr : own ? p.gv : part_v, p.gstate_out, p.gstate, seg[2], K, V, 0, 1, c};
+    if (own && p.gk) a.s[n++] = of_k;
+    if (own && (p.gv || p.gstate)) a.s[n++] = of_v;
+    launch_scans<T, T>(a, n, cut, vec, st);
     if (own) return;
     n = 0;
-    if (p.gk) a.s[n++] = Scan{p.v, p.go, p.q, share, 1, 1, part_k, p.gstate_out, nullptr, V, K, 1, 1, 1.f, c};
-    if (p.gv || p.gstate)
-        a.s[n++] = Scan{p.k, p.q, p.go, share, 1, 1, p.gv ? part_v : nullptr, p.gstate_out, p.gstate, K, V, 0, 1, 1.f, c};
-    launch_scans<T, float>(a, n, (int)p.n_seq, st);
+    if (p.gk) a.s[n++] = of_k;
+    if (p.gv || p.gstate) a.s[n++] = of_v;
+    launch_scans<T, float>(a, n, cut, vec, st);
     const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads;
     if (rows && p.gk) k_share<T><<<(unsigned)((rows * K + 255) / 256), 256, 0, st>>>(part_k, (T*)p.gk, share, K, rows * K);
     if (rows && p.gv) k_share<T><<<(unsigned)((rows * V + 255) / 256), 256, 0, st>>>(part_v, (T*)p.gv, share, V, rows * V);
@@ -249,13 +715,17 @@ using namespace fg;
 extern "C" {
 
 long long fm_attention_workspace(const fm_attention_args* a, int backward) {
-    return backward ? 4 * (shared_floats(*a, false) + shared_floats(*a, true)) : 0;
+    if (attention_wrong(*a, false, true)) return 0;
+    const Cut cut = cut_of(*a, backward ? 3 : 1);
+    return 4 * (segment_floats(*a, cut) * (backward ? 3 : 1) + (backward ? shared_floats(*a, false) + shared_floats(*a, true) : 0));
 }
 
 int fm_attention(const fm_attention_args* a, void* stream) {
     clear_error();
     if (!a) return fail("fm_attention: no arguments");
     if (const char* e = attention_wrong(*a, false)) return fail((std::string("fm_attention: ") + e).c_str());
+    const long long need = fm_attention_workspace(a, 0);
+    if (need && (!a->workspace || a->workspace_bytes < need)) return fail("fm_attention: the workspace is too small");
     if (a->dtype == FM_F32) attention_fwd<float>(*a, (hipStream_t)stream);
     else if (a->dtype == FM_BF16) attention_fwd<bf16>(*a, (hipStream_t)stream);
     else attention_fwd<f16>(*a, (hipStream_t)stream);
