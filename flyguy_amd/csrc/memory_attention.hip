@@ -7,8 +7,6 @@
 // the last moment's term does not decay; the second one's end state, decayed once more, is the start state's gradient.
 #include <hip/hip_runtime.h>
 
-#include <type_traits>
-
 #include "memory.h"
 
 namespace fg {
@@ -30,7 +28,7 @@ struct Scans {
     Scan s[3];
     const float* log_decay;
     const void* starts;
-    long long n_moments, L;              // L: moments per segment (a multiple of CHUNK)
+    long long n_moments, L;              // L: moments per segment (a multiple of CHUNK_MAX)
     int wide, heads, n_seq, nseg, slots; // slots of segments: n_seq x nseg, or an upper bound for packed stretches
 };
 
@@ -82,79 +80,142 @@ __device__ __forceinline__ float start_value(const Scan& s, size_t at, int k, in
     return s.backwards ? z : keep(z);
 }
 
-typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// v = hi + lo (+ what 16 bits do not hold), 8 values
-__device__ __forceinline__ void split2(const float (&v)[8], bf16x8& hi, bf16x8& lo) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi[i] = (bf16)v[i];
-        lo[i] = (bf16)(v[i] - (float)hi[i]);
-    }
-}
-__device__ __forceinline__ void split3(const float (&v)[8], bf16x8& hi, bf16x8& mid, bf16x8& lo) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi[i] = (bf16)v[i];
-        const float r = v[i] - (float)hi[i];
-        mid[i] = (bf16)r;
-        lo[i] = (bf16)(r - (float)mid[i]);
-    }
-}
-
-// A 4 x 16 block of 16-bit values in LDS, transposed: lane c of the 16 gets the block's column c, 4 rows.  p: this lane's
-// share of the block, 4 values of row c / 4.
-__device__ __forceinline__ bf16x4 columns4(const bf16* p) {
-    return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
-}
-__device__ __forceinline__ bf16x8 join(bf16x4 a, bf16x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// 8 values of a row from column c, zeros past the row's end or width
-template <bool VEC>
-__device__ __forceinline__ uint4 load8(const bf16* row, int c, int width, bool there) {
+// A number as a sum of bfloat16 terms, each the rest's nearest: 1, 2, 3 terms hold 8, 16, 24 bits.  A product of two sums
+// keeps the pairs of terms (i, j) with i + j < the longer one's terms: what is dropped is below its last bit.
+template <int P, int V>
+struct Sum {
+    typedef bf16 vec __attribute__((ext_vector_type(V)));
+    vec term[P];
+    __device__ __forceinline__ void of(const float (&v)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float r = v[i];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                term[p][i] = (bf16)r;
+                r -= (float)term[p][i];
+            }
+        }
+    }
+};
+template <int PA, int PB>
+__device__ __forceinline__ f32x4 mfma(const Sum<PA, 8>& a, const Sum<PB, 8>& b, f32x4 c) {
+    constexpr int most = PA > PB ? PA : PB;
+#pragma unroll
+    for (int o = most - 1; o >= 0; --o)                   // (the small ones first)
+#pragma unroll
+        for (int i = 0; i < PA; ++i)
+            if (o - i >= 0 && o - i < PB) c = mfma(a.term[i], b.term[o - i], c);
+    return c;
+}
+
+// How a value type goes through the matrix cores: X terms hold a value exactly; W terms a weight or the state where they
+// make an output (which has no more bits than these); a chunk's moments (what fits LDS with X planes of x, y and v).
+template <class T>
+struct Form;
+template <>
+struct Form<bf16> {
+    static constexpr int X = 1, W = 2, CHUNK = 64;
+};
+template <>
+struct Form<f16> {
+    static constexpr int X = 2, W = 2, CHUNK = 32;
+};
+template <>
+struct Form<float> {
+    static constexpr int X = 3, W = 3, CHUNK = 32;
+};
+constexpr int CHUNK_MAX = 64;
+constexpr int S_TERMS = 3;               // terms of v times its decay: the state is a float32 result
+
+// 16 bytes of a row from column c, zeros past the row's end or width
+template <class T, bool VEC>
+__device__ __forceinline__ uint4 load16(const T* row, int c, int width, bool there) {
     uint4 r = make_uint4(0, 0, 0, 0);
     if (!there || c >= width) return r;
     if (VEC) return *reinterpret_cast<const uint4*>(row + c);
-    unsigned short v[8];
+    typename Vec<T>::type v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < width ? reinterpret_cast<const unsigned short*>(row)[c + i] : 0;
-    r.x = v[0] | v[1] << 16;
-    r.y = v[2] | v[3] << 16;
-    r.z = v[4] | v[5] << 16;
-    r.w = v[6] | v[7] << 16;
-    return r;
+    for (int i = 0; i < Vec<T>::N; ++i) v[i] = c + i < width ? row[c + i] : (T)0.f;
+    return __builtin_bit_cast(uint4, v);
+}
+// ... as terms into its planes in LDS, `plane` apart
+template <class T>
+__device__ __forceinline__ void store_terms(uint4 r, bf16* to, int plane) {
+    if constexpr (Form<T>::X == 1) {
+        *reinterpret_cast<uint4*>(to) = r;
+    } else {
+        constexpr int V = Vec<T>::N;
+        const typename Vec<T>::type in = __builtin_bit_cast(typename Vec<T>::type, r);
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = widen(in[i]);
+        Sum<Form<T>::X, V> s;
+        s.of(v);
+#pragma unroll
+        for (int p = 0; p < Form<T>::X; ++p) *reinterpret_cast<typename Sum<1, V>::vec*>(to + p * plane) = s.term[p];
+    }
 }
 
-// The scan in chunks of 64 moments, bfloat16 values, on the matrix cores (v_mfma_f32_16x16x32_bf16).  With i, j the moments
-// inside a chunk of n and Z the state before it, decayed once (Z = l S),
+// 8 values side by side, of each plane
+template <int P>
+__device__ __forceinline__ Sum<P, 8> across(const bf16* p, int plane) {
+    Sum<P, 8> s;
+#pragma unroll
+    for (int i = 0; i < P; ++i) s.term[i] = *reinterpret_cast<const bf16x8*>(p + i * plane);
+    return s;
+}
+// Two 4 x 16 blocks of LDS, `apart` values apart, transposed: lane c of a block's 16 lanes gets its column c, 4 rows of each.
+// p: this lane's share of the first block, 4 values of row c / 4.
+__device__ __forceinline__ bf16x8 columns8(const bf16* p, int apart) {
+    typedef __attribute__((address_space(3))) s16x4* at;
+    const bf16x4 a = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)p));
+    const bf16x4 b = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(p + apart)));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <int P>
+__device__ __forceinline__ Sum<P, 8> down(const bf16* p, int apart, int plane) {
+    Sum<P, 8> s;
+#pragma unroll
+    for (int i = 0; i < P; ++i) s.term[i] = columns8(p + i * plane, apart);
+    return s;
+}
+
+// The scan in chunks, on the matrix cores (v_mfma_f32_16x16x32_bf16).  With i, j the moments inside a chunk of n and Z the
+// state before it, decayed once (Z = l S),
 //   out_i = c sum_{j <= i} l^(i-j) (x_i . y_j) v_j + c' l^i x_i Z,   Z' = l^n Z + sum_j c'' l^(n-j) y_j v_j^T
 // (forwards c' = c, c'' = 1; backwards c' = 1, c'' = c, so that the end state's gradient comes in and the start state's goes
-// out unscaled).
+// out unscaled).  A stretch's last chunk, where it is short, has its moments in the last rows and zeros before them, so that
+// its decays to the chunk's end are a whole chunk's.
 // A workgroup of WAVES waves walks one segment of one head; wave w owns the state's columns 16 w .., in accumulators all
 // along: a 16 x 16 accumulator block holds, in lane (column c, group g), rows 4g .. 4g + 3, which is also how a product's
 // operand wants it with the rows as the summed index.  So the state passes from product to product in registers, and the
 // order of the summed index (any, if both operands have it) is chosen so: state blocks 2b, 2b + 1 are the rows 32 b + 8g +
 // (0 .. 3), (4 .. 7), and a lane's 8 values of x or y are then side by side.  y^T and v^T come out of LDS by transposing
 // reads.  Outputs are formed transposed, so that a lane stores a row's values side by side.  The weights (x . y) l^(i-j) of
-// the chunk's six 16 x 32 pieces on and below the diagonal are formed by a wave each and shared through LDS.
-// Roundings: x, y, v are exact; weights and Z go into their products as two bfloat16 terms (2^-16), v times its decay as
-// three (2^-24: the state is a float32 result).
+// the chunk's 16 x 32 pieces on and below the diagonal are formed by a wave each and shared through LDS.
 // A value of v that is not finite reaches only the outputs from its moment on (there: NaN), though 0 weights meet it in the
 // products: such a chunk's products run with zeros in its place.
-constexpr int CHUNK = 64;
-template <int KT, int WAVES, bool VEC, bool OUT, class TO>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_scan16(Scans a) {
+template <class T, int KT, int WAVES, bool VEC, bool OUT, class TO>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
+    constexpr int X = Form<T>::X, W = Form<T>::W, CH = Form<T>::CHUNK, JB = CH / 16, VN = Vec<T>::N;
     constexpr int KW = 32 * KT, NW = 16 * WAVES, KP = KW + 8, NP = NW + 8;   // widths, and rows in LDS (no bank conflicts)
-    constexpr int XV = 4 * KT / WAVES, VV = 2;                               // a thread's 16-byte shares of x (y), of v
-    __shared__ __align__(16) bf16 sx[OUT ? CHUNK * KP : 8], sy[CHUNK * KP], sv[CHUNK * NP];
-    __shared__ __align__(16) bf16x8 sp[OUT ? 12 : 1][64];                    // the weights' pieces, two terms each
+    constexpr int XP = CH * KP, VP = CH * NP, PIECES = JB == 4 ? 6 : 2;
+    constexpr int XC = KW / VN, VC = NW / VN;                                // 16-byte shares of a row
+    constexpr int XR = 64 * WAVES / XC, VR = 64 * WAVES / VC;                // rows between a thread's shares
+    constexpr int XV = XR < CH ? CH / XR : 1, VV = CH / VR;                  // a thread's shares (XR > CH: of some threads)
+    static_assert((XV * XR == CH || XR > CH) && VV * VR == CH, "");
+    __shared__ __align__(16) bf16 sx[OUT ? X * XP : 8], sy[X * XP], sv[X * VP];
+    __shared__ __align__(16) bf16x8 sp[OUT ? PIECES : 1][W][64];
     const Scan& s = a.s[blockIdx.z];
     const int nblk = (s.N + NW - 1) / NW;
     const int slot = blockIdx.x / nblk, blk = blockIdx.x % nblk, h = blockIdx.y;
@@ -175,226 +236,224 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan16(Scans a) {
     f32x4 z[2 * KT];                                      // the state
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
     const int col = n0 + w0 + c;
+    const float* z0 = !OUT ? nullptr : s.seg ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : s.init ? s.init + at : nullptr;
     {
-        const Keep once(ld);
-        const float* from_seg = s.seg ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : nullptr;
+        const bool t = !s.seg && s.transposed;
+        const int zk = t ? 1 : s.N, zc = t ? s.K : 1;
+        const Keep once(!s.seg && !s.backwards && count ? ld : 0.f);      // (no moments: the state goes through as it is)
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int k = row_of(b, r);
-                z[b][r] = !OUT ? 0.f : from_seg ? (k < s.K && col < s.N ? from_seg[(size_t)k * s.N + col] : 0.f)
-                                                : start_value(s, at, k, col, once);
+                z[b][r] = z0 && k < s.K && col < s.N ? once(z0[k * zk + col * zc]) : 0.f;
             }
     }
 
     // this thread's shares of a chunk's rows
-    constexpr int XR = 64 * WAVES / (4 * KT), VR = CHUNK / VV;               // rows between a thread's shares
-    const int xrow = tid / (4 * KT), xcol = tid % (4 * KT) * 8, vrow = tid / (2 * WAVES), vcol = tid % (2 * WAVES) * 8;
+    const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
     const long long dir = s.backwards ? -1 : 1;
     const long long t0 = (a.starts ? first : 0) + (s.backwards ? count - 1 - from : from);
     auto base = [&](const fm_view& v, int share) {
-        return (const bf16*)v.data + (a.starts ? 0 : n * v.seq) + (h / share) * v.head + t0 * v.moment;
+        return (const T*)v.data + (a.starts ? 0 : n * v.seq) + (h / share) * v.head + t0 * v.moment;
     };
     const long long dx = dir * s.x.moment, dy = dir * s.y.moment, dv = dir * s.v.moment;
-    const bf16* px = OUT ? base(s.x, s.xs) + xrow * dx : nullptr;
-    const bf16* py = base(s.y, s.ys) + xrow * dy;
-    const bf16* pv = base(s.v, s.vs) + vrow * dv;
+    const T* px = OUT ? base(s.x, s.xs) + xrow * dx : nullptr;
+    const T* py = base(s.y, s.ys) + xrow * dy;
+    const T* pv = base(s.v, s.vs) + vrow * dv + n0;
     uint4 rx[XV], ry[XV], rv[VV];
-    auto fetch = [&](long long i0) {                      // the chunk from the segment's moment i0, where the pointers stand
-#pragma unroll
-        for (int i = 0; i < XV; ++i) {
-            const bool there = i0 + xrow + i * XR < left;
-            if (OUT) rx[i] = load8<VEC>(px + i * XR * dx, xcol, s.K, there);
-            ry[i] = load8<VEC>(py + i * XR * dy, xcol, s.K, there);
+    auto fetch = [&](int rows) {                          // the next chunk, of so many moments
+        const int pad = CH - rows;
+        if (pad) {
+            px -= OUT ? pad * dx : 0;
+            py -= pad * dy;
+            pv -= pad * dv;
         }
 #pragma unroll
-        for (int i = 0; i < VV; ++i) rv[i] = load8<VEC>(pv + i * VR * dv + n0, vcol, s.N - n0, i0 + vrow + i * VR < left);
-        if (OUT) px += CHUNK * dx;
-        py += CHUNK * dy;
-        pv += CHUNK * dv;
+        for (int i = 0; i < XV; ++i) {
+            const bool there = xrow + i * XR >= pad && (XR <= CH || xrow < CH);
+            if (OUT) rx[i] = load16<T, VEC>(px + i * XR * dx, xcol, s.K, there);
+            ry[i] = load16<T, VEC>(py + i * XR * dy, xcol, s.K, there);
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) rv[i] = load16<T, VEC>(pv + i * VR * dv, vcol, s.N - n0, vrow + i * VR >= pad);
+        if (OUT) px += CH * dx;
+        py += CH * dy;
+        pv += CH * dv;
     };
-    fetch(0);
+    auto rows_from = [&](long long i0) { return (int)(left - i0 < CH ? left - i0 : CH); };
+    if (left > 0) fetch(rows_from(0));
 
-    float rest[4];                                        // l^(16 - row in its block), times what backwards scales v with
     const float cv = s.backwards ? s.c : 1.f;
+    float rest[4];                                        // the decay from a 16-row block's row to its end, times c''
 #pragma unroll
     for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r);
-    const float row16 = (s.backwards ? 1.f : s.c) * power(c);
+    const float cz = s.backwards ? 1.f : s.c, row0 = cz * power(c);
     const float p16 = power(16), p32 = power(32), p48 = power(48);
-    const Keep chunk(ld * CHUNK);
-    TO* out = OUT ? (TO*)s.out : nullptr;
-    const long long out_row = (a.starts ? 0 : n * a.n_moments) + t0;
+    auto blocks = [&](int i) { return i == 0 ? 1.f : i == 1 ? p16 : i == 2 ? p32 : p48; };
+    const Keep chunk(ld * CH);
+    TO* const out = OUT ? (TO*)s.out : nullptr;
+    const long long drow = dir * a.heads * s.N;
+    TO* po = OUT ? out + (((a.starts ? 0 : n * a.n_moments) + t0) * a.heads + h) * s.N + c * drow + n0 + w0 + 4 * g : nullptr;
+    const bf16* const vdown = &sv[(4 * g + (c >> 2)) * NP + w0 + 4 * (c & 3)];
 
-    for (long long i0 = 0; i0 < left; i0 += CHUNK) {
-        const int rows = (int)(left - i0 < CHUNK ? left - i0 : CHUNK);
+    for (long long i0 = 0; i0 < left; i0 += CH) {
+        const int pad = CH - rows_from(i0);
         __syncthreads();                                  // (the chunk before is read)
 #pragma unroll
         for (int i = 0; i < XV; ++i) {
-            if (OUT) *reinterpret_cast<uint4*>(&sx[(xrow + i * XR) * KP + xcol]) = rx[i];
-            *reinterpret_cast<uint4*>(&sy[(xrow + i * XR) * KP + xcol]) = ry[i];
+            if (XR > CH && xrow >= CH) break;
+            if (OUT) store_terms<T>(rx[i], &sx[(xrow + i * XR) * KP + xcol], XP);
+            store_terms<T>(ry[i], &sy[(xrow + i * XR) * KP + xcol], XP);
         }
 #pragma unroll
-        for (int i = 0; i < VV; ++i) *reinterpret_cast<uint4*>(&sv[(vrow + i * VR) * NP + vcol]) = rv[i];
+        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], &sv[(vrow + i * VR) * NP + vcol], VP);
         __syncthreads();
-        if (i0 + CHUNK < left) fetch(i0 + CHUNK);
+        if (i0 + CH < left) fetch(rows_from(i0 + CH));
 
-        f32x4 o[4];
         if (OUT && out) {
-            // pieces of weights: rows 32 jj .., columns 16 i .. of (0,0) (1,0) (2,0) (3,0) (2,1) (3,1)
-            for (int piece = wave; piece < 6; piece += WAVES) {
+            // pieces of weights: rows 32 jj .., columns 16 i .. of (jj, i) = (0, 0) (0, 1) (0, 2) (0, 3) (1, 2) (1, 3)
+            for (int piece = wave; piece < PIECES; piece += WAVES) {
                 const int jj = piece >> 2, i = jj ? piece - 2 : piece;
-                f32x4 p0{0.f, 0.f, 0.f, 0.f}, p1{0.f, 0.f, 0.f, 0.f};
+                f32x4 p[2] = {};
 #pragma unroll
                 for (int b = 0; b < KT; ++b) {
-                    const bf16x8 xf = *reinterpret_cast<const bf16x8*>(&sx[(16 * i + c) * KP + 32 * b + 8 * g]);
+                    const Sum<X, 8> xf = across<X>(&sx[(16 * i + c) * KP + 32 * b + 8 * g], XP);
                     const bf16* y = &sy[(32 * jj + c) * KP + 32 * b + 8 * g];
-                    p0 = mfma(*reinterpret_cast<const bf16x8*>(y), xf, p0);
-                    p1 = mfma(*reinterpret_cast<const bf16x8*>(y + 16 * KP), xf, p1);
+                    p[0] = mfma(across<X>(y, XP), xf, p[0]);
+                    p[1] = mfma(across<X>(y + 16 * KP, XP), xf, p[1]);
                 }
                 float v[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     const int d = 16 * i + c - (32 * jj + 16 * (r >> 2) + 4 * g + (r & 3));
-                    v[r] = d >= 0 ? s.c * power(d) * (r < 4 ? p0[r] : p1[r - 4]) : 0.f;      // (whatever x . y is there)
+                    v[r] = d >= 0 ? s.c * power(d) * p[r >> 2][r & 3] : 0.f;      // (whatever x . y is there)
                 }
-                bf16x8 ph, pl;
-                split2(v, ph, pl);
-                sp[2 * piece][lane] = ph;
-                sp[2 * piece + 1][lane] = pl;
-            }
+                Sum<W, 8> w;
+                w.of(v);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < W; ++t) sp[piece][t][lane] = w.term[t];
+            }
+            f32x4 o[JB] = {};
 #pragma unroll
             for (int b = 0; b < KT; ++b) {
-                bf16x8 zh, zl;
                 float v[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) v[r] = z[2 * b + (r >> 2)][r & 3];
-                split2(v, zh, zl);
+                Sum<W, 8> zf;
+                zf.of(v);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bf16x8 xf = *reinterpret_cast<const bf16x8*>(&sx[(16 * i + c) * KP + 32 * b + 8 * g]);
-                    o[i] = mfma(zl, xf, o[i]);
-                    o[i] = mfma(zh, xf, o[i]);
-                }
+                for (int i = 0; i < JB; ++i) o[i] = mfma(zf, across<X>(&sx[(16 * i + c) * KP + 32 * b + 8 * g], XP), o[i]);
             }
-            __syncthreads();                              // (the pieces are there)
-        }
-
-        // v^T: block j's rows 4g .. of this wave's columns
-        bf16x4 vt[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vt[j] = columns4(&sv[(16 * j + 4 * g + (c >> 2)) * NP + w0 + 4 * (c & 3)]);
-        if (OUT && out) {
+            for (int i = 0; i < JB; ++i) o[i] *= pad ? cz * power(max(16 * i + c - pad, 0)) : row0 * blocks(i);
+            __syncthreads();                              // (the pieces are there)
             unsigned odd = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint2 u = __builtin_bit_cast(uint2, vt[j]);
-                odd |= ((u.x & 0x7f807f80u) + 0x00800080u) | ((u.y & 0x7f807f80u) + 0x00800080u);
-            }
-            const bool poisoned = __ballot((odd & 0x80008000u) != 0) != 0;
-            float since = 1e9f;                           // poisoned: the first row of column c that is not finite
-            bf16x4 vc[4];
+            for (int jj = 0; jj < JB / 2; ++jj) {
+                Sum<X, 8> vf = down<X>(vdown + 32 * jj * NP, 16 * NP, VP);
+                const uint4 u = __builtin_bit_cast(uint4, vf.term[0]);
+                const unsigned m = 0x7f807f80u, one = 0x00800080u;           // (an exponent of ones carries into the sign)
+                const unsigned bad = (((u.x & m) + one) | ((u.y & m) + one) | ((u.z & m) + one) | ((u.w & m) + one)) & 0x80008000u;
+                odd |= bad;
+                if (__ballot(bad != 0))
 #pragma unroll
-            for (int j = 0; j < 4; ++j) vc[j] = vt[j];
-            if (poisoned) {
+                    for (int r = 0; r < 8; ++r)
+                        if (!(fabsf((float)vf.term[0][r]) < INFINITY))
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                            for (int t = 0; t < X; ++t) vf.term[t][r] = (bf16)0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (!(fabsf((float)vt[j][r]) < INFINITY)) {
-                            vc[j][r] = (bf16)0.f;
-                            since = fminf(since, (float)(16 * j + 4 * g + r));
-                        }
-            }
+                for (int i = 2 * jj; i < JB; ++i) {
+                    Sum<W, 8> w;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[i] *= row16 * (i == 0 ? 1.f : i == 1 ? p16 : i == 2 ? p32 : p48);
-#pragma unroll
-                for (int jj = 0; jj <= i / 2; ++jj) {
-                    const int piece = jj ? i + 2 : i;
-                    const bf16x8 vf = join(vc[2 * jj], vc[2 * jj + 1]);
-                    o[i] = mfma(vf, sp[2 * piece + 1][lane], o[i]);
-                    o[i] = mfma(vf, sp[2 * piece][lane], o[i]);
+                    for (int t = 0; t < W; ++t) w.term[t] = sp[jj ? i + 2 : i][t][lane];
+                    o[i] = mfma(vf, w, o[i]);
                 }
             }
-            if (poisoned) {
+            if (__ballot(odd != 0)) {
+                float since = 1e9f;                       // the first row of column c that is not finite
+#pragma unroll
+                for (int jj = 0; jj < JB / 2; ++jj) {
+                    const bf16x8 v = columns8(vdown + 32 * jj * NP, 16 * NP);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (!(fabsf((float)v[r]) < INFINITY))
+                            since = fminf(since, (float)(32 * jj + 16 * (r >> 2) + 4 * g + (r & 3)));
+                }
                 since = fminf(since, __shfl_xor(since, 16));
                 since = fminf(since, __shfl_xor(since, 32));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float f = __shfl(since, 4 * g + r);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                    for (int i = 0; i < JB; ++i)
                         if ((float)(16 * i + c) >= f) o[i][r] = NAN;
                 }
             }
             const int oc = n0 + w0 + 4 * g;
+            if (pad) po -= pad * drow;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = 16 * i + c;
-                if (row >= rows) continue;
-                TO* to = out + ((out_row + dir * (i0 + row)) * a.heads + h) * s.N + oc;
-                if (VEC && oc + 4 <= s.N) {
+            for (int i = 0; i < JB; ++i) {
+                if (16 * i + c < pad) continue;
+                TO* to = po + 16 * i * drow;
+                if (VEC && oc < s.N) {
                     typedef TO vec __attribute__((ext_vector_type(4)));
                     vec v;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = narrow<TO>(o[i][r]);
                     *reinterpret_cast<vec*>(to) = v;
-                } else
+                } else if (!VEC)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (oc + r < s.N) to[r] = narrow<TO>(o[i][r]);
             }
+            po += CH * drow;
         }
 
         // the state after the chunk; of the stretch's last one forwards, S rather than l S
-        const bool ends = last && i0 + CHUNK >= left;
+        const bool ends = last && i0 + CH >= left;
         if (ends && !s.fin) break;
-        const int n1 = ends && !s.backwards ? rows - 1 : rows;
-        const bool whole = n1 == CHUNK;
-        const Keep keep = whole ? chunk : Keep(ld * (float)n1);
+        Keep keep = chunk;
+        if (ends) {
+            const int early = s.backwards ? 0 : 1;
+            keep = Keep(ld * (float)(CH - pad - early));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r - early);
+        }
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) z[b][r] = keep(z[b][r]);
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            bf16x8 wh, wm, wl;
+        for (int jj = 0; jj < JB / 2; ++jj) {
+            const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NP, 16 * NP, VP);
             float v[8];
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                const int jb = j + (r >> 2), row = 16 * jb + 4 * g + (r & 3);
-                float w = rest[r & 3] * (jb == 0 ? p48 : jb == 1 ? p32 : jb == 2 ? p16 : 1.f);
-                if (!whole) w = cv * power(n1 - row > 0 ? n1 - row : 0);
-                v[r] = w * (float)vt[jb][r & 3];
+                float x = 0.f;
+#pragma unroll
+                for (int t = X - 1; t >= 0; --t) x += (float)vf.term[t][r];
+                v[r] = x * (rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2)));
             }
-            split3(v, wh, wm, wl);
+            Sum<S_TERMS, 8> w;
+            w.of(v);
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
-                const bf16* p = &sy[(16 * j + 4 * g + (c >> 2)) * KP + 32 * (b >> 1) + 8 * (c & 3) + 4 * (b & 1)];
-                const bf16x8 yt = join(columns4(p), columns4(p + 16 * KP));
-                z[b] = mfma(yt, wl, z[b]);
-                z[b] = mfma(yt, wm, z[b]);
-                z[b] = mfma(yt, wh, z[b]);
+                const bf16* p = &sy[(32 * jj + 4 * g + (c >> 2)) * KP + 32 * (b >> 1) + 8 * (c & 3) + 4 * (b & 1)];
+                z[b] = mfma(down<X>(p, 16 * KP, XP), w, z[b]);
             }
         }
     }
 
-    float* to = !OUT ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : last ? s.fin : nullptr;
-    if (OUT && to) to += at;
-    if (to) {
-        const Keep none(0.f);
+    float* to = !OUT ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : last && s.fin ? s.fin + at : nullptr;
+    if (to)
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int k = row_of(b, r);
-                if (k < s.K && col < s.N)             // (no moments: the start state as it came)
-                    to[(size_t)k * s.N + col] = OUT && count == 0 ? start_value(s, at, k, col, none) : z[b][r];
+                if (k < s.K && col < s.N) to[k * s.N + col] = z[b][r];
             }
-    }
     if (OUT && a.starts && out && seg == 0 && (n == 0 || n == a.n_seq - 1)) {
         // moments of no stretch, before the first one and after the last, give zeros
         for (int e = tid; e < NW; e += 64 * WAVES) {
@@ -417,7 +476,7 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     long long first, count;
     stretch_of(a, n, first, count);
     const float ld = fmaxf(a.log_decay[h], -1e30f);
-    const Keep once(ld), keep(ld * (float)a.L);
+    const Keep once(count ? ld : 0.f), keep(ld * (float)a.L);    // (no moments: the state goes through as it is)
     float z = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, i / s.N, i % s.N, once);
     float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
     const size_t step = (size_t)a.heads * s.K * s.N;
@@ -428,77 +487,6 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
         if (!more) break;
         z = keep(z) + own;
     }
-}
-
-// Moment by moment: a workgroup holds 32 columns of a head's state, 4 columns and every 32nd row a lane.
-// grid (blocks of columns, heads, stretches x scans)
-template <class T, class TO>
-__global__ __launch_bounds__(256) void k_scan_simple(Scans a, int n_seq) {
-    __shared__ float xs[ATT_MAX], ys[ATT_MAX], part[4][32];
-    const Scan& s = a.s[blockIdx.z / n_seq];
-    const int n = blockIdx.z % n_seq, h = blockIdx.y, tid = threadIdx.x, cg = tid & 7, rg = tid >> 3;
-    const int c0 = blockIdx.x * 32 + 4 * cg, K = s.K, N = s.N;
-    if (blockIdx.x * 32 >= N) return;
-    long long first, count;
-    stretch_of(a, n, first, count);
-    const T* x = (const T*)s.x.data + (a.starts ? 0 : n * s.x.seq) + (h / s.xs) * s.x.head;
-    const T* y = (const T*)s.y.data + (a.starts ? 0 : n * s.y.seq) + (h / s.ys) * s.y.head;
-    const T* v = (const T*)s.v.data + (a.starts ? 0 : n * s.v.seq) + (h / s.vs) * s.v.head;
-    TO* out = (TO*)s.out + ((a.starts ? first : n * a.n_moments) * a.heads + h) * N;
-    const Keep keep(a.log_decay[h]);
-    float z[4][4] = {};
-    const size_t at = ((size_t)n * a.heads + h) * K * N;
-    if (s.init)
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int k = rg + 32 * i, c = c0 + j;
-                if (k < K && c < N) z[i][j] = s.init[at + (s.transposed ? (size_t)c * K + k : (size_t)k * N + c)];
-            }
-    for (long long i = 0; i < count; ++i) {
-        const long long t = s.backwards ? count - 1 - i : i;
-        __syncthreads();
-        for (int k = tid; k < K; k += 256) {
-            xs[k] = s.out ? widen(x[(first + t) * s.x.moment + k]) : 0.f;
-            ys[k] = widen(y[(first + t) * s.y.moment + k]);
-        }
-        __syncthreads();
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        float vv[4];
-        for (int j = 0; j < 4; ++j) vv[j] = c0 + j < N ? (s.backwards ? s.c : 1.f) * widen(v[(first + t) * s.v.moment + c0 + j]) : 0.f;
-        const bool first_back = s.backwards && i == 0;
-        for (int r = 0; r < 4; ++r) {
-            const int k = rg + 32 * r;
-            if (k >= K) break;
-            for (int j = 0; j < 4; ++j) z[r][j] = (first_back ? z[r][j] : keep(z[r][j])) + ys[k] * vv[j];
-            fma4(xs[k], make_float4(z[r][0], z[r][1], z[r][2], z[r][3]), o);
-        }
-        for (int m = 8; m < 64; m <<= 1) {
-            o.x += __shfl_xor(o.x, m);
-            o.y += __shfl_xor(o.y, m);
-            o.z += __shfl_xor(o.z, m);
-            o.w += __shfl_xor(o.w, m);
-        }
-        if ((tid & 63) < 8) *(float4*)&part[tid >> 6][4 * cg] = o;
-        __syncthreads();
-        if (s.out && tid < 32 && blockIdx.x * 32 + tid < N)
-            out[t * a.heads * N + blockIdx.x * 32 + tid] =
-                narrow<TO>((s.backwards ? 1.f : s.c) * (part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
-    }
-    if (a.starts && s.out) {             // moments of no stretch: those before the first one and after the last
-        TO* all = (TO*)s.out + (size_t)h * N + blockIdx.x * 32 + (tid & 31);
-        if (blockIdx.x * 32 + (tid & 31) < N) {
-            if (n == 0)
-                for (long long t = tid >> 5; t < first; t += 8) all[t * a.heads * N] = narrow<TO>(0.f);
-            if (n == n_seq - 1)
-                for (long long t = first + count + (tid >> 5); t < a.n_moments; t += 8) all[t * a.heads * N] = narrow<TO>(0.f);
-        }
-    }
-    if (s.fin)
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int k = rg + 32 * i, c = c0 + j;
-                if (k < K && c < N) s.fin[at + (size_t)k * N + c] = s.backwards && count ? keep(z[i][j]) : z[i][j];
-            }
 }
 
 // gradients of shared heads: out[m][j][d] = the sum over a key head's `share` query heads of part[m][share j + i][d]
@@ -590,9 +578,9 @@ Cut cut_of(const fm_attention_args& p, int scans) {
     const long long groups = p.n_seq * p.q_heads * scans;
     c.nseg = 1;
     c.slots = (int)p.n_seq;
-    c.L = (p.n_moments + CHUNK - 1) / CHUNK * CHUNK;
+    c.L = (p.n_moments + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
     if (groups >= SEG_GROUPS / 2 || !groups) return c;
-    long long L = (moments * p.q_heads * scans / SEG_GROUPS + CHUNK - 1) / CHUNK * CHUNK;
+    long long L = (moments * p.q_heads * scans / SEG_GROUPS + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
     if (L < SEG_MIN) L = SEG_MIN;
     if (L >= p.n_moments) return c;
     c.L = L;
@@ -602,11 +590,11 @@ Cut cut_of(const fm_attention_args& p, int scans) {
 }
 // floats of segments' states of one scan
 long long segment_floats(const fm_attention_args& p, const Cut& c) {
-    return c.nseg == 1 || p.dtype != FM_BF16 ? 0 : (long long)c.slots * p.q_heads * p.k_dim * p.v_dim;
+    return c.nseg == 1 ? 0 : (long long)c.slots * p.q_heads * p.k_dim * p.v_dim;
 }
 
-template <int KT, int WAVES, bool VEC, class TO>
-void launch16(Scans& a, int count, hipStream_t st) {
+template <class T, int KT, int WAVES, bool VEC, class TO>
+void launch_form(Scans& a, int count, hipStream_t st) {
     int nblk = 1, most = 1;
     for (int i = 0; i < count; ++i) {
         const int b = (a.s[i].N + 16 * WAVES - 1) / (16 * WAVES), kn = a.s[i].K * a.s[i].N;
@@ -615,37 +603,31 @@ void launch16(Scans& a, int count, hipStream_t st) {
     }
     const dim3 grid(a.slots * nblk, a.heads, count);
     if (a.nseg > 1) {
-        k_scan16<KT, WAVES, VEC, false, TO><<<grid, 64 * WAVES, 0, st>>>(a);
+        k_scan<T, KT, WAVES, VEC, false, TO><<<grid, 64 * WAVES, 0, st>>>(a);
         k_scan_join<<<dim3((most + 255) / 256 * a.heads, a.n_seq, count), 256, 0, st>>>(a);
     }
-    k_scan16<KT, WAVES, VEC, true, TO><<<grid, 64 * WAVES, 0, st>>>(a);
+    k_scan<T, KT, WAVES, VEC, true, TO><<<grid, 64 * WAVES, 0, st>>>(a);
 }
-template <class TO>
-void launch16_of(Scans& a, int count, bool vec, hipStream_t st) {
+template <class T, class TO>
+void launch_sized(Scans& a, int count, bool vec, hipStream_t st) {
     int widest = 0, n = 0;
     for (int i = 0; i < count; ++i) {
         widest = a.s[i].K > widest ? a.s[i].K : widest;
         n = a.s[i].N > n ? a.s[i].N : n;
     }
-    if (widest <= 64 && n <= 64) vec ? launch16<2, 4, true, TO>(a, count, st) : launch16<2, 4, false, TO>(a, count, st);
-    else if (widest <= 64) vec ? launch16<2, 8, true, TO>(a, count, st) : launch16<2, 8, false, TO>(a, count, st);
-    else if (n <= 64) vec ? launch16<4, 4, true, TO>(a, count, st) : launch16<4, 4, false, TO>(a, count, st);
-    else vec ? launch16<4, 8, true, TO>(a, count, st) : launch16<4, 8, false, TO>(a, count, st);
+    if (widest <= 64 && n <= 64) vec ? launch_form<T, 2, 4, true, TO>(a, count, st) : launch_form<T, 2, 4, false, TO>(a, count, st);
+    else if (widest <= 64) vec ? launch_form<T, 2, 8, true, TO>(a, count, st) : launch_form<T, 2, 8, false, TO>(a, count, st);
+    else if (n <= 64) vec ? launch_form<T, 4, 4, true, TO>(a, count, st) : launch_form<T, 4, 4, false, TO>(a, count, st);
+    else vec ? launch_form<T, 4, 8, true, TO>(a, count, st) : launch_form<T, 4, 8, false, TO>(a, count, st);
 }
 
 template <class T, class TO>
 void launch_scans(Scans& a, int count, const Cut& cut, bool vec, hipStream_t st) {
     if (!a.n_seq || !count) return;
-    if constexpr (sizeof(T) == 2 && !std::is_same<T, f16>::value) {
-        a.L = cut.L > 0 ? cut.L : CHUNK;
-        a.nseg = cut.nseg;
-        a.slots = cut.slots;
-        launch16_of<TO>(a, count, vec, st);
-    } else {
-        int widest = 0;
-        for (int i = 0; i < count; ++i) widest = a.s[i].N > widest ? a.s[i].N : widest;
-        k_scan_simple<T, TO><<<dim3((widest + 31) / 32, a.heads, a.n_seq * count), 256, 0, st>>>(a, a.n_seq);
-    }
+    a.L = cut.L > 0 ? cut.L : CHUNK_MAX;
+    a.nseg = cut.nseg;
+    a.slots = cut.slots;
+    launch_sized<T, TO>(a, count, vec, st);
 }
 
 Scans scans_of(const fm_attention_args& p) {
@@ -659,10 +641,10 @@ Scans scans_of(const fm_attention_args& p) {
     return a;
 }
 
-// 16-byte loads and stores: heads of a multiple of 8 values, everything aligned
+// 16-byte loads, whole stores: heads of a multiple of 16 bytes, everything aligned
 bool wide_rows(const fm_attention_args& p, bool bwd) {
     const int size = p.dtype == FM_F32 ? 4 : 2;
-    if (p.k_dim % 8 || p.v_dim % 8 || !aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
+    if (p.k_dim * size % 16 || p.v_dim * size % 16 || !aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
     if (bwd) return aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv | (uintptr_t)p.workspace) & 15);
     return !((uintptr_t)p.o & 15);
 }

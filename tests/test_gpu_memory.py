@@ -226,7 +226,7 @@ def test_attention_and_its_gradients(gpu_lib, case):
 
 
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
-@pytest.mark.parametrize("lengths", [[0], [1], [0, 3, 0, 64, 1, 129, 0], [65, 63, 2, 700, 17, 16], [1200, 5]])
+@pytest.mark.parametrize("lengths", [[0], [1], [0, 3, 0, 64, 1, 129, 0], [65, 63, 2, 700, 17, 16], [1200, 5], [0, 700, 0, 600, 0]])
 def test_packed_stretches(gpu_lib, dt, lengths):
     say(f"packed {lengths} {dt}")
     gen = torch.Generator().manual_seed(len(lengths))
@@ -372,6 +372,21 @@ def test_pieces_of_a_stretch_and_single_moments(gpu_lib):
         for a, b in ((o, e), (torch.cat([o1, o2], 1), e2), (torch.stack(outs, 1), live)):
             ref.within(a, want[0], mag[0], 64 + 32 + 150 + 200, "o", extra)
             ref.within(b, want[1], mag[1], 64 + 32 + 150 + 200, "state", extra)
+
+
+def test_long_stretches_keep_their_precision(gpu_lib):
+    """20,000 moments of heads that hardly forget: the end state within a few roundings of its own size, as its moments'
+    random signs add (errors of 20,000 roundings in one direction, as a rounded decay taken 300 times gives, would show)."""
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(12)
+    g = torch.tensor([-1e-5, -3e-4], device="cuda")
+    for dt in (F32, BF16):
+        q, k, v, _ = inputs(gen, 1, 20000, 2, 2, 16, 16, dt, "dense", False)
+        _, e = decay_attention(q, k, v, g)
+        f = [x.cpu().double() for x in (k, v)]
+        w = torch.exp(g.cpu().double()[:, None] * torch.arange(19999, -1, -1, dtype=torch.float64))
+        want = torch.einsum("ht,thk,thv->hkv", w, f[0][0], f[1][0])
+        assert float((e[0].cpu().double() - want).norm() / want.norm()) <= 1e-6
 
 
 def test_far_strides(gpu_lib):
