@@ -94,19 +94,17 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 template <int P, int V>
 struct Sum {
     typedef bf16 vec __attribute__((ext_vector_type(V)));
+    typedef float wide __attribute__((ext_vector_type(V)));
     vec term[P];
-    __device__ __forceinline__ void of(const float (&v)[V]) {
+    __device__ __forceinline__ void of(wide r) {          // (whole vectors: two values a conversion)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float r = v[i];
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                term[p][i] = (bf16)r;
-                r -= (float)term[p][i];
-            }
+        for (int p = 0; p < P; ++p) {
+            term[p] = __builtin_convertvector(r, vec);
+            if (p + 1 < P) r -= __builtin_convertvector(term[p], wide);
         }
     }
 };
+typedef Sum<1, 8>::wide f32x8;
 template <int PA, int PB>
 __device__ __forceinline__ f32x4 mfma(const Sum<PA, 8>& a, const Sum<PB, 8>& b, f32x4 c) {
     constexpr int most = PA > PB ? PA : PB;
@@ -156,11 +154,8 @@ __device__ __forceinline__ void store_terms(uint4 r, bf16* to, int plane) {
     } else {
         constexpr int V = Vec<T>::N;
         const typename Vec<T>::type in = __builtin_bit_cast(typename Vec<T>::type, r);
-        float v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = widen(in[i]);
         Sum<Form<T>::X, V> s;
-        s.of(v);
+        s.of(__builtin_convertvector(in, typename Sum<1, V>::wide));
 #pragma unroll
         for (int p = 0; p < Form<T>::X; ++p) *reinterpret_cast<typename Sum<1, V>::vec*>(to + p * plane) = s.term[p];
     }
@@ -205,11 +200,33 @@ __device__ __forceinline__ Sum<P, 8> down(const bf16* p, int apart, int plane) {
 // the chunk's 16 x 32 pieces on and below the diagonal are formed by a wave each and shared through LDS.
 // A value of v that is not finite reaches only the outputs from its moment on (there: NaN), though 0 weights meet it in the
 // products: such a chunk's products run with zeros in its place.
+template <class T, int KT, int WAVES, bool OUT>
+struct Tile {
+    static constexpr int CH = Form<T>::CHUNK, KW = 32 * KT, NW = 16 * WAVES;
+    static constexpr int KP = KW + 8, NP = NW + 8;        // rows in LDS: no bank conflicts
+    static constexpr int XP = CH * KP, VP = CH * NP, PIECES = CH == 64 ? 6 : 2;
+    static constexpr int LDS = Form<T>::X * 2 * (XP * (OUT ? 2 : 1) + VP) + (OUT ? PIECES * Form<T>::W * 1024 : 0);
+    // waves a SIMD that LDS lets in, at most 4 (128 registers)
+    static constexpr int FIT = 160 * 1024 / LDS * WAVES / 4;
+    static constexpr int PER_SIMD = FIT < 1 ? 1 : FIT > 4 ? 4 : FIT;
+};
+// an opaque copy: what is computed from it stays where it is used, instead of in registers all along
+template <class V>
+__device__ __forceinline__ V here(V v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// a value that all lanes share, in a scalar register
+__device__ __forceinline__ float shared_by_all(float v) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
 template <class T, int KT, int WAVES, bool VEC, bool OUT, class TO>
-__global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
-    constexpr int X = Form<T>::X, W = Form<T>::W, CH = Form<T>::CHUNK, JB = CH / 16, VN = Vec<T>::N;
-    constexpr int KW = 32 * KT, NW = 16 * WAVES, KP = KW + 8, NP = NW + 8;   // widths, and rows in LDS (no bank conflicts)
-    constexpr int XP = CH * KP, VP = CH * NP, PIECES = JB == 4 ? 6 : 2;
+__global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) void k_scan(Scans a) {
+    using S = Tile<T, KT, WAVES, OUT>;
+    constexpr int X = Form<T>::X, W = Form<T>::W, CH = S::CH, JB = CH / 16, VN = Vec<T>::N;
+    constexpr int KW = S::KW, NW = S::NW, KP = S::KP, NP = S::NP, XP = S::XP, VP = S::VP, PIECES = S::PIECES;
     constexpr int XC = KW / VN, VC = NW / VN;                                // 16-byte shares of a row
     constexpr int XR = 64 * WAVES / XC, VR = 64 * WAVES / VC;                // rows between a thread's shares
     constexpr int XV = XR < CH ? CH / XR : 1, VV = CH / VR;                  // a thread's shares (XR > CH: of some threads)
@@ -228,10 +245,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
     const long long from = seg * a.L, left = count - from < a.L ? count - from : a.L;
     const bool last = from + left == count;
     if (!OUT && last) return;                             // (the last segment's own state is needed by none)
-    const float ld = fmaxf(a.log_decay[h], -1e30f);       // (-inf: 0 times it would not be 0)
+    const float ld = shared_by_all(fmaxf(a.log_decay[h], -1e30f));        // (-inf: 0 times it would not be 0)
     const size_t at = ((size_t)n * a.heads + h) * s.K * s.N;
-    const float e2 = ld * 1.44269504f;
-    auto power = [&](int i) { return exp2f(e2 * (float)i); };
+    const float e2 = shared_by_all(ld * 1.44269504f);
+    auto power = [&](int i) { return __builtin_amdgcn_exp2f(e2 * (float)i); };
 
     f32x4 z[2 * KT];                                      // the state
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
@@ -242,12 +259,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
         const int zk = t ? 1 : s.N, zc = t ? s.K : 1;
         const Keep once(!s.seg && !s.backwards && count ? ld : 0.f);      // (no moments: the state goes through as it is)
 #pragma unroll
-        for (int b = 0; b < 2 * KT; ++b)
+        for (int b = 0; b < 2 * KT; ++b) z[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (z0) {
+            const float* p = z0 + min(col, s.N - 1) * zc;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int k = row_of(b, r);
-                z[b][r] = z0 && k < s.K && col < s.N ? once(z0[k * zk + col * zc]) : 0.f;
-            }
+            for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[b][r] = p[min(row_of(b, r), s.K - 1) * zk];
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[b][r] = row_of(b, r) < s.K && col < s.N ? once(z[b][r]) : 0.f;
+        }
     }
 
     // this thread's shares of a chunk's rows
@@ -289,9 +312,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r);
     const float cz = s.backwards ? 1.f : s.c, row0 = cz * power(c);
-    const float p16 = power(16), p32 = power(32), p48 = power(48);
+    const float p16 = shared_by_all(power(16)), p32 = shared_by_all(power(32)), p48 = shared_by_all(power(48));
     auto blocks = [&](int i) { return i == 0 ? 1.f : i == 1 ? p16 : i == 2 ? p32 : p48; };
-    const Keep chunk(ld * CH);
+    Keep keep(ld * CH);                                   // over a whole chunk
+    keep.one = shared_by_all(keep.one);
+    keep.f = shared_by_all(keep.f);
     TO* const out = OUT ? (TO*)s.out : nullptr;
     const long long drow = dir * a.heads * s.N;
     TO* po = OUT ? out + (((a.starts ? 0 : n * a.n_moments) + t0) * a.heads + h) * s.N + c * drow + n0 + w0 + 4 * g : nullptr;
@@ -309,12 +334,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
 #pragma unroll
         for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], &sv[(vrow + i * VR) * NP + vcol], VP);
         __syncthreads();
-        if (i0 + CH < left) fetch(rows_from(i0 + CH));
 
+        f32x4 o[JB] = {};
         if (OUT && out) {
             // pieces of weights: rows 32 jj .., columns 16 i .. of (jj, i) = (0, 0) (0, 1) (0, 2) (0, 3) (1, 2) (1, 3)
             for (int piece = wave; piece < PIECES; piece += WAVES) {
-                const int jj = piece >> 2, i = jj ? piece - 2 : piece;
+                const int jj = piece >> 2, i = jj ? piece - 2 : piece, d0 = here(16 * i + c - 32 * jj - 4 * g);
                 f32x4 p[2] = {};
 #pragma unroll
                 for (int b = 0; b < KT; ++b) {
@@ -323,10 +348,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
                     p[0] = mfma(across<X>(y, XP), xf, p[0]);
                     p[1] = mfma(across<X>(y + 16 * KP, XP), xf, p[1]);
                 }
-                float v[8];
+                f32x8 v;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    const int d = 16 * i + c - (32 * jj + 16 * (r >> 2) + 4 * g + (r & 3));
+                    const int d = d0 - 16 * (r >> 2) - (r & 3);
                     v[r] = d >= 0 ? s.c * power(d) * p[r >> 2][r & 3] : 0.f;      // (whatever x . y is there)
                 }
                 Sum<W, 8> w;
@@ -334,20 +359,26 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
 #pragma unroll
                 for (int t = 0; t < W; ++t) sp[piece][t][lane] = w.term[t];
             }
-            f32x4 o[JB] = {};
 #pragma unroll
             for (int b = 0; b < KT; ++b) {
-                float v[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] = z[2 * b + (r >> 2)][r & 3];
                 Sum<W, 8> zf;
-                zf.of(v);
+                zf.of(__builtin_shufflevector(z[2 * b], z[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                 for (int i = 0; i < JB; ++i) o[i] = mfma(zf, across<X>(&sx[(16 * i + c) * KP + 32 * b + 8 * g], XP), o[i]);
             }
+            const int c1 = here(c) - pad;
+            const float f0 = here(row0);
 #pragma unroll
-            for (int i = 0; i < JB; ++i) o[i] *= pad ? cz * power(max(16 * i + c - pad, 0)) : row0 * blocks(i);
+            for (int i = 0; i < JB; ++i) {
+                const float f = pad ? cz * power(max(16 * i + c1, 0)) : f0 * blocks(i);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[i][r] *= f;
+            }
             __syncthreads();                              // (the pieces are there)
+        }
+        // (the next chunk on its way from here: earlier, its registers push the products' operands out)
+        if (i0 + CH < left) fetch(rows_from(i0 + CH));
+        if (OUT && out) {
             unsigned odd = 0;
 #pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
@@ -371,30 +402,31 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
                 }
             }
             if (__ballot(odd != 0)) {
-                float since = 1e9f;                       // the first row of column c that is not finite
+                int since = CH;                           // the first row of column c that is not finite
+                const int g4 = here(4 * g), c1 = here(c);
 #pragma unroll
                 for (int jj = 0; jj < JB / 2; ++jj) {
                     const bf16x8 v = columns8(vdown + 32 * jj * NP, 16 * NP);
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
                         if (!(fabsf((float)v[r]) < INFINITY))
-                            since = fminf(since, (float)(32 * jj + 16 * (r >> 2) + 4 * g + (r & 3)));
+                            since = min(since, 32 * jj + 16 * (r >> 2) + g4 + (r & 3));
                 }
-                since = fminf(since, __shfl_xor(since, 16));
-                since = fminf(since, __shfl_xor(since, 32));
+                since = min(since, __shfl_xor(since, 16));
+                since = min(since, __shfl_xor(since, 32));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float f = __shfl(since, 4 * g + r);
+                    const int f = __shfl(since, g4 + r);
 #pragma unroll
                     for (int i = 0; i < JB; ++i)
-                        if ((float)(16 * i + c) >= f) o[i][r] = NAN;
+                        if (16 * i + c1 >= f) o[i][r] = NAN;
                 }
             }
             const int oc = n0 + w0 + 4 * g;
             if (pad) po -= pad * drow;
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
-                if (16 * i + c < pad) continue;
+                if (c < pad - 16 * i) continue;
                 TO* to = po + 16 * i * drow;
                 if (VEC && oc < s.N) {
                     typedef TO vec __attribute__((ext_vector_type(4)));
@@ -413,10 +445,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
         // the state after the chunk; of the stretch's last one forwards, S rather than l S
         const bool ends = last && i0 + CH >= left;
         if (ends && !s.fin) break;
-        Keep keep = chunk;
         if (ends) {
             const int early = s.backwards ? 0 : 1;
-            keep = Keep(ld * (float)(CH - pad - early));
+            const Keep k(ld * (float)(CH - pad - early));
+            keep.one = shared_by_all(k.one);
+            keep.f = shared_by_all(k.f);
 #pragma unroll
             for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r - early);
         }
@@ -427,14 +460,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
             const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NP, 16 * NP, VP);
-            float v[8];
+            f32x8 v = __builtin_convertvector(vf.term[X - 1], f32x8);
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                float x = 0.f;
+            for (int t = X - 2; t >= 0; --t) v += __builtin_convertvector(vf.term[t], f32x8);
 #pragma unroll
-                for (int t = X - 1; t >= 0; --t) x += (float)vf.term[t][r];
-                v[r] = x * (rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2)));
-            }
+            for (int r = 0; r < 8; ++r) v[r] *= rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2));
             Sum<S_TERMS, 8> w;
             w.of(v);
 #pragma unroll
@@ -446,14 +476,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void k_scan(Scans a) {
     }
 
     float* to = !OUT ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : last && s.fin ? s.fin + at : nullptr;
-    if (to)
+    if (to) {
+        const int k0 = here(8 * g), c0 = here(col);
+        if (c0 < s.N)
 #pragma unroll
-        for (int b = 0; b < 2 * KT; ++b)
+            for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int k = row_of(b, r);
-                if (k < s.K && col < s.N) to[k * s.N + col] = z[b][r];
-            }
+                for (int r = 0; r < 4; ++r) {
+                    const int k = k0 + 32 * (b >> 1) + 4 * (b & 1) + r;
+                    if (k < s.K) to[k * s.N + c0] = z[b][r];
+                }
+    }
     if (OUT && a.starts && out && seg == 0 && (n == 0 || n == a.n_seq - 1)) {
         // moments of no stretch, before the first one and after the last, give zeros
         for (int e = tid; e < NW; e += 64 * WAVES) {
@@ -502,16 +535,21 @@ __global__ __launch_bounds__(256) void k_share(const float* __restrict__ part, T
     out[i] = narrow<T>(s);
 }
 
-// One moment: a workgroup takes 32 columns of a row's state of one head.  grid (blocks of columns, heads, rows)
-template <class T>
+// One moment: a workgroup takes CB columns of a row's state of one head, CB / 4 lanes a row of it, every (1024 / CB)th row a
+// lane, all a lane's loads under way at once; the lanes' shares of q S are joined over rows by shuffles, then in LDS.
+// VEC: 16-byte loads and stores of the states (v_dim a multiple of 4, states aligned).
+// grid (blocks of columns, heads, rows)
+template <class T, int CB, bool VEC>
 __global__ __launch_bounds__(256) void k_step(fm_step_args a) {
-    __shared__ float part[4][32];
-    const int tid = threadIdx.x, cg = tid & 7, rg = tid >> 3, h = blockIdx.y, K = (int)a.k_dim, N = (int)a.v_dim;
-    const int c0 = blockIdx.x * 32 + 4 * cg;
+    constexpr int LR = CB / 4, RG = 256 / LR, ROWS = ATT_MAX / RG;
+    __shared__ float part[4][CB];
+    const int tid = threadIdx.x, cg = tid % LR, rg = tid / LR, h = blockIdx.y, K = (int)a.k_dim, N = (int)a.v_dim;
+    const int c0 = blockIdx.x * CB + 4 * cg;
     const long long n = blockIdx.z, slot = a.slots ? a.slots[n] : n;
-    T* o = (T*)a.o + (n * a.q_heads + h) * N;
+    T* o = (T*)a.o + (n * a.q_heads + h) * N + blockIdx.x * CB;
+    const int cols = min(CB, N - (int)blockIdx.x * CB);
     if (slot < 0 || slot >= a.n_states) {
-        if (tid < 32 && blockIdx.x * 32 + tid < N) o[blockIdx.x * 32 + tid] = narrow<T>(slot < 0 ? 0.f : NAN);
+        if (tid < cols) o[tid] = narrow<T>(slot < 0 ? 0.f : NAN);
         return;
     }
     const int hk = h / (int)(a.q_heads / a.k_heads);
@@ -519,22 +557,51 @@ __global__ __launch_bounds__(256) void k_step(fm_step_args a) {
     const T* k = (const T*)a.k.data + n * a.k.seq + hk * a.k.head;
     const T* v = (const T*)a.v.data + n * a.v.seq + hk * a.v.head;
     const size_t at = ((size_t)slot * a.q_heads + h) * K * N;
-    const Keep keep(a.log_decay[h]);
-    float acc[4] = {};
-    for (int r = rg; r < K; r += 32)
-        for (int j = 0; j < 4; ++j)
-            if (c0 + j < N) {
-                const float s = keep(a.state[at + (size_t)r * N + c0 + j]) + widen(k[r]) * widen(v[c0 + j]);
-                a.next[at + (size_t)r * N + c0 + j] = s;
-                acc[j] += widen(q[r]) * s;
-            }
-    for (int j = 0; j < 4; ++j) {
-        for (int m = 8; m < 64; m <<= 1) acc[j] += __shfl_xor(acc[j], m);
-        if ((tid & 63) < 8) part[tid >> 6][4 * cg + j] = acc[j];
+    float4 s[ROWS];
+    float kr[ROWS], qr[ROWS], vv[4];
+    auto load = [&](const float* p) {
+        if (VEC) return c0 < N ? *reinterpret_cast<const float4*>(p + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
+        return make_float4(c0 < N ? p[c0] : 0.f, c0 + 1 < N ? p[c0 + 1] : 0.f, c0 + 2 < N ? p[c0 + 2] : 0.f,
+                           c0 + 3 < N ? p[c0 + 3] : 0.f);
+    };
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = rg + i * RG;
+        s[i] = r < K ? load(a.state + at + (size_t)r * N) : make_float4(0.f, 0.f, 0.f, 0.f);
+        kr[i] = r < K ? widen(k[r]) : 0.f;
+        qr[i] = r < K ? widen(q[r]) : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = c0 + j < N ? widen(v[c0 + j]) : 0.f;
+    const Keep keep(a.log_decay[h]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = rg + i * RG;
+        if (r >= K) break;
+        s[i] = make_float4(fmaf(kr[i], vv[0], keep(s[i].x)), fmaf(kr[i], vv[1], keep(s[i].y)),
+                           fmaf(kr[i], vv[2], keep(s[i].z)), fmaf(kr[i], vv[3], keep(s[i].w)));
+        float* p = a.next + at + (size_t)r * N + c0;
+        if (VEC) {
+            if (c0 < N) *reinterpret_cast<float4*>(p) = s[i];
+        } else {
+            if (c0 < N) p[0] = s[i].x;
+            if (c0 + 1 < N) p[1] = s[i].y;
+            if (c0 + 2 < N) p[2] = s[i].z;
+            if (c0 + 3 < N) p[3] = s[i].w;
+        }
+        fma4(qr[i], s[i], acc);
+    }
+#pragma unroll
+    for (int m = LR; m < 64; m <<= 1) {
+        acc.x += __shfl_xor(acc.x, m);
+        acc.y += __shfl_xor(acc.y, m);
+        acc.z += __shfl_xor(acc.z, m);
+        acc.w += __shfl_xor(acc.w, m);
+    }
+    if ((tid & 63) < LR) *reinterpret_cast<float4*>(&part[tid >> 6][4 * cg]) = acc;
     __syncthreads();
-    if (tid < 32 && blockIdx.x * 32 + tid < N)
-        o[blockIdx.x * 32 + tid] = narrow<T>((float)a.scale * (part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
+    if (tid < cols) o[tid] = narrow<T>((float)a.scale * (part[0][tid] + part[1][tid] + part[2][tid] + part[3][tid]));
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -690,6 +757,17 @@ void attention_bwd(const fm_attention_args& p, hipStream_t st) {
     if (rows && p.gv) k_share<T><<<(unsigned)((rows * V + 255) / 256), 256, 0, st>>>(part_v, (T*)p.gv, share, V, rows * V);
 }
 
+#ifndef STEPCB
+#define STEPCB 32
+#endif
+template <class T>
+void step_of_type(const fm_step_args& a, hipStream_t st) {
+    constexpr int CB = STEPCB;
+    const dim3 grid((unsigned)((a.v_dim + CB - 1) / CB), (unsigned)a.q_heads, (unsigned)a.n);
+    if (a.v_dim % 4 || (((uintptr_t)a.state | (uintptr_t)a.next) & 15)) k_step<T, CB, false><<<grid, 256, 0, st>>>(a);
+    else k_step<T, CB, true><<<grid, 256, 0, st>>>(a);
+}
+
 }  // namespace fg
 
 using namespace fg;
@@ -736,10 +814,9 @@ int fm_step(const fm_step_args* a, void* stream) {
     if (!a->n) return 0;
     if (!a->q.data || !a->k.data || !a->v.data || !a->log_decay || !a->state || !a->next || !a->o) return fail("fm_step: a null tensor");
     if (!a->slots && a->n_states < a->n) return fail("fm_step: fewer states than rows");
-    const dim3 grid((unsigned)((a->v_dim + 31) / 32), (unsigned)a->q_heads, (unsigned)a->n);
-    if (a->dtype == FM_F32) k_step<float><<<grid, 256, 0, (hipStream_t)stream>>>(*a);
-    else if (a->dtype == FM_BF16) k_step<bf16><<<grid, 256, 0, (hipStream_t)stream>>>(*a);
-    else k_step<f16><<<grid, 256, 0, (hipStream_t)stream>>>(*a);
+    if (a->dtype == FM_F32) step_of_type<float>(*a, (hipStream_t)stream);
+    else if (a->dtype == FM_BF16) step_of_type<bf16>(*a, (hipStream_t)stream);
+    else step_of_type<f16>(*a, (hipStream_t)stream);
     FG_CHECK(hipGetLastError(), -1);
     return 0;
 }

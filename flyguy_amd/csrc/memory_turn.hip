@@ -30,9 +30,234 @@ __device__ __forceinline__ const float* table_line(const fm_turn_args& a, long l
     return p >= 0 && p < a.n_positions ? a.table + p * a.rotated : nullptr;
 }
 
-// One wave per row (a head of a moment), lanes over its values; a partner's value is read again (a cache hit).
+// Heads of whole 16-byte units (V values), turned ones in whole units: a group of `lanes` lanes (a power of two) takes HB
+// heads of a moment; lane j holds two units of a head, such that its pairs are its own: units j and j + R / 2V of the turned
+// part where pairs lie half apart, units 2j and 2j + 1 where they lie side by side; the rest goes two units a lane.  The
+// lane's V angles, the weights and the moment's addresses serve all HB heads, and all their loads are under way at once.
+struct Lanes {
+    int lanes, shift, q_chunks, chunks;  // lanes = 1 << shift; chunks of HB heads of queries, in all
+};
+template <class T, bool IL>
+struct Units {
+    static constexpr int V = Vec<T>::N;
+    int a, b;                            // first values of the lane's units (b: dim or more: none)
+    bool ta, tb;                         // turned?
+    float c[V], s[V];
+    __device__ __forceinline__ Units(int j, int D, int R) {
+        const int ru = IL ? 0 : R / (2 * V);
+        a = IL ? 2 * j * V : j < ru ? j * V : (2 * j) * V;
+        b = IL ? a + V : j < ru ? (j + ru) * V : a + V;
+        ta = a < R;
+        tb = b < R;
+    }
+    __device__ __forceinline__ void angles(const float* cs, int j, float sign) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool t = IL ? (i < V / 2 ? ta : tb) : ta;
+            if (!t) continue;
+            const float2 f = cs ? reinterpret_cast<const float2*>(cs)[j * V + i] : make_float2(NAN, NAN);
+            c[i] = f.x;
+            s[i] = sign * f.y;
+        }
+    }
+    // x, y: the values of units a, b (one that is not turned is not touched: its values may be anything)
+    __device__ __forceinline__ void turn(float (&x)[V], float (&y)[V]) const {
+        if constexpr (IL) {
+            if (ta) side_by_side(x, 0);
+            if (tb) side_by_side(y, V / 2);
+        } else if (ta)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float p = x[i], q = y[i];
+                x[i] = p * c[i] - q * s[i];
+                y[i] = q * c[i] + p * s[i];
+            }
+    }
+    __device__ __forceinline__ void side_by_side(float (&x)[V], int at) const {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float p = x[2 * i], q = x[2 * i + 1];
+            x[2 * i] = p * c[at + i] - q * s[at + i];
+            x[2 * i + 1] = q * c[at + i] + p * s[at + i];
+        }
+    }
+    __device__ __forceinline__ static void read(const T* p, bool there, typename Vec<T>::type& v) {
+        if (there) v = *reinterpret_cast<const typename Vec<T>::type*>(p);
+        else
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = (T)0.f;
+    }
+    __device__ __forceinline__ static void write(T* p, bool there, const float (&x)[V]) {
+        if (!there) return;
+        typename Vec<T>::type v;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = narrow<T>(x[i]);
+        *reinterpret_cast<typename Vec<T>::type*>(p) = v;
+    }
+    __device__ __forceinline__ static void read_weight(const float* w, int e, bool there, float (&f)[V]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = there ? w[e + i] : 0.f;
+    }
+};
+
+// sums of HB values over the lanes of a group, side by side
+template <int HB>
+__device__ __forceinline__ void group_sums(float (&v)[HB], int lanes) {
+    for (int m = 1; m < lanes; m <<= 1)
+#pragma unroll
+        for (int i = 0; i < HB; ++i) v[i] += __shfl_xor(v[i], m);
+}
+
+template <class T, bool IL, bool NORM, int HB>
+__global__ __launch_bounds__(256) void k_turn_units(fm_turn_args a, Lanes l, float sign) {
+    constexpr int V = Vec<T>::N;
+    const int D = (int)a.dim, R = (int)a.rotated, j = threadIdx.x & (l.lanes - 1);
+    const long long item = (long long)blockIdx.x * (256 >> l.shift) + (threadIdx.x >> l.shift);
+    const long long m = item / l.chunks, n = m / a.n_moments, t = m - n * a.n_moments;
+    if (n >= a.n_seq) return;                             // (a wave's lanes of other groups go on: sums stay in a group)
+    int chunk = (int)(item - m * l.chunks);
+    const int which = chunk >= l.q_chunks;
+    if (which) chunk -= l.q_chunks;
+    const fm_view xv = which ? a.x[1] : a.x[0], yv = which ? a.y[1] : a.y[0];
+    const int h0 = chunk * HB, hn = min(HB, (int)(which ? a.heads[1] : a.heads[0]) - h0);
+    const T* x = (const T*)xv.data + n * xv.seq + t * xv.moment + h0 * xv.head;
+    T* y = (T*)yv.data + n * yv.seq + t * yv.moment + h0 * yv.head;
+    Units<T, IL> u(j, D, R);
+    const bool ha = u.a < D, hb = u.b < D;
+    typename Vec<T>::type va[HB], vb[HB];
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+        u.read(x + i * xv.head + u.a, ha && i < hn, va[i]);
+        u.read(x + i * xv.head + u.b, hb && i < hn, vb[i]);
+    }
+    u.angles(R ? table_line(a, n, t) : nullptr, j, sign);
+    const float* w = which ? a.weight[1] : a.weight[0];
+    float wa[V], wb[V];
+    if (NORM && w) {
+        u.read_weight(w, u.a, ha, wa);
+        u.read_weight(w, u.b, hb, wb);
+    }
+    float sum[HB] = {};
+    if (NORM && w) {
+#pragma unroll
+        for (int i = 0; i < HB; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[i] += widen(va[i][e]) * widen(va[i][e]) + widen(vb[i][e]) * widen(vb[i][e]);
+        group_sums(sum, l.lanes);
+    }
+#pragma unroll
+    for (int i = 0; i < HB; ++i) {
+        float p[V], q[V];
+        const float r = NORM && w ? rsqrtf(sum[i] / D + (float)a.eps) : 1.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            p[e] = widen(va[i][e]);
+            q[e] = widen(vb[i][e]);
+            if (NORM && w) {
+                p[e] *= r * wa[e];
+                q[e] *= r * wb[e];
+            }
+        }
+        u.turn(p, q);
+        u.write(y + i * yv.head + u.a, ha && i < hn, p);
+        u.write(y + i * yv.head + u.b, hb && i < hn, q);
+    }
+}
+
+// The gradient with a norm: the turn undone (the sine's sign flipped), then, with xh = x r and u = g' w, gx = r (u - xh
+// mean(u xh)).  The weights' gradients sum g' xh over rows: a lane keeps its values' sums over its groups' rows, a
+// workgroup's groups are added in LDS, k_turn_gweight adds the workgroups; always in the same order.
+// partial [queries, keys][dim][blocks].  grid (blocks, queries and keys)
+template <class T, bool IL, int HB>
+__global__ __launch_bounds__(256) void k_turn_units_bwd(fm_turn_args a, Lanes l) {
+    constexpr int V = Vec<T>::N;
+    __shared__ float shared[256 * 2 * V];                 // [groups][dim]: dim <= lanes x 2V
+    const int D = (int)a.dim, R = (int)a.rotated, j = threadIdx.x & (l.lanes - 1), group = threadIdx.x >> l.shift;
+    const int groups = 256 >> l.shift, which = blockIdx.y;
+    const fm_view xv = a.x[which], yv = a.y[which], gv = a.g[which];
+    const float* w = a.weight[which];
+    const int H = (int)a.heads[which], chunks = which ? l.chunks - l.q_chunks : l.q_chunks;
+    Units<T, IL> u(j, D, R);
+    const bool ha = u.a < D, hb = u.b < D;
+    float wa[V], wb[V], sa[V] = {}, sb[V] = {};
+    if (w) {
+        u.read_weight(w, u.a, ha, wa);
+        u.read_weight(w, u.b, hb, wb);
+    }
+    const long long items = a.n_seq * a.n_moments * chunks;
+    for (long long item = (long long)blockIdx.x * groups + group; item < items; item += (long long)gridDim.x * groups) {
+        const long long m = item / chunks, n = m / a.n_moments, t = m - n * a.n_moments;
+        const int h0 = (int)(item - m * chunks) * HB, hn = min(HB, H - h0);
+        const T* g = (const T*)gv.data + n * gv.seq + t * gv.moment + h0 * gv.head;
+        const T* x = (const T*)xv.data + n * xv.seq + t * xv.moment + h0 * xv.head;
+        T* y = (T*)yv.data + n * yv.seq + t * yv.moment + h0 * yv.head;
+        typename Vec<T>::type ga[HB], gb[HB], va[HB], vb[HB];
+#pragma unroll
+        for (int i = 0; i < HB; ++i) {
+            u.read(g + i * gv.head + u.a, ha && i < hn, ga[i]);
+            u.read(g + i * gv.head + u.b, hb && i < hn, gb[i]);
+            if (!w) continue;
+            u.read(x + i * xv.head + u.a, ha && i < hn, va[i]);
+            u.read(x + i * xv.head + u.b, hb && i < hn, vb[i]);
+        }
+        u.angles(R ? table_line(a, n, t) : nullptr, j, -1.f);
+        // mean(u xh) = mean((g' w) x) r: both sums over x at once
+        float p[HB][V], q[HB][V], sums[2 * HB] = {};
+#pragma unroll
+        for (int i = 0; i < HB; ++i) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                p[i][e] = widen(ga[i][e]);
+                q[i][e] = widen(gb[i][e]);
+            }
+            u.turn(p[i], q[i]);
+            if (!w) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float x0 = widen(va[i][e]), x1 = widen(vb[i][e]);
+                sums[i] += x0 * x0 + x1 * x1;
+                sums[HB + i] += p[i][e] * wa[e] * x0 + q[i][e] * wb[e] * x1;
+            }
+        }
+        if (w) group_sums(sums, l.lanes);
+#pragma unroll
+        for (int i = 0; i < HB; ++i) {
+            if (w) {
+                const float r = rsqrtf(sums[i] / D + (float)a.eps), dot = sums[HB + i] * r / D;
+                const bool real = i < hn;                 // (a head past the last adds nothing, also where its r is not finite)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float x0 = widen(va[i][e]) * r, x1 = widen(vb[i][e]) * r;
+                    if (real) {
+                        sa[e] += p[i][e] * x0;
+                        sb[e] += q[i][e] * x1;
+                    }
+                    p[i][e] = r * (p[i][e] * wa[e] - x0 * dot);
+                    q[i][e] = r * (q[i][e] * wb[e] - x1 * dot);
+                }
+            }
+            u.write(y + i * yv.head + u.a, ha && i < hn, p[i]);
+            u.write(y + i * yv.head + u.b, hb && i < hn, q[i]);
+        }
+    }
+    if (!a.gweight[which]) return;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        if (ha) shared[group * D + u.a + e] = sa[e];
+        if (hb) shared[group * D + u.b + e] = sb[e];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < D; e += 256) {
+        float s = 0.f;
+        for (int i = 0; i < groups; ++i) s += shared[i * D + e];
+        a.partial[((size_t)which * D + e) * gridDim.x + blockIdx.x] = s;
+    }
+}
+
+// Any sizes and strides: one wave per row (a head of a moment), lanes over its values; a partner's value is read again (a
+// cache hit).
 template <class T, int NE>
-__global__ __launch_bounds__(64 * TURN_ROWS) void k_turn(fm_turn_args a) {
+__global__ __launch_bounds__(64 * TURN_ROWS) void k_turn(fm_turn_args a, float sign) {
     const int H = (int)(a.heads[0] + a.heads[1]), lane = threadIdx.x & 63, D = (int)a.dim, R = (int)a.rotated;
     const long long row = (long long)blockIdx.x * TURN_ROWS + (threadIdx.x >> 6);
     if (row >= a.n_seq * a.n_moments * H) return;
@@ -40,10 +265,10 @@ __global__ __launch_bounds__(64 * TURN_ROWS) void k_turn(fm_turn_args a) {
     int h = (int)(row % H);
     const int which = h >= a.heads[0];
     if (which) h -= (int)a.heads[0];
-    const fm_view &xv = a.x[which], &yv = a.y[which];
+    const fm_view xv = which ? a.x[1] : a.x[0], yv = which ? a.y[1] : a.y[0];
     const T* x = (const T*)xv.data + n * xv.seq + t * xv.moment + h * xv.head;
     T* y = (T*)yv.data + n * yv.seq + t * yv.moment + h * yv.head;
-    const float* w = a.weight[which];
+    const float* w = which ? a.weight[1] : a.weight[0];
     const float* cs = R ? table_line(a, n, t) : nullptr;
     float v[NE], r = 1.f, sum = 0.f;
 #pragma unroll
@@ -60,25 +285,23 @@ __global__ __launch_bounds__(64 * TURN_ROWS) void k_turn(fm_turn_args a) {
         float z = v[i] * r * (w ? w[e] : 1.f);
         if (e < R) {
             const Turn u = turn_of(e, cs, R, a.interleaved);
-            z = z * u.c + widen(x[u.partner]) * r * (w ? w[u.partner] : 1.f) * u.s;
+            z = z * u.c + widen(x[u.partner]) * r * (w ? w[u.partner] : 1.f) * (sign * u.s);
         }
         y[e] = narrow<T>(z);
     }
 }
 
-// Its gradient: the turn undone (the sine's sign flipped), then, with xh = x r and u = g' w, gx = r (u - xh mean(u xh));
-// the weights' gradients sum g' xh over rows: a wave keeps its rows' sums in registers (rows of queries and of keys in
-// launches' halves of their own), a workgroup's waves are added in LDS in wave order, k_turn_gweight adds the workgroups.
+// Its gradient with a norm (see k_turn_units_bwd).
 template <class T, int NE>
-__global__ __launch_bounds__(64 * TURN_ROWS) void k_turn_bwd(fm_turn_args a, int blocks) {
+__global__ __launch_bounds__(64 * TURN_ROWS) void k_turn_bwd(fm_turn_args a) {
     __shared__ float sums[TURN_ROWS][64 * NE];
     const int which = blockIdx.y, H = (int)a.heads[which], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int D = (int)a.dim, R = (int)a.rotated;
-    const fm_view &xv = a.x[which], &yv = a.y[which], &gv = a.g[which];
+    const fm_view xv = a.x[which], yv = a.y[which], gv = a.g[which];
     const float* w = a.weight[which];
     float gw[NE] = {};
     const long long rows = a.n_seq * a.n_moments * H;
-    for (long long row = (long long)blockIdx.x * TURN_ROWS + wave; row < rows; row += (long long)blocks * TURN_ROWS) {
+    for (long long row = (long long)blockIdx.x * TURN_ROWS + wave; row < rows; row += (long long)gridDim.x * TURN_ROWS) {
         const long long m = row / H, n = m / a.n_moments, t = m % a.n_moments;
         const int h = (int)(row % H);
         const T* g = (const T*)gv.data + n * gv.seq + t * gv.moment + h * gv.head;
@@ -127,24 +350,26 @@ __global__ __launch_bounds__(64 * TURN_ROWS) void k_turn_bwd(fm_turn_args a, int
     for (int e = threadIdx.x; e < D; e += 64 * TURN_ROWS) {
         float s = 0.f;
         for (int i = 0; i < TURN_ROWS; ++i) s += sums[i][e];
-        a.partial[((size_t)which * blocks + blockIdx.x) * D + e] = s;
+        a.partial[((size_t)which * D + e) * gridDim.x + blockIdx.x] = s;
     }
 }
 
-// gweight[which][e] = the sum of the workgroups' partials, in order: one wave per value, the lanes' strided sums joined
+// gweight[which][e] = the sum of the workgroups' partials: one wave per value, the lanes' strided sums joined
 __global__ __launch_bounds__(64) void k_turn_gweight(fm_turn_args a, int blocks) {
-    const int which = blockIdx.y, e = blockIdx.x, D = (int)a.dim;
+    const int which = blockIdx.y, e = blockIdx.x;
     if (!a.gweight[which]) return;
+    const float* p = a.partial + ((size_t)which * a.dim + e) * blocks;
     float s = 0.f;
-    for (int b = threadIdx.x; b < blocks; b += 64) s += a.partial[((size_t)which * blocks + b) * D + e];
+    for (int b = threadIdx.x; b < blocks; b += 64) s += p[b];
     s = wave_sum(s, 64);
     if (threadIdx.x == 0) a.gweight[which][e] = s;
 }
 
+// workgroups of a gradient with a norm: 4 a CU
 inline int turn_blocks(const fm_turn_args& a) {
     const long long rows = a.n_seq * a.n_moments * (a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1]);
     const long long b = (rows + TURN_ROWS - 1) / TURN_ROWS;
-    return (int)(b < 1 ? 1 : b > 2048 ? 2048 : b);
+    return (int)(b < 1 ? 1 : b > 1024 ? 1024 : b);
 }
 
 const char* turn_args_wrong(const fm_turn_args& a, bool bwd) {
@@ -167,34 +392,90 @@ const char* turn_args_wrong(const fm_turn_args& a, bool bwd) {
 }
 
 template <class T, int NE>
-void launch_turn(const fm_turn_args& a, bool bwd, hipStream_t st) {
-    if (bwd) {
-        const int blocks = turn_blocks(a);
-        k_turn_bwd<T, NE><<<dim3(blocks, a.heads[1] ? 2 : 1), 64 * TURN_ROWS, 0, st>>>(a, blocks);
-        if (a.gweight[0] || a.gweight[1])
-            k_turn_gweight<<<dim3((unsigned)a.dim, 2), 64, 0, st>>>(a, blocks);
+void launch_any(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
+    if (grad) {
+        k_turn_bwd<T, NE><<<dim3(turn_blocks(a), a.heads[1] ? 2 : 1), 64 * TURN_ROWS, 0, st>>>(a);
         return;
     }
     const long long rows = a.n_seq * a.n_moments * (a.heads[0] + a.heads[1]);
-    if (rows) k_turn<T, NE><<<(unsigned)((rows + TURN_ROWS - 1) / TURN_ROWS), 64 * TURN_ROWS, 0, st>>>(a);
+    k_turn<T, NE><<<(unsigned)((rows + TURN_ROWS - 1) / TURN_ROWS), 64 * TURN_ROWS, 0, st>>>(a, sign);
+}
+
+template <class T, bool IL, int HB>
+Lanes lanes_of(const fm_turn_args& a) {
+    Lanes l;
+    const int units = (int)a.dim / Vec<T>::N;
+    for (l.shift = 0; 2 << l.shift < units; ++l.shift) {}
+    l.lanes = 1 << l.shift;
+    l.q_chunks = ((int)a.heads[0] + HB - 1) / HB;
+    l.chunks = l.q_chunks + ((int)a.heads[1] + HB - 1) / HB;
+    return l;
+}
+#ifndef HBF
+#define HBF 4
+#define HBG 4
+#endif
+constexpr int HEADS_FWD = HBF, HEADS_BWD = HBG;
+template <class T, bool IL>
+void launch_units(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
+    if (grad) {
+        const Lanes l = lanes_of<T, IL, HEADS_BWD>(a);
+        k_turn_units_bwd<T, IL, HEADS_BWD><<<dim3(turn_blocks(a), a.heads[1] ? 2 : 1), 256, 0, st>>>(a, l);
+        return;
+    }
+    const Lanes l = lanes_of<T, IL, HEADS_FWD>(a);
+    const int groups = 256 >> l.shift;
+    const unsigned grid = (unsigned)((a.n_seq * a.n_moments * l.chunks + groups - 1) / groups);
+    if (a.weight[0] || a.weight[1]) k_turn_units<T, IL, true, HEADS_FWD><<<grid, 256, 0, st>>>(a, l, sign);
+    else k_turn_units<T, IL, false, HEADS_FWD><<<grid, 256, 0, st>>>(a, l, sign);
+}
+
+// heads of whole 16-byte units, all aligned, turned in whole units (k_turn_units), or anything (k_turn)
+template <class T>
+bool in_units(const fm_turn_args& a, bool grad) {
+    constexpr int V = Vec<T>::N;
+    if (a.dim % V || a.rotated % (a.interleaved ? V : 2 * V) || ((uintptr_t)a.table & 7)) return false;
+    for (int i = 0; i < 2; ++i)
+        if (a.heads[i] && (!aligned16(a.x[i], sizeof(T)) || !aligned16(a.y[i], sizeof(T)) ||
+                           (grad && !aligned16(a.g[i], sizeof(T)))))
+            return false;
+    return true;
 }
 
 template <class T>
-void turn_of_type(const fm_turn_args& a, bool bwd, hipStream_t st) {
-    if (a.dim <= 64) launch_turn<T, 1>(a, bwd, st);
-    else if (a.dim <= 128) launch_turn<T, 2>(a, bwd, st);
-    else if (a.dim <= 256) launch_turn<T, 4>(a, bwd, st);
-    else launch_turn<T, 8>(a, bwd, st);
+void turn_of_type(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
+    if (in_units<T>(a, grad)) {
+        a.interleaved ? launch_units<T, true>(a, grad, sign, st) : launch_units<T, false>(a, grad, sign, st);
+        return;
+    }
+    if (a.dim <= 64) launch_any<T, 1>(a, grad, sign, st);
+    else if (a.dim <= 128) launch_any<T, 2>(a, grad, sign, st);
+    else if (a.dim <= 256) launch_any<T, 4>(a, grad, sign, st);
+    else launch_any<T, 8>(a, grad, sign, st);
 }
 
-int turn(const fm_turn_args* a, bool bwd, void* stream) {
+int turn(const fm_turn_args* args, bool bwd, void* stream) {
     clear_error();
-    if (!a) return fail("fm_turn: no arguments");
-    if (const char* e = turn_args_wrong(*a, bwd)) return fail((std::string(bwd ? "fm_turn_bwd: " : "fm_turn: ") + e).c_str());
-    if (a->dtype == FM_F32) turn_of_type<float>(*a, bwd, (hipStream_t)stream);
-    else if (a->dtype == FM_BF16) turn_of_type<bf16>(*a, bwd, (hipStream_t)stream);
-    else turn_of_type<f16>(*a, bwd, (hipStream_t)stream);
-    FG_CHECK(hipGetLastError(), -1);
+    if (!args) return fail("fm_turn: no arguments");
+    if (const char* e = turn_args_wrong(*args, bwd)) return fail((std::string(bwd ? "fm_turn_bwd: " : "fm_turn: ") + e).c_str());
+    fm_turn_args a = *args;
+    hipStream_t st = (hipStream_t)stream;
+    const bool grad = bwd && (a.weight[0] || a.weight[1]);
+    if (bwd && !grad)                        // without a norm: g turned back
+        for (int i = 0; i < 2; ++i) a.x[i] = a.g[i];
+    if (!a.heads[1]) a.gweight[1] = nullptr;
+    const bool any = a.n_seq * a.n_moments * (a.heads[0] + a.heads[1]) > 0;
+    if (any || grad) {
+        const float sign = bwd ? -1.f : 1.f;
+        if (a.dtype == FM_F32) turn_of_type<float>(a, grad, sign, st);
+        else if (a.dtype == FM_BF16) turn_of_type<bf16>(a, grad, sign, st);
+        else turn_of_type<f16>(a, grad, sign, st);
+        FG_CHECK(hipGetLastError(), -1);
+    }
+    if (grad && (a.gweight[0] || a.gweight[1])) {
+        k_turn_gweight<<<dim3((unsigned)a.dim, 2), 64, 0, st>>>(a, turn_blocks(a));
+        FG_CHECK(hipGetLastError(), -1);
+    }
     return 0;
 }
 

@@ -24,6 +24,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TURN = struct.Struct("=44qd")
 _ATTENTION = struct.Struct("=36qd")
 _STEP = struct.Struct("=24qd")
+_PARTIAL_ROWS = 2 * 1024                # fm_turn_partial's most, in rows of a head's values
 
 
 def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -59,24 +60,15 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: str =
 
 
 # ------------------------------------------------------------------------------------------------ calls
-def _call(name: str, args: bytes, stream) -> None:
-    if getattr(lib(), name)(args, stream):
+def _call(name: str, x: torch.Tensor, args: bytes) -> None:
+    """The call on x's device and its current stream."""
+    dev = x.get_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _call(name, x, args)
+    if getattr(lib(), name)(args, torch._C._cuda_getCurrentRawStream(dev)):
         check(name)
         raise LibraryError(f"{name} failed")
-
-
-def _on(x: torch.Tensor):
-    """The current stream of x's device (None: another device is current; see _there)."""
-    return torch.cuda.current_stream(x.device).cuda_stream
-
-
-def _there(x: torch.Tensor, name: str, args: bytes) -> None:
-    """The call on x's device and its current stream."""
-    if x.device.index == torch.cuda.current_device():
-        _call(name, args, _on(x))
-    else:
-        with torch.cuda.device(x.device):
-            _call(name, args, _on(x))
 
 
 def _ptr(x: torch.Tensor | None) -> int:
@@ -165,9 +157,8 @@ def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
 
 def _turn(p: _Plan, q, k, wq, wk):
     q, k = _rows(q), None if k is None else _rows(k)
-    yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    yk = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _there(q, "fm_turn", p.pack((q, k), (yq, yk), (None, None), (wq, wk), (None, None), None))
+    yq, yk = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    _call("fm_turn", q, p.pack((q, k), (yq, yk), (None, None), (wq, wk), (None, None), None))
     return yq, yk
 
 
@@ -178,7 +169,6 @@ class TurnHip(torch.autograd.Function):
     def forward(ctx, q, k, wq, wk, p):
         ctx.p = p
         ctx.save_for_backward(*((q, k) if wq is not None else (None, None)), wq, wk)
-        ctx.like = (q.dtype, q.device)
         return _turn(p, q, k, wq, wk)
 
     @staticmethod
@@ -187,15 +177,13 @@ class TurnHip(torch.autograd.Function):
         p = ctx.p
         q, k, gq = None if q is None else _rows(q), None if k is None else _rows(k), _rows(gq)
         gk = None if not p.heads[1] else _rows(gk)
-        yq = torch.empty(gq.shape, dtype=ctx.like[0], device=ctx.like[1])
-        yk = None if gk is None else torch.empty(gk.shape, dtype=ctx.like[0], device=ctx.like[1])
+        yq, yk = gq.new_empty(gq.shape), None if gk is None else gk.new_empty(gk.shape)
         gwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         gwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
         partial = None
         if gwq is not None or gwk is not None:
-            n = lib().fm_turn_partial(p.pack((q, k), (yq, yk), (gq, gk), (wq, wk), (gwq, gwk), None))
-            partial = torch.empty(n, device=gq.device)
-        _there(gq, "fm_turn_bwd", p.pack((q, k), (yq, yk), (gq, gk), (wq, wk), (gwq, gwk), partial))
+            partial = wq.new_empty(_PARTIAL_ROWS * p.shape[2])
+        _call("fm_turn_bwd", gq, p.pack((q, k), (yq, yk), (gq, gk), (wq, wk), (gwq, gwk), partial))
         return yq, yk, gwq, gwk, None
 
 
@@ -248,10 +236,10 @@ class _Stretches:
 
 def _attend(p: _Stretches, q, k, v, state):
     q, k, v = _rows(q), _rows(k), _rows(v)
-    o = torch.empty(*q.shape[:-1], p.V, dtype=q.dtype, device=q.device)
-    state_out = torch.empty(p.n, p.q_heads, p.K, p.V, device=q.device)
+    o = q.new_empty((*q.shape[:-1], p.V))
+    state_out = p.log_decay.new_empty((p.n, p.q_heads, p.K, p.V))
     work = p.workspace(q, k, v, False)
-    _there(q, "fm_attention", p.pack(q, k, v, state=state, o=o, state_out=state_out, work=work))
+    _call("fm_attention", q, p.pack(q, k, v, state=state, o=o, state_out=state_out, work=work))
     return o, state_out
 
 
@@ -271,14 +259,14 @@ class DecayHip(torch.autograd.Function):
         q, k, v, state = ctx.saved_tensors
         want = ctx.needs_input_grad
         q, k, v = _rows(q), _rows(k), _rows(v)
-        go = torch.zeros(*q.shape[:-1], p.V, dtype=q.dtype, device=q.device) if go is None else _rows(go)
+        go = q.new_zeros((*q.shape[:-1], p.V)) if go is None else _rows(go)
         gstate_out = None if gstate_out is None else gstate_out.contiguous()
-        gq, gk, gv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if w else None
+        gq, gk, gv = (x.new_empty(x.shape) if w else None
                       for x, w in zip((q, k, v), want))
         gstate = torch.empty_like(state) if state is not None and want[3] else None
         given = dict(go=go, state=state, gstate_out=gstate_out, gq=gq, gk=gk, gv=gv, gstate=gstate)
         work = p.workspace(q, k, v, True, **given)
-        _there(q, "fm_attention_bwd", p.pack(q, k, v, work=work, **given))
+        _call("fm_attention_bwd", q, p.pack(q, k, v, work=work, **given))
         return gq, gk, gv, gstate, None
 
 
@@ -358,9 +346,9 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
         slots = slots.contiguous()
     log_decay = _decays(what, log_decay, Hq, dev)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    o = torch.empty(n, Hq, V, dtype=q.dtype, device=dev)
+    o = q.new_empty((n, Hq, V))
     views = [f for x in (q, k, v) for f in (x.data_ptr(), x.stride(0), 0, x.stride(1))]
-    _there(q, "fm_step", _STEP.pack(*views, log_decay.data_ptr(), state.data_ptr(), into.data_ptr(), _ptr(slots),
+    _call("fm_step", q, _STEP.pack(*views, log_decay.data_ptr(), state.data_ptr(), into.data_ptr(), _ptr(slots),
                                     o.data_ptr(), n, state.shape[0], Hq, k.shape[1], K, V, _TYPES[q.dtype],
                                     float(K ** -0.5 if scale is None else scale)))
     return o

@@ -141,6 +141,25 @@ def test_positions(gpu_lib):
     assert torch.isnan(rotary(q, None, table, 18)[0][:, 2:, :, :8]).all()
 
 
+@pytest.mark.parametrize("il", [False, True])
+def test_values_that_are_not_turned_pass_through(gpu_lib, il):
+    """Whatever they are: infinities and NaN among them touch nothing else, turned values' only their own pair."""
+    from flyguy_amd.memory_hip import rotary, rotary_table
+    gen = torch.Generator().manual_seed(7)
+    for dt in (F32, BF16):
+        q = draw(gen, 2, 5, 3, 96, dtype=dt)
+        table = rotary_table(5, 32).cuda()
+        clean = rotary(q, None, table, interleaved=il)[0]
+        bad = q.clone()
+        bad[0, 1, 2, 40], bad[0, 1, 2, 95], bad[1, 4, 0, 57], bad[1, 2, 1, 4] = (float(x) for x in ("inf", "nan", "-inf", "inf"))
+        got = rotary(bad, None, table, interleaved=il)[0]
+        assert torch.equal(got[..., 32:].view(torch.uint8), bad[..., 32:].view(torch.uint8))
+        off = ~torch.isfinite(got[..., :32])
+        pair = torch.zeros_like(off)
+        pair[1, 2, 1, [4, 5] if il else [4, 20]] = True
+        assert torch.equal(off, pair) and torch.equal(got[..., :32][~pair], clean[..., :32][~pair])
+
+
 def test_a_norm_keeps_rows_apart(gpu_lib):
     """A row of zeros, one of infinity and one of NaN: the others are what they are without them, the row of zeros is zeros."""
     from flyguy_amd.memory_hip import norm_rotary, rotary_table
