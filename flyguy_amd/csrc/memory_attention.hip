@@ -91,17 +91,42 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 
 // A number as a sum of bfloat16 terms, each the rest's nearest: 1, 2, 3 terms hold 8, 16, 24 bits.  A product of two sums
 // keeps the pairs of terms (i, j) with i + j < the longer one's terms: what is dropped is below its last bit.
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 template <int P, int V>
 struct Sum {
     typedef bf16 vec __attribute__((ext_vector_type(V)));
     typedef float wide __attribute__((ext_vector_type(V)));
     vec term[P];
-    __device__ __forceinline__ void of(wide r) {          // (whole vectors: two values a conversion)
+    // values of any places (whole vectors: two values a conversion)
+    __device__ __forceinline__ void of(wide r) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             term[p] = __builtin_convertvector(r, vec);
             if (p + 1 < P) r -= __builtin_convertvector(term[p], wide);
         }
+    }
+    // values that one sum takes: a term is taken off, exactly, by its pair's product with (-1, 0), without widening it; one that
+    // is not finite spoils its neighbour, and the sum is not finite then anyway
+    __device__ __forceinline__ void of_summed(wide r) {
+        unsigned one = 0x0000bf80u, two = 0xbf800000u;    // (in registers: as constants of this instruction they come out
+        asm("" : "+s"(one), "+s"(two));                   // as other numbers)
+        const bf16x2 first = __builtin_bit_cast(bf16x2, one), second = __builtin_bit_cast(bf16x2, two);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            term[p] = __builtin_convertvector(r, vec);
+            if (p + 1 == P) break;
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const bf16x2 t = pair(term[p], i);
+                r[i] = __builtin_amdgcn_fdot2_f32_bf16(t, first, r[i], false);
+                r[i + 1] = __builtin_amdgcn_fdot2_f32_bf16(t, second, r[i + 1], false);
+            }
+        }
+    }
+    __device__ __forceinline__ static bf16x2 pair(vec v, int i) {
+        if constexpr (V == 4) return i ? __builtin_shufflevector(v, v, 2, 3) : __builtin_shufflevector(v, v, 0, 1);
+        else return i == 0 ? __builtin_shufflevector(v, v, 0, 1) : i == 2 ? __builtin_shufflevector(v, v, 2, 3)
+                  : i == 4 ? __builtin_shufflevector(v, v, 4, 5) : __builtin_shufflevector(v, v, 6, 7);
     }
 };
 typedef Sum<1, 8>::wide f32x8;
@@ -203,13 +228,21 @@ __device__ __forceinline__ Sum<P, 8> down(const bf16* p, int apart, int plane) {
 template <class T, int KT, int WAVES, bool OUT>
 struct Tile {
     static constexpr int CH = Form<T>::CHUNK, KW = 32 * KT, NW = 16 * WAVES;
-    static constexpr int KP = KW + 8, NP = NW + 8;        // rows in LDS: no bank conflicts
-    static constexpr int XP = CH * KP, VP = CH * NP, PIECES = CH == 64 ? 6 : 2;
+    static constexpr int XP = CH * KW, VP = CH * NW, PIECES = CH == 64 ? 6 : 2;
     static constexpr int LDS = Form<T>::X * 2 * (XP * (OUT ? 2 : 1) + VP) + (OUT ? PIECES * Form<T>::W * 1024 : 0);
     // waves a SIMD that LDS lets in, at most 4 (128 registers)
     static constexpr int FIT = 160 * 1024 / LDS * WAVES / 4;
     static constexpr int PER_SIMD = FIT < 1 ? 1 : FIT > 4 ? 4 : FIT;
 };
+// Where a row's 8-value share q stands in LDS: rows of 8 or 16 shares, unpadded, the shares of row 4g + r (of 16) exchanged
+// by q ^ (r, g), so that both the 16 rows of a share and the 4 shares of 4 rows that a transposing read takes lie in banks
+// of their own.  place(row, q + 4b) = place(row, q) ^ 32 b where q < 4.
+template <int WIDTH>
+__device__ __forceinline__ int place(int row, int q) {
+    const int r = row & 3, g = row >> 2 & 3, swap = (g & 1) << 1 | g >> 1;
+    return row * WIDTH + 8 * (q ^ (WIDTH == 128 ? r << 2 | swap : (r & 2) << 1 | swap));
+}
+
 // an opaque copy: what is computed from it stays where it is used, instead of in registers all along
 template <class V>
 __device__ __forceinline__ V here(V v) {
@@ -226,7 +259,7 @@ template <class T, int KT, int WAVES, bool VEC, bool OUT, class TO>
 __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) void k_scan(Scans a) {
     using S = Tile<T, KT, WAVES, OUT>;
     constexpr int X = Form<T>::X, W = Form<T>::W, CH = S::CH, JB = CH / 16, VN = Vec<T>::N;
-    constexpr int KW = S::KW, NW = S::NW, KP = S::KP, NP = S::NP, XP = S::XP, VP = S::VP, PIECES = S::PIECES;
+    constexpr int KW = S::KW, NW = S::NW, XP = S::XP, VP = S::VP, PIECES = S::PIECES;
     constexpr int XC = KW / VN, VC = NW / VN;                                // 16-byte shares of a row
     constexpr int XR = 64 * WAVES / XC, VR = 64 * WAVES / VC;                // rows between a thread's shares
     constexpr int XV = XR < CH ? CH / XR : 1, VV = CH / VR;                  // a thread's shares (XR > CH: of some threads)
@@ -320,7 +353,8 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     TO* const out = OUT ? (TO*)s.out : nullptr;
     const long long drow = dir * a.heads * s.N;
     TO* po = OUT ? out + (((a.starts ? 0 : n * a.n_moments) + t0) * a.heads + h) * s.N + c * drow + n0 + w0 + 4 * g : nullptr;
-    const bf16* const vdown = &sv[(4 * g + (c >> 2)) * NP + w0 + 4 * (c & 3)];
+    const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
+    const bf16* const vdown = sv + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
 
     for (long long i0 = 0; i0 < left; i0 += CH) {
         const int pad = CH - rows_from(i0);
@@ -328,11 +362,12 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
 #pragma unroll
         for (int i = 0; i < XV; ++i) {
             if (XR > CH && xrow >= CH) break;
-            if (OUT) store_terms<T>(rx[i], &sx[(xrow + i * XR) * KP + xcol], XP);
-            store_terms<T>(ry[i], &sy[(xrow + i * XR) * KP + xcol], XP);
+            const int to = place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7);
+            if (OUT) store_terms<T>(rx[i], sx + to, XP);
+            store_terms<T>(ry[i], sy + to, XP);
         }
 #pragma unroll
-        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], &sv[(vrow + i * VR) * NP + vcol], VP);
+        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], sv + place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7), VP);
         __syncthreads();
 
         f32x4 o[JB] = {};
@@ -343,10 +378,11 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
                 f32x4 p[2] = {};
 #pragma unroll
                 for (int b = 0; b < KT; ++b) {
-                    const Sum<X, 8> xf = across<X>(&sx[(16 * i + c) * KP + 32 * b + 8 * g], XP);
-                    const bf16* y = &sy[(32 * jj + c) * KP + 32 * b + 8 * g];
+                    const int at = here(xat) ^ 32 * b;
+                    const Sum<X, 8> xf = across<X>(sx + 16 * i * KW + at, XP);
+                    const bf16* y = sy + 32 * jj * KW + at;
                     p[0] = mfma(across<X>(y, XP), xf, p[0]);
-                    p[1] = mfma(across<X>(y + 16 * KP, XP), xf, p[1]);
+                    p[1] = mfma(across<X>(y + 16 * KW, XP), xf, p[1]);
                 }
                 f32x8 v;
 #pragma unroll
@@ -355,16 +391,17 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
                     v[r] = d >= 0 ? s.c * power(d) * p[r >> 2][r & 3] : 0.f;      // (whatever x . y is there)
                 }
                 Sum<W, 8> w;
-                w.of(v);
+                w.of_summed(v);
 #pragma unroll
                 for (int t = 0; t < W; ++t) sp[piece][t][lane] = w.term[t];
             }
 #pragma unroll
             for (int b = 0; b < KT; ++b) {
                 Sum<W, 8> zf;
-                zf.of(__builtin_shufflevector(z[2 * b], z[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                zf.of_summed(__builtin_shufflevector(z[2 * b], z[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                const int at = here(xat) ^ 32 * b;
 #pragma unroll
-                for (int i = 0; i < JB; ++i) o[i] = mfma(zf, across<X>(&sx[(16 * i + c) * KP + 32 * b + 8 * g], XP), o[i]);
+                for (int i = 0; i < JB; ++i) o[i] = mfma(zf, across<X>(sx + 16 * i * KW + at, XP), o[i]);
             }
             const int c1 = here(c) - pad;
             const float f0 = here(row0);
@@ -382,7 +419,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
             unsigned odd = 0;
 #pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
-                Sum<X, 8> vf = down<X>(vdown + 32 * jj * NP, 16 * NP, VP);
+                Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW, 16 * NW, VP);
                 const uint4 u = __builtin_bit_cast(uint4, vf.term[0]);
                 const unsigned m = 0x7f807f80u, one = 0x00800080u;           // (an exponent of ones carries into the sign)
                 const unsigned bad = (((u.x & m) + one) | ((u.y & m) + one) | ((u.z & m) + one) | ((u.w & m) + one)) & 0x80008000u;
@@ -406,7 +443,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
                 const int g4 = here(4 * g), c1 = here(c);
 #pragma unroll
                 for (int jj = 0; jj < JB / 2; ++jj) {
-                    const bf16x8 v = columns8(vdown + 32 * jj * NP, 16 * NP);
+                    const bf16x8 v = columns8(vdown + 32 * jj * NW, 16 * NW);
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
                         if (!(fabsf((float)v[r]) < INFINITY))
@@ -453,24 +490,31 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
 #pragma unroll
             for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r - early);
         }
+        if (keep.one != 0.f) {                            // (one instruction a value, either way)
 #pragma unroll
-        for (int b = 0; b < 2 * KT; ++b)
+            for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) z[b][r] = keep(z[b][r]);
+                for (int r = 0; r < 4; ++r) z[b][r] = fmaf(keep.f, z[b][r], z[b][r]);
+        } else {
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[b][r] *= keep.f;
+        }
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
-            const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NP, 16 * NP, VP);
+            const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW, 16 * NW, VP);
             f32x8 v = __builtin_convertvector(vf.term[X - 1], f32x8);
 #pragma unroll
             for (int t = X - 2; t >= 0; --t) v += __builtin_convertvector(vf.term[t], f32x8);
 #pragma unroll
             for (int r = 0; r < 8; ++r) v[r] *= rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2));
             Sum<S_TERMS, 8> w;
-            w.of(v);
+            w.of_summed(v);
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
-                const bf16* p = &sy[(32 * jj + 4 * g + (c >> 2)) * KP + 32 * (b >> 1) + 8 * (c & 3) + 4 * (b & 1)];
-                z[b] = mfma(down<X>(p, 16 * KP, XP), w, z[b]);
+                const bf16* p = sy + 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
+                z[b] = mfma(down<X>(p, 16 * KW, XP), w, z[b]);
             }
         }
     }
@@ -513,12 +557,17 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     float z = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, i / s.N, i % s.N, once);
     float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
     const size_t step = (size_t)a.heads * s.K * s.N;
-    for (long long from = 0;; from += a.L, p += step) {
-        const bool more = from + a.L < count;
-        const float own = more ? *p : 0.f;
-        *p = z;
-        if (!more) break;
-        z = keep(z) + own;
+    // (8 segments' states under way at once)
+    for (long long from = 0; from < count || from == 0; from += 8 * a.L, p += 8 * step) {
+        float own[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) own[j] = from + (j + 1) * a.L < count ? p[j * step] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j && from + j * a.L >= count) return;
+            p[j * step] = z;
+            z = keep(z) + own[j];
+        }
     }
 }
 
@@ -634,7 +683,10 @@ long long shared_floats(const fm_attention_args& a, bool of_v) {
 
 // How a launch's scans are cut into segments: one segment a stretch where the stretches' heads alone fill the chip, else so
 // that about SEG_GROUPS workgroups run, of at least SEG_MIN moments.
-constexpr int SEG_GROUPS = 768, SEG_MIN = 256;
+#ifndef SEGG
+#define SEGG 512
+#endif
+constexpr int SEG_GROUPS = SEGG, SEG_MIN = 256;
 struct Cut {
     int nseg, slots;
     long long L;
