@@ -160,12 +160,10 @@ struct Form<float> {
 constexpr int CHUNK_MAX = 64;
 constexpr int S_TERMS = 3;               // terms of v times its decay: the state is a float32 result
 
-// 16 bytes of a row from column c, zeros past the row's end or width
-template <class T, bool VEC>
+// 16 bytes of a row from column c, value by value, zeros past the width
+template <class T>
 __device__ __forceinline__ uint4 load16(const T* row, int c, int width, bool there) {
-    uint4 r = make_uint4(0, 0, 0, 0);
-    if (!there || c >= width) return r;
-    if (VEC) return *reinterpret_cast<const uint4*>(row + c);
+    if (!there || c >= width) return make_uint4(0, 0, 0, 0);
     typename Vec<T>::type v;
 #pragma unroll
     for (int i = 0; i < Vec<T>::N; ++i) v[i] = c + i < width ? row[c + i] : (T)0.f;
@@ -255,6 +253,21 @@ __device__ __forceinline__ float shared_by_all(float v) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
 }
 
+__device__ __forceinline__ long long shared_by_all(long long v) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+
+// A chunk's rows in memory, `rows` of them `step` bytes apart from p, of `width` bytes: loads outside give zeros, stores
+// outside are dropped, so that lanes without a row or column need no branch.  NOWHERE: such a lane's offset.
+constexpr unsigned NOWHERE = 0xc0000000u;
+constexpr long long STRIDE_MOST = 1 << 22;               // values from row to row: 64 rows end below 2^30 bytes
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int rows, long long step, int width) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)((rows - 1) * step) + width, 0x00020000);
+}
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
 template <class T, int KT, int WAVES, bool VEC, bool OUT, class TO>
 __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) void k_scan(Scans a) {
     using S = Tile<T, KT, WAVES, OUT>;
@@ -263,7 +276,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     constexpr int XC = KW / VN, VC = NW / VN;                                // 16-byte shares of a row
     constexpr int XR = 64 * WAVES / XC, VR = 64 * WAVES / VC;                // rows between a thread's shares
     constexpr int XV = XR < CH ? CH / XR : 1, VV = CH / VR;                  // a thread's shares (XR > CH: of some threads)
-    static_assert((XV * XR == CH || XR > CH) && VV * VR == CH, "");
+    static_assert((XV * XR == CH || XR > CH) && VV * VR == CH && VR % 16 == 0, "");
     __shared__ __align__(16) bf16 sx[OUT ? X * XP : 8], sy[X * XP], sv[X * VP];
     __shared__ __align__(16) bf16x8 sp[OUT ? PIECES : 1][W][64];
     const Scan& s = a.s[blockIdx.z];
@@ -273,6 +286,10 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     int n, seg;
     long long first, count;
     if (!segment_of(a, slot, n, seg, first, count)) return;
+    n = __builtin_amdgcn_readfirstlane(n);
+    seg = __builtin_amdgcn_readfirstlane(seg);
+    first = shared_by_all(first);
+    count = shared_by_all(count);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int n0 = blk * NW, w0 = 16 * wave;              // this workgroup's columns, this wave's from there
     const long long from = seg * a.L, left = count - from < a.L ? count - from : a.L;
@@ -308,69 +325,88 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
 
     // this thread's shares of a chunk's rows
     const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
-    const long long dir = s.backwards ? -1 : 1;
-    const long long t0 = (a.starts ? first : 0) + (s.backwards ? count - 1 - from : from);
-    auto base = [&](const fm_view& v, int share) {
-        return (const T*)v.data + (a.starts ? 0 : n * v.seq) + (h / share) * v.head + t0 * v.moment;
-    };
-    const long long dx = dir * s.x.moment, dy = dir * s.y.moment, dv = dir * s.v.moment;
-    const T* px = OUT ? base(s.x, s.xs) + xrow * dx : nullptr;
-    const T* py = base(s.y, s.ys) + xrow * dy;
-    const T* pv = base(s.v, s.vs) + vrow * dv + n0;
-    uint4 rx[XV], ry[XV], rv[VV];
-    auto fetch = [&](int rows) {                          // the next chunk, of so many moments
-        const int pad = CH - rows;
-        if (pad) {
-            px -= OUT ? pad * dx : 0;
-            py -= pad * dy;
-            pv -= pad * dv;
-        }
-#pragma unroll
-        for (int i = 0; i < XV; ++i) {
-            const bool there = xrow + i * XR >= pad && (XR <= CH || xrow < CH);
-            if (OUT) rx[i] = load16<T, VEC>(px + i * XR * dx, xcol, s.K, there);
-            ry[i] = load16<T, VEC>(py + i * XR * dy, xcol, s.K, there);
-        }
-#pragma unroll
-        for (int i = 0; i < VV; ++i) rv[i] = load16<T, VEC>(pv + i * VR * dv, vcol, s.N - n0, vrow + i * VR >= pad);
-        if (OUT) px += CH * dx;
-        py += CH * dy;
-        pv += CH * dv;
-    };
     auto rows_from = [&](long long i0) { return (int)(left - i0 < CH ? left - i0 : CH); };
-    if (left > 0) fetch(rows_from(0));
+    // the chunk from the segment's moment i0: its moment lowest in memory, and a row's place from there
+    auto lowest = [&](long long i0, int rows) { return (a.starts ? first : 0) + (s.backwards ? count - from - i0 - rows : from + i0); };
+    auto in_memory = [&](int row, int pad) { return s.backwards ? CH - 1 - row : row - pad; };
+    auto base = [&](const fm_view& v, int share, long long low) {
+        return (const T*)v.data + (a.starts ? 0 : n * v.seq) + (h / share) * v.head + low * v.moment;
+    };
+    const int sx_ = (int)s.x.moment * (int)sizeof(T), sy_ = (int)s.y.moment * (int)sizeof(T), sv_ = (int)s.v.moment * (int)sizeof(T);
+    const int row_sign = s.backwards ? -1 : 1;
+    uint4 rx[XV], ry[XV], rv[VV];
+    auto fetch = [&](long long i0) {                      // the chunk from the segment's moment i0
+        const int rows = rows_from(i0), pad = CH - rows;
+        const long long low = lowest(i0, rows);
+        const T *px = OUT ? base(s.x, s.xs, low) : nullptr, *py = base(s.y, s.ys, low), *pv = base(s.v, s.vs, low) + n0;
+        if constexpr (VEC) {
+            const auto bx = rows_at(px, rows, sx_, s.K * (int)sizeof(T)), by = rows_at(py, rows, sy_, s.K * (int)sizeof(T));
+            const auto bv = rows_at(pv, rows, sv_, (s.N - n0) * (int)sizeof(T));
+            // (the lanes' places anew each time, from the thread's number: kept, they cost registers that the products need)
+            const int t = here(tid), xr = t / XC, xc = t % XC * VN, vr = t / VC, vc = t % VC * VN;
+            const bool in_x = xc < s.K && (XR <= CH || xr < CH);
+            const unsigned ax = in_x ? in_memory(xr, 0) * sx_ + xc * (int)sizeof(T) : NOWHERE;
+            const unsigned ay = in_x ? in_memory(xr, 0) * sy_ + xc * (int)sizeof(T) : NOWHERE;
+            const unsigned av = vc < s.N - n0 ? in_memory(vr, 0) * sv_ + vc * (int)sizeof(T) : NOWHERE;
+            auto load = [&](__amdgpu_buffer_rsrc_t r, unsigned at, int row, int step) {
+                if (pad) at = row < pad ? NOWHERE : at - (s.backwards ? 0 : pad * step);
+                return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+            };
+#pragma unroll
+            for (int i = 0; i < XV; ++i) {
+                if (OUT) rx[i] = load(bx, ax + i * XR * row_sign * sx_, xr + i * XR, sx_);
+                ry[i] = load(by, ay + i * XR * row_sign * sy_, xr + i * XR, sy_);
+            }
+#pragma unroll
+            for (int i = 0; i < VV; ++i) rv[i] = load(bv, av + i * VR * row_sign * sv_, vr + i * VR, sv_);
+        } else {
+#pragma unroll
+            for (int i = 0; i < XV; ++i) {
+                const int row = xrow + i * XR;
+                const bool there = row >= pad && (XR <= CH || xrow < CH);
+                if (OUT) rx[i] = load16(px + in_memory(row, pad) * s.x.moment, xcol, s.K, there);
+                ry[i] = load16(py + in_memory(row, pad) * s.y.moment, xcol, s.K, there);
+            }
+#pragma unroll
+            for (int i = 0; i < VV; ++i)
+                rv[i] = load16(pv + in_memory(vrow + i * VR, pad) * s.v.moment, vcol, s.N - n0, vrow + i * VR >= pad);
+        }
+    };
+    if (left > 0) fetch(0);
 
     const float cv = s.backwards ? s.c : 1.f;
     float rest[4];                                        // the decay from a 16-row block's row to its end, times c''
 #pragma unroll
     for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r);
-    const float cz = s.backwards ? 1.f : s.c, row0 = cz * power(c);
+    const float cz = s.backwards ? 1.f : s.c;
     const float p16 = shared_by_all(power(16)), p32 = shared_by_all(power(32)), p48 = shared_by_all(power(48));
     auto blocks = [&](int i) { return i == 0 ? 1.f : i == 1 ? p16 : i == 2 ? p32 : p48; };
     Keep keep(ld * CH);                                   // over a whole chunk
     keep.one = shared_by_all(keep.one);
     keep.f = shared_by_all(keep.f);
     TO* const out = OUT ? (TO*)s.out : nullptr;
-    const long long drow = dir * a.heads * s.N;
-    TO* po = OUT ? out + (((a.starts ? 0 : n * a.n_moments) + t0) * a.heads + h) * s.N + c * drow + n0 + w0 + 4 * g : nullptr;
+    const long long out_first = a.starts ? 0 : n * a.n_moments;
+    const int so_ = a.heads * s.N * (int)sizeof(TO), oc = w0 + 4 * g;
+    const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
     const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
     const bf16* const vdown = sv + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
 
     for (long long i0 = 0; i0 < left; i0 += CH) {
-        const int pad = CH - rows_from(i0);
+        const int rows = rows_from(i0), pad = CH - rows;
         __syncthreads();                                  // (the chunk before is read)
 #pragma unroll
         for (int i = 0; i < XV; ++i) {
             if (XR > CH && xrow >= CH) break;
-            const int to = place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7);
+            // (a row 16 on has its shares in the same order)
+            const int to = XR % 16 ? place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7) : xto + i * XR * KW;
             if (OUT) store_terms<T>(rx[i], sx + to, XP);
             store_terms<T>(ry[i], sy + to, XP);
         }
 #pragma unroll
-        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], sv + place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7), VP);
+        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], sv + vto + i * VR * NW, VP);
         __syncthreads();
 
-        f32x4 o[JB] = {};
+        f32x4 o[JB];
         if (OUT && out) {
             // pieces of weights: rows 32 jj .., columns 16 i .. of (jj, i) = (0, 0) (0, 1) (0, 2) (0, 3) (1, 2) (1, 3)
             for (int piece = wave; piece < PIECES; piece += WAVES) {
@@ -388,7 +424,8 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
                     const int d = d0 - 16 * (r >> 2) - (r & 3);
-                    v[r] = d >= 0 ? s.c * power(d) * p[r >> 2][r & 3] : 0.f;      // (whatever x . y is there)
+                    const float f = s.c * power(max(d, 0));
+                    v[r] = d >= 0 ? f * p[r >> 2][r & 3] : 0.f;   // (whatever x . y is there)
                 }
                 Sum<W, 8> w;
                 w.of_summed(v);
@@ -401,30 +438,40 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
                 zf.of_summed(__builtin_shufflevector(z[2 * b], z[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
                 const int at = here(xat) ^ 32 * b;
 #pragma unroll
-                for (int i = 0; i < JB; ++i) o[i] = mfma(zf, across<X>(sx + 16 * i * KW + at, XP), o[i]);
+                for (int i = 0; i < JB; ++i)
+                    o[i] = mfma(zf, across<X>(sx + 16 * i * KW + at, XP), b ? o[i] : f32x4{0.f, 0.f, 0.f, 0.f});
             }
-            const int c1 = here(c) - pad;
-            const float f0 = here(row0);
+            float f[JB];
+            if (pad) {
+                const int c1 = here(c) - pad;
 #pragma unroll
-            for (int i = 0; i < JB; ++i) {
-                const float f = pad ? cz * power(max(16 * i + c1, 0)) : f0 * blocks(i);
+                for (int i = 0; i < JB; ++i) f[i] = cz * power(max(16 * i + c1, 0));
+            } else {
+                const float f0 = cz * power(here(c));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[i][r] *= f;
+                for (int i = 0; i < JB; ++i) f[i] = f0 * blocks(i);
             }
+#pragma unroll
+            for (int i = 0; i < JB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[i][r] *= f[i];
             __syncthreads();                              // (the pieces are there)
         }
         // (the next chunk on its way from here: earlier, its registers push the products' operands out)
-        if (i0 + CH < left) fetch(rows_from(i0 + CH));
+        if (i0 + CH < left) fetch(i0 + CH);
         if (OUT && out) {
-            unsigned odd = 0;
+            float odd = 0.f;                              // (0 times what is not finite is NaN)
+            unsigned none = 0;
+            asm("" : "+s"(none));
 #pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
                 Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW, 16 * NW, VP);
-                const uint4 u = __builtin_bit_cast(uint4, vf.term[0]);
-                const unsigned m = 0x7f807f80u, one = 0x00800080u;           // (an exponent of ones carries into the sign)
-                const unsigned bad = (((u.x & m) + one) | ((u.y & m) + one) | ((u.z & m) + one) | ((u.w & m) + one)) & 0x80008000u;
-                odd |= bad;
-                if (__ballot(bad != 0))
+                float bad = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; r += 2)
+                    bad = __builtin_amdgcn_fdot2_f32_bf16(Sum<1, 8>::pair(vf.term[0], r), __builtin_bit_cast(bf16x2, none), bad, false);
+                odd += bad;
+                if (__ballot(!(bad == 0.f)))
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
                         if (!(fabsf((float)vf.term[0][r]) < INFINITY))
@@ -438,7 +485,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
                     o[i] = mfma(vf, w, o[i]);
                 }
             }
-            if (__ballot(odd != 0)) {
+            if (__ballot(!(odd == 0.f))) {
                 int since = CH;                           // the first row of column c that is not finite
                 const int g4 = here(4 * g), c1 = here(c);
 #pragma unroll
@@ -459,24 +506,29 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
                         if (16 * i + c1 >= f) o[i][r] = NAN;
                 }
             }
-            const int oc = n0 + w0 + 4 * g;
-            if (pad) po -= pad * drow;
+            TO* const po = out + ((out_first + lowest(i0, rows)) * a.heads + h) * s.N + n0;
+            if constexpr (VEC) {
+                const auto bo = rows_at(po, rows, so_, (s.N - n0) * (int)sizeof(TO));
+                const int c1 = here(c), oc1 = here(oc);
+                const unsigned at = n0 + oc1 < s.N ? in_memory(c1, pad) * so_ + oc1 * (int)sizeof(TO) : NOWHERE;       // (a row before the first, or past the last: outside)
 #pragma unroll
-            for (int i = 0; i < JB; ++i) {
-                if (c < pad - 16 * i) continue;
-                TO* to = po + 16 * i * drow;
-                if (VEC && oc < s.N) {
+                for (int i = 0; i < JB; ++i) {
                     typedef TO vec __attribute__((ext_vector_type(4)));
-                    vec v;
+                    const vec v = __builtin_convertvector(o[i], vec);
+                    const unsigned to = at + 16 * i * row_sign * so_;
+                    if constexpr (sizeof(TO) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), bo, to, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), bo, to, 0, 0);
+                }
+            } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = narrow<TO>(o[i][r]);
-                    *reinterpret_cast<vec*>(to) = v;
-                } else if (!VEC)
+                for (int i = 0; i < JB; ++i) {
+                    if (16 * i + c < pad) continue;
+                    TO* to = po + (long long)in_memory(16 * i + c, pad) * a.heads * s.N + oc;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (oc + r < s.N) to[r] = narrow<TO>(o[i][r]);
+                        if (n0 + oc + r < s.N) to[r] = narrow<TO>(o[i][r]);
+                }
             }
-            po += CH * drow;
         }
 
         // the state after the chunk; of the stretch's last one forwards, S rather than l S
@@ -760,11 +812,13 @@ Scans scans_of(const fm_attention_args& p) {
     return a;
 }
 
-// 16-byte loads, whole stores: heads of a multiple of 16 bytes, everything aligned
+// 16-byte loads, whole stores: heads of a multiple of 16 bytes, everything aligned, a chunk's rows within 2^30 bytes
 bool wide_rows(const fm_attention_args& p, bool bwd) {
     const int size = p.dtype == FM_F32 ? 4 : 2;
     if (p.k_dim * size % 16 || p.v_dim * size % 16 || !aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
-    if (bwd) return aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv | (uintptr_t)p.workspace) & 15);
+    auto near = [](long long s) { return s >= 0 && s < STRIDE_MOST; };
+    if (!near(p.q.moment) || !near(p.k.moment) || !near(p.v.moment) || !near(p.q_heads * ATT_MAX)) return false;
+    if (bwd) return near(p.go.moment) && aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv | (uintptr_t)p.workspace) & 15);
     return !((uintptr_t)p.o & 15);
 }
 
