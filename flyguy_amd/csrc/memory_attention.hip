@@ -7,6 +7,8 @@
 // the last moment's term does not decay; the second one's end state, decayed once more, is the start state's gradient.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "memory.h"
 
 namespace fg {
@@ -16,11 +18,11 @@ constexpr int ATT_MAX = 128;             // values of a head
 struct Scan {
     fm_view x, y, v;
     int xs, ys, vs;                      // query heads per head of x, y, v (1, or q_heads / k_heads)
-    void* out;                           // dense [moments][heads][N]; 0: no output
+    void* out;                           // dense [moments][heads][N], of the values' type or (wide) float32; 0: no output
     const float* init;                   // start state [n_seq][heads][K][N] (transposed: [N][K]); 0: zeros
     float* fin;                          // end state [n_seq][heads][K][N]; 0: not wanted
     float* seg;                          // [slots][heads][K][N]: segments' own states, then their start states
-    int K, N, transposed, backwards;
+    int K, N, transposed, backwards, wide;
     float c;
 };
 
@@ -223,14 +225,14 @@ __device__ __forceinline__ Sum<P, 8> down(const bf16* p, int apart, int plane) {
 // the chunk's 16 x 32 pieces on and below the diagonal are formed by a wave each and shared through LDS.
 // A value of v that is not finite reaches only the outputs from its moment on (there: NaN), though 0 weights meet it in the
 // products: such a chunk's products run with zeros in its place.
-template <class T, int KT, int WAVES, bool OUT>
+template <class T, int KT, int NT, int WAVES, bool OUT>
 struct Tile {
-    static constexpr int CH = Form<T>::CHUNK, KW = 32 * KT, NW = 16 * WAVES;
+    static constexpr int CH = Form<T>::CHUNK, KW = 32 * KT, NW = 16 * NT * WAVES;
     static constexpr int XP = CH * KW, VP = CH * NW, PIECES = CH == 64 ? 6 : 2;
     static constexpr int LDS = Form<T>::X * 2 * (XP * (OUT ? 2 : 1) + VP) + (OUT ? PIECES * Form<T>::W * 1024 : 0);
-    // waves a SIMD that LDS lets in, at most 4 (128 registers)
-    static constexpr int FIT = 160 * 1024 / LDS * WAVES / 4;
-    static constexpr int PER_SIMD = FIT < 1 ? 1 : FIT > 4 ? 4 : FIT;
+    // waves a SIMD that LDS lets in, at most 4 (128 registers); two blocks of columns a wave: 3 or 2
+    static constexpr int FIT = 160 * 1024 / LDS * WAVES / 4, MOST = NT == 1 ? 4 : KT == 2 ? 3 : 2;
+    static constexpr int PER_SIMD = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
 };
 // Where a row's 8-value share q stands in LDS: rows of 8 or 16 shares, unpadded, the shares of row 4g + r (of 16) exchanged
 // by q ^ (r, g), so that both the 16 rows of a share and the 4 shares of 4 rows that a transposing read takes lie in banks
@@ -268,21 +270,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int row
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-template <class T, int KT, int WAVES, bool VEC, bool OUT, class TO>
-__global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) void k_scan(Scans a) {
-    using S = Tile<T, KT, WAVES, OUT>;
+template <class T, int KT, int NT, int WAVES, bool VEC, bool OUT>
+__global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)) void k_scan(Scans a) {
+    using S = Tile<T, KT, NT, WAVES, OUT>;
     constexpr int X = Form<T>::X, W = Form<T>::W, CH = S::CH, JB = CH / 16, VN = Vec<T>::N;
     constexpr int KW = S::KW, NW = S::NW, XP = S::XP, VP = S::VP, PIECES = S::PIECES;
     constexpr int XC = KW / VN, VC = NW / VN;                                // 16-byte shares of a row
     constexpr int XR = 64 * WAVES / XC, VR = 64 * WAVES / VC;                // rows between a thread's shares
     constexpr int XV = XR < CH ? CH / XR : 1, VV = CH / VR;                  // a thread's shares (XR > CH: of some threads)
-    static_assert((XV * XR == CH || XR > CH) && VV * VR == CH && VR % 16 == 0, "");
+    static_assert((XV * XR == CH || XR > CH) && VV * VR == CH, "");
     __shared__ __align__(16) bf16 sx[OUT ? X * XP : 8], sy[X * XP], sv[X * VP];
     __shared__ __align__(16) bf16x8 sp[OUT ? PIECES : 1][W][64];
     const Scan& s = a.s[blockIdx.z];
-    const int nblk = (s.N + NW - 1) / NW;
-    const int slot = blockIdx.x / nblk, blk = blockIdx.x % nblk, h = blockIdx.y;
-    if (slot >= a.slots) return;
+    const int slot = blockIdx.x, h = blockIdx.y;
     int n, seg;
     long long first, count;
     if (!segment_of(a, slot, n, seg, first, count)) return;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     first = shared_by_all(first);
     count = shared_by_all(count);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const int n0 = blk * NW, w0 = 16 * wave;              // this workgroup's columns, this wave's from there
+    const int w0 = 16 * NT * wave;                        // this wave's columns from here
     const long long from = seg * a.L, left = count - from < a.L ? count - from : a.L;
     const bool last = from + left == count;
     if (!OUT && last) return;                             // (the last segment's own state is needed by none)
@@ -300,26 +300,30 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     const float e2 = shared_by_all(ld * 1.44269504f);
     auto power = [&](int i) { return __builtin_amdgcn_exp2f(e2 * (float)i); };
 
-    f32x4 z[2 * KT];                                      // the state
+    f32x4 z[2 * KT][NT];                                  // the state
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
-    const int col = n0 + w0 + c;
+    // the column of lane c in block t; a lane's outputs are then side by side
+    auto col_of = [&](int t, int m) { return w0 + (NT == 2 ? 8 * (m >> 2) + 4 * t + (m & 3) : m); };
     const float* z0 = !OUT ? nullptr : s.seg ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : s.init ? s.init + at : nullptr;
     {
-        const bool t = !s.seg && s.transposed;
-        const int zk = t ? 1 : s.N, zc = t ? s.K : 1;
+        const bool flip = !s.seg && s.transposed;
+        const int zk = flip ? 1 : s.N, zc = flip ? s.K : 1;
         const Keep once(!s.seg && !s.backwards && count ? ld : 0.f);      // (no moments: the state goes through as it is)
 #pragma unroll
-        for (int b = 0; b < 2 * KT; ++b) z[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (z0) {
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) z[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (!z0) continue;
+            const int col = col_of(t, c);
             const float* p = z0 + min(col, s.N - 1) * zc;
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[b][r] = p[min(row_of(b, r), s.K - 1) * zk];
+                for (int r = 0; r < 4; ++r) z[b][t][r] = p[min(row_of(b, r), s.K - 1) * zk];
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[b][r] = row_of(b, r) < s.K && col < s.N ? once(z[b][r]) : 0.f;
+                for (int r = 0; r < 4; ++r) z[b][t][r] = row_of(b, r) < s.K && col < s.N ? once(z[b][t][r]) : 0.f;
         }
     }
 
@@ -338,16 +342,16 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     auto fetch = [&](long long i0) {                      // the chunk from the segment's moment i0
         const int rows = rows_from(i0), pad = CH - rows;
         const long long low = lowest(i0, rows);
-        const T *px = OUT ? base(s.x, s.xs, low) : nullptr, *py = base(s.y, s.ys, low), *pv = base(s.v, s.vs, low) + n0;
+        const T *px = OUT ? base(s.x, s.xs, low) : nullptr, *py = base(s.y, s.ys, low), *pv = base(s.v, s.vs, low);
         if constexpr (VEC) {
             const auto bx = rows_at(px, rows, sx_, s.K * (int)sizeof(T)), by = rows_at(py, rows, sy_, s.K * (int)sizeof(T));
-            const auto bv = rows_at(pv, rows, sv_, (s.N - n0) * (int)sizeof(T));
+            const auto bv = rows_at(pv, rows, sv_, s.N * (int)sizeof(T));
             // (the lanes' places anew each time, from the thread's number: kept, they cost registers that the products need)
             const int t = here(tid), xr = t / XC, xc = t % XC * VN, vr = t / VC, vc = t % VC * VN;
             const bool in_x = xc < s.K && (XR <= CH || xr < CH);
             const unsigned ax = in_x ? in_memory(xr, 0) * sx_ + xc * (int)sizeof(T) : NOWHERE;
             const unsigned ay = in_x ? in_memory(xr, 0) * sy_ + xc * (int)sizeof(T) : NOWHERE;
-            const unsigned av = vc < s.N - n0 ? in_memory(vr, 0) * sv_ + vc * (int)sizeof(T) : NOWHERE;
+            const unsigned av = vc < s.N ? in_memory(vr, 0) * sv_ + vc * (int)sizeof(T) : NOWHERE;
             auto load = [&](__amdgpu_buffer_rsrc_t r, unsigned at, int row, int step) {
                 if (pad) at = row < pad ? NOWHERE : at - (s.backwards ? 0 : pad * step);
                 return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
             }
 #pragma unroll
             for (int i = 0; i < VV; ++i)
-                rv[i] = load16(pv + in_memory(vrow + i * VR, pad) * s.v.moment, vcol, s.N - n0, vrow + i * VR >= pad);
+                rv[i] = load16(pv + in_memory(vrow + i * VR, pad) * s.v.moment, vcol, s.N, vrow + i * VR >= pad);
         }
     };
     if (left > 0) fetch(0);
@@ -384,12 +388,19 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
     Keep keep(ld * CH);                                   // over a whole chunk
     keep.one = shared_by_all(keep.one);
     keep.f = shared_by_all(keep.f);
-    TO* const out = OUT ? (TO*)s.out : nullptr;
+    char* const out = OUT ? (char*)s.out : nullptr;
+    const int size = s.wide ? 4 : (int)sizeof(T);
     const long long out_first = a.starts ? 0 : n * a.n_moments;
-    const int so_ = a.heads * s.N * (int)sizeof(TO), oc = w0 + 4 * g;
+    const int so_ = a.heads * s.N * size, oc = w0 + 4 * NT * g;
     const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
     const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
-    const bf16* const vdown = sv + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+    const bf16* const vdown = sv + (NT == 2 ? place<NW>(4 * g + (c >> 2), 4 * wave + (c & 3))
+                                            : place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1));
+    if (OUT)                                              // the pieces' blocks above the diagonal: zeros for good
+        for (int i = tid; i < W * 64; i += 64 * WAVES) {
+            reinterpret_cast<bf16x4*>(&sp[0][0][i])[1] = bf16x4{};
+            if (PIECES == 6) reinterpret_cast<bf16x4*>(&sp[4][0][i])[1] = bf16x4{};
+        }
 
     for (long long i0 = 0; i0 < left; i0 += CH) {
         const int rows = rows_from(i0), pad = CH - rows;
@@ -403,43 +414,45 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
             store_terms<T>(ry[i], sy + to, XP);
         }
 #pragma unroll
-        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], sv + vto + i * VR * NW, VP);
+        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], sv + (VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW), VP);
         __syncthreads();
 
-        f32x4 o[JB];
+        f32x4 o[JB][NT];
         if (OUT && out) {
-            // pieces of weights: rows 32 jj .., columns 16 i .. of (jj, i) = (0, 0) (0, 1) (0, 2) (0, 3) (1, 2) (1, 3)
-            for (int piece = wave; piece < PIECES; piece += WAVES) {
-                const int jj = piece >> 2, i = jj ? piece - 2 : piece, d0 = here(16 * i + c - 32 * jj - 4 * g);
-                f32x4 p[2] = {};
+            // the weights' 16 x 16 blocks, rows j, columns i >= j; two of rows 32 jj .. make a piece: (jj, i) = (0, 0) (0, 1)
+            // (0, 2) (0, 3) (1, 2) (1, 3)
+            for (int block = wave; block < JB * (JB + 1) / 2; block += WAVES) {
+                const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3, j = block - i * (i + 1) / 2;
+                const int d0 = here(16 * (i - j) + c - 4 * g);
+                f32x4 p;
 #pragma unroll
                 for (int b = 0; b < KT; ++b) {
                     const int at = here(xat) ^ 32 * b;
-                    const Sum<X, 8> xf = across<X>(sx + 16 * i * KW + at, XP);
-                    const bf16* y = sy + 32 * jj * KW + at;
-                    p[0] = mfma(across<X>(y, XP), xf, p[0]);
-                    p[1] = mfma(across<X>(y + 16 * KW, XP), xf, p[1]);
+                    p = mfma(across<X>(sy + 16 * j * KW + at, XP), across<X>(sx + 16 * i * KW + at, XP),
+                             b ? p : f32x4{0.f, 0.f, 0.f, 0.f});
                 }
-                f32x8 v;
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int d = d0 - 16 * (r >> 2) - (r & 3);
-                    const float f = s.c * power(max(d, 0));
-                    v[r] = d >= 0 ? f * p[r >> 2][r & 3] : 0.f;   // (whatever x . y is there)
+                for (int r = 0; r < 4; ++r) {
+                    const float f = s.c * power(max(d0 - r, 0));
+                    p[r] = d0 >= r ? f * p[r] : 0.f;      // (whatever x . y is there)
                 }
-                Sum<W, 8> w;
-                w.of_summed(v);
+                Sum<W, 4> w;
+                w.of_summed(p);
 #pragma unroll
-                for (int t = 0; t < W; ++t) sp[piece][t][lane] = w.term[t];
+                for (int t = 0; t < W; ++t) reinterpret_cast<bf16x4*>(&sp[j < 2 ? i : i + 2][t][lane])[j & 1] = w.term[t];
             }
 #pragma unroll
             for (int b = 0; b < KT; ++b) {
-                Sum<W, 8> zf;
-                zf.of_summed(__builtin_shufflevector(z[2 * b], z[2 * b + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                Sum<W, 8> zf[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) zf[t].of_summed(__builtin_shufflevector(z[2 * b][t], z[2 * b + 1][t], 0, 1, 2, 3, 4, 5, 6, 7));
                 const int at = here(xat) ^ 32 * b;
 #pragma unroll
-                for (int i = 0; i < JB; ++i)
-                    o[i] = mfma(zf, across<X>(sx + 16 * i * KW + at, XP), b ? o[i] : f32x4{0.f, 0.f, 0.f, 0.f});
+                for (int i = 0; i < JB; ++i) {
+                    const Sum<X, 8> xf = across<X>(sx + 16 * i * KW + at, XP);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) o[i][t] = mfma(zf[t], xf, b ? o[i][t] : f32x4{0.f, 0.f, 0.f, 0.f});
+                }
             }
             float f[JB];
             if (pad) {
@@ -454,7 +467,9 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
 #pragma unroll
             for (int i = 0; i < JB; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[i][r] *= f[i];
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[i][t][r] *= f[i];
             __syncthreads();                              // (the pieces are there)
         }
         // (the next chunk on its way from here: earlier, its registers push the products' operands out)
@@ -465,68 +480,94 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
             asm("" : "+s"(none));
 #pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
-                Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW, 16 * NW, VP);
+                Sum<X, 8> vf[NT];
                 float bad = 0.f;
 #pragma unroll
-                for (int r = 0; r < 8; r += 2)
-                    bad = __builtin_amdgcn_fdot2_f32_bf16(Sum<1, 8>::pair(vf.term[0], r), __builtin_bit_cast(bf16x2, none), bad, false);
+                for (int t = 0; t < NT; ++t) {
+                    vf[t] = down<X>(vdown + 32 * jj * NW + 4 * t, 16 * NW, VP);
+#pragma unroll
+                    for (int r = 0; r < 8; r += 2)
+                        bad = __builtin_amdgcn_fdot2_f32_bf16(Sum<1, 8>::pair(vf[t].term[0], r), __builtin_bit_cast(bf16x2, none), bad, false);
+                }
                 odd += bad;
                 if (__ballot(!(bad == 0.f)))
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (!(fabsf((float)vf.term[0][r]) < INFINITY))
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                            for (int t = 0; t < X; ++t) vf.term[t][r] = (bf16)0.f;
+                        for (int r = 0; r < 8; ++r)
+                            if (!(fabsf((float)vf[t].term[0][r]) < INFINITY))
+#pragma unroll
+                                for (int p = 0; p < X; ++p) vf[t].term[p][r] = (bf16)0.f;
 #pragma unroll
                 for (int i = 2 * jj; i < JB; ++i) {
                     Sum<W, 8> w;
 #pragma unroll
                     for (int t = 0; t < W; ++t) w.term[t] = sp[jj ? i + 2 : i][t][lane];
-                    o[i] = mfma(vf, w, o[i]);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) o[i][t] = mfma(vf[t], w, o[i][t]);
                 }
             }
             if (__ballot(!(odd == 0.f))) {
-                int since = CH;                           // the first row of column c that is not finite
                 const int g4 = here(4 * g), c1 = here(c);
 #pragma unroll
-                for (int jj = 0; jj < JB / 2; ++jj) {
-                    const bf16x8 v = columns8(vdown + 32 * jj * NW, 16 * NW);
+                for (int t = 0; t < NT; ++t) {
+                    int since = CH;                       // the first row of the lane's column that is not finite
 #pragma unroll
-                    for (int r = 0; r < 8; ++r)
-                        if (!(fabsf((float)v[r]) < INFINITY))
-                            since = min(since, 32 * jj + 16 * (r >> 2) + g4 + (r & 3));
-                }
-                since = min(since, __shfl_xor(since, 16));
-                since = min(since, __shfl_xor(since, 32));
+                    for (int jj = 0; jj < JB / 2; ++jj) {
+                        const bf16x8 v = columns8(vdown + 32 * jj * NW + 4 * t, 16 * NW);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int f = __shfl(since, g4 + r);
+                        for (int r = 0; r < 8; ++r)
+                            if (!(fabsf((float)v[r]) < INFINITY))
+                                since = min(since, 32 * jj + 16 * (r >> 2) + g4 + (r & 3));
+                    }
+                    since = min(since, __shfl_xor(since, 16));
+                    since = min(since, __shfl_xor(since, 32));
 #pragma unroll
-                    for (int i = 0; i < JB; ++i)
-                        if (16 * i + c1 >= f) o[i][r] = NAN;
+                    for (int r = 0; r < 4; ++r) {
+                        const int f = __shfl(since, g4 + r);
+#pragma unroll
+                        for (int i = 0; i < JB; ++i)
+                            if (16 * i + c1 >= f) o[i][t][r] = NAN;
+                    }
                 }
             }
-            TO* const po = out + ((out_first + lowest(i0, rows)) * a.heads + h) * s.N + n0;
+            char* const po = out + ((out_first + lowest(i0, rows)) * a.heads + h) * s.N * size;
             if constexpr (VEC) {
-                const auto bo = rows_at(po, rows, so_, (s.N - n0) * (int)sizeof(TO));
+                const auto bo = rows_at(po, rows, so_, s.N * size);
                 const int c1 = here(c), oc1 = here(oc);
-                const unsigned at = n0 + oc1 < s.N ? in_memory(c1, pad) * so_ + oc1 * (int)sizeof(TO) : NOWHERE;       // (a row before the first, or past the last: outside)
+                // (a row before the first, or past the last, is outside)
+                const unsigned at = oc1 < s.N ? in_memory(c1, pad) * so_ + oc1 * size : NOWHERE;
 #pragma unroll
                 for (int i = 0; i < JB; ++i) {
-                    typedef TO vec __attribute__((ext_vector_type(4)));
-                    const vec v = __builtin_convertvector(o[i], vec);
                     const unsigned to = at + 16 * i * row_sign * so_;
-                    if constexpr (sizeof(TO) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), bo, to, 0, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), bo, to, 0, 0);
+                    if (sizeof(T) == 4 || s.wide) {
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)      // (columns past the row's end would be the next one's)
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i][t]), bo, oc1 + 4 * t < s.N ? to + 16 * t : NOWHERE, 0, 0);
+                    } else if constexpr (sizeof(T) == 2) {
+                        typedef T vec __attribute__((ext_vector_type(4)));
+                        vec v[NT];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) v[t] = __builtin_convertvector(o[i][t], vec);
+                        if constexpr (NT == 2)
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[NT - 1], 0, 1, 2, 3, 4, 5, 6, 7)), bo, to, 0, 0);
+                        else
+                            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v[0]), bo, to, 0, 0);
+                    }
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < JB; ++i) {
                     if (16 * i + c < pad) continue;
-                    TO* to = po + (long long)in_memory(16 * i + c, pad) * a.heads * s.N + oc;
+                    char* to = po + (long long)in_memory(16 * i + c, pad) * so_ + oc * size;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n0 + oc + r < s.N) to[r] = narrow<TO>(o[i][r]);
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (oc + 4 * t + r >= s.N) continue;
+                            if (s.wide) reinterpret_cast<float*>(to)[4 * t + r] = o[i][t][r];
+                            else reinterpret_cast<T*>(to)[4 * t + r] = narrow<T>(o[i][t][r]);
+                        }
                 }
             }
         }
@@ -546,52 +587,60 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, WAVES, OUT>::PER_SIMD)) vo
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[b][r] = fmaf(keep.f, z[b][r], z[b][r]);
+                for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] = fmaf(keep.f, z[b][r >> 2][r & 3], z[b][r >> 2][r & 3]);
         } else {
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[b][r] *= keep.f;
+                for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] *= keep.f;
         }
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
-            const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW, 16 * NW, VP);
-            f32x8 v = __builtin_convertvector(vf.term[X - 1], f32x8);
+            Sum<S_TERMS, 8> w[NT];
 #pragma unroll
-            for (int t = X - 2; t >= 0; --t) v += __builtin_convertvector(vf.term[t], f32x8);
+            for (int t = 0; t < NT; ++t) {
+                const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW + 4 * t, 16 * NW, VP);
+                f32x8 v = __builtin_convertvector(vf.term[X - 1], f32x8);
 #pragma unroll
-            for (int r = 0; r < 8; ++r) v[r] *= rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2));
-            Sum<S_TERMS, 8> w;
-            w.of_summed(v);
+                for (int p = X - 2; p >= 0; --p) v += __builtin_convertvector(vf.term[p], f32x8);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] *= rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2));
+                w[t].of_summed(v);
+            }
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
                 const bf16* p = sy + 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
-                z[b] = mfma(down<X>(p, 16 * KW, XP), w, z[b]);
+                const Sum<X, 8> yt = down<X>(p, 16 * KW, XP);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) z[b][t] = mfma(yt, w[t], z[b][t]);
             }
         }
     }
 
     float* to = !OUT ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : last && s.fin ? s.fin + at : nullptr;
     if (to) {
-        const int k0 = here(8 * g), c0 = here(col);
-        if (c0 < s.N)
+        const int k0 = here(8 * g);
 #pragma unroll
-            for (int b = 0; b < 2 * KT; ++b)
+        for (int t = 0; t < NT; ++t) {
+            const int c0 = here(col_of(t, c));
+            if (c0 < s.N)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int k = k0 + 32 * (b >> 1) + 4 * (b & 1) + r;
-                    if (k < s.K) to[k * s.N + c0] = z[b][r];
-                }
+                for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int k = k0 + 32 * (b >> 1) + 4 * (b & 1) + r;
+                        if (k < s.K) to[k * s.N + c0] = z[b][t][r];
+                    }
+        }
     }
     if (OUT && a.starts && out && seg == 0 && (n == 0 || n == a.n_seq - 1)) {
         // moments of no stretch, before the first one and after the last, give zeros
-        for (int e = tid; e < NW; e += 64 * WAVES) {
-            if (n0 + e >= s.N) break;
-            TO* all = out + (size_t)h * s.N + n0 + e;
+        for (int e = tid; e < s.N * size; e += 64 * WAVES) {
+            char* all = out + (size_t)h * s.N * size + e;
             if (n == 0)
-                for (long long t = 0; t < first; ++t) all[t * a.heads * s.N] = narrow<TO>(0.f);
+                for (long long t = 0; t < first; ++t) all[t * so_] = 0;
             if (n == a.n_seq - 1)
-                for (long long t = first + count; t < a.n_moments; ++t) all[t * a.heads * s.N] = narrow<TO>(0.f);
+                for (long long t = first + count; t < a.n_moments; ++t) all[t * so_] = 0;
         }
     }
 }
@@ -623,14 +672,18 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     }
 }
 
-// gradients of shared heads: out[m][j][d] = the sum over a key head's `share` query heads of part[m][share j + i][d]
+// gradients of shared heads: out[m][j][d] = the sum over a key head's `share` query heads of part[m][share j + i][d]; the
+// first `first` workgroups those of k, the rest those of v
 template <class T>
-__global__ __launch_bounds__(256) void k_share(const float* __restrict__ part, T* __restrict__ out, int share, int D,
-                                               long long n) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const long long row = i / D;
-    const int d = (int)(i % D);
+__global__ __launch_bounds__(256) void k_share(const float* part_k, T* out_k, int K, long long nk, unsigned first,
+                                               const float* part_v, T* out_v, int V, long long nv, int share) {
+    const bool of_v = blockIdx.x >= first;
+    const float* part = of_v ? part_v : part_k;
+    T* out = of_v ? out_v : out_k;
+    const int D = of_v ? V : K;
+    const long long i = (long long)(blockIdx.x - (of_v ? first : 0)) * 256 + threadIdx.x, row = i / D;
+    if (i >= (of_v ? nv : nk)) return;
+    const int d = (int)(i - row * D);
     float s = 0.f;
     for (int j = 0; j < share; ++j) s += part[(row * share + j) * D + d];
     out[i] = narrow<T>(s);
@@ -733,30 +786,68 @@ long long shared_floats(const fm_attention_args& a, bool of_v) {
     return a.q_heads > a.k_heads ? moments * a.q_heads * (of_v ? a.v_dim : a.k_dim) : 0;
 }
 
-// How a launch's scans are cut into segments: one segment a stretch where the stretches' heads alone fill the chip, else so
-// that about SEG_GROUPS workgroups run, of at least SEG_MIN moments.
-#ifndef SEGG
-#define SEGG 512
-#endif
-constexpr int SEG_GROUPS = SEGG, SEG_MIN = 256;
+// The kernel's forms by the products' sizes: K up to 64 or 128 rows of state; N up to 64 columns, a block of 16 a wave, or up
+// to 128, two blocks a wave (a wave's reads of x and y then serve two: at N = 128, one block and 8 waves measured the same
+// within 1%, and 4 waves in two workgroups 6% more).
+template <class T, int KT, int NT>
+constexpr int groups_per_cu() { return Tile<T, KT, NT, 4, true>::PER_SIMD; }
+template <class T>
+int groups_per_cu(int K, int N) {
+    return K <= 64 ? (N <= 64 ? groups_per_cu<T, 2, 1>() : groups_per_cu<T, 2, 2>())
+                   : (N <= 64 ? groups_per_cu<T, 4, 1>() : groups_per_cu<T, 4, 2>());
+}
+
+// How a launch's scans are cut into segments: as the following estimate has it cheapest, in chunks' times.  A CU with w
+// workgroups takes about 0.9 + w for a chunk of each (measured: 7.6 us with one, 11.6 with two of 128 x 128 in bfloat16), a
+// workgroup 1.5 chunks to begin and end.  More than one segment a stretch cost a pass for their own states (0.45 of the main
+// one) and one to join them.  A packed stretch is taken to be the middle length, the longest twice that.
 struct Cut {
-    int nseg, slots;
+    int nseg, slots, K, N;
     long long L;
 };
 Cut cut_of(const fm_attention_args& p, int scans) {
     Cut c;
-    const long long moments = p.n_moments * (p.starts ? 1 : p.n_seq);
-    const long long groups = p.n_seq * p.q_heads * scans;
+    const int widest = (int)(p.k_dim > p.v_dim ? p.k_dim : p.v_dim);
+    c.K = scans == 1 ? (int)p.k_dim : widest;             // (a gradient's scans have them both ways round)
+    c.N = scans == 1 ? (int)p.v_dim : widest;
     c.nseg = 1;
     c.slots = (int)p.n_seq;
     c.L = (p.n_moments + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
-    if (groups >= SEG_GROUPS / 2 || !groups) return c;
-    long long L = (moments * p.q_heads * scans / SEG_GROUPS + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
-    if (L < SEG_MIN) L = SEG_MIN;
-    if (L >= p.n_moments) return c;
-    c.L = L;
-    c.nseg = (int)((p.n_moments + L - 1) / L);
-    c.slots = p.starts ? (int)(p.n_moments / L + p.n_seq) : (int)p.n_seq * c.nseg;
+    if (!c.L) c.L = CHUNK_MAX;
+    if (!p.n_seq || !p.n_moments) return c;
+    const int cap = p.dtype == FM_F32 ? groups_per_cu<float>(c.K, c.N) : p.dtype == FM_BF16 ? groups_per_cu<bf16>(c.K, c.N)
+                                                                                            : groups_per_cu<f16>(c.K, c.N);
+    const int chunk = p.dtype == FM_BF16 ? Form<bf16>::CHUNK : Form<float>::CHUNK;
+    const double middle = p.starts ? (double)p.n_moments / p.n_seq : (double)p.n_moments;
+    const double longest = p.starts && p.n_seq > 1 ? 2 * middle : middle;
+    const double chains = (double)p.n_seq * p.q_heads * scans;
+    auto pass = [&](double groups, double L) {
+        double left = groups / 256, t = 0;
+        for (; left > 0; left -= cap) {
+            if (left > 64 * cap) {                        // (many rounds: each full)
+                t += (0.9 + cap) * left / cap;
+                break;
+            }
+            t += 0.9 + (left < cap ? ceil(left) : cap);
+        }
+        return t * (L / chunk + 1.5);
+    };
+    double best = pass(chains, longest);
+    for (int nseg = 2; nseg <= 1024; nseg += nseg < 4 ? 1 : nseg / 2) {
+        const long long L = ((long long)ceil(longest / nseg) + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
+        if (L >= longest) continue;
+        const double each = p.starts ? middle / L + 0.5 : ceil(middle / L);
+        const double t = pass(chains * each, (double)L) + 0.45 * pass(chains * (each - 1), (double)L) + 0.7 + each / 22;
+        if (t < best) {
+            best = t;
+            c.L = L;
+            c.nseg = nseg;
+        }
+        if (L == CHUNK_MAX) break;
+    }
+    if (c.nseg == 1) return c;
+    c.nseg = (int)((p.n_moments + c.L - 1) / c.L);
+    c.slots = p.starts ? (int)(p.n_moments / c.L + p.n_seq) : (int)p.n_seq * c.nseg;
     return c;
 }
 // floats of segments' states of one scan
@@ -764,41 +855,30 @@ long long segment_floats(const fm_attention_args& p, const Cut& c) {
     return c.nseg == 1 ? 0 : (long long)c.slots * p.q_heads * p.k_dim * p.v_dim;
 }
 
-template <class T, int KT, int WAVES, bool VEC, class TO>
+template <class T, int KT, int NT, bool VEC>
 void launch_form(Scans& a, int count, hipStream_t st) {
-    int nblk = 1, most = 1;
-    for (int i = 0; i < count; ++i) {
-        const int b = (a.s[i].N + 16 * WAVES - 1) / (16 * WAVES), kn = a.s[i].K * a.s[i].N;
-        nblk = b > nblk ? b : nblk;
-        most = kn > most ? kn : most;
-    }
-    const dim3 grid(a.slots * nblk, a.heads, count);
+    int most = 1;
+    for (int i = 0; i < count; ++i) most = a.s[i].K * a.s[i].N > most ? a.s[i].K * a.s[i].N : most;
+    const dim3 grid(a.slots, a.heads, count);
     if (a.nseg > 1) {
-        k_scan<T, KT, WAVES, VEC, false, TO><<<grid, 64 * WAVES, 0, st>>>(a);
+        k_scan<T, KT, NT, 4, VEC, false><<<grid, 256, 0, st>>>(a);
         k_scan_join<<<dim3((most + 255) / 256 * a.heads, a.n_seq, count), 256, 0, st>>>(a);
     }
-    k_scan<T, KT, WAVES, VEC, true, TO><<<grid, 64 * WAVES, 0, st>>>(a);
+    k_scan<T, KT, NT, 4, VEC, true><<<grid, 256, 0, st>>>(a);
 }
-template <class T, class TO>
-void launch_sized(Scans& a, int count, bool vec, hipStream_t st) {
-    int widest = 0, n = 0;
-    for (int i = 0; i < count; ++i) {
-        widest = a.s[i].K > widest ? a.s[i].K : widest;
-        n = a.s[i].N > n ? a.s[i].N : n;
-    }
-    if (widest <= 64 && n <= 64) vec ? launch_form<T, 2, 4, true, TO>(a, count, st) : launch_form<T, 2, 4, false, TO>(a, count, st);
-    else if (widest <= 64) vec ? launch_form<T, 2, 8, true, TO>(a, count, st) : launch_form<T, 2, 8, false, TO>(a, count, st);
-    else if (n <= 64) vec ? launch_form<T, 4, 4, true, TO>(a, count, st) : launch_form<T, 4, 4, false, TO>(a, count, st);
-    else vec ? launch_form<T, 4, 8, true, TO>(a, count, st) : launch_form<T, 4, 8, false, TO>(a, count, st);
+template <class T, bool VEC>
+void launch_sized(Scans& a, int count, const Cut& c, hipStream_t st) {
+    if (c.K <= 64) c.N <= 64 ? launch_form<T, 2, 1, VEC>(a, count, st) : launch_form<T, 2, 2, VEC>(a, count, st);
+    else c.N <= 64 ? launch_form<T, 4, 1, VEC>(a, count, st) : launch_form<T, 4, 2, VEC>(a, count, st);
 }
 
-template <class T, class TO>
+template <class T>
 void launch_scans(Scans& a, int count, const Cut& cut, bool vec, hipStream_t st) {
     if (!a.n_seq || !count) return;
-    a.L = cut.L > 0 ? cut.L : CHUNK_MAX;
+    a.L = cut.L;
     a.nseg = cut.nseg;
     a.slots = cut.slots;
-    launch_sized<T, TO>(a, count, vec, st);
+    vec ? launch_sized<T, true>(a, count, cut, st) : launch_sized<T, false>(a, count, cut, st);
 }
 
 Scans scans_of(const fm_attention_args& p) {
@@ -828,9 +908,9 @@ void attention_fwd(const fm_attention_args& p, hipStream_t st) {
     Scans a = scans_of(p);
     const Cut cut = cut_of(p, 1);
     float* seg = segment_floats(p, cut) ? (float*)p.workspace : nullptr;
-    a.s[0] = Scan{p.q, p.k, p.v, 1, share, share, p.o, p.state, p.state_out, seg, (int)p.k_dim, (int)p.v_dim, 0, 0,
+    a.s[0] = Scan{p.q, p.k, p.v, 1, share, share, p.o, p.state, p.state_out, seg, (int)p.k_dim, (int)p.v_dim, 0, 0, 0,
                   (float)p.scale};
-    launch_scans<T, T>(a, 1, cut, wide_rows(p, false), st);
+    launch_scans<T>(a, 1, cut, wide_rows(p, false), st);
 }
 
 template <class T>
@@ -838,29 +918,24 @@ void attention_bwd(const fm_attention_args& p, hipStream_t st) {
     const int share = (int)(p.q_heads / p.k_heads), K = (int)p.k_dim, V = (int)p.v_dim;
     const float c = (float)p.scale;
     const Cut cut = cut_of(p, 3);
-    const bool vec = wide_rows(p, true);
     const long long floats = segment_floats(p, cut);
     float* seg[3];
     for (int i = 0; i < 3; ++i) seg[i] = floats ? (float*)p.workspace + i * floats : nullptr;
+    // shared key / value heads: each query head's part in float32, then their sum
     float* part_k = (float*)p.workspace + 3 * floats;
     float* part_v = part_k + shared_floats(p, false);
-    const int own = share == 1;
+    const int part = share > 1;
     Scans a = scans_of(p);
     int n = 0;
-    if (p.gq) a.s[n++] = Scan{p.go, p.v, p.k, 1, share, share, p.gq, p.state, nullptr, seg[0], V, K, 1, 0, c};
-    const Scan of_k{p.v, p.go, p.q, share, 1, 1, own ? p.gk : part_k, p.gstate_out, nullptr, seg[1], V, K, 1, 1, c};
-    const Scan of_v{p.k, p.q, p.go, share, 1, 1, !p.gv ? nullptr : own ? p.gv : part_v, p.gstate_out, p.gstate, seg[2], K, V, 0, 1, c};
-    if (own && p.gk) a.s[n++] = of_k;
-    if (own && (p.gv || p.gstate)) a.s[n++] = of_v;
-    launch_scans<T, T>(a, n, cut, vec, st);
-    if (own) return;
-    n = 0;
-    if (p.gk) a.s[n++] = of_k;
-    if (p.gv || p.gstate) a.s[n++] = of_v;
-    launch_scans<T, float>(a, n, cut, vec, st);
-    const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads;
-    if (rows && p.gk) k_share<T><<<(unsigned)((rows * K + 255) / 256), 256, 0, st>>>(part_k, (T*)p.gk, share, K, rows * K);
-    if (rows && p.gv) k_share<T><<<(unsigned)((rows * V + 255) / 256), 256, 0, st>>>(part_v, (T*)p.gv, share, V, rows * V);
+    if (p.gq) a.s[n++] = Scan{p.go, p.v, p.k, 1, share, share, p.gq, p.state, nullptr, seg[0], V, K, 1, 0, 0, c};
+    if (p.gk) a.s[n++] = Scan{p.v, p.go, p.q, share, 1, 1, part ? part_k : p.gk, p.gstate_out, nullptr, seg[1], V, K, 1, 1, part, c};
+    if (p.gv || p.gstate)
+        a.s[n++] = Scan{p.k, p.q, p.go, share, 1, 1, part && p.gv ? part_v : p.gv, p.gstate_out, p.gstate, seg[2], K, V, 0, 1, part, c};
+    launch_scans<T>(a, n, cut, wide_rows(p, true), st);
+    if (!part) return;
+    const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads, nk = p.gk ? rows * K : 0, nv = p.gv ? rows * V : 0;
+    const unsigned bk = (unsigned)((nk + 255) / 256), bv = (unsigned)((nv + 255) / 256);
+    if (bk + bv) k_share<T><<<bk + bv, 256, 0, st>>>(part_k, (T*)p.gk, K, nk, bk, part_v, (T*)p.gv, V, nv, share);
 }
 
 #ifndef STEPCB
