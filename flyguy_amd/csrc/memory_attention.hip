@@ -32,6 +32,7 @@ struct Scans {
     const void* starts;
     long long n_moments, L;              // L: moments per segment (a multiple of CHUNK_MAX)
     int wide, heads, n_seq, nseg, slots; // slots of segments: n_seq x nseg, or an upper bound for packed stretches
+    int joined;                          // the segments' start states are there (k_scan_join)
 };
 
 // the moments of stretch n: [first, first + count) of the views
@@ -304,26 +305,35 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
     // the column of lane c in block t; a lane's outputs are then side by side
     auto col_of = [&](int t, int m) { return w0 + (NT == 2 ? 8 * (m >> 2) + 4 * t + (m & 3) : m); };
-    const float* z0 = !OUT ? nullptr : s.seg ? s.seg + ((size_t)slot * a.heads + h) * s.K * s.N : s.init ? s.init + at : nullptr;
     {
-        const bool flip = !s.seg && s.transposed;
-        const int zk = flip ? 1 : s.N, zc = flip ? s.K : 1;
-        const Keep once(!s.seg && !s.backwards && count ? ld : 0.f);      // (no moments: the state goes through as it is)
+        // the start state: the segment's where k_scan_join has left it, else the stretch's, decayed once where the scan goes
+        // forwards (not at all if there are no moments: it goes through as it is), joined with the segments' own before this one
+        const size_t step = (size_t)a.heads * s.K * s.N, mine = ((size_t)slot * a.heads + h) * s.K * s.N;
+        const bool ready = a.nseg > 1 && a.joined, flip = !ready && s.transposed;
+        const float* z0 = !OUT ? nullptr : ready ? s.seg + mine : s.init ? s.init + at : nullptr;
+        const int zk = flip ? 1 : s.N, zc = flip ? s.K : 1, before = OUT && a.nseg > 1 && !a.joined ? seg : 0;
+        const Keep once(!ready && !s.backwards && count ? ld : 0.f), over(ld * (float)a.L);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) z[b][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (!z0) continue;
-            const int col = col_of(t, c);
-            const float* p = z0 + min(col, s.N - 1) * zc;
+            const int col = min(col_of(t, c), s.N - 1);   // (what a lane without a row or column reads is dropped below)
+            if (z0)
+#pragma unroll
+                for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[b][t][r] = once(z0[min(row_of(b, r), s.K - 1) * zk + col * zc]);
+            for (int i = 0; i < before; ++i) {
+                const float* own = s.seg + mine - (size_t)(before - i) * step + col;
+#pragma unroll
+                for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z[b][t][r] = over(z[b][t][r]) + own[min(row_of(b, r), s.K - 1) * s.N];
+            }
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) z[b][t][r] = p[min(row_of(b, r), s.K - 1) * zk];
-#pragma unroll
-            for (int b = 0; b < 2 * KT; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) z[b][t][r] = row_of(b, r) < s.K && col < s.N ? once(z[b][t][r]) : 0.f;
+                for (int r = 0; r < 4; ++r) z[b][t][r] = row_of(b, r) < s.K && col_of(t, c) < s.N ? z[b][t][r] : 0.f;
         }
     }
 
@@ -645,29 +655,36 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
     }
 }
 
-// Segments' start states from their own: Z_0 = the stretch's, Z_{s+1} = l^L Z_s + own_s, in place.
-// grid (blocks of values x heads, stretches, scans)
+// Segments' start states from their own: Z_0 = the stretch's, Z_{s+1} = l^L Z_s + own_s, in place; 4 values a lane (K x N a
+// multiple of 4) or one.  grid (blocks of values x heads, stretches, scans)
+template <int V>
 __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
+    typedef float vec __attribute__((ext_vector_type(V)));
     const Scan& s = a.s[blockIdx.z];
-    const int h = blockIdx.x % a.heads, n = blockIdx.y, i = blockIdx.x / a.heads * 256 + threadIdx.x;
+    const int h = blockIdx.x % a.heads, n = blockIdx.y, i = (blockIdx.x / a.heads * 256 + threadIdx.x) * V;
     if (i >= s.K * s.N) return;
     long long first, count;
     stretch_of(a, n, first, count);
     const float ld = fmaxf(a.log_decay[h], -1e30f);
     const Keep once(count ? ld : 0.f), keep(ld * (float)a.L);    // (no moments: the state goes through as it is)
-    float z = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, i / s.N, i % s.N, once);
-    float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
+    vec z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z[j] = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, (i + j) / s.N, (i + j) % s.N, once);
     const size_t step = (size_t)a.heads * s.K * s.N;
+    float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
     // (8 segments' states under way at once)
     for (long long from = 0; from < count || from == 0; from += 8 * a.L, p += 8 * step) {
-        float own[8];
+        vec own[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) own[j] = from + (j + 1) * a.L < count ? p[j * step] : 0.f;
+        for (int j = 0; j < 8; ++j)
+            if (from + (j + 1) * a.L < count) own[j] = *reinterpret_cast<const vec*>(p + j * step);
+            else own[j] = (vec)0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (j && from + j * a.L >= count) return;
-            p[j * step] = z;
-            z = keep(z) + own[j];
+            *reinterpret_cast<vec*>(p + j * step) = z;
+#pragma unroll
+            for (int e = 0; e < V; ++e) z[e] = keep(z[e]) + own[j][e];
         }
     }
 }
@@ -802,15 +819,20 @@ int groups_per_cu(int K, int N) {
 // workgroup 1.5 chunks to begin and end.  More than one segment a stretch cost a pass for their own states (0.45 of the main
 // one) and one to join them.  A packed stretch is taken to be the middle length, the longest twice that.
 struct Cut {
-    int nseg, slots, K, N;
+    int nseg, slots, K, N, joined;
     long long L;
 };
+#ifndef JOINF
+#define JOINF 8
+#endif
+constexpr int JOIN_FROM = JOINF;
 Cut cut_of(const fm_attention_args& p, int scans) {
     Cut c;
     const int widest = (int)(p.k_dim > p.v_dim ? p.k_dim : p.v_dim);
     c.K = scans == 1 ? (int)p.k_dim : widest;             // (a gradient's scans have them both ways round)
     c.N = scans == 1 ? (int)p.v_dim : widest;
     c.nseg = 1;
+    c.joined = 0;
     c.slots = (int)p.n_seq;
     c.L = (p.n_moments + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
     if (!c.L) c.L = CHUNK_MAX;
@@ -846,6 +868,7 @@ Cut cut_of(const fm_attention_args& p, int scans) {
         if (L == CHUNK_MAX) break;
     }
     if (c.nseg == 1) return c;
+    c.joined = c.nseg >= JOIN_FROM;
     c.nseg = (int)((p.n_moments + c.L - 1) / c.L);
     c.slots = p.starts ? (int)(p.n_moments / c.L + p.n_seq) : (int)p.n_seq * c.nseg;
     return c;
@@ -862,7 +885,9 @@ void launch_form(Scans& a, int count, hipStream_t st) {
     const dim3 grid(a.slots, a.heads, count);
     if (a.nseg > 1) {
         k_scan<T, KT, NT, 4, VEC, false><<<grid, 256, 0, st>>>(a);
-        k_scan_join<<<dim3((most + 255) / 256 * a.heads, a.n_seq, count), 256, 0, st>>>(a);
+        auto blocks = [&](int v) { return dim3((most / v + 255) / 256 * a.heads, a.n_seq, count); };
+        if (a.joined && most % 4 == 0) k_scan_join<4><<<blocks(4), 256, 0, st>>>(a);
+        else if (a.joined) k_scan_join<1><<<blocks(1), 256, 0, st>>>(a);
     }
     k_scan<T, KT, NT, 4, VEC, true><<<grid, 256, 0, st>>>(a);
 }
@@ -878,6 +903,7 @@ void launch_scans(Scans& a, int count, const Cut& cut, bool vec, hipStream_t st)
     a.L = cut.L;
     a.nseg = cut.nseg;
     a.slots = cut.slots;
+    a.joined = cut.joined;
     vec ? launch_sized<T, true>(a, count, cut, st) : launch_sized<T, false>(a, count, cut, st);
 }
 

@@ -230,8 +230,16 @@ class _Stretches:
                                self.k_heads, self.K, self.V, self.type, self.scale)
 
     def workspace(self, q, k, v, backward: bool, **given) -> torch.Tensor | None:
-        n = lib().fm_attention_workspace(self.pack(q, k, v, **given), int(backward))
-        return torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        sizes = (self.starts is None, self.n, self.moments, self.q_heads, self.k_heads, self.K, self.V, self.type, backward)
+        n = _workspaces.get(sizes)
+        if n is None:
+            if len(_workspaces) >= 4096:
+                _workspaces.clear()
+            n = _workspaces[sizes] = lib().fm_attention_workspace(self.pack(q, k, v, **given), int(backward))
+        return q.new_empty(n, dtype=torch.uint8) if n else None
+
+
+_workspaces: dict = {}                  # bytes by sizes: the library's answer depends on nothing else
 
 
 def _attend(p: _Stretches, q, k, v, state):
