@@ -522,3 +522,48 @@ def test_in_a_graph(gpu_lib):
         want = decide(eager)
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]) and torch.equal(s, eager)
+
+
+# ------------------------------------------------------------------------------------------------ the actor that remembers
+def test_memory_actor_on_the_gpu(gpu_lib):
+    """MemoryActor through the library against its CPU form: logits, state and every gradient, to the bars of the actor's own
+    tests (1e-5 and 1e-4 of the largest entry, the latter for what passes float32 norms and sums on both sides); and a
+    stretch played moment by moment."""
+    import copy
+
+    from conftest import lively, toy
+    from flyguy_amd.fly import FlyActor
+    from flyguy_amd.memory import MemoryActor
+    from gpu_helpers import rel
+    torch.manual_seed(3)
+    f = lively(FlyActor(toy("b"), 517, 90, hops=3), 3)
+    f.kernel = "hip"
+    m = MemoryActor(f, heads=4, k_heads=2, dim=24, positions=128)
+    with torch.no_grad():
+        m.back.weight.normal_(0, 0.3)
+    x, R = torch.randn(3, 75, 517), torch.randn(3, 75, 90)
+    g = copy.deepcopy(m).cuda()
+    out, (mem, seen) = g(x.cuda())
+    (out * R.cuda()).sum().backward()
+    want, (want_mem, _) = m(x)
+    (want * R).sum().backward()
+    assert rel(out.detach().cpu(), want.detach()) <= 1e-4 and rel(mem.detach().cpu(), want_mem.detach()) <= 1e-4
+    for (name, p), (_, q) in zip(g.named_parameters(), m.named_parameters()):
+        assert p.grad is not None and rel(p.grad.cpu(), q.grad) <= 1e-4, name
+    live = g.state(3)
+    played = torch.stack([g.step(x[:, t].cuda(), live) for t in range(75)], 1)
+    assert rel(played.cpu(), out.detach().cpu()) <= 1e-4 and live[1].tolist() == [75] * 3
+
+
+def test_the_teaching_command_on_the_gpu(gpu_lib, tmp_path, capsys):
+    import numpy as np
+
+    from conftest import GOLDEN
+    from flyguy_amd.remember import main
+    from oracle import trainer as ot
+    rng = np.random.default_rng(4)
+    ot.write_chunk(tmp_path / "game.bin", rng.standard_normal((300, 517)).astype(np.float16),
+                   (3 * rng.standard_normal((300, 90))).astype(np.float16))
+    assert main(["--data", str(tmp_path / "game.bin"), "--graph", str(GOLDEN / "toy_a.npz"), "--stretch", "100", "--cars", "8",
+                 "--steps", "20", "--out", str(tmp_path / "m.pt")]) == 0
+    assert "first choice the same in" in capsys.readouterr().out

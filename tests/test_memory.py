@@ -1,0 +1,97 @@
+"""The actor that remembers (flyguy_amd.memory.MemoryActor) and its teaching command, on the CPU: a fresh one decides as its
+actor, a stretch in pieces or moment by moment is the stretch at once, nothing reaches an earlier moment, and a memory can be
+taught what no single moment shows."""
+from __future__ import annotations
+
+import re
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import GOLDEN, lively, toy
+from flyguy_amd.fly import FlyActor
+from flyguy_amd.memory import MemoryActor
+from flyguy_amd.remember import main
+from oracle import trainer as ot
+
+
+def net(**kw):
+    torch.manual_seed(1)
+    f = lively(FlyActor(toy("a"), 517, 90, hops=3), 1)
+    m = MemoryActor(f, **(dict(heads=4, k_heads=2, dim=16, positions=64) | kw))
+    with torch.no_grad():
+        m.back.weight.normal_(0, 0.3)
+    return m
+
+
+def test_a_fresh_memory_changes_nothing():
+    m = net()
+    torch.nn.init.zeros_(m.back.weight)
+    x = torch.randn(2, 7, 517)
+    with torch.no_grad():
+        want = m.actor(x.flatten(0, 1)).unflatten(0, (2, 7))
+        torch.testing.assert_close(m(x)[0], want, rtol=1e-5, atol=1e-5)
+
+
+def test_pieces_and_single_moments():
+    m = net()
+    x = torch.randn(3, 20, 517)
+    with torch.no_grad():
+        whole, (mem, seen) = m(x)
+        a, st = m(x[:, :8])
+        b, (mem2, seen2) = m(x[:, 8:], st)
+        live = m.state(3)
+        played = torch.stack([m.step(x[:, t], live) for t in range(20)], 1)
+    torch.testing.assert_close(torch.cat([a, b], 1), whole, rtol=1e-4, atol=1e-4)
+    torch.testing.assert_close(played, whole, rtol=1e-4, atol=1e-4)
+    torch.testing.assert_close(mem2, mem, rtol=1e-4, atol=1e-4)
+    torch.testing.assert_close(live[0], mem, rtol=1e-4, atol=1e-4)
+    assert seen.tolist() == seen2.tolist() == live[1].tolist() == [20] * 3
+
+
+def test_only_what_was_seen_counts():
+    m = net()
+    x = torch.randn(1, 12, 517)
+    y = x.clone()
+    y[:, 9:] = torch.randn(1, 3, 517)
+    with torch.no_grad():
+        a, b = m(x)[0], m(y)[0]
+    torch.testing.assert_close(a[:, :9], b[:, :9], rtol=1e-5, atol=1e-5)
+    assert (a[:, 9:] - b[:, 9:]).abs().max() > 1e-3
+
+
+def test_heads_must_share():
+    with pytest.raises(ValueError, match="multiple"):
+        net(heads=4, k_heads=3)
+
+
+def test_teaching_a_memory(tmp_path, capsys):
+    """Answers that depend on the moment before: with a memory the distance falls."""
+    rng = np.random.default_rng(4)
+    obs = rng.standard_normal((400, 517)).astype(np.float16)
+    ans = np.zeros((400, 90), np.float16)
+    side = np.concatenate([[False], obs[:-1, 0] > 0])
+    ans[side, 3], ans[~side, 7] = 6, 6
+    data = tmp_path / "game.bin"
+    ot.write_chunk(data, obs, ans)
+    torch.manual_seed(5)
+    f = lively(FlyActor(toy("a"), 517, 90, hops=3), 5)
+    ck = tmp_path / "actor.pt"
+    torch.save({"model": {"actor." + k: v for k, v in f.state_dict().items()}}, ck)
+    out = tmp_path / "memory.pt"
+    assert main(["--data", str(data), "--graph", str(GOLDEN / "toy_a.npz"), "--start", str(ck), "--stretch", "24", "--cars", "4",
+                 "--steps", "40", "--heads", "2", "--dim", "8", "--lr", "1e-2", "--device", "cpu", "--out", str(out)]) == 0
+    text = capsys.readouterr().out
+    first, last = (float(v) for v in re.search(r"KL ([0-9.]+) -> ([0-9.]+)", text).groups())
+    assert last < 0.7 * first
+    assert float(re.search(r"off by ([0-9.e+-]+)", text).group(1)) <= 1e-4
+    saved = torch.load(out, weights_only=True)
+    assert set(saved["memory"]) == {"proj.weight", "wq", "wk", "back.weight", "log_decay"}
+
+
+def test_too_short_a_recording(tmp_path):
+    data = tmp_path / "game.bin"
+    ot.write_chunk(data, np.zeros((5, 517), np.float16), np.zeros((5, 90), np.float16))
+    with pytest.raises(SystemExit, match="no file holds"):
+        main(["--data", str(data), "--graph", str(GOLDEN / "toy_a.npz"), "--device", "cpu"])
