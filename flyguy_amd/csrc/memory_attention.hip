@@ -672,15 +672,15 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     for (int j = 0; j < V; ++j) z[j] = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, (i + j) / s.N, (i + j) % s.N, once);
     const size_t step = (size_t)a.heads * s.K * s.N;
     float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
-    // (8 segments' states under way at once)
-    for (long long from = 0; from < count || from == 0; from += 8 * a.L, p += 8 * step) {
-        vec own[8];
+    constexpr int AHEAD = 16;                             // segments' states under way at once
+    for (long long from = 0; from < count || from == 0; from += AHEAD * a.L, p += AHEAD * step) {
+        vec own[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < AHEAD; ++j)
             if (from + (j + 1) * a.L < count) own[j] = *reinterpret_cast<const vec*>(p + j * step);
             else own[j] = (vec)0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < AHEAD; ++j) {
             if (j && from + j * a.L >= count) return;
             *reinterpret_cast<vec*>(p + j * step) = z;
 #pragma unroll
@@ -822,10 +822,10 @@ struct Cut {
     int nseg, slots, K, N, joined;
     long long L;
 };
-#ifndef JOINF
-#define JOINF 8
-#endif
-constexpr int JOIN_FROM = JOINF;
+// From this many values of a chain's segments up they are joined by a kernel of its own; fewer, each segment of the main pass
+// joins those before it as it begins (a launch less; 4 segments of 64 x 64: 143 us a learning step against 149 with the
+// kernel, 4 of 128 x 128: 786 against 776).
+constexpr int JOIN_FROM = 65536;
 Cut cut_of(const fm_attention_args& p, int scans) {
     Cut c;
     const int widest = (int)(p.k_dim > p.v_dim ? p.k_dim : p.v_dim);
@@ -868,7 +868,7 @@ Cut cut_of(const fm_attention_args& p, int scans) {
         if (L == CHUNK_MAX) break;
     }
     if (c.nseg == 1) return c;
-    c.joined = c.nseg >= JOIN_FROM;
+    c.joined = (long long)c.nseg * c.K * c.N >= JOIN_FROM;
     c.nseg = (int)((p.n_moments + c.L - 1) / c.L);
     c.slots = p.starts ? (int)(p.n_moments / c.L + p.n_seq) : (int)p.n_seq * c.nseg;
     return c;

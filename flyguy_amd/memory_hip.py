@@ -60,13 +60,19 @@ def rotary_table(positions: int, dim: int, base: float = 10000.0, scaling: str =
 
 
 # ------------------------------------------------------------------------------------------------ calls
+_functions: dict = {}
+
+
 def _call(name: str, x: torch.Tensor, args: bytes) -> None:
     """The call on x's device and its current stream."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(lib(), name)
     dev = x.get_device()
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _call(name, x, args)
-    if getattr(lib(), name)(args, torch._C._cuda_getCurrentRawStream(dev)):
+    if fn(args, torch._C._cuda_getCurrentRawStream(dev)):
         check(name)
         raise LibraryError(f"{name} failed")
 
@@ -80,22 +86,22 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _heads(what: str, like: torch.Tensor | None, dims: int, **tensors) -> None:
+def _heads(what: str, dims: int, *tensors) -> None:
     """Every tensor on one GPU, of one type and `dims` dimensions."""
-    for name, x in tensors.items():
+    first = tensors[0]
+    for i, x in enumerate(tensors):
         if not isinstance(x, torch.Tensor) or not x.is_cuda:
-            raise ValueError(f"{what}: {name} must be a tensor on the GPU")
+            raise ValueError(f"{what}: {'qkv'[i]} must be a tensor on the GPU")
         if x.dtype not in _TYPES or x.dim() != dims:
-            raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16 of {dims} dimensions")
-        like = x if like is None else like
-        if x.dtype != like.dtype or x.device != like.device:
-            raise ValueError(f"{what}: {name} is of another type or on another device")
+            raise ValueError(f"{what}: {'qkv'[i]} must be float32, bfloat16 or float16 of {dims} dimensions")
+        if x.dtype != first.dtype or x.device != first.device:
+            raise ValueError(f"{what}: {'qkv'[i]} is of another type or on another device")
 
 
 def _floats(what: str, name: str, x, shape: tuple, device) -> torch.Tensor:
-    if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != device or tuple(x.shape) != shape:
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != device or x.shape != shape:
         raise ValueError(f"{what}: {name} must be float32 {list(shape)} on the same GPU")
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _wants_grad(*tensors) -> bool:
@@ -107,6 +113,10 @@ _NONE = (0, 0, 0, 0)
 
 def _view4(x: torch.Tensor | None) -> tuple:
     return _NONE if x is None else (x.data_ptr(), *x.stride()[:3])
+
+
+def _view3(x: torch.Tensor | None) -> tuple:
+    return _NONE if x is None else (x.data_ptr(), 0, *x.stride()[:2])
 
 
 # ------------------------------------------------------------------------------------------------ rotation and norm
@@ -122,7 +132,7 @@ class _Plan:
 
 
 def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
-    _heads(what, None, 4, q=q) if k is None else _heads(what, None, 4, q=q, k=k)
+    _heads(what, 4, q) if k is None else _heads(what, 4, q, k)
     N, T, H, D = q.shape
     if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != D):
         raise ValueError(f"{what}: q and k must be of the same stretches, moments and values per head")
@@ -134,7 +144,7 @@ def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
         if not isinstance(table, torch.Tensor) or table.dim() != 3 or table.shape[2] != 2 or \
                 table.dtype != torch.float32 or table.device != q.device:
             raise ValueError(f"{what}: the table must be float32 [positions, rotated / 2, 2] on the same GPU (rotary_table)")
-        table = table.detach().contiguous()
+        table = table if table.is_contiguous() else table.contiguous()
         p.rotated = 2 * table.shape[1]
         if p.rotated > D:
             raise ValueError(f"{what}: the table turns more values than a head has")
@@ -144,7 +154,7 @@ def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
                 positions.dim() < 1:
             raise ValueError(f"{what}: positions must be int32 or int64 [moments] or [stretches, moments] on the same GPU")
         try:
-            p.positions = positions.expand(N, T)
+            p.positions = positions if positions.shape == (N, T) else positions.expand(N, T)
         except RuntimeError:
             raise ValueError(f"{what}: positions do not fit [stretches, moments]") from None
         p.pos = (*p.positions.stride(), 0, int(positions.dtype == torch.int64))
@@ -157,7 +167,7 @@ def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
 
 def _turn(p: _Plan, q, k, wq, wk):
     q, k = _rows(q), None if k is None else _rows(k)
-    yq, yk = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
+    yq, yk = torch.empty_like(q), None if k is None else torch.empty_like(k)
     _call("fm_turn", q, p.pack((q, k), (yq, yk), (None, None), (wq, wk), (None, None), None))
     return yq, yk
 
@@ -177,7 +187,7 @@ class TurnHip(torch.autograd.Function):
         p = ctx.p
         q, k, gq = None if q is None else _rows(q), None if k is None else _rows(k), _rows(gq)
         gk = None if not p.heads[1] else _rows(gk)
-        yq, yk = gq.new_empty(gq.shape), None if gk is None else gk.new_empty(gk.shape)
+        yq, yk = torch.empty_like(gq), None if gk is None else torch.empty_like(gk)
         gwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         gwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
         partial = None
@@ -191,7 +201,7 @@ def rotary(q, k, table, positions=None, interleaved: bool = False):
     """q and k (k may be None) turned by their positions: the pairs of the first 2 table.shape[1] values of each head, (i,
     i + half) or, interleaved, (2i, 2i + 1); the rest passes through.  positions: int32 / int64 tensor [moments] or
     [stretches, moments], the first moment's position (an int), or None for 0, 1, ...  A position outside the table gives
-    NaN.  Returns the turned (q, k), dense."""
+    NaN.  Returns the turned (q, k), without gaps."""
     if table is None:
         raise ValueError("rotary: no table")
     p = _plan("rotary", q, k, table, positions, interleaved, 0.0)
@@ -216,21 +226,18 @@ def norm_rotary(q, k, wq, wk, table=None, positions=None, interleaved: bool = Fa
 
 # ------------------------------------------------------------------------------------------------ linear attention
 class _Stretches:
-    __slots__ = ("starts", "wide", "n", "moments", "q_heads", "k_heads", "K", "V", "type", "scale", "log_decay")
+    __slots__ = ("starts", "sizes", "state", "V", "scale", "log_decay")
 
     def pack(self, q, k, v, go=None, state=None, o=None, state_out=None, gstate_out=None, gq=None, gk=None, gv=None,
              gstate=None, work=None) -> bytes:
-        views = []
-        for x in (q, k, v, go):
-            s = (0, 0, 0) if x is None else x.stride()[:-1]
-            views += [_ptr(x), *(s if len(s) == 3 else (0, *s))]
-        return _ATTENTION.pack(*views, _ptr(self.log_decay), _ptr(state), _ptr(self.starts), _ptr(o), _ptr(state_out),
-                               _ptr(gstate_out), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(gstate), _ptr(work),
-                               0 if work is None else work.numel(), self.wide, self.n, self.moments, self.q_heads,
-                               self.k_heads, self.K, self.V, self.type, self.scale)
+        vq, vk, vv, vg = (_view4(q), _view4(k), _view4(v), _view4(go)) if self.starts is None else \
+            (_view3(q), _view3(k), _view3(v), _view3(go))
+        return _ATTENTION.pack(*vq, *vk, *vv, *vg, _ptr(self.log_decay), _ptr(state), _ptr(self.starts), _ptr(o),
+                               _ptr(state_out), _ptr(gstate_out), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(gstate), _ptr(work),
+                               0 if work is None else work.numel(), *self.sizes, self.scale)
 
     def workspace(self, q, k, v, backward: bool, **given) -> torch.Tensor | None:
-        sizes = (self.starts is None, self.n, self.moments, self.q_heads, self.k_heads, self.K, self.V, self.type, backward)
+        sizes = (self.starts is None, backward, *self.sizes)
         n = _workspaces.get(sizes)
         if n is None:
             if len(_workspaces) >= 4096:
@@ -245,7 +252,7 @@ _workspaces: dict = {}                  # bytes by sizes: the library's answer d
 def _attend(p: _Stretches, q, k, v, state):
     q, k, v = _rows(q), _rows(k), _rows(v)
     o = q.new_empty((*q.shape[:-1], p.V))
-    state_out = p.log_decay.new_empty((p.n, p.q_heads, p.K, p.V))
+    state_out = p.log_decay.new_empty(p.state)
     work = p.workspace(q, k, v, False)
     _call("fm_attention", q, p.pack(q, k, v, state=state, o=o, state_out=state_out, work=work))
     return o, state_out
@@ -302,23 +309,26 @@ def decay_attention(q, k, v, log_decay, state=None, starts=None, scale: float | 
     Returns (o in q's type, the state after each stretch).  Gradients of q, k, v and state; the decays are fixed."""
     what = "decay_attention"
     dims = 4 if starts is None else 3
-    _heads(what, None, dims, q=q, k=k, v=v)
+    _heads(what, dims, q, k, v)
     _shared(what, q, k, v, dims - 2)
     p = _Stretches()
-    p.starts, p.wide = None, 0
+    p.starts, wide = None, 0
     if starts is None:
-        p.n, p.moments = q.shape[:2]
+        n, moments = q.shape[:2]
     else:
         if not isinstance(starts, torch.Tensor) or starts.dtype not in (torch.int32, torch.int64) or starts.dim() != 1 or \
                 starts.numel() < 1 or starts.device != q.device:
             raise ValueError(f"{what}: starts must be int32 or int64 [stretches + 1] on the same GPU")
-        p.starts, p.wide = starts.contiguous(), int(starts.dtype == torch.int64)
-        p.n, p.moments = starts.numel() - 1, q.shape[0]
-    p.q_heads, p.k_heads, p.K, p.V = q.shape[-2], k.shape[-2], q.shape[-1], v.shape[-1]
-    p.type, p.scale = _TYPES[q.dtype], float(p.K ** -0.5 if scale is None else scale)
-    p.log_decay = _decays(what, log_decay, p.q_heads, q.device)
+        p.starts, wide = starts.contiguous(), int(starts.dtype == torch.int64)
+        n, moments = starts.numel() - 1, q.shape[0]
+    H, K = q.shape[-2:]
+    p.V = v.shape[-1]
+    p.state = (n, H, K, p.V)
+    p.sizes = (wide, n, moments, H, k.shape[-2], K, p.V, _TYPES[q.dtype])
+    p.scale = float(K ** -0.5 if scale is None else scale)
+    p.log_decay = _decays(what, log_decay, H, q.device)
     if state is not None:
-        state = _floats(what, "state", state, (p.n, p.q_heads, p.K, p.V), q.device)
+        state = _floats(what, "state", state, p.state, q.device)
     if _wants_grad(q, k, v, state):
         return DecayHip.apply(q, k, v, state, p)
     return _attend(p, q, k, v, state)
@@ -331,7 +341,7 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
     number; below 0: the row is idle (zeros, no state touched); past the states: NaN, no state touched.  No two rows of a
     call may name one slot.  No gradients."""
     what = "decay_step"
-    _heads(what, None, 3, q=q, k=k, v=v)
+    _heads(what, 3, q, k, v)
     _shared(what, q, k, v, 1)
     if _wants_grad(q, k, v, state):
         raise ValueError(f"{what}: has no gradients; decay_attention has")
