@@ -30,55 +30,83 @@ __device__ __forceinline__ const float* table_line(const fm_turn_args& a, long l
     return p >= 0 && p < a.n_positions ? a.table + p * a.rotated : nullptr;
 }
 
-// Heads of whole 16-byte units (V values), turned ones in whole units: a group of `lanes` lanes (a power of two) takes HB
-// heads of a moment; lane j holds two units of a head, such that its pairs are its own: units j and j + R / 2V of the turned
-// part where pairs lie half apart, units 2j and 2j + 1 where they lie side by side; the rest goes two units a lane.  The
-// lane's V angles, the weights and the moment's addresses serve all HB heads, and all their loads are under way at once.
+// Heads of whole 16-byte units (V values): a group of `lanes` lanes (a power of two) takes HB heads of a moment; lane j holds
+// two units of a head.  Where pairs lie half apart and the turned part is whole units, units j and j + R / 2V of it, so that the
+// lane's pairs are its own (HALVES; the rest goes two units a lane); side by side, units 2j and 2j + 1 (SIDE).  Half apart at
+// any place (SPREAD), units 2j and 2j + 1 too, and partners pass through LDS inside the group: 27 us instead of the 62 of a
+// wave per row at 8 x 981 moments of 16 float32 heads of 128 values, 106 of them turned.  The lane's angles, the weights and
+// the moment's addresses serve all HB heads, and all their loads are under way at once.
+enum Pairs { HALVES, SIDE, SPREAD };
 struct Lanes {
     int lanes, shift, q_chunks, chunks;  // lanes = 1 << shift; chunks of HB heads of queries, in all
 };
-template <class T, bool IL>
+template <class T, Pairs P>
 struct Units {
-    static constexpr int V = Vec<T>::N;
-    int a, b;                            // first values of the lane's units (b: dim or more: none)
-    bool ta, tb;                         // turned?
-    float c[V], s[V];
-    __device__ __forceinline__ Units(int j, int D, int R) {
-        const int ru = IL ? 0 : R / (2 * V);
-        a = IL ? 2 * j * V : j < ru ? j * V : (2 * j) * V;
-        b = IL ? a + V : j < ru ? (j + ru) * V : a + V;
-        ta = a < R;
-        tb = b < R;
+    static constexpr int V = Vec<T>::N, ANGLES = P == SPREAD ? 2 * V : V;
+    int a, b, R;                         // first values of the lane's units (b: dim or more: none); values turned
+    float c[ANGLES], s[ANGLES];
+    __device__ __forceinline__ Units(int j, int D, int turned) : R(turned) {
+        const int ru = R / (2 * V);
+        a = P == HALVES && j < ru ? j * V : 2 * j * V;
+        b = P == HALVES && j < ru ? (j + ru) * V : a + V;
     }
     __device__ __forceinline__ void angles(const float* cs, int j, float sign) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const bool t = IL ? (i < V / 2 ? ta : tb) : ta;
-            if (!t) continue;
-            const float2 f = cs ? reinterpret_cast<const float2*>(cs)[j * V + i] : make_float2(NAN, NAN);
+        for (int i = 0; i < ANGLES; ++i) {
+            const int e = a + i, second = P == SPREAD && e >= R / 2;           // SPREAD: of value e
+            const int pair = P == SPREAD ? (second ? e - R / 2 : e) : j * V + i;
+            if (P == SPREAD ? e >= R : P == SIDE && i >= V / 2 ? b >= R : a >= R) continue;
+            const float2 f = cs ? reinterpret_cast<const float2*>(cs)[P == SIDE ? min(pair, R / 2 - 1) : pair] : make_float2(NAN, NAN);
             c[i] = f.x;
-            s[i] = sign * f.y;
+            s[i] = P == SPREAD && !second ? -sign * f.y : sign * f.y;
         }
     }
-    // x, y: the values of units a, b (one that is not turned is not touched: its values may be anything)
-    __device__ __forceinline__ void turn(float (&x)[V], float (&y)[V]) const {
-        if constexpr (IL) {
-            if (ta) side_by_side(x, 0);
-            if (tb) side_by_side(y, V / 2);
-        } else if (ta)
+    // x, y: the values of units a, b (one that is not turned is not touched: it may be anything); row: the group's 2V floats a
+    // lane of LDS (SPREAD)
+    __device__ __forceinline__ void turn(float (&x)[V], float (&y)[V], float* row) const {
+        if constexpr (P == SIDE) {
+            side_by_side(x, a, 0);
+            side_by_side(y, b, V / 2);
+        } else if constexpr (P == HALVES) {
+            if (a < R)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float p = x[i], q = y[i];
+                    x[i] = p * c[i] - q * s[i];
+                    y[i] = q * c[i] + p * s[i];
+                }
+        } else {
+            // (one wave's LDS operations go in order: the compiler only has to leave them so)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float p = x[i], q = y[i];
-                x[i] = p * c[i] - q * s[i];
-                y[i] = q * c[i] + p * s[i];
+                row[a + i] = x[i];
+                row[b + i] = y[i];
             }
+            asm volatile("" ::: "memory");
+            partners(x, a, 0, row);
+            partners(y, b, V, row);
+            asm volatile("" ::: "memory");
+        }
     }
-    __device__ __forceinline__ void side_by_side(float (&x)[V], int at) const {
+    __device__ __forceinline__ void side_by_side(float (&x)[V], int first, int at) const {
+        if (first + V <= R) {
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-            const float p = x[2 * i], q = x[2 * i + 1];
-            x[2 * i] = p * c[at + i] - q * s[at + i];
-            x[2 * i + 1] = q * c[at + i] + p * s[at + i];
+            for (int i = 0; i < V / 2; ++i) pair(x, i, at);
+        } else if (first < R)
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i)
+                if (first + 2 * i < R) pair(x, i, at);
+    }
+    __device__ __forceinline__ void pair(float (&x)[V], int i, int at) const {
+        const float p = x[2 * i], q = x[2 * i + 1];
+        x[2 * i] = p * c[at + i] - q * s[at + i];
+        x[2 * i + 1] = q * c[at + i] + p * s[at + i];
+    }
+    __device__ __forceinline__ void partners(float (&x)[V], int first, int at, const float* row) const {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int e = first + i;
+            if (e < R) x[i] = x[i] * c[at + i] + row[e < R / 2 ? e + R / 2 : e - R / 2] * s[at + i];
         }
     }
     __device__ __forceinline__ static void read(const T* p, bool there, typename Vec<T>::type& v) {
@@ -108,10 +136,12 @@ __device__ __forceinline__ void group_sums(float (&v)[HB], int lanes) {
         for (int i = 0; i < HB; ++i) v[i] += __shfl_xor(v[i], m);
 }
 
-template <class T, bool IL, bool NORM, int HB>
+template <class T, Pairs P, bool NORM, int HB>
 __global__ __launch_bounds__(256) void k_turn_units(fm_turn_args a, Lanes l, float sign) {
     constexpr int V = Vec<T>::N;
+    __shared__ float rows[P == SPREAD ? 256 * 2 * V : 1];
     const int D = (int)a.dim, R = (int)a.rotated, j = threadIdx.x & (l.lanes - 1);
+    float* const row = rows + (P == SPREAD ? (threadIdx.x >> l.shift << l.shift) * 2 * V : 0);
     const long long item = (long long)blockIdx.x * (256 >> l.shift) + (threadIdx.x >> l.shift);
     const long long m = item / l.chunks, n = m / a.n_moments, t = m - n * a.n_moments;
     if (n >= a.n_seq) return;                             // (a wave's lanes of other groups go on: sums stay in a group)
@@ -122,7 +152,7 @@ __global__ __launch_bounds__(256) void k_turn_units(fm_turn_args a, Lanes l, flo
     const int h0 = chunk * HB, hn = min(HB, (int)(which ? a.heads[1] : a.heads[0]) - h0);
     const T* x = (const T*)xv.data + n * xv.seq + t * xv.moment + h0 * xv.head;
     T* y = (T*)yv.data + n * yv.seq + t * yv.moment + h0 * yv.head;
-    Units<T, IL> u(j, D, R);
+    Units<T, P> u(j, D, R);
     const bool ha = u.a < D, hb = u.b < D;
     typename Vec<T>::type va[HB], vb[HB];
 #pragma unroll
@@ -158,7 +188,7 @@ __global__ __launch_bounds__(256) void k_turn_units(fm_turn_args a, Lanes l, flo
                 q[e] *= r * wb[e];
             }
         }
-        u.turn(p, q);
+        u.turn(p, q, row);
         u.write(y + i * yv.head + u.a, ha && i < hn, p);
         u.write(y + i * yv.head + u.b, hb && i < hn, q);
     }
@@ -168,16 +198,16 @@ __global__ __launch_bounds__(256) void k_turn_units(fm_turn_args a, Lanes l, flo
 // mean(u xh)).  The weights' gradients sum g' xh over rows: a lane keeps its values' sums over its groups' rows, a
 // workgroup's groups are added in LDS, k_turn_gweight adds the workgroups; always in the same order.
 // partial [queries, keys][dim][blocks].  grid (blocks, queries and keys)
-template <class T, bool IL, int HB>
+template <class T, Pairs P, int HB>
 __global__ __launch_bounds__(256) void k_turn_units_bwd(fm_turn_args a, Lanes l) {
     constexpr int V = Vec<T>::N;
-    __shared__ float shared[256 * 2 * V];                 // [groups][dim]: dim <= lanes x 2V
+    __shared__ float shared[256 * 2 * V];                 // a group's row (SPREAD); then [groups][dim]: dim <= lanes x 2V
     const int D = (int)a.dim, R = (int)a.rotated, j = threadIdx.x & (l.lanes - 1), group = threadIdx.x >> l.shift;
     const int groups = 256 >> l.shift, which = blockIdx.y;
     const fm_view xv = a.x[which], yv = a.y[which], gv = a.g[which];
     const float* w = a.weight[which];
     const int H = (int)a.heads[which], chunks = which ? l.chunks - l.q_chunks : l.q_chunks;
-    Units<T, IL> u(j, D, R);
+    Units<T, P> u(j, D, R);
     const bool ha = u.a < D, hb = u.b < D;
     float wa[V], wb[V], sa[V] = {}, sb[V] = {};
     if (w) {
@@ -210,7 +240,7 @@ __global__ __launch_bounds__(256) void k_turn_units_bwd(fm_turn_args a, Lanes l)
                 p[i][e] = widen(ga[i][e]);
                 q[i][e] = widen(gb[i][e]);
             }
-            u.turn(p[i], q[i]);
+            u.turn(p[i], q[i], shared + (threadIdx.x >> l.shift << l.shift) * 2 * V);
             if (!w) continue;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -241,6 +271,7 @@ __global__ __launch_bounds__(256) void k_turn_units_bwd(fm_turn_args a, Lanes l)
         }
     }
     if (!a.gweight[which]) return;
+    __syncthreads();
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         if (ha) shared[group * D + u.a + e] = sa[e];
@@ -401,7 +432,11 @@ void launch_any(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
     k_turn<T, NE><<<(unsigned)((rows + TURN_ROWS - 1) / TURN_ROWS), 64 * TURN_ROWS, 0, st>>>(a, sign);
 }
 
-template <class T, bool IL, int HB>
+// 4 heads a group: queries and keys of 16 heads of 128 values in bfloat16, 8 x 2048 moments, forward and gradient with a norm:
+// 209 / 178 / 173 / 172 us with 1 / 2 / 4 / 8; turned only, 2 x 16384 moments of 20 heads: 144 / 140 / 144 / 150.  The gradient
+// with SPREAD pairs takes 2, which its registers hold: 280 us of the former (106 values turned), 330 with 1 or 4.
+constexpr int TURN_HEADS = 4, TURN_HEADS_SPREAD = 2;
+template <class T, int HB>
 Lanes lanes_of(const fm_turn_args& a) {
     Lanes l;
     const int units = (int)a.dim / Vec<T>::N;
@@ -411,30 +446,24 @@ Lanes lanes_of(const fm_turn_args& a) {
     l.chunks = l.q_chunks + ((int)a.heads[1] + HB - 1) / HB;
     return l;
 }
-#ifndef HBF
-#define HBF 4
-#define HBG 4
-#endif
-constexpr int HEADS_FWD = HBF, HEADS_BWD = HBG;
-template <class T, bool IL>
+template <class T, Pairs P>
 void launch_units(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
+    constexpr int HB = TURN_HEADS, HG = P == SPREAD ? TURN_HEADS_SPREAD : TURN_HEADS;
     if (grad) {
-        const Lanes l = lanes_of<T, IL, HEADS_BWD>(a);
-        k_turn_units_bwd<T, IL, HEADS_BWD><<<dim3(turn_blocks(a), a.heads[1] ? 2 : 1), 256, 0, st>>>(a, l);
+        k_turn_units_bwd<T, P, HG><<<dim3(turn_blocks(a), a.heads[1] ? 2 : 1), 256, 0, st>>>(a, lanes_of<T, HG>(a));
         return;
     }
-    const Lanes l = lanes_of<T, IL, HEADS_FWD>(a);
+    const Lanes l = lanes_of<T, HB>(a);
     const int groups = 256 >> l.shift;
     const unsigned grid = (unsigned)((a.n_seq * a.n_moments * l.chunks + groups - 1) / groups);
-    if (a.weight[0] || a.weight[1]) k_turn_units<T, IL, true, HEADS_FWD><<<grid, 256, 0, st>>>(a, l, sign);
-    else k_turn_units<T, IL, false, HEADS_FWD><<<grid, 256, 0, st>>>(a, l, sign);
+    if (a.weight[0] || a.weight[1]) k_turn_units<T, P, true, HB><<<grid, 256, 0, st>>>(a, l, sign);
+    else k_turn_units<T, P, false, HB><<<grid, 256, 0, st>>>(a, l, sign);
 }
 
-// heads of whole 16-byte units, all aligned, turned in whole units (k_turn_units), or anything (k_turn)
+// heads of whole 16-byte units, all aligned (k_turn_units), or anything (k_turn)
 template <class T>
 bool in_units(const fm_turn_args& a, bool grad) {
-    constexpr int V = Vec<T>::N;
-    if (a.dim % V || a.rotated % (a.interleaved ? V : 2 * V) || ((uintptr_t)a.table & 7)) return false;
+    if (a.dim % Vec<T>::N || ((uintptr_t)a.table & 7)) return false;
     for (int i = 0; i < 2; ++i)
         if (a.heads[i] && (!aligned16(a.x[i], sizeof(T)) || !aligned16(a.y[i], sizeof(T)) ||
                            (grad && !aligned16(a.g[i], sizeof(T)))))
@@ -445,7 +474,9 @@ bool in_units(const fm_turn_args& a, bool grad) {
 template <class T>
 void turn_of_type(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
     if (in_units<T>(a, grad)) {
-        a.interleaved ? launch_units<T, true>(a, grad, sign, st) : launch_units<T, false>(a, grad, sign, st);
+        if (a.interleaved) launch_units<T, SIDE>(a, grad, sign, st);
+        else if (a.rotated % (2 * Vec<T>::N) == 0) launch_units<T, HALVES>(a, grad, sign, st);
+        else launch_units<T, SPREAD>(a, grad, sign, st);
         return;
     }
     if (a.dim <= 64) launch_any<T, 1>(a, grad, sign, st);

@@ -57,6 +57,13 @@ TURNS = [  # N, T, Hq, Hk, D, R, interleaved, type, layout
     (1, 1, 1, 1, 1, 0, False, F32, "dense"),
     (1, 65, 2, 2, 24, 8, True, BF16, "packed"),
     (1, 65, 2, 2, 40, 16, False, BF16, "packed"),
+    (2, 37, 5, 3, 128, 106, False, F32, "packed"),
+    (1, 130, 9, 1, 128, 34, False, BF16, "packed"),
+    (3, 11, 4, 4, 64, 62, False, F16, "dense"),
+    (1, 9, 3, 2, 512, 298, False, BF16, "dense"),
+    (2, 21, 4, 2, 64, 50, True, BF16, "packed"),
+    (1, 5, 6, 6, 16, 2, False, F32, "dense"),
+    (1, 5, 6, 6, 8, 6, False, BF16, "dense"),
 ]
 
 
