@@ -32,11 +32,11 @@ __device__ __forceinline__ const float* table_line(const fm_turn_args& a, long l
 
 // Heads of whole 16-byte units (V values): a group of `lanes` lanes (a power of two) takes HB heads of a moment; lane j holds
 // two units of a head.  Where pairs lie half apart and the turned part is whole units, units j and j + R / 2V of it, so that the
-// lane's pairs are its own (HALVES; the rest goes two units a lane); side by side, units 2j and 2j + 1 (SIDE).  Half apart at
-// any place (SPREAD), units 2j and 2j + 1 too, and partners pass through LDS inside the group: 27 us instead of the 62 of a
+// lane's pairs are its own (HALVES; the rest goes two units a lane); side by side, units 2j and 2j + 1 (SIDE; SIDE_ANY: the turned
+// part ends inside a unit, which costs the others 5% if they ask for it).  Half apart at any place (SPREAD), units 2j and 2j + 1 too, and partners pass through LDS inside the group: 27 us instead of the 62 of a
 // wave per row at 8 x 981 moments of 16 float32 heads of 128 values, 106 of them turned.  The lane's angles, the weights and
 // the moment's addresses serve all HB heads, and all their loads are under way at once.
-enum Pairs { HALVES, SIDE, SPREAD };
+enum Pairs { HALVES, SIDE, SIDE_ANY, SPREAD };
 struct Lanes {
     int lanes, shift, q_chunks, chunks;  // lanes = 1 << shift; chunks of HB heads of queries, in all
 };
@@ -51,22 +51,41 @@ struct Units {
         b = P == HALVES && j < ru ? (j + ru) * V : a + V;
     }
     __device__ __forceinline__ void angles(const float* cs, int j, float sign) {
+        if (a >= R) return;
+        if constexpr (P == SPREAD) {                      // of value e of the lane's
 #pragma unroll
-        for (int i = 0; i < ANGLES; ++i) {
-            const int e = a + i, second = P == SPREAD && e >= R / 2;           // SPREAD: of value e
-            const int pair = P == SPREAD ? (second ? e - R / 2 : e) : j * V + i;
-            if (P == SPREAD ? e >= R : P == SIDE && i >= V / 2 ? b >= R : a >= R) continue;
-            const float2 f = cs ? reinterpret_cast<const float2*>(cs)[P == SIDE ? min(pair, R / 2 - 1) : pair] : make_float2(NAN, NAN);
-            c[i] = f.x;
-            s[i] = P == SPREAD && !second ? -sign * f.y : sign * f.y;
+            for (int i = 0; i < ANGLES; ++i) {
+                const int e = a + i;
+                const bool second = e >= R / 2;
+                if (e < R) angle(cs, second ? e - R / 2 : e, i, second ? sign : -sign);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (P == HALVES || (P == SIDE ? i < V / 2 || b < R : 2 * (j * V + i) < R)) angle(cs, j * V + i, i, sign);
         }
+    }
+    __device__ __forceinline__ void angle(const float* cs, int pair, int i, float sign) {
+        const float2 f = cs ? reinterpret_cast<const float2*>(cs)[pair] : make_float2(NAN, NAN);
+        c[i] = f.x;
+        s[i] = sign * f.y;
     }
     // x, y: the values of units a, b (one that is not turned is not touched: it may be anything); row: the group's 2V floats a
     // lane of LDS (SPREAD)
     __device__ __forceinline__ void turn(float (&x)[V], float (&y)[V], float* row) const {
         if constexpr (P == SIDE) {
-            side_by_side(x, a, 0);
-            side_by_side(y, b, V / 2);
+            if (a < R)
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) pair(x, i, 0);
+            if (b < R)
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) pair(y, i, V / 2);
+        } else if constexpr (P == SIDE_ANY) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                if (a + 2 * i < R) pair(x, i, 0);
+                if (b + 2 * i < R) pair(y, i, V / 2);
+            }
         } else if constexpr (P == HALVES) {
             if (a < R)
 #pragma unroll
@@ -87,15 +106,6 @@ struct Units {
             partners(y, b, V, row);
             asm volatile("" ::: "memory");
         }
-    }
-    __device__ __forceinline__ void side_by_side(float (&x)[V], int first, int at) const {
-        if (first + V <= R) {
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) pair(x, i, at);
-        } else if (first < R)
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i)
-                if (first + 2 * i < R) pair(x, i, at);
     }
     __device__ __forceinline__ void pair(float (&x)[V], int i, int at) const {
         const float p = x[2 * i], q = x[2 * i + 1];
@@ -474,7 +484,8 @@ bool in_units(const fm_turn_args& a, bool grad) {
 template <class T>
 void turn_of_type(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
     if (in_units<T>(a, grad)) {
-        if (a.interleaved) launch_units<T, SIDE>(a, grad, sign, st);
+        if (a.interleaved && a.rotated % Vec<T>::N == 0) launch_units<T, SIDE>(a, grad, sign, st);
+        else if (a.interleaved) launch_units<T, SIDE_ANY>(a, grad, sign, st);
         else if (a.rotated % (2 * Vec<T>::N) == 0) launch_units<T, HALVES>(a, grad, sign, st);
         else launch_units<T, SPREAD>(a, grad, sign, st);
         return;
