@@ -480,11 +480,55 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) o[i][t][r] *= f[i];
-            __syncthreads();                              // (the pieces are there)
         }
         // (the next chunk on its way from here: earlier, its registers push the products' operands out)
         if (i0 + CH < left) fetch(i0 + CH);
+        // the state after the chunk; of the stretch's last one forwards, S rather than l S
+        const bool ends = last && i0 + CH >= left;
+        if (!ends || s.fin) {
+            if (ends) {
+                const int early = s.backwards ? 0 : 1;
+                const Keep k(ld * (float)(CH - pad - early));
+                keep.one = shared_by_all(k.one);
+                keep.f = shared_by_all(k.f);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r - early);
+            }
+            if (keep.one != 0.f) {                            // (one instruction a value, either way)
+#pragma unroll
+                for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] = fmaf(keep.f, z[b][r >> 2][r & 3], z[b][r >> 2][r & 3]);
+            } else {
+#pragma unroll
+                for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                    for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] *= keep.f;
+            }
+#pragma unroll
+            for (int jj = 0; jj < JB / 2; ++jj) {
+                Sum<S_TERMS, 8> w[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW + 4 * t, 16 * NW, VP);
+                    f32x8 v = __builtin_convertvector(vf.term[X - 1], f32x8);
+#pragma unroll
+                    for (int p = X - 2; p >= 0; --p) v += __builtin_convertvector(vf.term[p], f32x8);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) v[r] *= rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2));
+                    w[t].of_summed(v);
+                }
+#pragma unroll
+                for (int b = 0; b < 2 * KT; ++b) {
+                    const bf16* p = sy + 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
+                    const Sum<X, 8> yt = down<X>(p, 16 * KW, XP);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) z[b][t] = mfma(yt, w[t], z[b][t]);
+                }
+            }
+        }
         if (OUT && out) {
+            __syncthreads();                              // (the weights' pieces are there, long since: the state came between)
             float odd = 0.f;                              // (0 times what is not finite is NaN)
             unsigned none = 0;
             asm("" : "+s"(none));
@@ -579,50 +623,6 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
                             else reinterpret_cast<T*>(to)[4 * t + r] = narrow<T>(o[i][t][r]);
                         }
                 }
-            }
-        }
-
-        // the state after the chunk; of the stretch's last one forwards, S rather than l S
-        const bool ends = last && i0 + CH >= left;
-        if (ends && !s.fin) break;
-        if (ends) {
-            const int early = s.backwards ? 0 : 1;
-            const Keep k(ld * (float)(CH - pad - early));
-            keep.one = shared_by_all(k.one);
-            keep.f = shared_by_all(k.f);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r - early);
-        }
-        if (keep.one != 0.f) {                            // (one instruction a value, either way)
-#pragma unroll
-            for (int b = 0; b < 2 * KT; ++b)
-#pragma unroll
-                for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] = fmaf(keep.f, z[b][r >> 2][r & 3], z[b][r >> 2][r & 3]);
-        } else {
-#pragma unroll
-            for (int b = 0; b < 2 * KT; ++b)
-#pragma unroll
-                for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] *= keep.f;
-        }
-#pragma unroll
-        for (int jj = 0; jj < JB / 2; ++jj) {
-            Sum<S_TERMS, 8> w[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const Sum<X, 8> vf = down<X>(vdown + 32 * jj * NW + 4 * t, 16 * NW, VP);
-                f32x8 v = __builtin_convertvector(vf.term[X - 1], f32x8);
-#pragma unroll
-                for (int p = X - 2; p >= 0; --p) v += __builtin_convertvector(vf.term[p], f32x8);
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] *= rest[r & 3] * blocks(JB - 1 - 2 * jj - (r >> 2));
-                w[t].of_summed(v);
-            }
-#pragma unroll
-            for (int b = 0; b < 2 * KT; ++b) {
-                const bf16* p = sy + 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
-                const Sum<X, 8> yt = down<X>(p, 16 * KW, XP);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) z[b][t] = mfma(yt, w[t], z[b][t]);
             }
         }
     }
