@@ -39,6 +39,13 @@ __device__ __forceinline__ long long index_at(const void* p, long long i, bool w
     return wide ? reinterpret_cast<const long long*>(p)[i] : reinterpret_cast<const int*>(p)[i];
 }
 
+// a launch of any number of workgroups (a grid's x holds 2^32 threads)
+inline dim3 blocks_of(long long n) {
+    const long long x = n < 1 << 20 ? n : 1 << 20;
+    return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+}
+__device__ __forceinline__ long long block_number() { return (long long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline bool aligned16(const fm_view& v, int size) {
     return !(((uintptr_t)v.data | (uintptr_t)(v.seq * size) | (uintptr_t)(v.moment * size) | (uintptr_t)(v.head * size)) & 15);
 }

@@ -692,13 +692,14 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
 // gradients of shared heads: out[m][j][d] = the sum over a key head's `share` query heads of part[m][share j + i][d]; the
 // first `first` workgroups those of k, the rest those of v
 template <class T>
-__global__ __launch_bounds__(256) void k_share(const float* part_k, T* out_k, int K, long long nk, unsigned first,
+__global__ __launch_bounds__(256) void k_share(const float* part_k, T* out_k, int K, long long nk, long long first,
                                                const float* part_v, T* out_v, int V, long long nv, int share) {
-    const bool of_v = blockIdx.x >= first;
+    const long long block = block_number();
+    const bool of_v = block >= first;
     const float* part = of_v ? part_v : part_k;
     T* out = of_v ? out_v : out_k;
     const int D = of_v ? V : K;
-    const long long i = (long long)(blockIdx.x - (of_v ? first : 0)) * 256 + threadIdx.x, row = i / D;
+    const long long i = (block - (of_v ? first : 0)) * 256 + threadIdx.x, row = i / D;
     if (i >= (of_v ? nv : nk)) return;
     const int d = (int)(i - row * D);
     float s = 0.f;
@@ -960,8 +961,8 @@ void attention_bwd(const fm_attention_args& p, hipStream_t st) {
     launch_scans<T>(a, n, cut, wide_rows(p, true), st);
     if (!part) return;
     const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads, nk = p.gk ? rows * K : 0, nv = p.gv ? rows * V : 0;
-    const unsigned bk = (unsigned)((nk + 255) / 256), bv = (unsigned)((nv + 255) / 256);
-    if (bk + bv) k_share<T><<<bk + bv, 256, 0, st>>>(part_k, (T*)p.gk, K, nk, bk, part_v, (T*)p.gv, V, nv, share);
+    const long long bk = (nk + 255) / 256, bv = (nv + 255) / 256;
+    if (bk + bv) k_share<T><<<blocks_of(bk + bv), 256, 0, st>>>(part_k, (T*)p.gk, K, nk, bk, part_v, (T*)p.gv, V, nv, share);
 }
 
 // 32 columns a workgroup: 416 rows of 8 states of 128 x 128, 90 us with 32 or 64 columns, 101 with 128; one row of 8 states of
@@ -981,7 +982,7 @@ using namespace fg;
 extern "C" {
 
 long long fm_attention_workspace(const fm_attention_args* a, int backward) {
-    if (attention_wrong(*a, false, true)) return 0;
+    if (!a || attention_wrong(*a, false, true)) return 0;
     const Cut cut = cut_of(*a, backward ? 3 : 1);
     return 4 * (segment_floats(*a, cut) * (backward ? 3 : 1) + (backward ? shared_floats(*a, false) + shared_floats(*a, true) : 0));
 }

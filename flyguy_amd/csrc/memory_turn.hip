@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256) void k_turn_units(fm_turn_args a, Lanes l, flo
     __shared__ float rows[P == SPREAD ? 256 * 2 * V : 1];
     const int D = (int)a.dim, R = (int)a.rotated, j = threadIdx.x & (l.lanes - 1);
     float* const row = rows + (P == SPREAD ? (threadIdx.x >> l.shift << l.shift) * 2 * V : 0);
-    const long long item = (long long)blockIdx.x * (256 >> l.shift) + (threadIdx.x >> l.shift);
+    const long long item = block_number() * (256 >> l.shift) + (threadIdx.x >> l.shift);
     const long long m = item / l.chunks, n = m / a.n_moments, t = m - n * a.n_moments;
     if (n >= a.n_seq) return;                             // (a wave's lanes of other groups go on: sums stay in a group)
     int chunk = (int)(item - m * l.chunks);
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void k_turn_units_bwd(fm_turn_args a, Lanes l)
 template <class T, int NE>
 __global__ __launch_bounds__(64 * TURN_ROWS) void k_turn(fm_turn_args a, float sign) {
     const int H = (int)(a.heads[0] + a.heads[1]), lane = threadIdx.x & 63, D = (int)a.dim, R = (int)a.rotated;
-    const long long row = (long long)blockIdx.x * TURN_ROWS + (threadIdx.x >> 6);
+    const long long row = block_number() * TURN_ROWS + (threadIdx.x >> 6);
     if (row >= a.n_seq * a.n_moments * H) return;
     const long long m = row / H, n = m / a.n_moments, t = m % a.n_moments;
     int h = (int)(row % H);
@@ -439,7 +439,7 @@ void launch_any(const fm_turn_args& a, bool grad, float sign, hipStream_t st) {
         return;
     }
     const long long rows = a.n_seq * a.n_moments * (a.heads[0] + a.heads[1]);
-    k_turn<T, NE><<<(unsigned)((rows + TURN_ROWS - 1) / TURN_ROWS), 64 * TURN_ROWS, 0, st>>>(a, sign);
+    k_turn<T, NE><<<blocks_of((rows + TURN_ROWS - 1) / TURN_ROWS), 64 * TURN_ROWS, 0, st>>>(a, sign);
 }
 
 // 4 heads a group: queries and keys of 16 heads of 128 values in bfloat16, 8 x 2048 moments, forward and gradient with a norm:
@@ -465,7 +465,7 @@ void launch_units(const fm_turn_args& a, bool grad, float sign, hipStream_t st) 
     }
     const Lanes l = lanes_of<T, HB>(a);
     const int groups = 256 >> l.shift;
-    const unsigned grid = (unsigned)((a.n_seq * a.n_moments * l.chunks + groups - 1) / groups);
+    const dim3 grid = blocks_of((a.n_seq * a.n_moments * l.chunks + groups - 1) / groups);
     if (a.weight[0] || a.weight[1]) k_turn_units<T, P, true, HB><<<grid, 256, 0, st>>>(a, l, sign);
     else k_turn_units<T, P, false, HB><<<grid, 256, 0, st>>>(a, l, sign);
 }
@@ -529,6 +529,6 @@ extern "C" {
 
 int fm_turn(const fm_turn_args* a, void* stream) { return turn(a, false, stream); }
 int fm_turn_bwd(const fm_turn_args* a, void* stream) { return turn(a, true, stream); }
-long long fm_turn_partial(const fm_turn_args* a) { return 2LL * turn_blocks(*a) * a->dim; }
+long long fm_turn_partial(const fm_turn_args* a) { return a ? 2LL * turn_blocks(*a) * a->dim : 0; }
 
 }  // extern "C"

@@ -148,6 +148,18 @@ def test_positions(gpu_lib):
     assert torch.isnan(rotary(q, None, table, 18)[0][:, 2:, :, :8]).all()
 
 
+def test_many_rows(gpu_lib):
+    """70 million heads of two values: more workgroups than a grid's x takes threads for."""
+    from flyguy_amd.memory_hip import rotary, rotary_table
+    q = torch.randn(1, 70, 1000000, 2, device="cuda").bfloat16()
+    table = rotary_table(70, 2).cuda()
+    got = rotary(q, None, table)[0]
+    c, s = table[:, 0, 0, None], table[:, 0, 1, None]
+    a, b = q[0, ..., 0].float(), q[0, ..., 1].float()
+    for x, y in ((got[0, ..., 0], a * c - b * s), (got[0, ..., 1], b * c + a * s)):
+        assert float((x.float() - y).abs().max()) <= 2.0 ** -8 * float(y.abs().max())
+
+
 @pytest.mark.parametrize("il", [False, True])
 def test_values_that_are_not_turned_pass_through(gpu_lib, il):
     """Whatever they are: infinities and NaN among them touch nothing else, turned values' only their own pair."""
