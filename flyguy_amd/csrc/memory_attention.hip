@@ -1,10 +1,11 @@
 // Linear attention with a decay for each head (include/flyguy_memory.h: fm_attention, fm_attention_bwd, fm_step).
 //
 // One scan computes everything: with x, y, v of K, K, N values a moment, a state Z [K][N] and l = exp(log_decay),
-//   Z_i = l Z_{i-1} + cz y_i v_i^T,   out_i = co x_i Z_i.
+//   Z_i = l Z_{i-1} + y_i v_i^T,   out_i = c x_i Z_i.
 // The forward is the scan of (q, k, v); the gradient of q that of (go, v, k), with the start state transposed; the
 // gradients of k and v those of (v, go, q) and (k, q, go) over the moments backwards, from the end state's gradient, which
-// the last moment's term does not decay; the second one's end state, decayed once more, is the start state's gradient.
+// the last moment's term does not decay (c on what is added instead); the second one's end state, decayed once more, is the
+// start state's gradient.  A gradient's three scans are one launch.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -32,7 +33,7 @@ struct Scans {
     const void* starts;
     long long n_moments, L;              // L: moments per segment (a multiple of CHUNK_MAX)
     int wide, heads, n_seq, nseg, slots; // slots of segments: n_seq x nseg, or an upper bound for packed stretches
-    int joined;                          // the segments' start states are there (k_scan_join)
+    int joined, scans;                   // the segments' start states are there (k_scan_join); the launch's scans
 };
 
 // the moments of stretch n: [first, first + count) of the views
@@ -49,31 +50,49 @@ __device__ __forceinline__ void stretch_of(const Scans& a, int n, long long& fir
     count = e - b;
 }
 
+// Whole segments before moment `first` (at most n_moments <= 2^31, as L - 64 is).
+__device__ __forceinline__ int segments_before(const Scans& a, long long first) { return (int)((unsigned)first / (unsigned)a.L); }
+
 // The slot of a packed stretch's first segment: its segments and the next stretch's never share one, as floor(b / L) + 1 +
 // floor((b + c) / L) - floor(b / L) >= ceil(c / L), and 1 for a stretch without moments.
-__device__ __forceinline__ int first_slot(const Scans& a, int n) {
-    if (!a.starts || a.nseg == 1) return n * a.nseg;
-    long long b = index_at(a.starts, n, a.wide);
-    b = b < 0 ? 0 : b > a.n_moments ? a.n_moments : b;
-    return (int)(b / a.L) + n;
+__device__ __forceinline__ int first_slot(const Scans& a, int n, long long first) {
+    return !a.starts || a.nseg == 1 ? n * a.nseg : segments_before(a, first) + n;
 }
-// (stretch, segment) of a slot; false: the slot is empty
-__device__ __forceinline__ bool segment_of(const Scans& a, int slot, int& n, int& seg, long long& first, long long& count) {
+// (stretch, segment, slot) of a workgroup; false: it has none.  Packed stretches: the first n_seq workgroups take their first
+// segments, workgroup n_seq + e the segment s > 0 of the stretch with floor(b / L) + s - 1 = e, which all 64 lanes look for.
+// So most search nothing, and those without a segment come last (k_scan): 37 stretches of 1,531 moments in the middle, 4 heads
+// of 64 x 128 values in bfloat16, take 98 us, 110 with a binary search by every workgroup and slots in the stretches' order.
+__device__ __forceinline__ bool segment_of(const Scans& a, int block, int& n, int& seg, int& slot, long long& first,
+                                           long long& count) {
     if (!a.starts || a.nseg == 1) {
-        n = slot / a.nseg;
-        seg = slot % a.nseg;
+        n = block / a.nseg;
+        seg = block % a.nseg;
+    } else if (block < a.n_seq) {
+        n = block;
+        seg = 0;
     } else {
-        int lo = 0, hi = a.n_seq - 1;    // the last stretch whose first slot is not past this one
+        const int e = block - a.n_seq, lane = threadIdx.x & 63;
+        int lo = 0, hi = a.n_seq - 1;    // the last stretch that does not begin past it
         while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (first_slot(a, mid) <= slot) lo = mid;
-            else hi = mid - 1;
+            const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
+            bool before = at <= hi;
+            if (before) {
+                const long long b = index_at(a.starts, at, a.wide);
+                before = segments_before(a, b < 0 ? 0 : b > a.n_moments ? a.n_moments : b) <= e;
+            }
+            lo += __popcll(__ballot(before)) * step;
+            hi = min(hi, lo + step - 1);
         }
         n = lo;
-        seg = slot - first_slot(a, n);
+        seg = -1;
     }
     stretch_of(a, n, first, count);
-    return seg == 0 || (seg > 0 && seg * a.L < count);
+    if (seg < 0) {
+        seg = block - a.n_seq - segments_before(a, first) + 1;
+        if (seg < 1) return false;
+    }
+    slot = first_slot(a, n, first) + seg;
+    return seg == 0 || seg * a.L < count;
 }
 
 // A state's value at (k, c) of the start state of stretch n, decayed once where the scan goes forwards (Z = l S).
@@ -217,16 +236,23 @@ __device__ __forceinline__ Sum<P, 8> down(const bf16* p, int apart, int plane) {
 // (forwards c' = c, c'' = 1; backwards c' = 1, c'' = c, so that the end state's gradient comes in and the start state's goes
 // out unscaled).  A stretch's last chunk, where it is short, has its moments in the last rows and zeros before them, so that
 // its decays to the chunk's end are a whole chunk's.
-// A workgroup of WAVES waves walks one segment of one head; wave w owns the state's columns 16 w .., in accumulators all
+// A workgroup of 4 waves walks one segment of one head; wave w owns the state's columns 16 NT w .., in accumulators all
 // along: a 16 x 16 accumulator block holds, in lane (column c, group g), rows 4g .. 4g + 3, which is also how a product's
 // operand wants it with the rows as the summed index.  So the state passes from product to product in registers, and the
 // order of the summed index (any, if both operands have it) is chosen so: state blocks 2b, 2b + 1 are the rows 32 b + 8g +
 // (0 .. 3), (4 .. 7), and a lane's 8 values of x or y are then side by side.  y^T and v^T come out of LDS by transposing
 // reads.  Outputs are formed transposed, so that a lane stores a row's values side by side.  The weights (x . y) l^(i-j) of
-// the chunk's 16 x 32 pieces on and below the diagonal are formed by a wave each and shared through LDS.
+// the chunk's 16 x 16 blocks on and below the diagonal are dealt to the waves and shared through LDS; the state's additions,
+// which do not need them, run before the barrier that waits for them (780 -> 759 us a learning step of 8 x 4096 moments of 16
+// heads of 128 values, bfloat16).
 // A value of v that is not finite reaches only the outputs from its moment on (there: NaN), though 0 weights meet it in the
 // products: such a chunk's products run with zeros in its place.
-template <class T, int KT, int NT, int WAVES, bool OUT>
+// What bounds it: latency between a chunk's three barriers, with the two workgroups a CU that the registers of 128 x 128 states
+// allow.  32,768 moments of 8 such heads in bfloat16, 57 segments, take 96 us: 1.6 waves a SIMD, whose vector instructions
+// (sums of terms, decays) take 38% of the time and matrix instructions 26%; LDS is read 22% of it.  512 heads of 4,096 moments
+// in one segment each: 620 us, 3.5 TB/s of a copy's 5.2; 477 without loads and stores, 480 without the products.
+constexpr int WAVES = 4;
+template <class T, int KT, int NT, bool OUT>
 struct Tile {
     static constexpr int CH = Form<T>::CHUNK, KW = 32 * KT, NW = 16 * NT * WAVES;
     static constexpr int XP = CH * KW, VP = CH * NW, PIECES = CH == 64 ? 6 : 2;
@@ -271,24 +297,29 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int row
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-template <class T, int KT, int NT, int WAVES, bool VEC, bool OUT>
-__global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)) void k_scan(Scans a) {
-    using S = Tile<T, KT, NT, WAVES, OUT>;
+template <class T, int KT, int NT, bool VEC, bool OUT>
+__global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void k_scan(Scans a) {
+    using S = Tile<T, KT, NT, OUT>;
     constexpr int X = Form<T>::X, W = Form<T>::W, CH = S::CH, JB = CH / 16, VN = Vec<T>::N;
     constexpr int KW = S::KW, NW = S::NW, XP = S::XP, VP = S::VP, PIECES = S::PIECES;
     constexpr int XC = KW / VN, VC = NW / VN;                                // 16-byte shares of a row
     constexpr int XR = 64 * WAVES / XC, VR = 64 * WAVES / VC;                // rows between a thread's shares
-    constexpr int XV = XR < CH ? CH / XR : 1, VV = CH / VR;                  // a thread's shares (XR > CH: of some threads)
-    static_assert((XV * XR == CH || XR > CH) && VV * VR == CH, "");
+    constexpr int XV = CH / XR, VV = CH / VR;                                // a thread's shares
+    static_assert(XV * XR == CH && VV * VR == CH, "");
     __shared__ __align__(16) bf16 sx[OUT ? X * XP : 8], sy[X * XP], sv[X * VP];
     __shared__ __align__(16) bf16x8 sp[OUT ? PIECES : 1][W][64];
-    const Scan& s = a.s[blockIdx.z];
-    const int slot = blockIdx.x, h = blockIdx.y;
-    int n, seg;
+    // (heads first, then scans: a packed launch's workgroups without a segment come last, or some CUs would get only such; and
+    // a gradient's scans read the same moments at about the same time)
+    const unsigned block = (unsigned)block_number(), group = block / a.heads, place_in = group / a.scans;
+    const int h = (int)(block - group * a.heads);
+    const Scan& s = a.s[group - place_in * a.scans];
+    if (place_in >= (unsigned)a.slots) return;
+    int n, seg, slot;
     long long first, count;
-    if (!segment_of(a, slot, n, seg, first, count)) return;
+    if (!segment_of(a, (int)place_in, n, seg, slot, first, count)) return;
     n = __builtin_amdgcn_readfirstlane(n);
     seg = __builtin_amdgcn_readfirstlane(seg);
+    slot = __builtin_amdgcn_readfirstlane(slot);
     first = shared_by_all(first);
     count = shared_by_all(count);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
@@ -341,7 +372,9 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
     const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
     auto rows_from = [&](long long i0) { return (int)(left - i0 < CH ? left - i0 : CH); };
     // the chunk from the segment's moment i0: its moment lowest in memory, and a row's place from there
-    auto lowest = [&](long long i0, int rows) { return (a.starts ? first : 0) + (s.backwards ? count - from - i0 - rows : from + i0); };
+    auto lowest = [&](long long i0, int rows) {
+        return (a.starts ? first : 0) + (s.backwards ? count - from - i0 - rows : from + i0);
+    };
     auto in_memory = [&](int row, int pad) { return s.backwards ? CH - 1 - row : row - pad; };
     auto base = [&](const fm_view& v, int share, long long low) {
         return (const T*)v.data + (a.starts ? 0 : n * v.seq) + (h / share) * v.head + low * v.moment;
@@ -358,9 +391,8 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
             const auto bv = rows_at(pv, rows, sv_, s.N * (int)sizeof(T));
             // (the lanes' places anew each time, from the thread's number: kept, they cost registers that the products need)
             const int t = here(tid), xr = t / XC, xc = t % XC * VN, vr = t / VC, vc = t % VC * VN;
-            const bool in_x = xc < s.K && (XR <= CH || xr < CH);
-            const unsigned ax = in_x ? in_memory(xr, 0) * sx_ + xc * (int)sizeof(T) : NOWHERE;
-            const unsigned ay = in_x ? in_memory(xr, 0) * sy_ + xc * (int)sizeof(T) : NOWHERE;
+            const unsigned ax = xc < s.K ? in_memory(xr, 0) * sx_ + xc * (int)sizeof(T) : NOWHERE;
+            const unsigned ay = xc < s.K ? in_memory(xr, 0) * sy_ + xc * (int)sizeof(T) : NOWHERE;
             const unsigned av = vc < s.N ? in_memory(vr, 0) * sv_ + vc * (int)sizeof(T) : NOWHERE;
             auto load = [&](__amdgpu_buffer_rsrc_t r, unsigned at, int row, int step) {
                 if (pad) at = row < pad ? NOWHERE : at - (s.backwards ? 0 : pad * step);
@@ -377,7 +409,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
 #pragma unroll
             for (int i = 0; i < XV; ++i) {
                 const int row = xrow + i * XR;
-                const bool there = row >= pad && (XR <= CH || xrow < CH);
+                const bool there = row >= pad;
                 if (OUT) rx[i] = load16(px + in_memory(row, pad) * s.x.moment, xcol, s.K, there);
                 ry[i] = load16(py + in_memory(row, pad) * s.y.moment, xcol, s.K, there);
             }
@@ -417,14 +449,16 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
         __syncthreads();                                  // (the chunk before is read)
 #pragma unroll
         for (int i = 0; i < XV; ++i) {
-            if (XR > CH && xrow >= CH) break;
             // (a row 16 on has its shares in the same order)
             const int to = XR % 16 ? place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7) : xto + i * XR * KW;
             if (OUT) store_terms<T>(rx[i], sx + to, XP);
             store_terms<T>(ry[i], sy + to, XP);
         }
 #pragma unroll
-        for (int i = 0; i < VV; ++i) store_terms<T>(rv[i], sv + (VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW), VP);
+        for (int i = 0; i < VV; ++i) {
+            const int to = VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW;
+            store_terms<T>(rv[i], sv + to, VP);
+        }
         __syncthreads();
 
         f32x4 o[JB][NT];
@@ -455,7 +489,8 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
             for (int b = 0; b < KT; ++b) {
                 Sum<W, 8> zf[NT];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) zf[t].of_summed(__builtin_shufflevector(z[2 * b][t], z[2 * b + 1][t], 0, 1, 2, 3, 4, 5, 6, 7));
+                for (int t = 0; t < NT; ++t)
+                    zf[t].of_summed(__builtin_shufflevector(z[2 * b][t], z[2 * b + 1][t], 0, 1, 2, 3, 4, 5, 6, 7));
                 const int at = here(xat) ^ 32 * b;
 #pragma unroll
                 for (int i = 0; i < JB; ++i) {
@@ -597,16 +632,19 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
                     if (sizeof(T) == 4 || s.wide) {
 #pragma unroll
                         for (int t = 0; t < NT; ++t)      // (columns past the row's end would be the next one's)
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i][t]), bo, oc1 + 4 * t < s.N ? to + 16 * t : NOWHERE, 0, 0);
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i][t]), bo,
+                                                                   oc1 + 4 * t < s.N ? to + 16 * t : NOWHERE, 0, 0);
                     } else if constexpr (sizeof(T) == 2) {
                         typedef T vec __attribute__((ext_vector_type(4)));
                         vec v[NT];
 #pragma unroll
                         for (int t = 0; t < NT; ++t) v[t] = __builtin_convertvector(o[i][t], vec);
-                        if constexpr (NT == 2)
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[NT - 1], 0, 1, 2, 3, 4, 5, 6, 7)), bo, to, 0, 0);
-                        else
+                        if constexpr (NT == 2) {
+                            const auto both = __builtin_shufflevector(v[0], v[NT - 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, both), bo, to, 0, 0);
+                        } else {
                             __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v[0]), bo, to, 0, 0);
+                        }
                     }
                 }
             } else {
@@ -656,7 +694,8 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, WAVES, OUT>::PER_SIMD)
 }
 
 // Segments' start states from their own: Z_0 = the stretch's, Z_{s+1} = l^L Z_s + own_s, in place; 4 values a lane (K x N a
-// multiple of 4) or one.  grid (blocks of values x heads, stretches, scans)
+// multiple of 4) or one.  A value's chain is as long as its segments are many, so 16 of them are under way at once.
+// grid (blocks of values x heads, stretches, scans)
 template <int V>
 __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     typedef float vec __attribute__((ext_vector_type(V)));
@@ -669,9 +708,10 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     const Keep once(count ? ld : 0.f), keep(ld * (float)a.L);    // (no moments: the state goes through as it is)
     vec z;
 #pragma unroll
-    for (int j = 0; j < V; ++j) z[j] = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, (i + j) / s.N, (i + j) % s.N, once);
+    for (int j = 0; j < V; ++j)
+        z[j] = start_value(s, ((size_t)n * a.heads + h) * s.K * s.N, (i + j) / s.N, (i + j) % s.N, once);
     const size_t step = (size_t)a.heads * s.K * s.N;
-    float* p = s.seg + ((size_t)first_slot(a, n) * a.heads + h) * s.K * s.N + i;
+    float* p = s.seg + ((size_t)first_slot(a, n, first) * a.heads + h) * s.K * s.N + i;
     constexpr int AHEAD = 16;                             // segments' states under way at once
     for (long long from = 0; from < count || from == 0; from += AHEAD * a.L, p += AHEAD * step) {
         vec own[AHEAD];
@@ -808,25 +848,29 @@ long long shared_floats(const fm_attention_args& a, bool of_v) {
 // to 128, two blocks a wave (a wave's reads of x and y then serve two: at N = 128, one block and 8 waves measured the same
 // within 1%, and 4 waves in two workgroups 6% more).
 template <class T, int KT, int NT>
-constexpr int groups_per_cu() { return Tile<T, KT, NT, 4, true>::PER_SIMD; }
+constexpr int groups_per_cu() { return Tile<T, KT, NT, true>::PER_SIMD; }
 template <class T>
 int groups_per_cu(int K, int N) {
     return K <= 64 ? (N <= 64 ? groups_per_cu<T, 2, 1>() : groups_per_cu<T, 2, 2>())
                    : (N <= 64 ? groups_per_cu<T, 4, 1>() : groups_per_cu<T, 4, 2>());
 }
 
-// How a launch's scans are cut into segments: as the following estimate has it cheapest, in chunks' times.  A CU with w
-// workgroups takes about 0.9 + w for a chunk of each (measured: 7.6 us with one, 11.6 with two of 128 x 128 in bfloat16), a
-// workgroup 1.5 chunks to begin and end.  More than one segment a stretch cost a pass for their own states (0.45 of the main
-// one) and one to join them.  A packed stretch is taken to be the middle length, the longest twice that.
+// How a launch's scans are cut into segments: as the following estimate (us) has it cheapest.  A CU with w workgroups takes
+// 1.7 + b w (3 + K N / 1024) for a chunk of each, K and N as the kernel's form has them, b = 0.207 for bfloat16 (64 moments a
+// chunk), 0.147 for binary16, 0.257 for float32 (32); the longest workgroup ends alone.  More than one segment a stretch cost a
+// pass for their own states (0.55 of the constant, 0.2 of the rest; a stretch's last segment needs none), its launch, and the
+// joining's traffic.  Packed stretches, whose lengths only the device knows, are taken to be of any length up to twice the
+// middle one.  Fitted to 550 measured times (13% rms): 15 sets of stretches of one or of mixed lengths, forward and gradient, 5
+// to 12 cuts of each.  The cut so chosen takes 5% (rms) more than the best of them where the host knows the lengths, 6% where
+// packed ones are mixed, 20% where packed ones are all the same, 15% where one of them is four times the others.
 struct Cut {
     int nseg, slots, K, N, joined;
     long long L;
 };
 // From this many values of a chain's segments up they are joined by a kernel of its own; fewer, each segment of the main pass
 // joins those before it as it begins (a launch less; 4 segments of 64 x 64: 143 us a learning step against 149 with the
-// kernel, 4 of 128 x 128: 786 against 776).
-constexpr int JOIN_FROM = 65536;
+// kernel, 4 of 128 x 128: 786 against 776, 6 of 64 x 128: 113 us a packed forward pass against 98).
+constexpr int JOIN_FROM = 49152;
 Cut cut_of(const fm_attention_args& p, int scans) {
     Cut c;
     const int widest = (int)(p.k_dim > p.v_dim ? p.k_dim : p.v_dim);
@@ -841,37 +885,49 @@ Cut cut_of(const fm_attention_args& p, int scans) {
     const int cap = p.dtype == FM_F32 ? groups_per_cu<float>(c.K, c.N) : p.dtype == FM_BF16 ? groups_per_cu<bf16>(c.K, c.N)
                                                                                             : groups_per_cu<f16>(c.K, c.N);
     const int chunk = p.dtype == FM_BF16 ? Form<bf16>::CHUNK : Form<float>::CHUNK;
-    const double middle = p.starts ? (double)p.n_moments / p.n_seq : (double)p.n_moments;
-    const double longest = p.starts && p.n_seq > 1 ? 2 * middle : middle;
+    const double one = (p.dtype == FM_BF16 ? 0.207 : p.dtype == FM_F16 ? 0.147 : 0.257) *
+                       (3 + (c.K <= 64 ? 1 : 2) * (c.N <= 64 ? 1 : 2) * 4.0);
+    const bool packed = p.starts && p.n_seq > 1;
+    const double middle = (double)p.n_moments / (packed ? p.n_seq : 1), longest = packed ? 2 * middle : middle;
     const double chains = (double)p.n_seq * p.q_heads * scans;
-    auto pass = [&](double groups, double L) {
+    // each, most: moments of a group in the middle, of the longest
+    auto pass = [&](double groups, double each, double most, double a, double b) {
         double left = groups / 256, t = 0;
+        if (left <= 0) return 0.0;
         for (; left > 0; left -= cap) {
             if (left > 64 * cap) {                        // (many rounds: each full)
-                t += (0.9 + cap) * left / cap;
+                t += (a + b * cap) * left / cap;
                 break;
             }
-            t += 0.9 + (left < cap ? ceil(left) : cap);
+            t += a + b * (left < cap ? ceil(left) : cap);
         }
-        return t * (L / chunk + 1.5);
+        return t * (each / chunk + 0.3) + (a + b) * (most - each) / chunk;
     };
-    double best = pass(chains, longest);
+    double best = 0.95 * pass(chains, middle, longest, 1.7, one);     // (whole where it is about the same)
     for (int nseg = 2; nseg <= 1024; nseg += nseg < 4 ? 1 : nseg / 2) {
         const long long L = ((long long)ceil(longest / nseg) + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
         if (L >= longest) continue;
-        const double each = p.starts ? middle / L + 0.5 : ceil(middle / L);
-        const double t = pass(chains * each, (double)L) + 0.45 * pass(chains * (each - 1), (double)L) + 0.7 + each / 22;
+        const double each = packed ? middle / L + 0.5 : ceil(middle / L), states = chains * each * c.K * c.N * 4;
+        const int joined = ceil(longest / L) * c.K * c.N >= JOIN_FROM;
+        const double t = pass(chains * each, packed ? middle / each : (double)L, (double)L, 1.7, one) +
+                         pass(chains * (each - 1), (double)L, (double)L, 0.55 * 1.7, 0.2 * one) +
+                         (joined ? 28 + states * 2 / 5.7e6 : 14 + states * (each - 1) / 2 / 5.7e6);
         if (t < best) {
             best = t;
             c.L = L;
             c.nseg = nseg;
+            c.joined = joined;
         }
         if (L == CHUNK_MAX) break;
     }
-    if (c.nseg == 1) return c;
-    c.joined = (long long)c.nseg * c.K * c.N >= JOIN_FROM;
+    // a packed launch that is best left whole cuts stretches past 8 times the middle all the same: that costs the others up to
+    // 7 us, and spares one long stretch among many from being walked alone
+    if (packed && c.nseg == 1 && p.n_seq > 8) {
+        c.L = ((long long)ceil(8 * middle) + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
+        c.joined = 0;
+    }
     c.nseg = (int)((p.n_moments + c.L - 1) / c.L);
-    c.slots = p.starts ? (int)(p.n_moments / c.L + p.n_seq) : (int)p.n_seq * c.nseg;
+    if (c.nseg > 1) c.slots = p.starts ? (int)(p.n_moments / c.L + p.n_seq) : (int)p.n_seq * c.nseg;
     return c;
 }
 // floats of segments' states of one scan
@@ -883,14 +939,15 @@ template <class T, int KT, int NT, bool VEC>
 void launch_form(Scans& a, int count, hipStream_t st) {
     int most = 1;
     for (int i = 0; i < count; ++i) most = a.s[i].K * a.s[i].N > most ? a.s[i].K * a.s[i].N : most;
-    const dim3 grid(a.slots, a.heads, count);
+    const dim3 grid = blocks_of((long long)a.slots * a.heads * count);
+    a.scans = count;
     if (a.nseg > 1) {
-        k_scan<T, KT, NT, 4, VEC, false><<<grid, 256, 0, st>>>(a);
+        k_scan<T, KT, NT, VEC, false><<<grid, 64 * WAVES, 0, st>>>(a);
         auto blocks = [&](int v) { return dim3((most / v + 255) / 256 * a.heads, a.n_seq, count); };
         if (a.joined && most % 4 == 0) k_scan_join<4><<<blocks(4), 256, 0, st>>>(a);
         else if (a.joined) k_scan_join<1><<<blocks(1), 256, 0, st>>>(a);
     }
-    k_scan<T, KT, NT, 4, VEC, true><<<grid, 256, 0, st>>>(a);
+    k_scan<T, KT, NT, VEC, true><<<grid, 64 * WAVES, 0, st>>>(a);
 }
 template <class T, bool VEC>
 void launch_sized(Scans& a, int count, const Cut& c, hipStream_t st) {
@@ -922,11 +979,13 @@ Scans scans_of(const fm_attention_args& p) {
 // 16-byte loads, whole stores: heads of a multiple of 16 bytes, everything aligned, a chunk's rows within 2^30 bytes
 bool wide_rows(const fm_attention_args& p, bool bwd) {
     const int size = p.dtype == FM_F32 ? 4 : 2;
-    if (p.k_dim * size % 16 || p.v_dim * size % 16 || !aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
+    if (p.k_dim * size % 16 || p.v_dim * size % 16) return false;
+    if (!aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
     auto near = [](long long s) { return s >= 0 && s < STRIDE_MOST; };
     if (!near(p.q.moment) || !near(p.k.moment) || !near(p.v.moment) || !near(p.q_heads * ATT_MAX)) return false;
-    if (bwd) return near(p.go.moment) && aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv | (uintptr_t)p.workspace) & 15);
-    return !((uintptr_t)p.o & 15);
+    if (!bwd) return !((uintptr_t)p.o & 15);
+    return near(p.go.moment) && aligned16(p.go, size) &&
+           !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv | (uintptr_t)p.workspace) & 15);
 }
 
 template <class T>
@@ -960,7 +1019,8 @@ void attention_bwd(const fm_attention_args& p, hipStream_t st) {
         a.s[n++] = Scan{p.k, p.q, p.go, share, 1, 1, part && p.gv ? part_v : p.gv, p.gstate_out, p.gstate, seg[2], K, V, 0, 1, part, c};
     launch_scans<T>(a, n, cut, wide_rows(p, true), st);
     if (!part) return;
-    const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads, nk = p.gk ? rows * K : 0, nv = p.gv ? rows * V : 0;
+    const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads;
+    const long long nk = p.gk ? rows * K : 0, nv = p.gv ? rows * V : 0;
     const long long bk = (nk + 255) / 256, bv = (nv + 255) / 256;
     if (bk + bv) k_share<T><<<blocks_of(bk + bv), 256, 0, st>>>(part_k, (T*)p.gk, K, nk, bk, part_v, (T*)p.gv, V, nv, share);
 }
@@ -1016,10 +1076,12 @@ int fm_attention_bwd(const fm_attention_args* a, void* stream) {
 int fm_step(const fm_step_args* a, void* stream) {
     clear_error();
     if (!a) return fail("fm_step: no arguments");
-    if (const char* e = heads_wrong(a->dtype, a->q_heads, a->k_heads, a->k_dim, a->v_dim)) return fail((std::string("fm_step: ") + e).c_str());
+    if (const char* e = heads_wrong(a->dtype, a->q_heads, a->k_heads, a->k_dim, a->v_dim))
+        return fail((std::string("fm_step: ") + e).c_str());
     if (a->n < 0 || a->n > 65535 || a->n_states < 0) return fail("fm_step: other than 0 to 65535 rows");
     if (!a->n) return 0;
-    if (!a->q.data || !a->k.data || !a->v.data || !a->log_decay || !a->state || !a->next || !a->o) return fail("fm_step: a null tensor");
+    if (!a->q.data || !a->k.data || !a->v.data || !a->log_decay || !a->state || !a->next || !a->o)
+        return fail("fm_step: a null tensor");
     if (!a->slots && a->n_states < a->n) return fail("fm_step: fewer states than rows");
     if (a->dtype == FM_F32) step_of_type<float>(*a, (hipStream_t)stream);
     else if (a->dtype == FM_BF16) step_of_type<bf16>(*a, (hipStream_t)stream);

@@ -32,10 +32,11 @@ __device__ __forceinline__ const float* table_line(const fm_turn_args& a, long l
 
 // Heads of whole 16-byte units (V values): a group of `lanes` lanes (a power of two) takes HB heads of a moment; lane j holds
 // two units of a head.  Where pairs lie half apart and the turned part is whole units, units j and j + R / 2V of it, so that the
-// lane's pairs are its own (HALVES; the rest goes two units a lane); side by side, units 2j and 2j + 1 (SIDE; SIDE_ANY: the turned
-// part ends inside a unit, which costs the others 5% if they ask for it).  Half apart at any place (SPREAD), units 2j and 2j + 1 too, and partners pass through LDS inside the group: 27 us instead of the 62 of a
-// wave per row at 8 x 981 moments of 16 float32 heads of 128 values, 106 of them turned.  The lane's angles, the weights and
-// the moment's addresses serve all HB heads, and all their loads are under way at once.
+// lane's pairs are its own (HALVES; the rest goes two units a lane); side by side, units 2j and 2j + 1 (SIDE; SIDE_ANY: the
+// turned part ends inside a unit, which costs the others 5% if they ask for it).  Half apart at any place (SPREAD), units 2j
+// and 2j + 1 too, and partners pass through LDS inside the group: 27 us instead of the 62 of a wave per row at 8 x 981 moments
+// of 16 float32 heads of 128 values, 106 of them turned.  The lane's angles, the weights and the moment's addresses serve all
+// HB heads, and all their loads are under way at once.
 enum Pairs { HALVES, SIDE, SIDE_ANY, SPREAD };
 struct Lanes {
     int lanes, shift, q_chunks, chunks;  // lanes = 1 << shift; chunks of HB heads of queries, in all
