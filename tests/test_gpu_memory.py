@@ -3,6 +3,7 @@ restatements, at the sizes, layouts and values where such kernels go wrong."""
 from __future__ import annotations
 
 import math
+import random
 
 import pytest
 import torch
@@ -274,6 +275,22 @@ def test_packed_stretches(gpu_lib, dt, lengths):
     H, Hk, K, V = 4, 2, 48, 40
     q, k, v = (draw(gen, starts[-1], h, d, dtype=dt) for h, d in ((H, K), (Hk, K), (Hk, V)))
     check_attention(q, k, v, decays(H), draw(gen, len(lengths), H, K, V), starts)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_many_short_stretches_and_a_few_long_ones(gpu_lib, dt):
+    """The long ones are cut, wherever they lie among the short ones; moments before the first stretch belong to none."""
+    say(f"many packed {dt}")
+    rng = random.Random(5)
+    lengths = [rng.randint(0, 12) for _ in range(300)]
+    for n, at in ((64, 0), (500, 1), (65, 70), (129, 200), (777, 299)):
+        lengths[at] = n
+    gen = torch.Generator().manual_seed(6)
+    starts = [70]
+    for n in lengths:
+        starts.append(starts[-1] + n)
+    q, k, v = (draw(gen, starts[-1], h, d, dtype=dt) for h, d in ((2, 24), (1, 24), (1, 32)))
+    check_attention(q, k, v, decays(2), draw(gen, len(lengths), 2, 24, 32), starts)
 
 
 def test_starts_of_another_kind(gpu_lib):
