@@ -48,13 +48,14 @@ int fm_turn(const fm_turn_args* a, void* stream);
 int fm_turn_bwd(const fm_turn_args* a, void* stream);
 long long fm_turn_partial(const fm_turn_args* a);
 
-/* Linear attention with a decay for each query head, l = exp(log_decay[h]); query head h reads key / value head
- * h / (q_heads / k_heads):
+/* Linear attention with a decay for each query head, l = exp(log_decay[h]) (log_decay 0 keeps everything, -inf nothing; above 0
+ * states grow until they overflow); query head h reads key / value head h / (q_heads / k_heads):
  *   S_t = l S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   S_{-1} = state (0: zeros)
  * k_dim, v_dim <= 128.  A value that is not finite reaches no output of an earlier moment (no gradient of a later one), and no
  * other stretch; the outputs that it does reach are NaN, or infinite.
  * Stretches: n_seq of n_moments moments each, or (starts not 0) packed: n_moments in all, stretch n being moments starts[n] ..
- * starts[n+1] - 1 (int32, or int64 if wide; out of [0, n_moments] or falling: clamped), the views' seq unread.  o: dense [moments][q_heads][v_dim].  state, state_out: float32 [n_seq][q_heads][k_dim][v_dim]
+ * starts[n+1] - 1 (int32, or int64 if wide; out of [0, n_moments] or falling: clamped), the views' seq unread.  o: dense
+ * [moments][q_heads][v_dim].  state, state_out: float32 [n_seq][q_heads][k_dim][v_dim]
  * (state_out 0: not wanted; it must not overlap state).  A stretch without moments passes its state on.
  * Gradients (fm_attention_bwd): go of o, gstate_out of state_out (0: zeros); gq, gk, gv dense like their tensors, gstate
  * float32; each 0 where not wanted.  workspace: fm_attention_workspace(a, backward) bytes. */
