@@ -50,6 +50,12 @@ __device__ __forceinline__ void stretch_of(const Scans& a, int n, long long& fir
     count = e - b;
 }
 
+// (-inf: 0 times it would not be 0; NaN stays NaN)
+__device__ __forceinline__ float log_decay_of(const Scans& a, int h) {
+    const float d = a.log_decay[h];
+    return d < -1e30f ? -1e30f : d;
+}
+
 // Whole segments before moment `first` (at most n_moments <= 2^31, as L - 64 is).
 __device__ __forceinline__ int segments_before(const Scans& a, long long first) { return (int)((unsigned)first / (unsigned)a.L); }
 
@@ -327,7 +333,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
     const long long from = seg * a.L, left = count - from < a.L ? count - from : a.L;
     const bool last = from + left == count;
     if (!OUT && last) return;                             // (the last segment's own state is needed by none)
-    const float ld = shared_by_all(fmaxf(a.log_decay[h], -1e30f));        // (-inf: 0 times it would not be 0)
+    const float ld = shared_by_all(log_decay_of(a, h));
     const size_t at = ((size_t)n * a.heads + h) * s.K * s.N;
     const float e2 = shared_by_all(ld * 1.44269504f);
     auto power = [&](int i) { return __builtin_amdgcn_exp2f(e2 * (float)i); };
@@ -704,7 +710,7 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     if (i >= s.K * s.N) return;
     long long first, count;
     stretch_of(a, n, first, count);
-    const float ld = fmaxf(a.log_decay[h], -1e30f);
+    const float ld = log_decay_of(a, h);
     const Keep once(count ? ld : 0.f), keep(ld * (float)a.L);    // (no moments: the state goes through as it is)
     vec z;
 #pragma unroll
@@ -824,6 +830,11 @@ const char* heads_wrong(long long dtype, long long qh, long long kh, long long k
     return nullptr;
 }
 
+// two arrays of n floats share memory
+bool overlap(const float* a, const float* b, long long n) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + 4 * n && (uintptr_t)b < (uintptr_t)a + 4 * n;
+}
+
 const char* attention_wrong(const fm_attention_args& a, bool bwd, bool sizes_only = false) {
     if (const char* e = heads_wrong(a.dtype, a.q_heads, a.k_heads, a.k_dim, a.v_dim)) return e;
     if (a.n_seq < 0 || a.n_seq > 16384) return "other than 0 to 16384 stretches";
@@ -833,7 +844,7 @@ const char* attention_wrong(const fm_attention_args& a, bool bwd, bool sizes_onl
     const bool any = a.n_seq && a.n_moments;
     if (any && (!a.q.data || !a.k.data || !a.v.data)) return "a null tensor";
     if (!bwd && any && !a.o) return "a null tensor";
-    if (!bwd && a.state && a.state_out == a.state) return "state_out must not be state";
+    if (!bwd && overlap(a.state, a.state_out, a.n_seq * a.q_heads * a.k_dim * a.v_dim)) return "state_out must not be state";
     if (bwd && any && !a.go.data) return "a null tensor";
     return nullptr;
 }
@@ -1083,6 +1094,8 @@ int fm_step(const fm_step_args* a, void* stream) {
     if (!a->q.data || !a->k.data || !a->v.data || !a->log_decay || !a->state || !a->next || !a->o)
         return fail("fm_step: a null tensor");
     if (!a->slots && a->n_states < a->n) return fail("fm_step: fewer states than rows");
+    if (a->next != a->state && overlap(a->state, a->next, a->n_states * a->q_heads * a->k_dim * a->v_dim))
+        return fail("fm_step: next must be state or lie outside it");
     if (a->dtype == FM_F32) step_of_type<float>(*a, (hipStream_t)stream);
     else if (a->dtype == FM_BF16) step_of_type<bf16>(*a, (hipStream_t)stream);
     else step_of_type<f16>(*a, (hipStream_t)stream);

@@ -17,6 +17,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from ._lib import LibraryError, check, lib
 
@@ -119,6 +120,12 @@ def _view3(x: torch.Tensor | None) -> tuple:
     return _NONE if x is None else (x.data_ptr(), 0, *x.stride()[:2])
 
 
+def _once(what: str) -> None:
+    """A gradient that is asked for with a graph of its own (create_graph) would be taken for a constant there."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: its gradient has no gradient (create_graph)")
+
+
 # ------------------------------------------------------------------------------------------------ rotation and norm
 class _Plan:
     """What a turn of queries and keys shares with its gradient."""
@@ -178,12 +185,14 @@ class TurnHip(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, p):
         ctx.p = p
-        ctx.save_for_backward(*((q, k) if wq is not None else (None, None)), wq, wk)
+        # (table and positions, so that one that is changed before the gradient is found out)
+        ctx.save_for_backward(*((q, k) if wq is not None else (None, None)), wq, wk, p.table, p.positions)
         return _turn(p, q, k, wq, wk)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        q, k, wq, wk = ctx.saved_tensors
+        _once("rotary, norm_rotary")
+        q, k, wq, wk = ctx.saved_tensors[:4]
         p = ctx.p
         q, k, gq = None if q is None else _rows(q), None if k is None else _rows(k), _rows(gq)
         gk = None if not p.heads[1] else _rows(gk)
@@ -265,13 +274,14 @@ class DecayHip(torch.autograd.Function):
     def forward(ctx, q, k, v, state, p):
         ctx.p = p
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, state)
+        ctx.save_for_backward(q, k, v, state, p.log_decay, p.starts)
         return _attend(p, q, k, v, state)
 
     @staticmethod
     def backward(ctx, go, gstate_out):
+        _once("decay_attention")
         p = ctx.p
-        q, k, v, state = ctx.saved_tensors
+        q, k, v, state = ctx.saved_tensors[:4]
         want = ctx.needs_input_grad
         q, k, v = _rows(q), _rows(k), _rows(v)
         go = q.new_zeros((*q.shape[:-1], p.V)) if go is None else _rows(go)
@@ -337,9 +347,9 @@ def decay_attention(q, k, v, log_decay, state=None, starts=None, scale: float | 
 def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None, into=None):
     """One new moment of decay_attention for each row: q [rows, q heads, values], k, v -> o [rows, q heads, v values].
     state (float32 [states, q heads, values, v values], dense) is updated in place, or the new states are written to
-    `into`, another tensor like it.  slots (int32 [rows] on the GPU): the state each row goes on from, by default its own
-    number; below 0: the row is idle (zeros, no state touched); past the states: NaN, no state touched.  No two rows of a
-    call may name one slot.  No gradients."""
+    `into`, another tensor like it that shares none of its memory.  slots (int32 [rows] on the GPU): the state each row goes
+    on from, by default its own number; below 0: the row is idle (zeros, no state touched); past the states: NaN, no state
+    touched.  No two rows of a call may name one slot.  No gradients."""
     what = "decay_step"
     _heads(what, 3, q, k, v)
     _shared(what, q, k, v, 1)
@@ -369,4 +379,6 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
     _call("fm_step", q, _STEP.pack(*views, log_decay.data_ptr(), state.data_ptr(), into.data_ptr(), _ptr(slots),
                                     o.data_ptr(), n, state.shape[0], Hq, k.shape[1], K, V, _TYPES[q.dtype],
                                     float(K ** -0.5 if scale is None else scale)))
+    if not into.is_inference():
+        increment_version(into)               # (autograd does not see the library's write)
     return o

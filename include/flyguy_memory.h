@@ -80,9 +80,9 @@ long long fm_attention_workspace(const fm_attention_args* a, int backward);
 
 /* One moment of it for n rows: q, k, v (views without moments) and
  *   next[s] = l state[s] + k v^T,  o = scale q next[s]     (o: dense [n][q_heads][v_dim])
- * s = slots[row] (int32; 0: s = row), state and next float32 [n_states][q_heads][k_dim][v_dim] (next == state: in place).
- * A slot below 0 gives a row of zeros and touches no state; one past the states gives NaN and touches none.  No two rows
- * may name the same slot. */
+ * s = slots[row] (int32; 0: s = row), state and next float32 [n_states][q_heads][k_dim][v_dim] (next == state: in place;
+ * else outside it).  A slot below 0 gives a row of zeros and touches no state; one past the states gives NaN and touches none.
+ * No two rows may name the same slot. */
 typedef struct fm_step_args {
     fm_view q, k, v;
     const float* log_decay;

@@ -407,6 +407,62 @@ def test_parts_of_the_gradient(gpu_lib):
                     assert torch.equal(x, whole[i]), (Hk, outs, wanted, i)
 
 
+def test_a_gradient_is_refused_where_it_would_be_wrong(gpu_lib):
+    """Gradients of gradients, and a gradient after its inputs, positions, starts or decays were changed in place."""
+    from flyguy_amd.memory_hip import decay_attention, norm_rotary, rotary_table
+    gen = torch.Generator().manual_seed(12)
+    q, k, v = (draw(gen, 6, 2, 16).requires_grad_() for _ in range(3))
+    w = torch.ones(16, device="cuda", requires_grad=True)
+    g, starts = decays(2), torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda")
+    at, table = torch.arange(6, dtype=torch.int32, device="cuda"), rotary_table(8, 16, device="cuda")
+
+    def attend():
+        return decay_attention(q, k, v, g, None, starts)[0]
+
+    def turn():
+        return norm_rotary(q[None], k[None], w, w, table, at)[0]
+    for f in (attend, turn):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(f().sum(), q, create_graph=True)
+    for f, changed in ((attend, g), (attend, starts), (turn, at), (turn, table)):
+        out = f().sum()
+        changed.add_(0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            out.backward()
+
+
+def test_a_state_that_a_step_has_changed_is_found_out(gpu_lib):
+    """A step's write counts as a change in place; in inference mode it is done all the same."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step
+    gen = torch.Generator().manual_seed(13)
+    q, k, v = (draw(gen, 1, 3, 2, 16).requires_grad_() for _ in range(3))
+    s = draw(gen, 1, 2, 16, 16)
+    o, _ = decay_attention(q, k, v, decays(2), s)
+    with torch.no_grad():
+        decay_step(q[:, 0], k[:, 0], v[:, 0], decays(2), s)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        o.sum().backward()
+    with torch.inference_mode():
+        t = torch.zeros(1, 2, 16, 16, device="cuda")
+        decay_step(q[:, 0], k[:, 0], v[:, 0], decays(2), t)
+        assert (t != 0).any()
+
+
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_a_decay_that_is_not_a_number(gpu_lib, dt):
+    """Its head's outputs and states are not numbers either; the other head's stay as they are."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step
+    gen = torch.Generator().manual_seed(14)
+    q, k, v = (draw(gen, 1, 70, 2, 32, dtype=dt) for _ in range(3))
+    s = draw(gen, 1, 2, 32, 32)
+    clean, bad = (torch.tensor([-0.1, x], device="cuda") for x in (-0.2, math.nan))
+    for f in (lambda g: decay_attention(q, k, v, g, s),
+              lambda g: (decay_step(q[:, 0], k[:, 0], v[:, 0], g, s, into=(n := torch.empty_like(s))), n)):
+        (o, e), (ob, eb) = f(clean), f(bad)
+        assert torch.equal(o[..., 0, :], ob[..., 0, :]) and torch.equal(e[:, 0], eb[:, 0])
+        assert ob[..., 1, :].isnan().all() and eb[:, 1].isnan().all()
+
+
 def test_pieces_of_a_stretch_and_single_moments(gpu_lib):
     """A stretch read in two pieces, or moment by moment with decay_step, is the stretch read at once, up to rounding."""
     from flyguy_amd.memory_hip import decay_attention, decay_step

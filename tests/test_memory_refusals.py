@@ -95,6 +95,13 @@ def test_the_library_refuses_attention(given):
     refuses("fm_attention", attention(**given))
 
 
+def test_the_library_refuses_states_that_share_memory():
+    refuses("fm_attention", attention(state=256, end=512))
+    refuses("fm_attention", attention(state=512, end=256))
+    refuses("fm_step", step(state=256, next=768))
+    refuses("fm_step", step(state=768, next=256))
+
+
 def test_the_library_refuses_attention_gradients():
     refuses("fm_attention_bwd", attention(go=0, gk=256))
     refuses("fm_attention_bwd", attention(gk=256))                         # shared heads: a workspace is needed
