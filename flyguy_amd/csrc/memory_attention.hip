@@ -31,7 +31,7 @@ struct Scans {
     Scan s[3];
     const float* log_decay;
     const void* starts;
-    long long n_moments, L;              // L: moments per segment (a multiple of CHUNK_MAX)
+    long long n_moments, L, L0;          // L: moments per segment, L0: of a stretch's first one (multiples of CHUNK_MAX)
     int wide, heads, n_seq, nseg, slots; // slots of segments: n_seq x nseg, or an upper bound for packed stretches
     int joined, scans;                   // the segments' start states are there (k_scan_join); the launch's scans
 };
@@ -56,6 +56,9 @@ __device__ __forceinline__ float log_decay_of(const Scans& a, int h) {
     return d < -1e30f ? -1e30f : d;
 }
 
+// the first moment of segment s of a stretch
+__device__ __forceinline__ long long start_of(const Scans& a, long long s) { return s ? a.L0 + (s - 1) * a.L : 0; }
+
 // Whole segments before moment `first` (at most n_moments <= 2^31, as L - 64 is).
 __device__ __forceinline__ int segments_before(const Scans& a, long long first) { return (int)((unsigned)first / (unsigned)a.L); }
 
@@ -71,8 +74,9 @@ __device__ __forceinline__ int first_slot(const Scans& a, int n, long long first
 __device__ __forceinline__ bool segment_of(const Scans& a, int block, int& n, int& seg, int& slot, long long& first,
                                            long long& count) {
     if (!a.starts || a.nseg == 1) {
-        n = block / a.nseg;
-        seg = block % a.nseg;
+        seg = block / a.n_seq;
+        n = block - seg * a.n_seq;
+        if (a.L0 != a.L) seg = a.nseg - 1 - seg;          // (the long segments first)
     } else if (block < a.n_seq) {
         n = block;
         seg = 0;
@@ -98,7 +102,7 @@ __device__ __forceinline__ bool segment_of(const Scans& a, int block, int& n, in
         if (seg < 1) return false;
     }
     slot = first_slot(a, n, first) + seg;
-    return seg == 0 || seg * a.L < count;
+    return seg == 0 || start_of(a, seg) < count;
 }
 
 // A state's value at (k, c) of the start state of stretch n, decayed once where the scan goes forwards (Z = l S).
@@ -330,7 +334,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
     count = shared_by_all(count);
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int w0 = 16 * NT * wave;                        // this wave's columns from here
-    const long long from = seg * a.L, left = count - from < a.L ? count - from : a.L;
+    const long long from = start_of(a, seg), most = seg ? a.L : a.L0, left = count - from < most ? count - from : most;
     const bool last = from + left == count;
     if (!OUT && last) return;                             // (the last segment's own state is needed by none)
     const float ld = shared_by_all(log_decay_of(a, h));
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
         const bool ready = a.nseg > 1 && a.joined, flip = !ready && s.transposed;
         const float* z0 = !OUT ? nullptr : ready ? s.seg + mine : s.init ? s.init + at : nullptr;
         const int zk = flip ? 1 : s.N, zc = flip ? s.K : 1, before = OUT && a.nseg > 1 && !a.joined ? seg : 0;
-        const Keep once(!ready && !s.backwards && count ? ld : 0.f), over(ld * (float)a.L);
+        const Keep once(!ready && !s.backwards && count ? ld : 0.f), over(ld * (float)a.L), over0(ld * (float)a.L0);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -365,7 +369,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
 #pragma unroll
                 for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) z[b][t][r] = over(z[b][t][r]) + own[min(row_of(b, r), s.K - 1) * s.N];
+                    for (int r = 0; r < 4; ++r) z[b][t][r] = (i ? over : over0)(z[b][t][r]) + own[min(row_of(b, r), s.K - 1) * s.N];
             }
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
@@ -711,7 +715,8 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     long long first, count;
     stretch_of(a, n, first, count);
     const float ld = log_decay_of(a, h);
-    const Keep once(count ? ld : 0.f), keep(ld * (float)a.L);    // (no moments: the state goes through as it is)
+    // (no moments: the state goes through as it is)
+    const Keep once(count ? ld : 0.f), keep(ld * (float)a.L), keep0(ld * (float)a.L0);
     vec z;
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -719,18 +724,19 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     const size_t step = (size_t)a.heads * s.K * s.N;
     float* p = s.seg + ((size_t)first_slot(a, n, first) * a.heads + h) * s.K * s.N + i;
     constexpr int AHEAD = 16;                             // segments' states under way at once
-    for (long long from = 0; from < count || from == 0; from += AHEAD * a.L, p += AHEAD * step) {
+    for (long long first_of = 0; !first_of || start_of(a, first_of) < count; first_of += AHEAD, p += AHEAD * step) {
         vec own[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j)
-            if (from + (j + 1) * a.L < count) own[j] = *reinterpret_cast<const vec*>(p + j * step);
+            if (start_of(a, first_of + j + 1) < count) own[j] = *reinterpret_cast<const vec*>(p + j * step);
             else own[j] = (vec)0.f;
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            if (j && from + j * a.L >= count) return;
+            if (j && start_of(a, first_of + j) >= count) return;
             *reinterpret_cast<vec*>(p + j * step) = z;
+            const Keep& over = first_of + j ? keep : keep0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) z[e] = keep(z[e]) + own[j][e];
+            for (int e = 0; e < V; ++e) z[e] = over(z[e]) + own[j][e];
         }
     }
 }
@@ -876,7 +882,7 @@ int groups_per_cu(int K, int N) {
 // packed ones are mixed, 20% where packed ones are all the same, 15% where one of them is four times the others.
 struct Cut {
     int nseg, slots, K, N, joined;
-    long long L;
+    long long L, L0;
 };
 // From this many values of a chain's segments up they are joined by a kernel of its own; fewer, each segment of the main pass
 // joins those before it as it begins (a launch less; 4 segments of 64 x 64: 143 us a learning step against 149 with the
@@ -892,6 +898,7 @@ Cut cut_of(const fm_attention_args& p, int scans) {
     c.slots = (int)p.n_seq;
     c.L = (p.n_moments + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
     if (!c.L) c.L = CHUNK_MAX;
+    c.L0 = c.L;
     if (!p.n_seq || !p.n_moments) return c;
     const int cap = p.dtype == FM_F32 ? groups_per_cu<float>(c.K, c.N) : p.dtype == FM_BF16 ? groups_per_cu<bf16>(c.K, c.N)
                                                                                             : groups_per_cu<f16>(c.K, c.N);
@@ -938,6 +945,25 @@ Cut cut_of(const fm_attention_args& p, int scans) {
         c.joined = 0;
     }
     c.nseg = (int)((p.n_moments + c.L - 1) / c.L);
+    c.L0 = c.L;
+    // More chains than half the workgroups that fit, but not all of them: a first segment so short that those left over, one
+    // after another, walk the first segments while the chains' workgroups walk the rest (8 x 4096 moments of 16 heads of 128
+    // values in bfloat16, the gradient's 384 chains:
+    // 753 -> 715 us a learning step).
+    const double fit = 256.0 * cap;
+    if (!packed && chains < fit && 2 * chains > fit) {
+        const double turns = ceil(chains / (fit - chains));
+        const long long L0 = (long long)(middle / (1 + turns)) / CHUNK_MAX * CHUNK_MAX;
+        const double rest = middle - L0, states = chains * c.K * c.N * 8;
+        const double t = (1.7 + one * cap) * (fmax(rest, turns * L0) / chunk + 0.3 * (1 + turns)) +
+                         pass(chains, (double)L0, (double)L0, 0.55 * 1.7, 0.2 * one) + 14 + states / 2 / 5.7e6;
+        if (L0 && t < best) {
+            c.L0 = L0;
+            c.L = (p.n_moments - L0 + CHUNK_MAX - 1) / CHUNK_MAX * CHUNK_MAX;
+            c.nseg = 2;
+            c.joined = 0;
+        }
+    }
     if (c.nseg > 1) c.slots = p.starts ? (int)(p.n_moments / c.L + p.n_seq) : (int)p.n_seq * c.nseg;
     return c;
 }
@@ -970,6 +996,7 @@ template <class T>
 void launch_scans(Scans& a, int count, const Cut& cut, bool vec, hipStream_t st) {
     if (!a.n_seq || !count) return;
     a.L = cut.L;
+    a.L0 = cut.L0;
     a.nseg = cut.nseg;
     a.slots = cut.slots;
     a.joined = cut.joined;

@@ -293,6 +293,29 @@ def test_many_short_stretches_and_a_few_long_ones(gpu_lib, dt):
     check_attention(q, k, v, decays(2), draw(gen, len(lengths), 2, 24, 32), starts)
 
 
+def test_more_chains_than_half_of_what_fits(gpu_lib):
+    """So many heads that the gradient's first segments are shorter than the rest: a few heads against the restatement."""
+    say("uneven segments")
+    from flyguy_amd.memory_hip import decay_attention
+    gen = torch.Generator().manual_seed(8)
+    H, T, K = 128, 2100, 128
+    q, k, v, go = (draw(gen, 1, T, H, K, dtype=BF16) for _ in range(4))
+    s, ge, g = draw(gen, 1, H, K, K), draw(gen, 1, H, K, K), decays(H)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, s)]
+    o, end = decay_attention(*leaves[:3], g, leaves[3])
+    grads = torch.autograd.grad([o, end], leaves, [go, ge])
+    few = [0, 61, 127]
+    f = [x[..., few, :].cpu().double() for x in (q, k, v)] + [x[:, few].cpu().double() for x in (s, ge)]
+    args = dict(log_decay=g[few].cpu(), starts=None, scale=K ** -0.5)
+    do = go[..., few, :].cpu().double()
+    want = ref.attention(*f[:3], state=f[3], go=do, gs=f[4], **args)
+    m = [x.abs() for x in f]
+    mag = ref.attention(*m[:3], state=m[3], go=do.abs(), gs=m[4], **args)
+    for i, (got, what) in enumerate(zip((o, end, *grads), ("o", "end state", "gradient of q", "of k", "of v", "of the state"))):
+        got = got[:, few] if i in (1, 5) else got[..., few, :]
+        ref.within(got, want[i], mag[i], 2 * K + T + 200, what, 2.0 ** -16)
+
+
 def test_starts_of_another_kind(gpu_lib):
     """int64 starts give the int32 ones' results; moments of no stretch give zeros, and take no gradient; starts beyond the
     moments, or falling, read nothing outside."""
