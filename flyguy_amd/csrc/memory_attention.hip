@@ -948,10 +948,9 @@ Cut cut_of(const fm_attention_args& p, int scans) {
     c.L0 = c.L;
     // More chains than half the workgroups that fit, but not all of them: a first segment so short that those left over, one
     // after another, walk the first segments while the chains' workgroups walk the rest (8 x 4096 moments of 16 heads of 128
-    // values in bfloat16, the gradient's 384 chains:
-    // 753 -> 715 us a learning step).
+    // values in bfloat16, the gradient's 384 chains: 753 -> 715 us a learning step).
     const double fit = 256.0 * cap;
-    if (!packed && chains < fit && 2 * chains > fit) {
+    if (!p.starts && chains < fit && 2 * chains > fit) {      // (packed stretches find their segments by L alone)
         const double turns = ceil(chains / (fit - chains));
         const long long L0 = (long long)(middle / (1 + turns)) / CHUNK_MAX * CHUNK_MAX;
         const double rest = middle - L0, states = chains * c.K * c.N * 8;
