@@ -759,6 +759,13 @@ __global__ __launch_bounds__(256) void k_share(const float* part_k, T* out_k, in
     out[i] = narrow<T>(s);
 }
 
+// moments of no stretch at all
+template <class T>
+__global__ __launch_bounds__(256) void k_zeros(T* out, long long n) {
+    const long long i = block_number() * 256 + threadIdx.x;
+    if (i < n) out[i] = (T)0.f;
+}
+
 // One moment: a workgroup takes CB columns of a row's state of one head, CB / 4 lanes a row of it, every (1024 / CB)th row a
 // lane, all a lane's loads under way at once; the lanes' shares of q S are joined over rows by shuffles, then in LDS.
 // VEC: 16-byte loads and stores of the states (v_dim a multiple of 4, states aligned).
@@ -849,7 +856,7 @@ const char* attention_wrong(const fm_attention_args& a, bool bwd, bool sizes_onl
     if (!a.log_decay) return "no decays";
     const bool any = a.n_seq && a.n_moments;
     if (any && (!a.q.data || !a.k.data || !a.v.data)) return "a null tensor";
-    if (!bwd && any && !a.o) return "a null tensor";
+    if (!bwd && a.n_moments && (a.n_seq || a.starts) && !a.o) return "a null tensor";
     if (!bwd && overlap(a.state, a.state_out, a.n_seq * a.q_heads * a.k_dim * a.v_dim)) return "state_out must not be state";
     if (bwd && any && !a.go.data) return "a null tensor";
     return nullptr;
@@ -1026,8 +1033,17 @@ bool wide_rows(const fm_attention_args& p, bool bwd) {
 }
 
 template <class T>
+void zeros(void* out, long long n, hipStream_t st) {
+    if (out && n) k_zeros<T><<<blocks_of((n + 255) / 256), 256, 0, st>>>((T*)out, n);
+}
+
+template <class T>
 void attention_fwd(const fm_attention_args& p, hipStream_t st) {
     const int share = (int)(p.q_heads / p.k_heads);
+    if (p.starts && !p.n_seq) {
+        zeros<T>(p.o, p.n_moments * p.q_heads * p.v_dim, st);
+        return;
+    }
     Scans a = scans_of(p);
     const Cut cut = cut_of(p, 1);
     float* seg = segment_floats(p, cut) ? (float*)p.workspace : nullptr;
@@ -1040,6 +1056,12 @@ template <class T>
 void attention_bwd(const fm_attention_args& p, hipStream_t st) {
     const int share = (int)(p.q_heads / p.k_heads), K = (int)p.k_dim, V = (int)p.v_dim;
     const float c = (float)p.scale;
+    if (p.starts && !p.n_seq) {
+        zeros<T>(p.gq, p.n_moments * p.q_heads * K, st);
+        zeros<T>(p.gk, p.n_moments * p.k_heads * K, st);
+        zeros<T>(p.gv, p.n_moments * p.k_heads * V, st);
+        return;
+    }
     const Cut cut = cut_of(p, 3);
     const long long floats = segment_floats(p, cut);
     float* seg[3];

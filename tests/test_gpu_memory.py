@@ -351,6 +351,28 @@ def test_no_moments(gpu_lib, dt):
     assert o.shape == (0, 0, 2, 24) and e.shape == (0, 2, 16, 24)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("Hk", [4, 2])
+def test_moments_of_no_stretch_at_all(gpu_lib, dt, Hk):
+    """Packed moments and no stretches: zeros, and gradients of zero, whatever the memory held before."""
+    from flyguy_amd.memory_hip import decay_attention
+    say(f"no stretch {dt} {Hk}")
+    gen = torch.Generator().manual_seed(18)
+    q, k, v = (draw(gen, 200, h, d, dtype=dt).requires_grad_() for h, d in ((4, 24), (Hk, 24), (Hk, 40)))
+    starts = torch.zeros(1, dtype=torch.int32, device="cuda")
+    go = draw(gen, 200, 4, 40, dtype=dt)
+    for _ in range(3):
+        held = [torch.full((200, 4, d), float("nan"), dtype=dt, device="cuda") for d in (24, 40, 24, 40)]
+        del held
+        o, e = decay_attention(q, k, v, decays(4), None, starts)
+        assert (o == 0).all() and e.shape == (0, 4, 24, 40)
+        held = [torch.full((200, 4, d), float("nan"), dtype=dt, device="cuda") for d in (24, 24, 40, 40)]
+        del held
+        for x, g in zip((q, k, v), torch.autograd.grad(o, (q, k, v), go)):
+            assert g.shape == x.shape and (g == 0).all()
+    decay_attention(q[:0], k[:0], v[:0], decays(4), None, starts)
+
+
 @pytest.mark.parametrize("dt,K,V", [(F32, 64, 64), (BF16, 64, 128), (BF16, 128, 48), (F16, 40, 40)])
 def test_a_later_moment_does_not_reach_an_earlier_one(gpu_lib, dt, K, V):
     """NaN and infinities at a moment leave the outputs before it, and the gradients after it, as they were, bit for bit;

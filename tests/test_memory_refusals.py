@@ -95,6 +95,10 @@ def test_the_library_refuses_attention(given):
     refuses("fm_attention", attention(**given))
 
 
+def test_the_library_refuses_packed_moments_without_an_output():
+    refuses("fm_attention", attention(n=0, starts=256, o=0))
+
+
 def test_the_library_refuses_states_that_share_memory():
     refuses("fm_attention", attention(state=256, end=512))
     refuses("fm_attention", attention(state=512, end=256))
