@@ -36,18 +36,69 @@ struct Scans {
     int joined, scans;                   // the segments' start states are there (k_scan_join); the launch's scans
 };
 
+// bound i of packed stretches: their start i, brought into the moments (past the last one: past every moment)
+__device__ __forceinline__ unsigned bound_of(const Scans& a, int i) {
+    const long long b = index_at(a.starts, min(i, a.n_seq), a.wide);
+    return i > a.n_seq ? ~0u : b < 0 ? 0u : b > a.n_moments ? (unsigned)a.n_moments : (unsigned)b;
+}
+
+// Packed moments belong to leaves of a search in rows of 8 bounds, in each row to the last one before the first bound past the
+// moment: leaf n < n_seq is stretch n, leaf n_seq what lies past the last one.  As such a search never goes back while the
+// moment goes on, leaves lie in order and share no moment whatever the starts are; where these do not fall, leaf n is
+// [starts[n], starts[n+1]).  Its moments are those from the largest of the bounds that the search passes, to the least of those
+// it stops at: the rows' 5 x 8 bounds in one load, and then the ends are bounds n and n + 1 unless a ballot finds others.
+// All 64 lanes come here together.
+constexpr int ROW_BITS = 3, ROWS = 5;    // 8^5 leaves
+__device__ __forceinline__ void leaf_of(const Scans& a, int n, long long& first, long long& count) {
+    n = __builtin_amdgcn_readfirstlane(n);
+    const int lane = threadIdx.x & 63, at = lane & 7, shift = (lane >> ROW_BITS) * ROW_BITS, digit = n >> shift & 7;
+    const unsigned bound = bound_of(a, ((n >> shift & ~7) + at) << shift);
+    const int row = __builtin_ctz(~n) / ROW_BITS;         // (bound n + 1 stands in the first row that it does not overflow)
+    unsigned low = __builtin_amdgcn_readlane((int)bound, n & 7);
+    unsigned high = __builtin_amdgcn_readlane((int)bound, 8 * row + (n >> row * ROW_BITS & 7) + 1);
+    high = min(high, (unsigned)a.n_moments);
+    if (__ballot((at <= digit && bound > low) || (at == digit + 1 && bound < high))) {
+        unsigned most = at <= digit ? bound : 0, least = at == digit + 1 ? bound : high;
+        for (int m = 1; m < 64; m <<= 1) {
+            most = max(most, (unsigned)__shfl_xor((int)most, m));
+            least = min(least, (unsigned)__shfl_xor((int)least, m));
+        }
+        low = __builtin_amdgcn_readfirstlane((int)most);
+        high = __builtin_amdgcn_readfirstlane((int)least);
+    }
+    first = low;
+    count = high > low ? high - low : 0;
+}
+// the leaf that moment t lies in, and its moments; -1: t lies before the first
+__device__ __forceinline__ int leaf_at(const Scans& a, unsigned t, long long& first, long long& count) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = a.n_seq;            // the last bound that is not past it, if none falls
+    while (lo < hi) {
+        const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
+        lo += __popcll(__ballot(at <= hi && bound_of(a, at) <= t)) * step;
+        hi = min(hi, lo + step - 1);
+    }
+    leaf_of(a, lo, first, count);
+    if (t >= first && t < first + count) return lo;
+    lo = 0;                              // some do, or t lies before the first: row by row
+    for (int shift = (ROWS - 1) * ROW_BITS; shift >= 0; shift -= ROW_BITS) {
+        const unsigned long long past = __ballot(lane > 7 || bound_of(a, lo + (lane << shift)) > t);
+        const int before = __builtin_ctzll(past);
+        if (!before) return -1;
+        lo += (before - 1) << shift;
+    }
+    leaf_of(a, lo, first, count);
+    return lo;
+}
+
 // the moments of stretch n: [first, first + count) of the views
 __device__ __forceinline__ void stretch_of(const Scans& a, int n, long long& first, long long& count) {
-    if (!a.starts) {
-        first = 0;
-        count = a.n_moments;
+    if (a.starts) {
+        leaf_of(a, n, first, count);
         return;
     }
-    long long b = index_at(a.starts, n, a.wide), e = index_at(a.starts, n + 1, a.wide);
-    b = b < 0 ? 0 : b > a.n_moments ? a.n_moments : b;
-    e = e < b ? b : e > a.n_moments ? a.n_moments : e;
-    first = b;
-    count = e - b;
+    first = 0;
+    count = a.n_moments;
 }
 
 // (-inf: 0 times it would not be 0; NaN stays NaN)
@@ -62,44 +113,34 @@ __device__ __forceinline__ long long start_of(const Scans& a, long long s) { ret
 // Whole segments before moment `first` (at most n_moments <= 2^31, as L - 64 is).
 __device__ __forceinline__ int segments_before(const Scans& a, long long first) { return (int)((unsigned)first / (unsigned)a.L); }
 
-// The slot of a packed stretch's first segment: its segments and the next stretch's never share one, as floor(b / L) + 1 +
-// floor((b + c) / L) - floor(b / L) >= ceil(c / L), and 1 for a stretch without moments.
+// The slot of a packed stretch's first segment: its segments and the next one's that has moments never share one, as floor(b /
+// L) + 1 + floor((b + c) / L) - floor(b / L) >= ceil(c / L).  (A stretch without moments uses none.)
 __device__ __forceinline__ int first_slot(const Scans& a, int n, long long first) {
     return !a.starts || a.nseg == 1 ? n * a.nseg : segments_before(a, first) + n;
 }
 // (stretch, segment, slot) of a workgroup; false: it has none.  Packed stretches: the first n_seq workgroups take their first
-// segments, workgroup n_seq + e the segment s > 0 of the stretch with floor(b / L) + s - 1 = e, which all 64 lanes look for.
-// So most search nothing, and those without a segment come last (k_scan): 37 stretches of 1,531 moments in the middle, 4 heads
-// of 64 x 128 values in bfloat16, take 98 us, 110 with a binary search by every workgroup and slots in the stretches' order.
+// segments, workgroup n_seq + e the segment s > 0 of the stretch with floor(b / L) + s - 1 = e, the one that moment (e + 1) L - 1
+// lies in.  So most search nothing, and those without a segment come last (k_scan): 37 stretches of 1,531 moments in the middle,
+// 4 heads of 64 x 128 values in bfloat16, take 98 us, 110 with a binary search by every workgroup and slots in the stretches'
+// order.
 __device__ __forceinline__ bool segment_of(const Scans& a, int block, int& n, int& seg, int& slot, long long& first,
                                            long long& count) {
     if (!a.starts || a.nseg == 1) {
         seg = block / a.n_seq;
         n = block - seg * a.n_seq;
         if (a.L0 != a.L) seg = a.nseg - 1 - seg;          // (the long segments first)
-    } else if (block < a.n_seq) {
-        n = block;
-        seg = 0;
+        stretch_of(a, n, first, count);
     } else {
-        const int e = block - a.n_seq, lane = threadIdx.x & 63;
-        int lo = 0, hi = a.n_seq - 1;    // the last stretch that does not begin past it
-        while (lo < hi) {
-            const int step = (hi - lo + 63) >> 6, at = lo + (lane + 1) * step;
-            bool before = at <= hi;
-            if (before) {
-                const long long b = index_at(a.starts, at, a.wide);
-                before = segments_before(a, b < 0 ? 0 : b > a.n_moments ? a.n_moments : b) <= e;
-            }
-            lo += __popcll(__ballot(before)) * step;
-            hi = min(hi, lo + step - 1);
+        const int e = block - a.n_seq;
+        if (e < 0) {
+            n = block;
+            seg = 0;
+            stretch_of(a, n, first, count);
+        } else {
+            n = leaf_at(a, (unsigned)((e + 1) * a.L - 1), first, count);
+            if (n < 0 || n == a.n_seq) return false;
+            seg = e - segments_before(a, first) + 1;
         }
-        n = lo;
-        seg = -1;
-    }
-    stretch_of(a, n, first, count);
-    if (seg < 0) {
-        seg = block - a.n_seq - segments_before(a, first) + 1;
-        if (seg < 1) return false;
     }
     slot = first_slot(a, n, first) + seg;
     return seg == 0 || start_of(a, seg) < count;
@@ -350,7 +391,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
         // the start state: the segment's where k_scan_join has left it, else the stretch's, decayed once where the scan goes
         // forwards (not at all if there are no moments: it goes through as it is), joined with the segments' own before this one
         const size_t step = (size_t)a.heads * s.K * s.N, mine = ((size_t)slot * a.heads + h) * s.K * s.N;
-        const bool ready = a.nseg > 1 && a.joined, flip = !ready && s.transposed;
+        const bool ready = a.nseg > 1 && a.joined && count, flip = !ready && s.transposed;
         const float* z0 = !OUT ? nullptr : ready ? s.seg + mine : s.init ? s.init + at : nullptr;
         const int zk = flip ? 1 : s.N, zc = flip ? s.K : 1, before = OUT && a.nseg > 1 && !a.joined ? seg : 0;
         const Keep once(!ready && !s.backwards && count ? ld : 0.f), over(ld * (float)a.L), over0(ld * (float)a.L0);
@@ -693,12 +734,14 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
     }
     if (OUT && a.starts && out && seg == 0 && (n == 0 || n == a.n_seq - 1)) {
         // moments of no stretch, before the first one and after the last, give zeros
+        long long past, rest;
+        leaf_of(a, a.n_seq, past, rest);
         for (int e = tid; e < s.N * size; e += 64 * WAVES) {
             char* all = out + (size_t)h * s.N * size + e;
             if (n == 0)
                 for (long long t = 0; t < first; ++t) all[t * so_] = 0;
             if (n == a.n_seq - 1)
-                for (long long t = first + count; t < a.n_moments; ++t) all[t * so_] = 0;
+                for (long long t = past; t < past + rest; ++t) all[t * so_] = 0;
         }
     }
 }
@@ -711,12 +754,11 @@ __global__ __launch_bounds__(256) void k_scan_join(Scans a) {
     typedef float vec __attribute__((ext_vector_type(V)));
     const Scan& s = a.s[blockIdx.z];
     const int h = blockIdx.x % a.heads, n = blockIdx.y, i = (blockIdx.x / a.heads * 256 + threadIdx.x) * V;
-    if (i >= s.K * s.N) return;
     long long first, count;
     stretch_of(a, n, first, count);
+    if (i >= s.K * s.N || !count) return;                 // (without moments there are no segments)
     const float ld = log_decay_of(a, h);
-    // (no moments: the state goes through as it is)
-    const Keep once(count ? ld : 0.f), keep(ld * (float)a.L), keep0(ld * (float)a.L0);
+    const Keep once(ld), keep(ld * (float)a.L), keep0(ld * (float)a.L0);
     vec z;
 #pragma unroll
     for (int j = 0; j < V; ++j)

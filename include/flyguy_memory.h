@@ -54,7 +54,8 @@ long long fm_turn_partial(const fm_turn_args* a);
  * k_dim, v_dim <= 128.  A value that is not finite reaches no output of an earlier moment (no gradient of a later one), and no
  * other stretch; the outputs that it does reach are NaN, or infinite.
  * Stretches: n_seq of n_moments moments each, or (starts not 0) packed: n_moments in all, stretch n being moments starts[n] ..
- * starts[n+1] - 1 (int32, or int64 if wide; out of [0, n_moments] or falling: clamped), the views' seq unread.  o: dense
+ * starts[n+1] - 1 (int32, or int64 if wide; out of [0, n_moments]: brought into it), the views' seq unread.  Where starts fall,
+ * stretches are cut short so that no two share a moment.  o: dense
  * [moments][q_heads][v_dim].  state, state_out: float32 [n_seq][q_heads][k_dim][v_dim]
  * (state_out 0: not wanted; it must not overlap state).  A stretch without moments passes its state on.
  * Gradients (fm_attention_bwd): go of o, gstate_out of state_out (0: zeros); gq, gk, gv dense like their tensors, gstate

@@ -78,6 +78,24 @@ def attention(q, k, v, log_decay, state, scale, starts=None, go=None, gs=None):
             dv.unflatten(1, (-1, share)).sum(2).reshape(shape["v"]), ds)
 
 
+def risen(starts, moments):
+    """Starts that do not fall, with the same stretches as `starts` where the library gives each moment to one of them: a search
+    in rows of 8 bounds, in each up to the first bound past the moment."""
+    b, n_seq = [min(max(x, 0), moments) for x in starts], len(starts) - 1
+    out = [b[0]]
+    for n in range(n_seq):
+        lo, low, high = 0, 0, moments
+        for step in (4096, 512, 64, 8, 1):
+            passed = (n - lo) // step + 1
+            low = max(low, *(b[lo + i * step] for i in range(passed)), 0)
+            if passed < 8 and lo + passed * step <= n_seq:
+                high = min(high, b[lo + passed * step])
+            lo += (passed - 1) * step
+        assert high <= low or low == out[-1]       # (stretches follow each other)
+        out.append(max(high, out[-1]) if high > low else out[-1])
+    return out
+
+
 def within(got, want, magnitude, count, what, extra=0.0):
     """|got - want| at most (count u + extra) magnitude plus the rounding of got's type (and of its smallest numbers)."""
     got64 = got.detach().cpu().double()

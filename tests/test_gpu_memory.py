@@ -337,6 +337,46 @@ def test_starts_of_another_kind(gpu_lib):
     torch.cuda.synchronize()
 
 
+FALLING = [[150, 20, 400, -3], [0, 60, 30, 200], [7, 190, 3, 195, 100, 110, 200], [200, 0], [90, 10, 20, 30], [0, 0, -9, 5, 5]]
+
+
+@pytest.mark.parametrize("dt,wide", [(F32, False), (BF16, True)])
+@pytest.mark.parametrize("case", range(len(FALLING) + 5))
+def test_starts_that_fall(gpu_lib, case, dt, wide):
+    """No two stretches share a moment, whatever the starts: values and gradients are those of starts that do not fall with the
+    same stretches; of a few stretches, those that begin at the largest start so far."""
+    from flyguy_amd.memory_hip import decay_attention
+    say(f"falling {case} {dt}")
+    rng = random.Random(case)
+    if case < len(FALLING):
+        starts, M = FALLING[case], 200
+    else:
+        n_seq, M = ((5, 3000), (63, 4000), (64, 4000), (700, 9000), (4100, 30000))[case - len(FALLING)]
+        starts = sorted(rng.randint(-50, M + 50) for _ in range(n_seq + 1))
+        for _ in range(max(2, n_seq // 9)):
+            starts[rng.randrange(n_seq + 1)] = rng.randint(-50, M + 50)
+    same = ref.risen(starts, M)
+    if len(starts) <= 8:
+        b, top = [min(max(x, 0), M) for x in starts], 0
+        for n, x in enumerate(b):
+            top = max(top, x)
+            assert same[n] == top
+    gen = torch.Generator().manual_seed(case)
+    q, k, v = (draw(gen, M, h, d, dtype=dt).requires_grad_() for h, d in ((2, 24), (1, 24), (1, 32)))
+    n = len(starts) - 1
+    s, go, ge = draw(gen, n, 2, 24, 32).requires_grad_(), draw(gen, M, 2, 32, dtype=dt), draw(gen, n, 2, 24, 32)
+    outs = []
+    for st in (starts, same):
+        st = torch.tensor(st, dtype=torch.int64 if wide else torch.int32, device="cuda")
+        held = [torch.full((M, 2, 32), float("nan"), dtype=dt, device="cuda") for _ in range(6)]
+        del held
+        o, e = decay_attention(q, k, v, decays(2), s, st)
+        outs.append((o, e, *torch.autograd.grad([o, e], [q, k, v, s], [go, ge])))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert (outs[0][0][:same[0]] == 0).all() and (outs[0][0][same[-1]:] == 0).all()
+
+
 @pytest.mark.parametrize("dt", [F32, BF16])
 def test_no_moments(gpu_lib, dt):
     """No moments pass the state on, both ways; no stretches give nothing."""
