@@ -34,6 +34,7 @@ struct Scans {
     long long n_moments, L, L0;          // L: moments per segment, L0: of a stretch's first one (multiples of CHUNK_MAX)
     int wide, heads, n_seq, nseg, slots; // slots of segments: n_seq x nseg, or an upper bound for packed stretches
     int joined, scans;                   // the segments' start states are there (k_scan_join); the launch's scans
+    int clearing;                        // places after the slots' for the outputs of moments that are in no stretch
 };
 
 // bound i of packed stretches: their start i, brought into the moments (past the last one: past every moment)
@@ -348,6 +349,26 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int row
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
+// The outputs of the moments before the first stretch and after the last one: zeros, by all 256 threads of each of the workgroups
+// that come after the slots'.  (A pack of 4,096 moments in a place for 262,144, 8 heads of 128 values, bfloat16: 6,014 us cleared byte by byte
+// in the stretches' own workgroups, 438 by these.)
+__device__ __forceinline__ void clear_outside(const Scans& a, const Scan& s, int size, long long share) {
+    const long long shares = (long long)a.clearing * a.heads, row = (long long)a.heads * s.N * size;
+    if (!s.out || share >= shares) return;
+    long long past, rest;
+    leaf_of(a, a.n_seq, past, rest);
+    auto clear = [&](uintptr_t from, uintptr_t to) {      // (the ends up to a multiple of 16 bytes one by one)
+        const uintptr_t up = (from + 15) & ~(uintptr_t)15, down = to & ~(uintptr_t)15, lo = up < to ? up : to,
+                        hi = down > lo ? down : lo;
+        if (share == 0 && threadIdx.x < lo - from) ((char*)from)[threadIdx.x] = 0;
+        if (share == 0 && threadIdx.x < to - hi) ((char*)hi)[threadIdx.x] = 0;
+        for (uintptr_t p = lo + 16 * (share * 256 + threadIdx.x); p < hi; p += 16 * 256 * shares)
+            *(uint4*)p = make_uint4(0, 0, 0, 0);
+    };
+    clear((uintptr_t)s.out, (uintptr_t)s.out + bound_of(a, 0) * row);
+    clear((uintptr_t)s.out + past * row, (uintptr_t)s.out + (past + rest) * row);
+}
+
 template <class T, int KT, int NT, bool VEC, bool OUT>
 __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void k_scan(Scans a) {
     using S = Tile<T, KT, NT, OUT>;
@@ -364,7 +385,11 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
     const unsigned block = (unsigned)block_number(), group = block / a.heads, place_in = group / a.scans;
     const int h = (int)(block - group * a.heads);
     const Scan& s = a.s[group - place_in * a.scans];
-    if (place_in >= (unsigned)a.slots) return;
+    if (place_in >= (unsigned)a.slots) {
+        if (OUT && a.clearing)
+            clear_outside(a, s, s.wide ? 4 : (int)sizeof(T), (long long)(place_in - a.slots) * a.heads + h);
+        return;
+    }
     int n, seg, slot;
     long long first, count;
     if (!segment_of(a, (int)place_in, n, seg, slot, first, count)) return;
@@ -732,18 +757,6 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
                     }
         }
     }
-    if (OUT && a.starts && out && seg == 0 && (n == 0 || n == a.n_seq - 1)) {
-        // moments of no stretch, before the first one and after the last, give zeros
-        long long past, rest;
-        leaf_of(a, a.n_seq, past, rest);
-        for (int e = tid; e < s.N * size; e += 64 * WAVES) {
-            char* all = out + (size_t)h * s.N * size + e;
-            if (n == 0)
-                for (long long t = 0; t < first; ++t) all[t * so_] = 0;
-            if (n == a.n_seq - 1)
-                for (long long t = past; t < past + rest; ++t) all[t * so_] = 0;
-        }
-    }
 }
 
 // Segments' start states from their own: Z_0 = the stretch's, Z_{s+1} = l^L Z_s + own_s, in place; 4 values a lane (K x N a
@@ -1020,19 +1033,21 @@ long long segment_floats(const fm_attention_args& p, const Cut& c) {
     return c.nseg == 1 ? 0 : (long long)c.slots * p.q_heads * p.k_dim * p.v_dim;
 }
 
+constexpr int CLEARING = 256;            // workgroups of a packed launch that clear: one a CU
 template <class T, int KT, int NT, bool VEC>
 void launch_form(Scans& a, int count, hipStream_t st) {
     int most = 1;
     for (int i = 0; i < count; ++i) most = a.s[i].K * a.s[i].N > most ? a.s[i].K * a.s[i].N : most;
     const dim3 grid = blocks_of((long long)a.slots * a.heads * count);
     a.scans = count;
+    a.clearing = a.starts ? (CLEARING + a.heads * count - 1) / (a.heads * count) : 0;
     if (a.nseg > 1) {
         k_scan<T, KT, NT, VEC, false><<<grid, 64 * WAVES, 0, st>>>(a);
         auto blocks = [&](int v) { return dim3((most / v + 255) / 256 * a.heads, a.n_seq, count); };
         if (a.joined && most % 4 == 0) k_scan_join<4><<<blocks(4), 256, 0, st>>>(a);
         else if (a.joined) k_scan_join<1><<<blocks(1), 256, 0, st>>>(a);
     }
-    k_scan<T, KT, NT, VEC, true><<<grid, 64 * WAVES, 0, st>>>(a);
+    k_scan<T, KT, NT, VEC, true><<<blocks_of((long long)(a.slots + a.clearing) * a.heads * count), 64 * WAVES, 0, st>>>(a);
 }
 template <class T, bool VEC>
 void launch_sized(Scans& a, int count, const Cut& c, hipStream_t st) {

@@ -337,6 +337,32 @@ def test_starts_of_another_kind(gpu_lib):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dt,V", [(F32, 24), (BF16, 7), (F16, 40)])
+@pytest.mark.parametrize("Hk", [3, 1])
+def test_a_pack_with_room_before_and_behind(gpu_lib, dt, V, Hk):
+    """Two stretches in the middle of a place for many times as much: the values and gradients of the stretches alone, zeros
+    elsewhere, whatever the memory held."""
+    from flyguy_amd.memory_hip import decay_attention
+    say(f"room {dt} {V} {Hk}")
+    gen = torch.Generator().manual_seed(19)
+    M, b, n = 5003, 1501, 333
+    q, k, v, go = (draw(gen, M, h, d, dtype=dt) for h, d in ((3, 8), (Hk, 8), (Hk, V), (3, V)))
+
+    def both(q, k, v, go, starts):
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+        held = [torch.full((M, 3, d), float("nan"), dtype=dt, device="cuda") for d in (8, 8, V, V, V)]
+        del held
+        o, e = decay_attention(*leaves, decays(3), None, torch.tensor(starts, dtype=torch.int32, device="cuda"))
+        return (o, *torch.autograd.grad([o, e], leaves, [go, torch.ones_like(e)])), e
+    got, e = both(q, k, v, go, [b, b + 100, b + n])
+    want, e2 = both(*(x[b:b + n] for x in (q, k, v, go)), [0, 100, n])
+    for x, y in zip(got, want):
+        small = {F32: 1e-5, BF16: 2.0 ** -7, F16: 2.0 ** -10}[dt]      # (other segments: sums in another order, one more rounding)
+        torch.testing.assert_close(x[b:b + n], y, rtol=small, atol=small * float(y.detach().abs().max()))
+        assert (x[:b] == 0).all() and (x[b + n:] == 0).all()
+    torch.testing.assert_close(e, e2, rtol=1e-5, atol=1e-5 * float(e2.detach().abs().max()))
+
+
 FALLING = [[150, 20, 400, -3], [0, 60, 30, 200], [7, 190, 3, 195, 100, 110, 200], [200, 0], [90, 10, 20, 30], [0, 0, -9, 5, 5]]
 
 
