@@ -56,6 +56,7 @@ struct Pool {
     std::atomic<unsigned> sense{0};
     const float* x = nullptr;              // the car being decided
     float* out = nullptr;
+    float* firing = nullptr;
     unsigned char* tap = nullptr;
 };
 
@@ -106,7 +107,7 @@ void barrier(CpuNet& n, unsigned& local) {
 
 // Thread t's part of one car.  Rows [r0, r1) of every layer are its own: it computes and fires them (and writes
 // their tap bytes); the sources it reads are every thread's rows of the layer below, final after the barrier.
-void decide_part(CpuNet& n, int t, const float* x, float* out, unsigned char* tap, unsigned& local) {
+void decide_part(CpuNet& n, int t, const float* x, float* out, float* firing, unsigned char* tap, unsigned& local) {
     const bool multi = n.threads > 1;
     float* cur = n.a.data();
     float* nxt = n.b.data();
@@ -173,6 +174,8 @@ void decide_part(CpuNet& n, int t, const float* x, float* out, unsigned char* ta
             barrier(n, local);
         }
     }
+    if (firing && t == 0)
+        for (int j = 0; j < n.n_dn; ++j) firing[j] = cur[n.readout_rows[j]];
     const int a0 = multi ? n.act_r[t] : 0, a1 = multi ? n.act_r[t + 1] : n.n_act;
     for (int a = a0; a < a1; ++a) {
         const float* wa = n.ro_w.data() + (size_t)a * n.n_dn;
@@ -200,7 +203,7 @@ void worker(CpuNet* n, int t) {
         }
         if (p.stop.load(std::memory_order_acquire)) return;
         seen = j;
-        decide_part(*n, t, p.x, p.out, p.tap, local);
+        decide_part(*n, t, p.x, p.out, p.firing, p.tap, local);
     }
 }
 
@@ -343,6 +346,10 @@ void fly_set_threads(void* p, int threads) {
 }
 
 void fly_forward(void* p, const float* obs, int batch, float* logits, unsigned char* tap) {
+    flyinfer_firing(p, obs, batch, logits, nullptr, tap);
+}
+
+void flyinfer_firing(void* p, const float* obs, int batch, float* logits, float* firing, unsigned char* tap) {
     CpuNet* n = (CpuNet*)p;
     if (!n || !n->ready() || !obs || !logits) return;
     if (n->threads > 1) {
@@ -363,11 +370,13 @@ void fly_forward(void* p, const float* obs, int batch, float* logits, unsigned c
     for (int c = 0; c < batch; ++c) {
         const float* x = obs + (size_t)c * n->obs_dim;
         float* out = logits + (size_t)c * n->n_act;
+        float* top = firing ? firing + (size_t)c * n->n_dn : nullptr;
         unsigned char* tp = c == 0 ? tap : nullptr;
         if (n->threads > 1) {
             Pool& pl = *n->pool;
             pl.x = x;
             pl.out = out;
+            pl.firing = top;
             pl.tap = tp;
             {
                 std::lock_guard<std::mutex> lk(pl.mu);
@@ -375,7 +384,7 @@ void fly_forward(void* p, const float* obs, int batch, float* logits, unsigned c
             }
             pl.cv.notify_all();
         }
-        decide_part(*n, 0, x, out, tp, local);
+        decide_part(*n, 0, x, out, top, tp, local);
     }
 }
 

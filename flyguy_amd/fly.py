@@ -28,6 +28,7 @@ from __future__ import annotations
 from collections.abc import Mapping
 from typing import NamedTuple
 import struct
+import threading
 from pathlib import Path
 
 import numpy as np
@@ -246,9 +247,9 @@ class FlyActor(nn.Module):
         return out
 
     def _walk(self, x: torch.Tensor, product, by_neuron: bool, watch=None, activate=None) -> torch.Tensor:
-        """Logits of a batch: the plug's product plus bias gives the sensory drive, each hop's product (plus the
-        drive of its re-driven sensory rows) the next layer's input, every neuron fires relu(gain z - softplus
-        theta), and the read-out maps the descending rows to the actions (fly.py:286-305 / 170-185 / 252-284).
+        """The descending neurons' firing [B, descending] of a batch, which the read-out maps to the actions: the plug's
+        product plus bias gives the sensory drive, each hop's product (plus the drive of its re-driven sensory rows) the
+        next layer's input, and every neuron fires relu(gain z - softplus theta) (fly.py:286-305 / 170-185 / 252-284).
         States are [rows, B] when by_neuron, else [B, rows]; product(k, layer, weights, states) is layer k's sparse
         product (k = 0: the plug).  activate(z, gain, threshold) computes the firing of [rows, B] states from the
         rows' gains and thresholds (default: PyTorch's elementwise operations).  watch(h) sees every layer's
@@ -283,7 +284,7 @@ class FlyActor(nn.Module):
             if watch is not None:
                 watch(h)
         top = h.index_select(axis, self.dn_rows)
-        return self.out(top.t() if by_neuron else top)
+        return top.t() if by_neuron else top
 
     def _walk_tiled(self, obs: torch.Tensor) -> torch.Tensor:
         """_walk on the library's float32 kernels with the states [B/32, rows, 32] throughout (HopHip's layer form): a
@@ -308,7 +309,7 @@ class FlyActor(nn.Module):
         for layer in layers[1:]:
             h = fire(product(layer, self.w.index_select(0, layer.edges), h, None, drive), layer.nid)
         top = h.index_select(1, self.dn_rows)
-        return self.out(top.transpose(1, 2).reshape(B, -1))
+        return top.transpose(1, 2).reshape(B, -1)
 
     # ---- CPU play
     def _host_decider(self) -> "_HostDecider | None":
@@ -342,26 +343,35 @@ class FlyActor(nn.Module):
         return held[1]
 
     @torch.no_grad()
-    def _play(self, obs: torch.Tensor) -> torch.Tensor:
+    def _play(self, obs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """A decision on the CPU (the bot): the CPU decision library when it is there, else sparse CSR products of
-        the current weights (fly.py:186-284).  A visualizer tap (self.tap) gets the first sample's firing."""
+        the current weights (fly.py:186-284) -> (logits, the descending neurons' firing).  A visualizer tap (self.tap)
+        gets the first sample's firing."""
         tap = getattr(self, "tap", None)
         dec = self._host_decider()
         if dec is not None:
             return dec.decide(obs, tap)
         mats = self._host_matrices()
         first = [] if tap is not None else None
-        logits = self._walk(obs.t().contiguous(), lambda k, layer, w, h: torch.sparse.mm(mats[k], h),
-                            by_neuron=True, watch=(lambda h: first.append(h[:, 0])) if first is not None else None)
+        top = self._walk(obs.t().contiguous(), lambda k, layer, w, h: torch.sparse.mm(mats[k], h),
+                         by_neuron=True, watch=(lambda h: first.append(h[:, 0])) if first is not None else None)
         if tap is not None:
             tap(first)
-        return logits
+        return self.out(top), top
 
     # ---- forward
     def forward(self, obs: torch.Tensor, extra: torch.Tensor | None = None) -> torch.Tensor:
+        return self.with_firing(obs)[0]
+
+    def with_firing(self, obs: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(the logits of a batch, the descending neurons' firing [B, descending] that they are read from)."""
         obs = obs.double() if self.w.dtype == torch.float64 else obs.float()    # (float64: an actor made .double())
         if not obs.is_cuda and not torch.is_grad_enabled():
             return self._play(obs)
+        top = self._firing(obs)
+        return self.out(top), top
+
+    def _firing(self, obs: torch.Tensor) -> torch.Tensor:
         if self.kernel != "torch" and obs.is_cuda and obs.shape[0] % 32 == 0:      # (at any batch size)
             from .fly_hip import FireHip, HopHip
             half = self.kernel == "cuda16"
@@ -457,7 +467,7 @@ class _HostDecider:
             vp, ci = ctypes.c_void_p, ctypes.c_int
             sig = {"fly_create": (vp, [ci, ci, ci]), "fly_set_plug": (None, [vp, ci, ci] + [vp] * 6),
                    "fly_set_hop": (None, [vp, ci, ci, ci, ci] + [vp] * 6), "fly_set_out": (None, [vp, ci, vp, vp, vp]),
-                   "fly_forward": (None, [vp, vp, ci, vp, vp]), "fly_free": (None, [vp]),
+                   "flyinfer_firing": (None, [vp, vp, ci, vp, vp, vp]), "fly_free": (None, [vp]),
                    "fly_set_threads": (None, [vp, ci])}
             for name, (res, args) in sig.items():
                 fn = getattr(L, name)
@@ -475,7 +485,8 @@ class _HostDecider:
             return a.ctypes.data
 
         i32, f32 = np.int32, np.float32
-        self.n_act = f.out.out_features
+        self.n_act, self.n_dn = f.out.out_features, f.out.in_features
+        self.busy = threading.Lock()       # (a handle decides for one thread at a time)
         with torch.no_grad():
             thr = nn.functional.softplus(f.theta)
             self.h = L.fly_create(f.obs_dim, self.n_act, f.hops)
@@ -495,19 +506,24 @@ class _HostDecider:
                 L.fly_set_threads(self.h, int(threads))
         self.shade = np.zeros(int(sum(f.sizes)), np.uint8)
 
-    def decide(self, obs: torch.Tensor, tap=None) -> torch.Tensor:
+    def decide(self, obs: torch.Tensor, tap=None) -> tuple[torch.Tensor, torch.Tensor]:
+        """(logits, the descending neurons' firing)."""
         x = np.ascontiguousarray(obs.detach().numpy(), dtype=np.float32)
-        out = np.empty((x.shape[0], self.n_act), np.float32)
-        self.library().fly_forward(self.h, x.ctypes.data, x.shape[0], out.ctypes.data,
-                                   self.shade.ctypes.data if tap is not None else None)
-        if tap is not None:
-            tap(self.shade)
-        return torch.from_numpy(out)
+        out, top = np.empty((x.shape[0], self.n_act), np.float32), np.empty((x.shape[0], self.n_dn), np.float32)
+        with self.busy:
+            if not self.h:
+                raise RuntimeError("FlyActor: a weight changed while another thread was deciding")
+            self.library().flyinfer_firing(self.h, x.ctypes.data, x.shape[0], out.ctypes.data, top.ctypes.data,
+                                              self.shade.ctypes.data if tap is not None else None)
+            if tap is not None:
+                tap(self.shade)
+        return torch.from_numpy(out), torch.from_numpy(top)
 
     def close(self) -> None:
-        if self.h:
-            self.library().fly_free(self.h)
-            self.h = None
+        with self.busy:
+            if self.h:
+                self.library().fly_free(self.h)
+                self.h = None
 
 
 class VizTap:

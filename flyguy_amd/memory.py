@@ -72,15 +72,8 @@ class MemoryActor(nn.Module):
         n = obs.shape[0]
         if obs.is_cuda and n % 32:                # (the library's products take batches of whole tiles)
             obs = torch.cat([obs, obs.new_zeros(-n % 32, obs.shape[1])])
-        seen = []
-        hook = self.actor.out.register_forward_pre_hook(lambda _, args: seen.append(args[0]))
-        try:
-            # (without gradients a CPU actor decides in compiled code, which keeps the firing to itself)
-            with torch.set_grad_enabled(torch.is_grad_enabled() or not obs.is_cuda):
-                logits = self.actor(obs)
-        finally:
-            hook.remove()
-        return logits[:n], seen[0][:n]
+        logits, firing = self.actor.with_firing(obs)
+        return logits[:n], firing[:n]
 
     def _heads(self, firing: torch.Tensor):
         return self.proj(firing).split([self.heads * self.dim, self.k_heads * self.dim, self.k_heads * self.dim], -1)

@@ -4,6 +4,7 @@ taught what no single moment shows."""
 from __future__ import annotations
 
 import re
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -59,6 +60,51 @@ def test_only_what_was_seen_counts():
         a, b = m(x)[0], m(y)[0]
     torch.testing.assert_close(a[:, :9], b[:, :9], rtol=1e-5, atol=1e-5)
     assert (a[:, 9:] - b[:, 9:]).abs().max() > 1e-3
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_threads_that_share_an_actor(grad):
+    """Two threads play through one MemoryActor, and a third through another with the same actor: each gets what it gets alone."""
+    m, other = net(), net()
+    other.actor = m.actor
+    xs = [torch.randn(60, 1, 517) for _ in range(3)]
+
+    def play(m, x):
+        live, out = m.state(1), []
+        with torch.set_grad_enabled(grad):
+            for t in range(60):
+                if grad:
+                    y, live = m(x[t][:, None], live)
+                    out.append(y[:, 0].detach())
+                else:
+                    out.append(m.step(x[t], live))
+        return torch.stack(out), live[0].detach()
+    nets = (m, m, other)
+    alone = [play(n, x) for n, x in zip(nets, xs)]
+    with ThreadPoolExecutor(3) as pool:
+        for _ in range(3):
+            for got, want in zip(pool.map(play, nets, xs), alone):
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_cpu_play_is_the_actors(monkeypatch):
+    """A step on the CPU decides in compiled code, without gradients: a fresh memory gives the actor's logits bit for bit, and
+    both forms of play the same firing."""
+    m = net()
+    torch.nn.init.zeros_(m.back.weight)
+    x, grads = torch.randn(4, 517), []
+    walk = FlyActor._walk
+    monkeypatch.setattr(FlyActor, "_walk", lambda *a, **kw: grads.append(torch.is_grad_enabled()) or walk(*a, **kw))
+    with torch.no_grad():
+        want = m.actor(x)
+        assert torch.equal(m.step(x, m.state(4)), want) and not grads
+        _, firing = m.actor.with_firing(x)
+        top = m.actor._firing(x)
+    assert grads == [False] and (firing > 0).any()
+    torch.testing.assert_close(firing, top, rtol=1e-5, atol=1e-5)
+    logits, again = m.actor.with_firing(x)                     # (with gradients)
+    torch.testing.assert_close(again, firing, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(logits, want, rtol=1e-5, atol=1e-5)
 
 
 def test_heads_must_share():
