@@ -9,7 +9,7 @@ the next (flyguy/fly.py:286-305 decides each moment alone).
 
 Queries and keys are [stretches, moments, heads, values] (decay_step: [rows, heads, values]), float32, bfloat16 or
 binary16, on the GPU, with any strides whose last is 1 (another last stride costs a copy); query heads share key / value
-heads in consecutive groups.  The first three have gradients.  Work goes to the current stream; nothing synchronises.
+heads in consecutive groups.  The first three have gradients (backwards, of the first order; tables and decays are fixed).  Work goes to the current stream; nothing synchronises.
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ import struct
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from ._lib import LibraryError, check, lib
@@ -109,6 +110,13 @@ def _wants_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors)
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """The library's calls take no tangents along: forward-mode derivatives would come out as zero."""
+    if forward_ad._current_level >= 0 and any(isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None
+                                              for x in tensors):
+        raise RuntimeError(f"{what}: has no forward-mode derivative")
+
+
 _NONE = (0, 0, 0, 0)
 
 
@@ -139,6 +147,7 @@ class _Plan:
 
 
 def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
+    _no_tangents(what, q, k, table)
     _heads(what, 4, q) if k is None else _heads(what, 4, q, k)
     N, T, H, D = q.shape
     if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != D):
@@ -151,6 +160,8 @@ def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
         if not isinstance(table, torch.Tensor) or table.dim() != 3 or table.shape[2] != 2 or \
                 table.dtype != torch.float32 or table.device != q.device:
             raise ValueError(f"{what}: the table must be float32 [positions, rotated / 2, 2] on the same GPU (rotary_table)")
+        if _wants_grad(table):
+            raise ValueError(f"{what}: the table is fixed; one that requires a gradient would get none")
         table = table if table.is_contiguous() else table.contiguous()
         p.rotated = 2 * table.shape[1]
         if p.rotated > D:
@@ -222,6 +233,7 @@ def rotary(q, k, table, positions=None, interleaved: bool = False):
 def norm_rotary(q, k, wq, wk, table=None, positions=None, interleaved: bool = False, eps: float = 1e-6):
     """Each head of q and k divided by its root mean square (eps added to the mean square) and multiplied by wq / wk
     (float32 [values], shared by the heads), then turned as by rotary (table None: not turned), in one pass over memory."""
+    _no_tangents("norm_rotary", wq, wk)
     p = _plan("norm_rotary", q, k, table, positions, interleaved, eps)
     D = q.shape[3]
     wq = _floats("norm_rotary", "wq", wq, (D,), q.device)
@@ -318,6 +330,7 @@ def decay_attention(q, k, v, log_decay, state=None, starts=None, scale: float | 
     moments starts[n] .. starts[n + 1] - 1 (any length, 0 too; moments of no stretch give zeros).
     Returns (o in q's type, the state after each stretch).  Gradients of q, k, v and state; the decays are fixed."""
     what = "decay_attention"
+    _no_tangents(what, q, k, v, log_decay, state)
     dims = 4 if starts is None else 3
     _heads(what, dims, q, k, v)
     _shared(what, q, k, v, dims - 2)
@@ -351,9 +364,10 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
     on from, by default its own number; below 0: the row is idle (zeros, no state touched); past the states: NaN, no state
     touched.  No two rows of a call may name one slot.  No gradients."""
     what = "decay_step"
+    _no_tangents(what, q, k, v, log_decay, state, into)
     _heads(what, 3, q, k, v)
     _shared(what, q, k, v, 1)
-    if _wants_grad(q, k, v, state):
+    if _wants_grad(q, k, v, state, into):
         raise ValueError(f"{what}: has no gradients; decay_attention has")
     n, Hq, K = q.shape
     V, dev = v.shape[2], q.device

@@ -7,6 +7,7 @@ import random
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import memory_helpers as ref
 from gpu_helpers import say
@@ -540,6 +541,24 @@ def test_a_gradient_is_refused_where_it_would_be_wrong(gpu_lib):
         changed.add_(0)
         with pytest.raises(RuntimeError, match="modified by an inplace"):
             out.backward()
+
+
+def test_what_gets_no_gradient_is_refused(gpu_lib):
+    """Tables, decays and a step's states that ask for one; where gradients are off, a table that would ask is taken."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step, norm_rotary, rotary, rotary_table
+    q, w, s, g = torch.zeros(1, 6, 2, 16, device="cuda"), torch.ones(16, device="cuda"), torch.zeros(1, 2, 16, 16, device="cuda"), decays(2)
+    table = rotary_table(8, 16, device="cuda").requires_grad_()
+    for f in (lambda: rotary(q, q, table), lambda: norm_rotary(q, q, w, w, table)):
+        with pytest.raises(ValueError, match="table is fixed"):
+            f()
+        with torch.no_grad():
+            f()
+    with pytest.raises(ValueError, match="decays are fixed"):
+        decay_attention(q, q, q, g.clone().requires_grad_())
+    with pytest.raises(ValueError, match="no gradients"):
+        decay_step(q[:, 0], q[:, 0], q[:, 0], g, s, into=torch.zeros_like(s).requires_grad_())
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        rotary(forward_ad.make_dual(q, q), None, table.detach())
 
 
 def test_a_state_that_a_step_has_changed_is_found_out(gpu_lib):

@@ -6,6 +6,7 @@ import math
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from flyguy_amd._lib import LibraryError, check, lib
 from flyguy_amd.memory_hip import _ATTENTION, _STEP, _TURN, decay_attention, decay_step, norm_rotary, rotary, rotary_table
@@ -48,6 +49,28 @@ def test_tensors_off_the_gpu():
                                                                                      torch.zeros(1, 3, 4, 4))):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_forward_mode():
+    """A tangent is refused wherever it comes in: it would be dropped."""
+    q, w, s, g = torch.zeros(1, 2, 3, 4), torch.ones(4), torch.zeros(1, 3, 4, 4), torch.zeros(3)
+    table = rotary_table(2, 4)
+    calls = {"rotary": (rotary, [q, q, table], (0, 1, 2)), "norm_rotary": (norm_rotary, [q, q, w, w, table], range(5)),
+             "decay_attention": (decay_attention, [q, q, q, g, s], range(5)),
+             "decay_step": (decay_step, [q[:, 0], q[:, 0], q[:, 0], g, s], range(5))}
+    for name, (f, args, places) in calls.items():
+        for i in places:
+            with forward_ad.dual_level():
+                given = [forward_ad.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate(args)]
+                with pytest.raises(RuntimeError, match=f"{name}: has no forward-mode"):
+                    f(*given)
+
+            def at(x):
+                return f(*[x if j == i else y for j, y in enumerate(args)])
+            with pytest.raises(RuntimeError, match=f"{name}: has no forward-mode"):
+                torch.func.jvp(at, (args[i],), (torch.ones_like(args[i]),))
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="GPU"):      # (no tangent among them)
+        rotary(q, q, table)
 
 
 def refuses(name, args):
