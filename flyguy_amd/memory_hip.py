@@ -88,6 +88,15 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _like(x: torch.Tensor | None) -> torch.Tensor | None:
+    """Memory for as many values as x, in x's order where that leaves a head's values side by side (views whose rows overlap,
+    as unfold's, can come out with another dimension innermost)."""
+    if x is None:
+        return None
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 or y.shape[-1] == 1 else x.new_empty(x.shape)
+
+
 def _heads(what: str, dims: int, *tensors) -> None:
     """Every tensor on one GPU, of one type and `dims` dimensions."""
     first = tensors[0]
@@ -185,7 +194,7 @@ def _plan(what, q, k, table, positions, interleaved, eps) -> _Plan:
 
 def _turn(p: _Plan, q, k, wq, wk):
     q, k = _rows(q), None if k is None else _rows(k)
-    yq, yk = torch.empty_like(q), None if k is None else torch.empty_like(k)
+    yq, yk = _like(q), _like(k)
     _call("fm_turn", q, p.pack((q, k), (yq, yk), (None, None), (wq, wk), (None, None), None))
     return yq, yk
 
@@ -207,7 +216,7 @@ class TurnHip(torch.autograd.Function):
         p = ctx.p
         q, k, gq = None if q is None else _rows(q), None if k is None else _rows(k), _rows(gq)
         gk = None if not p.heads[1] else _rows(gk)
-        yq, yk = torch.empty_like(gq), None if gk is None else torch.empty_like(gk)
+        yq, yk = _like(gq), _like(gk)
         gwq = torch.empty_like(wq) if wq is not None and ctx.needs_input_grad[2] else None
         gwk = torch.empty_like(wk) if wk is not None and ctx.needs_input_grad[3] else None
         partial = None

@@ -132,6 +132,35 @@ def test_norm_gradient_against_differences(gpu_lib):
         assert abs(float((grad.double() * way.double()).sum()) - float(want)) <= 8 * h * h * terms + noise
 
 
+OVERLAPPING = [((1, 3, 2, 4), (50, 8, 1, 1)), ((2, 5, 3, 64), (40, 3, 1, 1)), ((2, 9, 2, 8), (0, 1, 0, 1)),
+               ((2, 20, 1, 24), (64, 1, 1, 1)), ((1, 7, 3, 16), (0, 0, 0, 1))]
+
+
+@pytest.mark.parametrize("shape,strides", OVERLAPPING)
+def test_rows_that_overlap(gpu_lib, shape, strides):
+    """Views whose rows share values (windows, expanded tensors): what a copy of them gives, in memory of its own, and its
+    gradients too."""
+    from flyguy_amd.memory_hip import decay_attention, norm_rotary, rotary, rotary_table
+    say(f"overlapping {shape} {strides}")
+    gen = torch.Generator().manual_seed(20)
+    q = draw(gen, 400).as_strided(shape, strides)
+    D, w, g = shape[-1], draw(gen, shape[-1]), draw(gen, 400).as_strided(shape, strides)
+    table = rotary_table(shape[1], D, device="cuda")
+    d = decays(shape[2])
+
+    def all_of(q, g):
+        x = q.detach().requires_grad_()
+        a, b = rotary(x, x, table)
+        c, _ = norm_rotary(x, None, w, None, table)
+        o, _ = decay_attention(x, x, x, d)
+        for y in (a, b, c, o):
+            assert y.stride(-1) == 1
+        return [a, b, c, o, *(torch.autograd.grad(y, x, g, retain_graph=True)[0] for y in (a, b, c, o))]
+    # (the copy's strides may take another form of the kernels: the same numbers up to a few roundings)
+    for y, want in zip(all_of(q, g), all_of(q.contiguous(), g.contiguous())):
+        torch.testing.assert_close(y, want, rtol=1e-5, atol=1e-5 * float(want.detach().abs().max()))
+
+
 def test_positions(gpu_lib):
     """None, an int, one row for all, int32, int64, and strided positions name the same turns; outside the table: NaN."""
     from flyguy_amd.memory_hip import rotary, rotary_table

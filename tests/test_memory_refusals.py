@@ -9,7 +9,7 @@ import torch
 from torch.autograd import forward_ad
 
 from flyguy_amd._lib import LibraryError, check, lib
-from flyguy_amd.memory_hip import _ATTENTION, _STEP, _TURN, decay_attention, decay_step, norm_rotary, rotary, rotary_table
+from flyguy_amd.memory_hip import _ATTENTION, _STEP, _TURN, _like, decay_attention, decay_step, norm_rotary, rotary, rotary_table
 
 
 def test_tables():
@@ -49,6 +49,16 @@ def test_tensors_off_the_gpu():
                                                                                      torch.zeros(1, 3, 4, 4))):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_memory_like_a_view():
+    """As many values, a head's side by side, whatever view asks."""
+    for shape, strides in (((1, 3, 2, 4), (50, 8, 1, 1)), ((2, 5, 3, 64), (40, 3, 1, 1)), ((2, 9, 2, 8), (0, 1, 0, 1)),
+                           ((2, 3, 4, 8), (96, 8, 24, 1)), ((2, 3, 4, 1), (12, 4, 1, 7))):
+        y = _like(torch.zeros(1000).as_strided(shape, strides))
+        assert y.shape == shape and (y.stride(-1) == 1 or shape[-1] == 1) and y.untyped_storage().nbytes() == 4 * y.numel()
+    x = torch.zeros(2, 4, 3, 8).transpose(1, 2)
+    assert _like(x).stride() == x.stride() and _like(None) is None
 
 
 def test_forward_mode():
