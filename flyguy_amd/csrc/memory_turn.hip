@@ -296,6 +296,9 @@ __global__ __launch_bounds__(256) void k_turn_units_bwd(fm_turn_args a, Lanes l)
     }
 }
 
+// what this wave loads is there (other lanes' stores may follow, to the same places)
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // Any sizes and strides: one wave per row (a head of a moment), lanes over its values; a partner's value is read again (a
 // cache hit).
 template <class T, int NE>
@@ -321,16 +324,19 @@ __global__ __launch_bounds__(64 * TURN_ROWS) void k_turn(fm_turn_args a, float s
     }
     if (w) r = rsqrtf(wave_sum(sum, 64) / D + (float)a.eps);
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
+    for (int i = 0; i < NE; ++i) {                        // (all partners are read before anything is written: y may be x)
         const int e = lane + 64 * i;
         if (e >= D) continue;
-        float z = v[i] * r * (w ? w[e] : 1.f);
+        v[i] *= r * (w ? w[e] : 1.f);
         if (e < R) {
             const Turn u = turn_of(e, cs, R, a.interleaved);
-            z = z * u.c + widen(x[u.partner]) * r * (w ? w[u.partner] : 1.f) * (sign * u.s);
+            v[i] = v[i] * u.c + widen(x[u.partner]) * r * (w ? w[u.partner] : 1.f) * (sign * u.s);
         }
-        y[e] = narrow<T>(z);
     }
+    loads_done();
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+        if (lane + 64 * i < D) y[lane + 64 * i] = narrow<T>(v[i]);
 }
 
 // Its gradient with a norm (see k_turn_units_bwd).
@@ -381,6 +387,7 @@ __global__ __launch_bounds__(64 * TURN_ROWS) void k_turn_bwd(fm_turn_args a) {
 #pragma unroll
             for (int i = 0; i < NE; ++i) z[i] = r * (z[i] - v[i] * dot);
         }
+        loads_done();
 #pragma unroll
         for (int i = 0; i < NE; ++i)
             if (lane + 64 * i < D) y[lane + 64 * i] = narrow<T>(z[i]);

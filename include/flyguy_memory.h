@@ -32,7 +32,8 @@ typedef struct fm_view {
  * table: float32 [n_positions][rotated/2][2] (rotated 0: no rotation).  A moment's position is positions[n pos_seq + t
  * pos_moment] (int32, or int64 if wide) + first; positions 0: t + first.  A position outside the table gives NaN in the
  * rotated values.  Gradients (fm_turn_bwd): x the forward's inputs (read only where weight is not 0), g the gradients of y, y
- * the gradients of x, written; gweight: the weights' gradients, written; partial: fm_turn_partial() floats. */
+ * the gradients of x, written; gweight: the weights' gradients, written; partial: fm_turn_partial() floats.  y may be x itself
+ * (gradients: x or g), with the same strides; otherwise what is written must lie outside what is read. */
 typedef struct fm_turn_args {
     fm_view x[2], y[2], g[2];
     const float* weight[2];

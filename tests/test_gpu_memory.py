@@ -161,6 +161,40 @@ def test_rows_that_overlap(gpu_lib, shape, strides):
         torch.testing.assert_close(y, want, rtol=1e-5, atol=1e-5 * float(want.detach().abs().max()))
 
 
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("D,R,il,dt,how", [(100, 50, False, F32, "dense"), (100, 100, False, BF16, "odd"), (100, 98, True, F16, "odd"),
+                                           (33, 32, False, F32, "dense"), (511, 510, False, BF16, "dense"),
+                                           (128, 128, False, F32, "odd"), (128, 106, False, BF16, "dense"),
+                                           (64, 64, False, BF16, "packed"), (96, 64, True, F32, "packed"), (200, 130, False, F16, "odd")])
+def test_in_place(gpu_lib, D, R, il, dt, how, norm):
+    """The library writes over what it reads, queries and keys alike, bit for bit what it writes elsewhere; gradients over the
+    outputs' and over the inputs."""
+    from flyguy_amd.memory_hip import _call, _plan, rotary_table
+    say(f"in place {D} {R} {il} {dt} {how} {norm}")
+    gen = torch.Generator().manual_seed(21)
+    x = [laid_out(draw(gen, 2, 9, h, D, dtype=dt), how) for h in (3, 2)]
+    g = [laid_out(draw(gen, 2, 9, h, D, dtype=dt), how) for h in (3, 2)]
+    w = [1 + 0.2 * draw(gen, D) for _ in range(2)] if norm else [None, None]
+    p = _plan("test", *x, rotary_table(9, R, device="cuda"), None, il, 1e-6)
+
+    def copies(xs):
+        return [laid_out(y.contiguous().clone(), how) for y in xs]
+
+    def forward(xs, ys):
+        _call("fm_turn", xs[0], p.pack(xs, ys, (None, None), w, (None, None), None))
+        return ys
+
+    def backward(xs, gs, ys):
+        _call("fm_turn_bwd", gs[0], p.pack(xs, ys, gs, w, (None, None), None))
+        return ys
+    want, a = forward(x, copies(x)), copies(x)
+    for y, z in zip(want, forward(a, a)):
+        assert torch.equal(y, z)
+    want, a, b = backward(x, g, copies(x)), copies(g), copies(x)
+    for y, z, u in zip(want, backward(x, a, a), backward(b, g, b)):
+        assert torch.equal(y, z) and torch.equal(y, u)
+
+
 def test_positions(gpu_lib):
     """None, an int, one row for all, int32, int64, and strided positions name the same turns; outside the table: NaN."""
     from flyguy_amd.memory_hip import rotary, rotary_table
