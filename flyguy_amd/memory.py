@@ -43,11 +43,15 @@ def _decay_attention_cpu(q, k, v, log_decay, state):
 
 class MemoryActor(nn.Module):
     """actor: a FlyActor.  heads query heads of dim values share k_heads key / value heads; the slowest head remembers about
-    `longest` moments, the fastest 8.  positions: the most moments a car's stretch may have (the rotation's table)."""
+    `longest` moments, the fastest 8.  positions: moments of the rotation's table.  A stretch from an empty memory may not be
+    longer; a car that goes on past it keeps its memory, whose moments from there on all count as the table's last one, so that
+    newer ones are no longer told apart by their distance."""
 
     def __init__(self, actor: FlyActor, heads: int = 8, k_heads: int | None = None, dim: int = 64, longest: float = 2048.0,
                  positions: int = 65536):
         super().__init__()
+        if positions < 1:
+            raise ValueError("MemoryActor: at least one position")
         k_heads = heads if k_heads is None else k_heads
         if heads % k_heads:
             raise ValueError("MemoryActor: heads must be a multiple of k_heads")
@@ -78,14 +82,19 @@ class MemoryActor(nn.Module):
     def _heads(self, firing: torch.Tensor):
         return self.proj(firing).split([self.heads * self.dim, self.k_heads * self.dim, self.k_heads * self.dim], -1)
 
+    def _at(self, moments: torch.Tensor) -> torch.Tensor:
+        return moments.clamp_max(len(self.table) - 1)
+
     def forward(self, obs: torch.Tensor, state: tuple | None = None):
         """Stretches of consecutive moments obs [cars, moments, observation] -> (logits [cars, moments, actions], the
         memory after them)."""
         N, T = obs.shape[:2]
+        if state is None and T > len(self.table):
+            raise ValueError(f"MemoryActor: a stretch of {T} moments; positions is {len(self.table)}")
         mem, seen = self.state(N) if state is None else state
         logits, firing = self._see(obs.flatten(0, 1))
         q, k, v = (x.unflatten(-1, (-1, self.dim)) for x in self._heads(firing.unflatten(0, (N, T))))
-        at = seen[:, None] + torch.arange(T, device=obs.device, dtype=torch.int32)
+        at = self._at(seen[:, None] + torch.arange(T, device=obs.device, dtype=torch.int32))
         if obs.is_cuda:
             q, k = norm_rotary(q, k, self.wq, self.wk, self.table, at, eps=EPS)
             o, mem = decay_attention(q, k, v, self.log_decay, mem)
@@ -105,7 +114,7 @@ class MemoryActor(nn.Module):
             return logits[:, 0]
         logits, firing = self._see(obs)
         q, k, v = (x.unflatten(-1, (-1, self.dim)) for x in self._heads(firing))
-        q, k = norm_rotary(q[:, None], k[:, None], self.wq, self.wk, self.table, seen[:, None], eps=EPS)
+        q, k = norm_rotary(q[:, None], k[:, None], self.wq, self.wk, self.table, self._at(seen[:, None]), eps=EPS)
         o = decay_step(q[:, 0], k[:, 0], v, self.log_decay, mem)
         seen += 1
         return logits + self.back(o.flatten(-2))

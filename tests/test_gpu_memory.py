@@ -840,6 +840,30 @@ def test_memory_actor_on_the_gpu(gpu_lib):
     assert rel(played.cpu(), out.detach().cpu()) <= 1e-4 and live[1].tolist() == [75] * 3
 
 
+def test_an_actor_past_its_table(gpu_lib):
+    """Cars that play on past the table: the CPU form's logits and memory (to the bars above), by moments and by stretches."""
+    import copy
+
+    from conftest import lively, toy
+    from flyguy_amd.fly import FlyActor
+    from flyguy_amd.memory import MemoryActor
+    from gpu_helpers import rel
+    torch.manual_seed(4)
+    f = lively(FlyActor(toy("a"), 517, 90, hops=3), 4)
+    f.kernel = "hip"
+    m = MemoryActor(f, heads=4, k_heads=2, dim=24, positions=10)
+    with torch.no_grad():
+        m.back.weight.normal_(0, 0.3)
+        x, g = torch.randn(3, 25, 517), copy.deepcopy(m).cuda()
+        live, cpu = g.state(3), m.state(3)
+        played = torch.stack([g.step(x[:, t].cuda(), live) for t in range(25)], 1)
+        want = torch.stack([m.step(x[:, t], cpu) for t in range(25)], 1)
+        a, st = g(x[:, :7].cuda())
+        b, (mem, _) = g(x[:, 7:].cuda(), st)
+    assert rel(played.cpu(), want) <= 1e-4 and rel(live[0].cpu(), cpu[0]) <= 1e-4
+    assert rel(torch.cat([a, b], 1).cpu(), want) <= 1e-4 and rel(mem.cpu(), cpu[0]) <= 1e-4
+
+
 def test_the_teaching_command_on_the_gpu(gpu_lib, tmp_path, capsys):
     import numpy as np
 

@@ -62,6 +62,29 @@ def test_only_what_was_seen_counts():
     assert (a[:, 9:] - b[:, 9:]).abs().max() > 1e-3
 
 
+def test_past_the_table():
+    """A car that goes on past the table keeps a memory of numbers, its later moments at the table's last position, however it is
+    read; a stretch from the start that is longer is refused."""
+    m, x = net(positions=8), torch.randn(2, 30, 517)
+    far = net(positions=64)
+    far.table[8:] = far.table[7]
+    with torch.no_grad():
+        want, (mem, _) = far(x)
+        live = m.state(2)
+        played = torch.stack([m.step(x[:, t], live) for t in range(30)], 1)
+        a, st = m(x[:, :6])
+        b, (mem2, seen) = m(x[:, 6:], st)
+    assert torch.isfinite(played).all() and live[1].tolist() == seen.tolist() == [30] * 2
+    torch.testing.assert_close(played, want, rtol=1e-4, atol=1e-4)
+    torch.testing.assert_close(torch.cat([a, b], 1), want, rtol=1e-4, atol=1e-4)
+    for got in (live[0], mem2):
+        torch.testing.assert_close(got, mem, rtol=1e-4, atol=1e-4)
+    with pytest.raises(ValueError, match="positions is 8"):
+        m(x[:, :9])
+    with pytest.raises(ValueError, match="one position"):
+        net(positions=0)
+
+
 @pytest.mark.parametrize("grad", [False, True])
 def test_threads_that_share_an_actor(grad):
     """Two threads play through one MemoryActor, and a third through another with the same actor: each gets what it gets alone."""
