@@ -333,7 +333,7 @@ def _shared(what, q, k, v, first: int) -> None:
 
 
 def decay_attention(q, k, v, log_decay, state=None, starts=None, scale: float | None = None):
-    """Linear attention with a decay for each query head, l = exp(log_decay[head]): S_t = l S_{t-1} + k_t v_t^T, o_t = scale
+    """Linear attention with a decay for each query head, l = exp(log_decay[head]) (log_decay at most 1): S_t = l S_{t-1} + k_t v_t^T, o_t = scale
     q_t S_t (scale: values^-0.5 unless given), from `state` (float32 [stretches, q heads, values, v values]; None: zeros).
     starts (int32 / int64 [stretches + 1] on the GPU): q, k, v are packed, [moments, heads, values], and stretch n is
     moments starts[n] .. starts[n + 1] - 1 (any length, 0 too; moments of no stretch give zeros).

@@ -49,8 +49,8 @@ int fm_turn(const fm_turn_args* a, void* stream);
 int fm_turn_bwd(const fm_turn_args* a, void* stream);
 long long fm_turn_partial(const fm_turn_args* a);
 
-/* Linear attention with a decay for each query head, l = exp(log_decay[h]) (log_decay 0 keeps everything, -inf nothing; above 0
- * states grow until they overflow); query head h reads key / value head h / (q_heads / k_heads):
+/* Linear attention with a decay for each query head, l = exp(log_decay[h]) (log_decay 0 keeps everything, -inf nothing; above 0,
+ * at most 1, states grow until they overflow); query head h reads key / value head h / (q_heads / k_heads):
  *   S_t = l S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   S_{-1} = state (0: zeros)
  * k_dim, v_dim <= 128.  A value that is not finite reaches no output of an earlier moment (no gradient of a later one), and no
  * other stretch; the outputs that it does reach are NaN, or infinite.

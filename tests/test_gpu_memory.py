@@ -481,6 +481,79 @@ def test_no_moments(gpu_lib, dt):
     assert o.shape == (0, 0, 2, 24) and e.shape == (0, 2, 16, 24)
 
 
+@pytest.mark.parametrize("lengths", [None, [0, 0], [0, 5, 0], [70, 0, 2500, 0]])
+def test_no_moments_pass_any_state_on(gpu_lib, lengths):
+    """Infinities and NaN too, bit for bit, and so the end state's gradient; at any decay."""
+    from flyguy_amd.memory_hip import decay_attention
+    say(f"pass on {lengths}")
+    gen = torch.Generator().manual_seed(22)
+    n = 3 if lengths is None else len(lengths)
+    s, ge = (draw(gen, n, 6, 16, 24) for _ in range(2))
+    for x in (s, ge):
+        x[:, :, 3, 5], x[:, :, 0, 1], x[:, :, 15, 23] = math.inf, -math.inf, math.nan
+    if lengths is None:
+        q, k, v = (torch.empty(3, 0, 6, d, device="cuda") for d in (16, 16, 24))
+        st, empty = None, range(3)
+    else:
+        starts = [0]
+        for x in lengths:
+            starts.append(starts[-1] + x)
+        q, k, v = (draw(gen, starts[-1], 6, d) for d in (16, 16, 24))
+        st, empty = torch.tensor(starts, dtype=torch.int32, device="cuda"), [i for i, x in enumerate(lengths) if not x]
+    s.requires_grad_()
+    _, e = decay_attention(q, k, v, decays(6), s, st)
+    g, = torch.autograd.grad(e, s, ge)
+    for i in empty:
+        assert torch.equal(e[i].view(torch.int32), s[i].view(torch.int32)), i
+        assert torch.equal(g[i].view(torch.int32), ge[i].view(torch.int32)), i
+
+
+@pytest.mark.parametrize("T", [1, 64, 130, 3000])
+def test_a_state_kept_whole(gpu_lib, T):
+    """A decay of 1 leaves an infinite entry of the state infinite."""
+    from flyguy_amd.memory_hip import decay_attention, decay_step
+    gen = torch.Generator().manual_seed(23)
+    q, k, v, s = inputs(gen, 1, T, 1, 1, 32, 32, F32, "dense", True)
+    s[0, 0, 3, 5], s[0, 0, 9, 1] = math.inf, -math.inf
+    g, into = torch.zeros(1, device="cuda"), torch.empty_like(s)
+    decay_step(q[:, 0], k[:, 0], v[:, 0], g, s, into=into)
+    for e in (decay_attention(q, k, v, g, s)[1], into):
+        assert e[0, 0, 3, 5] == math.inf and e[0, 0, 9, 1] == -math.inf
+        assert torch.equal(torch.isfinite(e), torch.isfinite(s))
+
+
+@pytest.mark.parametrize("K,V", [(16, 16), (128, 128)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_growing_states_that_are_zero_for_long(gpu_lib, dt, K, V):
+    """log_decay 1: what is zero stays zero over any number of moments, forwards and backwards."""
+    from flyguy_amd.memory_hip import decay_attention
+    say(f"growing {dt} {K}")
+    gen = torch.Generator().manual_seed(24)
+    T, n = 65536, 40
+    q, k, v, go = (draw(gen, 1, T, 1, d, dtype=dt) for d in (K, K, V, V))
+    g = torch.ones(1, device="cuda")
+    late = k.clone()
+    late[:, :-n] = 0
+    o, e = decay_attention(q, late, v, g)
+    f = [x[:, -n:].cpu().double() for x in (q, k, v)]
+    want = ref.attention(*f, g.cpu(), None, K ** -0.5)
+    mag = ref.attention(*[x.abs() for x in f], g.cpu(), None, K ** -0.5)
+    extra = 2.0 ** -16 if dt == BF16 else 0.0
+    assert (o[:, :-n] == 0).all()
+    ref.within(o[:, -n:], want[0], mag[0], K + V + n + 200, "o", extra)
+    ref.within(e, want[1], mag[1], K + V + n + 200, "end state", extra)
+    early_q, leaves = q.clone(), [k.clone().requires_grad_(), v.clone().requires_grad_()]
+    early_q[:, n:] = 0
+    go[:, n:] = 0
+    grads = torch.autograd.grad(decay_attention(early_q, *leaves, g)[0], leaves, go)
+    f = [x[:, :n].cpu().double() for x in (q, k, v, go)]
+    want = ref.attention(*f[:3], g.cpu(), None, K ** -0.5, go=f[3])
+    mag = ref.attention(*[x.abs() for x in f[:3]], g.cpu(), None, K ** -0.5, go=f[3].abs())
+    for i, x in zip((3, 4), grads):
+        assert (x[:, n:] == 0).all()
+        ref.within(x[:, :n], want[i], mag[i], K + V + n + 200, "gradient", extra)
+
+
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
 @pytest.mark.parametrize("Hk", [4, 2])
 def test_moments_of_no_stretch_at_all(gpu_lib, dt, Hk):
