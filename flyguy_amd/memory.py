@@ -65,6 +65,26 @@ class MemoryActor(nn.Module):
         self.register_buffer("log_decay", -torch.exp2(-memory).float())
         self.register_buffer("table", rotary_table(positions, dim - dim % 2), persistent=False)
 
+    def checkpoint(self, graph: str) -> dict:
+        """What MemoryActor.load reads: the memory, and the actor that it was taught on (as flyguy_amd.teach writes actors)."""
+        held = {k: v.detach().cpu() for k, v in self.state_dict().items()}
+        return {"memory": {k: v for k, v in held.items() if not k.startswith("actor.")},
+                "model": {k: v for k, v in held.items() if k.startswith("actor.")},
+                "config": {"heads": self.heads, "k_heads": self.k_heads, "dim": self.dim, "positions": len(self.table),
+                           "observation": self.actor.obs_dim, "actions": self.actor.out.out_features,
+                           "model": {"fly_graph": str(graph), "fly_hops": self.actor.hops, "fly_fan": self.actor.fan}}}
+
+    @classmethod
+    def load(cls, path, graph: str | None = None) -> "MemoryActor":
+        """A MemoryActor from a checkpoint (flyguy_amd.remember writes them); graph: where the actor's graph lies now."""
+        ck = torch.load(path, map_location="cpu", weights_only=True)
+        c = ck["config"]
+        m = c["model"]
+        net = cls(FlyActor(graph or m["fly_graph"], c["observation"], c["actions"], hops=m["fly_hops"], fan=m["fly_fan"]),
+                  heads=c["heads"], k_heads=c["k_heads"], dim=c["dim"], positions=c["positions"])
+        net.load_state_dict({**ck["memory"], **ck["model"]})
+        return net
+
     def state(self, cars: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The memory of cars that have seen nothing: (states, moments seen)."""
         dev = self.log_decay.device

@@ -7,7 +7,8 @@
 DATA: FLYD files or FLYR recordings of the bot as flyguy_amd.teach reads them, their moments in the order they were played;
 the answers are those in the files, or a fly-actor --teacher's.  The actor itself (--start, or a fresh one) stays as it is:
 what is taught are the memory's projections, norms and read-out (MemoryActor), by KL(teacher || student) over whole
-stretches.  At the end a stretch is played moment by moment from an empty memory, and compared with the stretch read at once.
+stretches.  Memory and actor are written out together; flyguy_amd.memory.MemoryActor.load reads them.  At the end a stretch is
+played moment by moment from an empty memory, and compared with the stretch read at once.
 """
 from __future__ import annotations
 
@@ -25,9 +26,11 @@ from .teach import _actor_weights, kl_to, moments
 
 
 def _actor(graph: str, checkpoint: Path | None, hops: int, kernel: str) -> FlyActor:
-    f = FlyActor(graph, 517, 90, hops=hops)
-    if checkpoint is not None:
-        f.load_state_dict(_actor_weights(torch.load(checkpoint, map_location="cpu", weights_only=True)), strict=False)
+    ck = {} if checkpoint is None else torch.load(checkpoint, map_location="cpu", weights_only=True)
+    cfg = (ck.get("config") or {}).get("model", {})
+    f = FlyActor(graph, 517, 90, hops=int(cfg.get("fly_hops", hops)), fan=int(cfg.get("fly_fan", 16)))
+    if ck:
+        f.load_state_dict(_actor_weights(ck), strict=False)
     f.kernel = kernel
     return f.requires_grad_(False)
 
@@ -38,7 +41,7 @@ def main(argv=None) -> int:
     ap.add_argument("--graph", required=True)
     ap.add_argument("--start", type=Path, default=None)
     ap.add_argument("--teacher", type=Path, default=None)
-    ap.add_argument("--hops", type=int, default=3)
+    ap.add_argument("--hops", type=int, default=3, help="hops of an actor whose checkpoint does not say")
     ap.add_argument("--stretch", type=int, default=256)
     ap.add_argument("--cars", type=int, default=16, help="stretches per step")
     ap.add_argument("--steps", type=int, default=500)
@@ -51,6 +54,8 @@ def main(argv=None) -> int:
     ap.add_argument("--kernel", default="hip", choices=["hip", "torch"])
     ap.add_argument("--seed", type=int, default=0)
     args = ap.parse_args(argv)
+    if min(args.steps, args.cars, args.stretch) < 1:
+        raise SystemExit("--steps, --cars and --stretch are at least 1")
     dev = torch.device(args.device)
     torch.manual_seed(args.seed)
     rng = np.random.default_rng(args.seed)
@@ -94,8 +99,7 @@ def main(argv=None) -> int:
             print(f"step {step:,} | KL {now:.4f} | {step * x.shape[0] * x.shape[1] / (time.time() - began):,.0f} moments/s",
                   flush=True)
     args.out.parent.mkdir(parents=True, exist_ok=True)
-    torch.save({"memory": {k: v.detach().cpu() for k, v in net.state_dict().items() if not k.startswith("actor.")},
-                "config": {"heads": args.heads, "dim": args.dim}, "taught_steps": args.steps}, args.out)
+    torch.save({**net.checkpoint(args.graph), "taught_steps": args.steps}, args.out)
 
     x, _ = draw()
     with torch.no_grad():

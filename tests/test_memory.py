@@ -159,6 +159,39 @@ def test_teaching_a_memory(tmp_path, capsys):
     assert set(saved["memory"]) == {"proj.weight", "wq", "wk", "back.weight", "log_decay"}
 
 
+def test_a_taught_memory_is_read_back(tmp_path, monkeypatch):
+    """What the command writes decides as what it taught, with the actor it was taught on: a fresh one, or a checkpoint's with
+    hops and a fan of its own."""
+    rng = np.random.default_rng(6)
+    data = tmp_path / "game.bin"
+    ot.write_chunk(data, rng.standard_normal((60, 517)).astype(np.float16), (3 * rng.standard_normal((60, 90))).astype(np.float16))
+    f = lively(FlyActor(toy("a"), 517, 90, hops=2, fan=7), 6)
+    torch.save({"model": {"actor." + k: v for k, v in f.state_dict().items()}, "config": {"model": {"fly_hops": 2, "fly_fan": 7}}},
+               tmp_path / "actor.pt")
+    taught, init = [], MemoryActor.__init__
+    monkeypatch.setattr(MemoryActor, "__init__", lambda self, *a, **kw: taught.append(self) or init(self, *a, **kw))
+    x = torch.randn(2, 11, 517)
+    for start in ([], ["--start", str(tmp_path / "actor.pt")]):
+        assert main(["--data", str(data), "--graph", str(GOLDEN / "toy_a.npz"), "--stretch", "12", "--cars", "3", "--steps", "4",
+                     "--heads", "4", "--dim", "12", "--device", "cpu", "--out", str(tmp_path / "m.pt"), *start]) == 0
+        net = MemoryActor.load(tmp_path / "m.pt")
+        with torch.no_grad():
+            assert torch.equal(net(x)[0], taught[-2](x)[0])
+        assert net.actor.hops == (2 if start else 3) and len(net.table) == 65536
+        if start:
+            assert torch.equal(net.actor.w, f.w) and torch.equal(net.actor.in_w, f.in_w)
+    (tmp_path / "elsewhere.npz").write_bytes((GOLDEN / "toy_a.npz").read_bytes())
+    again = MemoryActor.load(tmp_path / "m.pt", graph=str(tmp_path / "elsewhere.npz"))
+    with torch.no_grad():
+        assert torch.equal(again(x)[0], net(x)[0])
+
+
+@pytest.mark.parametrize("what", ["--steps", "--cars", "--stretch"])
+def test_nothing_to_teach(tmp_path, what):
+    with pytest.raises(SystemExit, match="at least 1"):
+        main(["--data", str(tmp_path / "none.bin"), "--graph", str(GOLDEN / "toy_a.npz"), "--device", "cpu", what, "0"])
+
+
 def test_too_short_a_recording(tmp_path):
     data = tmp_path / "game.bin"
     ot.write_chunk(data, np.zeros((5, 517), np.float16), np.zeros((5, 90), np.float16))
