@@ -110,18 +110,22 @@ def silent_floor(ms: float, floor_ms: float, E: int, B: int) -> dict:
                     "share of the launch spent waiting on the memory system"}
 
 
+def kernel_sources() -> list[str]:
+    """The sources of what the benchmark runs: all in csrc/ but the memory over decisions, which it calls nothing of."""
+    d = os.path.join(os.path.dirname(os.path.abspath(__file__)), "flyguy_amd", "csrc")
+    return [os.path.join(d, n) for n in sorted(os.listdir(d)) if n.endswith((".hip", ".h")) and not n.startswith("memory")]
+
+
 def kernel_sources_sha() -> str:
-    """SHA-256 over the library's kernel sources without their comments and with runs of white space made one
-    space: a counter run recorded for other code is stale, one recorded before a change of comments only is not."""
+    """SHA-256 over kernel_sources() without their comments and with runs of white space made one space: a counter run
+    recorded for other code is stale, one recorded before a change of comments only is not."""
     import hashlib
     import re
     h = hashlib.sha256()
-    d = os.path.join(os.path.dirname(os.path.abspath(__file__)), "flyguy_amd", "csrc")
-    for n in sorted(os.listdir(d)):
-        if n.endswith((".hip", ".h")):
-            with open(os.path.join(d, n), encoding="utf-8") as fh:
-                code = re.sub(r"/\*.*?\*/|//[^\n]*", " ", fh.read(), flags=re.S)
-            h.update(n.encode() + b"\0" + " ".join(code.split()).encode())
+    for path in kernel_sources():
+        with open(path, encoding="utf-8") as fh:
+            code = re.sub(r"/\*.*?\*/|//[^\n]*", " ", fh.read(), flags=re.S)
+        h.update(os.path.basename(path).encode() + b"\0" + " ".join(code.split()).encode())
     return h.hexdigest()
 
 

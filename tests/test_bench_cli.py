@@ -26,3 +26,18 @@ def test_a_multi_rank_launch_is_refused():
     r = _run(env=env)
     assert r.returncode != 0
     assert "one GPU" in (r.stdout + r.stderr)
+
+
+def test_a_counter_run_goes_stale_with_the_sources_it_ran():
+    """What the benchmark hashes is closed under #include and holds every source of the library but the memory over decisions,
+    which nothing among them includes."""
+    import re
+    sys.path.insert(0, str(ROOT))
+    import bench
+    from flyguy_amd.build import SOURCES
+    hashed = {Path(p).name for p in bench.kernel_sources()}
+    assert hashed >= {p.name for p in SOURCES if not p.name.startswith("memory")}
+    assert not any(n.startswith("memory") for n in hashed)
+    for p in bench.kernel_sources():
+        included = re.findall(r'#include "([^"/]+)"', Path(p).read_text())
+        assert set(included) <= hashed, p
