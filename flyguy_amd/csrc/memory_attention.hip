@@ -299,10 +299,11 @@ __device__ __forceinline__ Sum<P, 8> down(const bf16* p, int apart, int plane) {
 // heads of 128 values, bfloat16).
 // A value of v that is not finite reaches only the outputs from its moment on (there: NaN), though 0 weights meet it in the
 // products: such a chunk's products run with zeros in its place.
-// What bounds it: latency between a chunk's three barriers, with the two workgroups a CU that the registers of 128 x 128 states
-// allow.  32,768 moments of 8 such heads in bfloat16, 57 segments, take 96 us: 1.6 waves a SIMD, whose vector instructions
-// (sums of terms, decays) take 38% of the time and matrix instructions 26%; LDS is read 22% of it.  512 heads of 4,096 moments
-// in one segment each: 620 us, 3.5 TB/s of a copy's 5.2; 477 without loads and stores, 480 without the products.
+// What bounds it: a chunk's phases between its three barriers, which do not overlap, with the two workgroups a CU that
+// registers and LDS (60 KB) of 128 x 128 states both allow.  32,768 moments of 8 such heads in bfloat16, 57 segments, take 96
+// us: 1.6 waves a SIMD, whose vector instructions (sums of terms, decays) take 38% of the time and matrix instructions 26%;
+// LDS is read 22% of it.  512 heads of 4,096 moments in one segment each: 620 us, 3.5 TB/s of a copy's 5.2; 477 without loads
+// and stores, 480 without the products.
 constexpr int WAVES = 4;
 template <class T, int KT, int NT, bool OUT>
 struct Tile {
@@ -314,8 +315,9 @@ struct Tile {
     static constexpr int PER_SIMD = FIT < 1 ? 1 : FIT > MOST ? MOST : FIT;
 };
 // Where a row's 8-value share q stands in LDS: rows of 8 or 16 shares, unpadded, the shares of row 4g + r (of 16) exchanged
-// by q ^ (r, g), so that both the 16 rows of a share and the 4 shares of 4 rows that a transposing read takes lie in banks
-// of their own.  place(row, q + 4b) = place(row, q) ^ 32 b where q < 4.
+// by q ^ (r, g), so that both the 16 rows of a share and the 4 shares of 4 rows that a transposing read takes are spread over
+// the banks.  (Conflicts are counted all the same, 39% of the cycles in which LDS is busy; one source is the weights' pieces,
+// written 8 bytes at a time 16 bytes apart.)  place(row, q + 4b) = place(row, q) ^ 32 b where q < 4.
 template <int WIDTH>
 __device__ __forceinline__ int place(int row, int q) {
     const int r = row & 3, g = row >> 2 & 3, swap = (g & 1) << 1 | g >> 1;
@@ -350,8 +352,8 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 // The outputs of the moments before the first stretch and after the last one: zeros, by all 256 threads of each of the workgroups
-// that come after the slots'.  (A pack of 4,096 moments in a place for 262,144, 8 heads of 128 values, bfloat16: 6,014 us cleared byte by byte
-// in the stretches' own workgroups, 438 by these.)
+// that come after the slots'.  (A pack of 4,096 moments in a place for 262,144, 8 heads of 128 values, bfloat16: 6,014 us cleared
+// byte by byte in the stretches' own workgroups, 438 by these.)
 __device__ __forceinline__ void clear_outside(const Scans& a, const Scan& s, int size, long long share) {
     const long long shares = (long long)a.clearing * a.heads, row = (long long)a.heads * s.N * size;
     if (!s.out || share >= shares) return;
@@ -938,19 +940,23 @@ int groups_per_cu(int K, int N) {
 
 // How a launch's scans are cut into segments: as the following estimate (us) has it cheapest.  A CU with w workgroups takes
 // 1.7 + b w (3 + K N / 1024) for a chunk of each, K and N as the kernel's form has them, b = 0.207 for bfloat16 (64 moments a
-// chunk), 0.147 for binary16, 0.257 for float32 (32); the longest workgroup ends alone.  More than one segment a stretch cost a
-// pass for their own states (0.55 of the constant, 0.2 of the rest; a stretch's last segment needs none), its launch, and the
-// joining's traffic.  Packed stretches, whose lengths only the device knows, are taken to be of any length up to twice the
-// middle one.  Fitted to 550 measured times (13% rms): 15 sets of stretches of one or of mixed lengths, forward and gradient, 5
-// to 12 cuts of each.  The cut so chosen takes 5% (rms) more than the best of them where the host knows the lengths, 6% where
-// packed ones are mixed, 20% where packed ones are all the same, 15% where one of them is four times the others.
+// chunk), 0.147 for binary16, 0.257 for float32 (32); the longest workgroup ends alone.  More than one segment a stretch cost
+// a pass for their own states (0.55 of the constant, 0.2 of the rest; a stretch's last segment needs none), its launch, and
+// the joining's traffic.  Packed stretches, whose lengths only the device knows, are taken to be of any length up to twice the
+// middle one.  (264 packs, all alike, of any length up to twice the middle, with one six times as long, or of exponential
+// lengths, a quarter each: against twice, 1.5 times takes 2% more, 2.5 and 3 times 2% less, but up to 47% more where all are
+// alike, 6 times the same.)  Fitted to 550 measured times (13% rms): 15 sets of stretches of one or of mixed lengths, forward
+// and gradient, 5 to 12 cuts of each.  The cut so chosen takes 5% (rms) more than the best of them where the host knows the
+// lengths, 6% where packed ones are mixed, 20% where packed ones are all the same, 15% where one of them is four times the
+// others.
 struct Cut {
     int nseg, slots, K, N, joined;
     long long L, L0;
 };
 // From this many values of a chain's segments up they are joined by a kernel of its own; fewer, each segment of the main pass
-// joins those before it as it begins (a launch less; 4 segments of 64 x 64: 143 us a learning step against 149 with the
-// kernel, 4 of 128 x 128: 786 against 776, 6 of 64 x 128: 113 us a packed forward pass against 98).
+// joins those before it as it begins (a launch less).  150 sets of stretches, alike and packed, states of 16 x 16 to 128 x
+// 128, forward and gradient: from 32,768 values up takes 0.5% more in the mean, from 98,304 2.5%, from 196,608 8%, always the
+// kernel 0.5% (small states prefer it, up to 1.45 times as fast; short packs the other way, 2.4 times), never the kernel 24%.
 constexpr int JOIN_FROM = 49152;
 Cut cut_of(const fm_attention_args& p, int scans) {
     Cut c;
@@ -1011,8 +1017,9 @@ Cut cut_of(const fm_attention_args& p, int scans) {
     c.nseg = (int)((p.n_moments + c.L - 1) / c.L);
     c.L0 = c.L;
     // More chains than half the workgroups that fit, but not all of them: a first segment so short that those left over, one
-    // after another, walk the first segments while the chains' workgroups walk the rest (8 x 4096 moments of 16 heads of 128
-    // values in bfloat16, the gradient's 384 chains: 753 -> 715 us a learning step).
+    // after another, walk the first segments while the chains' workgroups walk the rest.  (84 such sets, 55 to 92% of what fits, 700
+    // to 6,000 moments of each type: gradients take 2.4% less in the mean, 15% less at best, 12 x 2048 moments of 8 heads of 128
+    // float32 values 600 -> 508 us, and 6% more at worst, 12 x 700 in binary16 156 -> 166.)
     const double fit = 256.0 * cap;
     if (!p.starts && chains < fit && 2 * chains > fit) {      // (packed stretches find their segments by L alone)
         const double turns = ceil(chains / (fit - chains));

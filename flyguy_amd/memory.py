@@ -45,7 +45,7 @@ class MemoryActor(nn.Module):
     """actor: a FlyActor.  heads query heads of dim values share k_heads key / value heads; the slowest head remembers about
     `longest` moments, the fastest 8.  positions: moments of the rotation's table.  A stretch from an empty memory may not be
     longer; a car that goes on past it keeps its memory, whose moments from there on all count as the table's last one, so that
-    newer ones are no longer told apart by their distance."""
+    newer ones are no longer told apart by their distance.  On the GPU a call takes up to 16384 stretches, a step 65535 cars."""
 
     def __init__(self, actor: FlyActor, heads: int = 8, k_heads: int | None = None, dim: int = 64, longest: float = 2048.0,
                  positions: int = 65536):

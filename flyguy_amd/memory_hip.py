@@ -9,7 +9,8 @@ the next (flyguy/fly.py:286-305 decides each moment alone).
 
 Queries and keys are [stretches, moments, heads, values] (decay_step: [rows, heads, values]), float32, bfloat16 or
 binary16, on the GPU, with any strides whose last is 1 (another last stride costs a copy); query heads share key / value
-heads in consecutive groups.  The first three have gradients (backwards, of the first order; tables and decays are fixed).  Work goes to the current stream; nothing synchronises.
+heads in consecutive groups.  The first three have gradients (backwards, of the first order; tables and decays are fixed).
+Work goes to the current stream; nothing synchronises.
 """
 from __future__ import annotations
 
@@ -333,10 +334,11 @@ def _shared(what, q, k, v, first: int) -> None:
 
 
 def decay_attention(q, k, v, log_decay, state=None, starts=None, scale: float | None = None):
-    """Linear attention with a decay for each query head, l = exp(log_decay[head]) (log_decay at most 1): S_t = l S_{t-1} + k_t v_t^T, o_t = scale
-    q_t S_t (scale: values^-0.5 unless given), from `state` (float32 [stretches, q heads, values, v values]; None: zeros).
+    """Linear attention with a decay for each query head, l = exp(log_decay[head]) (log_decay at most 1): S_t = l S_{t-1} +
+    k_t v_t^T, o_t = scale q_t S_t (scale: values^-0.5 unless given), from `state` (float32 [stretches, q heads, values, v values]; None: zeros).
     starts (int32 / int64 [stretches + 1] on the GPU): q, k, v are packed, [moments, heads, values], and stretch n is
-    moments starts[n] .. starts[n + 1] - 1 (any length, 0 too; moments of no stretch give zeros).
+    moments starts[n] .. starts[n + 1] - 1 (any length, 0 too; moments of no stretch give zeros; where starts fall, stretches
+    are cut short so that no two share a moment).  At most 16384 stretches.
     Returns (o in q's type, the state after each stretch).  Gradients of q, k, v and state; the decays are fixed."""
     what = "decay_attention"
     _no_tangents(what, q, k, v, log_decay, state)
@@ -371,7 +373,7 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
     state (float32 [states, q heads, values, v values], dense) is updated in place, or the new states are written to
     `into`, another tensor like it that shares none of its memory.  slots (int32 [rows] on the GPU): the state each row goes
     on from, by default its own number; below 0: the row is idle (zeros, no state touched); past the states: NaN, no state
-    touched.  No two rows of a call may name one slot.  No gradients."""
+    touched.  No two rows of a call may name one slot.  At most 65535 rows.  No gradients."""
     what = "decay_step"
     _no_tangents(what, q, k, v, log_decay, state, into)
     _heads(what, 3, q, k, v)

@@ -31,9 +31,10 @@ typedef struct fm_view {
  *   y_a = z_a cos - z_b sin,  y_b = z_b cos + z_a sin,   (cos, sin) = table[position][i]
  * table: float32 [n_positions][rotated/2][2] (rotated 0: no rotation).  A moment's position is positions[n pos_seq + t
  * pos_moment] (int32, or int64 if wide) + first; positions 0: t + first.  A position outside the table gives NaN in the
- * rotated values.  Gradients (fm_turn_bwd): x the forward's inputs (read only where weight is not 0), g the gradients of y, y
- * the gradients of x, written; gweight: the weights' gradients, written; partial: fm_turn_partial() floats.  y may be x itself
- * (gradients: x or g), with the same strides; otherwise what is written must lie outside what is read. */
+ * rotated values.  At most 8e9 heads of moments.  Gradients (fm_turn_bwd): x the forward's inputs (read only where weight
+ * is not 0), g the gradients of y, y the gradients of x, written; gweight: the weights' gradients, written; partial:
+ * fm_turn_partial() floats.  y may be x itself (gradients: x or g), with the same strides; otherwise what is written must
+ * lie outside what is read. */
 typedef struct fm_turn_args {
     fm_view x[2], y[2], g[2];
     const float* weight[2];
@@ -52,13 +53,14 @@ long long fm_turn_partial(const fm_turn_args* a);
 /* Linear attention with a decay for each query head, l = exp(log_decay[h]) (log_decay 0 keeps everything, -inf nothing; above 0,
  * at most 1, states grow until they overflow); query head h reads key / value head h / (q_heads / k_heads):
  *   S_t = l S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   S_{-1} = state (0: zeros)
- * k_dim, v_dim <= 128.  A value that is not finite reaches no output of an earlier moment (no gradient of a later one), and no
- * other stretch; the outputs that it does reach are NaN, or infinite.
+ * k_dim, v_dim <= 128, q_heads <= 65535, n_seq <= 16384, n_moments <= 2^31.  A value that is not finite reaches no output of an
+ * earlier moment (no gradient of a later one), and no other stretch; the outputs and states that it does reach are NaN, or
+ * infinite.
  * Stretches: n_seq of n_moments moments each, or (starts not 0) packed: n_moments in all, stretch n being moments starts[n] ..
  * starts[n+1] - 1 (int32, or int64 if wide; out of [0, n_moments]: brought into it), the views' seq unread.  Where starts fall,
- * stretches are cut short so that no two share a moment.  o: dense
- * [moments][q_heads][v_dim].  state, state_out: float32 [n_seq][q_heads][k_dim][v_dim]
- * (state_out 0: not wanted; it must not overlap state).  A stretch without moments passes its state on.
+ * stretches are cut short so that no two share a moment.  o: dense [moments][q_heads][v_dim], zeros at moments of no stretch.
+ * state, state_out: float32 [n_seq][q_heads][k_dim][v_dim] (state_out 0: not wanted; it must not overlap state).  A stretch
+ * without moments passes its state on as it is.
  * Gradients (fm_attention_bwd): go of o, gstate_out of state_out (0: zeros); gq, gk, gv dense like their tensors, gstate
  * float32; each 0 where not wanted.  workspace: fm_attention_workspace(a, backward) bytes. */
 typedef struct fm_attention_args {
@@ -80,7 +82,7 @@ int fm_attention(const fm_attention_args* a, void* stream);
 int fm_attention_bwd(const fm_attention_args* a, void* stream);
 long long fm_attention_workspace(const fm_attention_args* a, int backward);
 
-/* One moment of it for n rows: q, k, v (views without moments) and
+/* One moment of it for n <= 65535 rows: q, k, v (views without moments) and
  *   next[s] = l state[s] + k v^T,  o = scale q next[s]     (o: dense [n][q_heads][v_dim])
  * s = slots[row] (int32; 0: s = row), state and next float32 [n_states][q_heads][k_dim][v_dim] (next == state: in place;
  * else outside it).  A slot below 0 gives a row of zeros and touches no state; one past the states gives NaN and touches none.
