@@ -312,6 +312,10 @@ class FlyActor(nn.Module):
         return top.transpose(1, 2).reshape(B, -1)
 
     # ---- CPU play
+    def __getstate__(self) -> dict:
+        """What copies and pickles hold: all but the decision library's handle, of which each actor sets up its own."""
+        return {k: v for k, v in self.__dict__.items() if k != "_decider"}
+
     def _host_decider(self) -> "_HostDecider | None":
         """The CPU decision library loaded with the current weights (rebuilt when a weight changed), or None when it
         is not built, FLYGUY_NATIVE=0 or the weights are not float32."""

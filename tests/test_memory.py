@@ -3,6 +3,8 @@ actor, a stretch in pieces or moment by moment is the stretch at once, nothing r
 taught what no single moment shows."""
 from __future__ import annotations
 
+import copy
+import pickle
 import re
 from concurrent.futures import ThreadPoolExecutor
 
@@ -128,6 +130,20 @@ def test_cpu_play_is_the_actors(monkeypatch):
     logits, again = m.actor.with_firing(x)                     # (with gradients)
     torch.testing.assert_close(again, firing, rtol=1e-5, atol=1e-5)
     torch.testing.assert_close(logits, want, rtol=1e-5, atol=1e-5)
+
+
+def test_copies_of_an_actor_that_has_played():
+    """A copy and a pickle of an actor that has decided on the CPU decide by themselves."""
+    m, x = net(), torch.randn(3, 517)
+    with torch.no_grad():
+        want = m.step(x, m.state(3))
+        copies = [copy.deepcopy(m), pickle.loads(pickle.dumps(m))]
+        m.actor.out.bias.add_(1.0)
+        moved = m.step(x, m.state(3))
+        for c in copies:
+            assert torch.equal(c.step(x, c.state(3)), want)
+            assert c.actor._decider[1] is not None and c.actor._decider[1] is not m.actor._decider[1]
+    torch.testing.assert_close(moved, want + 1.0)
 
 
 def test_heads_must_share():
