@@ -607,9 +607,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) rest[r] = cv * power(16 - 4 * g - r - early);
             }
-            if (keep.one != 0.f && keep.f == 0.f) {
-                // (as it is: it may hold an infinity)
-            } else if (keep.one != 0.f) {                     // (one instruction a value, either way)
+            if (keep.one != 0.f && keep.f != 0.f) {           // (one instruction a value, either way)
 #pragma unroll
                 for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
@@ -618,7 +616,7 @@ __global__ __launch_bounds__(64 * WAVES, (Tile<T, KT, NT, OUT>::PER_SIMD)) void 
 #pragma unroll
                 for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
-                    for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] *= keep.f;
+                    for (int r = 0; r < 4 * NT; ++r) z[b][r >> 2][r & 3] *= keep.one + keep.f;       // (one of them is 0)
             }
 #pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
