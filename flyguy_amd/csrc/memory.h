@@ -20,8 +20,11 @@ __device__ __forceinline__ T narrow(float v) { return (T)v; }
 struct Keep {
     float one, f;                        // exp(g) = one + f
     __device__ __forceinline__ explicit Keep(float g) : one(g > -0.5f ? 1.f : 0.f), f(g > -0.5f ? expm1f(g) : expf(g)) {}
+    // (of the common kind: neither of those)
+    __device__ __forceinline__ bool plain() const { return f != 0.f && f < INFINITY; }
+    __device__ __forceinline__ float times(float x) const { return fmaf(f, x, one * x); }
     __device__ __forceinline__ float operator()(float x) const {
-        return f == 0.f || x == 0.f ? one * x : fmaf(f, x, one * x);
+        return f == 0.f || (x == 0.f && f > 0.f) ? one * x : times(x);
     }
 };
 

@@ -729,6 +729,16 @@ def test_a_decay_that_is_not_a_number(gpu_lib, dt):
         assert ob[..., 1, :].isnan().all() and eb[:, 1].isnan().all()
 
 
+def test_a_decay_that_is_not_a_number_and_an_empty_state(gpu_lib):
+    from flyguy_amd.memory_hip import decay_attention, decay_step
+    gen = torch.Generator().manual_seed(25)
+    q, k, v = (draw(gen, 1, 3000, 2, 16) for _ in range(3))
+    g, s = torch.tensor([-0.1, math.nan], device="cuda"), torch.zeros(1, 2, 16, 16, device="cuda")
+    decay_step(q[:, 0], k[:, 0], v[:, 0], g, s)
+    for e in (s, decay_attention(q, k, v, g)[1], decay_attention(q, k, v, g, torch.zeros_like(s))[1]):
+        assert e[:, 1].isnan().all() and e[:, 0].isfinite().all()
+
+
 def test_pieces_of_a_stretch_and_single_moments(gpu_lib):
     """A stretch read in two pieces, or moment by moment with decay_step, is the stretch read at once, up to rounding."""
     from flyguy_amd.memory_hip import decay_attention, decay_step
