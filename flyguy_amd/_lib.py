@@ -78,6 +78,10 @@ _SIGS = {
     "fm_attention_bwd": (ci, [ctypes.c_char_p, vp]),
     "fm_attention_workspace": (cll, [ctypes.c_char_p, ci]),
     "fm_step": (ci, [ctypes.c_char_p, vp]),
+    "fm_norm": (ci, [ctypes.c_char_p, vp]),
+    "fm_norm_bwd": (ci, [ctypes.c_char_p, vp]),
+    "fm_norm_partial": (cll, [ctypes.c_char_p]),
+    "fm_drop": (ci, [ctypes.c_char_p, vp]),
     "fc_layers": (ci, [vp, ctypes.POINTER(ci), ci]),
     "fc_survey": (ci, [vp, vp, vp, ci, ci, cf, ci]),
     "fc_survey_read": (cll, [vp, vp, vp, ctypes.POINTER(ctypes.c_double)]),

@@ -99,6 +99,40 @@ typedef struct fm_step_args {
 } fm_step_args;
 int fm_step(const fm_step_args* a, void* stream);
 
+/* Layer norm of rows of `width` values (1 to 2^24), row i at x + i x_row (strides in values):
+ *   m = mean(x), r = (mean((x - m)^2) + eps)^-1/2, xh = (x - m) r, y = xh weight + bias   (weight 0: 1; bias 0: 0)
+ * stats: float32 [rows][2], (m, r) of each row, written if not 0.  Gradients (fm_norm_bwd): x, weight and stats the forward's,
+ * g the gradient of y; gx, gweight, gbias the gradients, each 0 where not wanted; partial: fm_norm_partial() floats.  weight,
+ * bias and their gradients are float32.  y may be x, gx may be x or g, with the same stride, where rows do not overlap; otherwise what is
+ * written must lie outside what is read. */
+typedef struct fm_norm_args {
+    const void* x;
+    void* y;
+    const void* g;
+    void* gx;
+    long long x_row, y_row, g_row, gx_row;
+    const float *weight, *bias;
+    float *gweight, *gbias, *stats, *partial;
+    long long rows, width, dtype;
+    double eps;
+} fm_norm_args;
+int fm_norm(const fm_norm_args* a, void* stream);
+int fm_norm_bwd(const fm_norm_args* a, void* stream);
+long long fm_norm_partial(const fm_norm_args* a);
+
+/* Dropout without a stored mask: number i = row width + column of rows x width (at most 1e12) becomes 0 where its draw is below
+ * t = round(65536 share), else 65536 / (65536 - t) times itself; share 1: all zeros.  Draws: Philox4x32 of 10 rounds, key = counter[0]
+ * (low word first), counter = (i / 8, counter[1]); draw i is half i % 8 of its four words, low halves first.  counter: device
+ * memory, read when the kernel runs.  y: dense.  The same call on y's gradient gives x's.  y may be x where x is dense. */
+typedef struct fm_drop_args {
+    const void* x;
+    void* y;
+    const unsigned long long* counter;
+    long long x_row, rows, width, dtype;
+    double share;
+} fm_drop_args;
+int fm_drop(const fm_drop_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
