@@ -78,6 +78,11 @@ _SIGS = {
     "fm_attention_bwd": (ci, [ctypes.c_char_p, vp]),
     "fm_attention_workspace": (cll, [ctypes.c_char_p, ci]),
     "fm_step": (ci, [ctypes.c_char_p, vp]),
+    "fm_delta": (ci, [ctypes.c_char_p, vp]),
+    "fm_delta_bwd": (ci, [ctypes.c_char_p, vp]),
+    "fm_delta_workspace": (cll, [ctypes.c_char_p, ci]),
+    "fm_delta_saved": (cll, [ctypes.c_char_p]),
+    "fm_delta_step": (ci, [ctypes.c_char_p, vp]),
     "fm_norm": (ci, [ctypes.c_char_p, vp]),
     "fm_norm_bwd": (ci, [ctypes.c_char_p, vp]),
     "fm_norm_partial": (cll, [ctypes.c_char_p]),

@@ -20,8 +20,8 @@ LIB = PKG / "libflyguy_core.so"
 EXE = PKG / "flyguy_train"
 CPU_LIB = PKG / "libfly_infer.so"          # decisions on the host CPU (include/fly_infer.h): no HIP
 SOURCES = [PKG / "csrc" / n for n in ("kernels.hip", "core.hip", "core16.hip", "readout.hip", "hop_api.hip", "half.hip", "train.hip", "probe.hip",
-                                       "memory_turn.hip", "memory_attention.hip", "memory_rows.hip")]
-HEADERS = [PKG / "csrc" / n for n in ("common.h", "kernels.h", "device.h", "core.h", "half.h", "memory.h")] + \
+                                       "memory_turn.hip", "memory_attention.hip", "memory_rows.hip", "memory_delta.hip")]
+HEADERS = [PKG / "csrc" / n for n in ("common.h", "kernels.h", "device.h", "core.h", "half.h", "memory.h", "memory_chunk.h")] + \
     [ROOT / "include" / "flyguy_core.h", ROOT / "include" / "flyguy_train.h", ROOT / "include" / "fly_infer.h",
      ROOT / "include" / "flyguy_memory.h"]
 ARCH = os.environ.get("FLYGUY_OFFLOAD_ARCH", "gfx950")

@@ -1,0 +1,1381 @@
+// The gated delta rule (include/flyguy_memory.h: fm_delta, fm_delta_bwd, fm_delta_step): a linear memory that moves what it holds
+// under a key towards the key's new value.  With a_t = exp(log_decay_t) and a state S [K][V] of each head,
+//   e_t = v_t - (a_t S_{t-1})^T k_t,   S_t = a_t S_{t-1} + beta_t k_t e_t^T,   o_t = c S_t^T q_t.
+//
+// In chunks of C moments, with G_i the sum of a chunk's log decays up to moment i, D_ij = exp(G_i - G_j) for j <= i, E = exp(G),
+// F = exp(G_end - G) and S the state before the chunk, the errors solve a triangular system:
+//   (I + N) e = v - E K S,  N = strict lower(K K^T D) beta;   with T = (I + N)^-1:
+//   e = T (v - E K S),   o = c E Q S + P e,  P = c lower(Q K^T D) beta,   S' = E_end S + K^T (F beta e).
+// Backwards, with X the gradient of S' and g that of o:
+//   y = T^T (P^T g + beta F K X) (the gradient of v),   X' = E_end X + Q^T (c E g) - K^T (E y),
+// and with H = c lower(g e^T) D, Z = -strict lower(y e^T) D:
+//   gq = c E g S^T + H beta K,   r = -E y S^T + Z beta K,   w = F e X^T + Z^T K + H^T Q,   gk = r + beta w,   gbeta = k . w,
+//   gG = q . gq + k . r - beta gbeta, and at the chunk's end E_end <S, X> + sum_i F_i beta_i k_i . (X e_i) besides; a log decay's
+//   gradient is the sum of gG from its moment to the chunk's end.
+// (beta_j, exp(-G_j) and a writing k_j stand only together, as do exp(G_i) and a reading q_i or k_i: so one dot product of a
+// row with its gradient is the factor's gradient.)
+//
+// T and P need no state: k_delta_prep makes them for all chunks at once.  k_delta_scan then walks each head's chunks with the
+// state in registers, and k_delta_back walks them backwards; k_delta_grads makes the gradients of all chunks at once from the
+// states and errors that the two walks leave.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "memory_chunk.h"
+
+namespace fg {
+
+constexpr int DELTA_MAX = 128;           // values of a head
+constexpr int T_TERMS = 3;               // terms of T, of what it multiplies and of the state: the state is a float32 result
+
+// A launch's view of its stretches, cut into chunks (memory_chunk.h: L is a chunk).
+struct Delta {
+    fm_view q, k, v, go;
+    const float *log_decay, *beta;
+    long long ld_seq, ld_moment, ld_head, be_seq, be_moment, be_head;
+    const void* starts;
+    long long n_moments, L, L0;
+    int wide, heads, share, n_seq, nseg, slots, K, V;
+    float c;
+    int vec;                             // 16-byte loads
+    // workspace, by chunk slot and head
+    char* prep;                          // T and P as the products' operands, then the chunk's factors
+    float *states, *errors;              // S before each chunk [KW][VW], e [CH][VW] (0: not kept)
+    float *grads, *ys;                   // X after each chunk, y, the same way
+    // whole tensors
+    const float* init;
+    float* fin;
+    void* o;
+    const float* gfin;
+    float* ginit;
+    void *gq, *gk, *gv;                  // gk, gv: of the values' type, or (shared heads) float32 parts of each query head
+    float *glog_decay, *gbeta;
+};
+
+template <class T>
+struct DeltaForm {
+    static constexpr int X = Form<T>::X, W = Form<T>::W, CH = Form<T>::CHUNK, JB = CH / 16, PIECES = JB == 4 ? 6 : 2;
+    // operands in units of 64 lanes x 16 bytes: P's terms, then T's
+    static constexpr int P_UNITS = PIECES * W, T_UNITS = PIECES * T_TERMS, UNITS = P_UNITS + T_UNITS;
+    // factors: E_end as 1 + x or x (Keep), the first moment that is not finite (as int), 0; then E, F beta, F, beta and G (high
+    // and low part) of each moment
+    static constexpr int FACTORS = 4 + 6 * CH;
+    static constexpr int PREP = UNITS * 1024 + FACTORS * 4;
+};
+enum { F_E = 4 };
+template <class T>
+__device__ __forceinline__ const float* factors_of(const char* prep) {
+    return reinterpret_cast<const float*>(prep + DeltaForm<T>::UNITS * 1024);
+}
+
+// piece of rows' block i and the pair jj of summed blocks 2jj, 2jj + 1 of a lower triangular matrix (JB 4: (0,0) (0,1) (0,2)
+// (0,3) (1,2) (1,3) as (jj, i)); of its transpose, pair ii and block j: (0,0) (0,1) (1,0) .. (1,3)
+__device__ __forceinline__ constexpr int piece_of(int jj, int i) { return jj ? i + 2 : i; }
+__device__ __forceinline__ constexpr int tpiece_of(int ii, int j) { return ii ? j + 2 : j; }
+// block n of the lower triangle, row by row
+__device__ __forceinline__ void block_of(int n, int& i, int& j) {
+    i = n < 1 ? 0 : n < 3 ? 1 : n < 6 ? 2 : 3;
+    j = n - i * (i + 1) / 2;
+}
+
+// ------------------------------------------------------------------------------------------------ a chunk's rows
+// rows of a chunk in memory: 16 bytes of row `row` from value `col`; zeros past the rows and columns
+template <class T>
+struct Chunk {
+    const T* p;
+    int rows, width, vec;
+    long long step;
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ Chunk(const T* data, int rows, long long step, int width, int vec)
+        : p(data), rows(rows), width(width), vec(vec), step(step),
+          rsrc(rows_at(data, rows, vec ? step * (int)sizeof(T) : 0, width * (int)sizeof(T))) {}
+    __device__ __forceinline__ uint4 operator()(int row, int col) const {
+        const bool there = row < rows && col < width;
+        if (vec) {
+            const unsigned at = there ? row * (int)step * (int)sizeof(T) + col * (int)sizeof(T) : NOWHERE;
+            return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
+        }
+        return load16(p + row * step, col, width, there);
+    }
+};
+template <class T>
+__device__ __forceinline__ Chunk<T> chunk_of(const Delta& a, const fm_view& v, int n, int head, long long moment, int rows, int width) {
+    return Chunk<T>((const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + moment * v.moment, rows, v.moment, width, a.vec);
+}
+// a value that is not finite among 16 bytes
+template <class T>
+__device__ __forceinline__ bool odd16(uint4 r) {
+    const typename Vec<T>::type v = __builtin_bit_cast(typename Vec<T>::type, r);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i) s = fmaf(widen(v[i]), 0.f, s);
+    return !(s == 0.f);
+}
+template <int P>
+__device__ __forceinline__ f32x8 widened(const Sum<P, 8>& s) {
+    f32x8 v = __builtin_convertvector(s.term[P - 1], f32x8);
+#pragma unroll
+    for (int p = P - 2; p >= 0; --p) v += __builtin_convertvector(s.term[p], f32x8);
+    return v;
+}
+template <int P>
+__device__ __forceinline__ f32x4 widened(const bf16* p, int plane) {
+    f32x4 v = __builtin_convertvector(*reinterpret_cast<const bf16x4*>(p + (P - 1) * plane), f32x4);
+#pragma unroll
+    for (int i = P - 2; i >= 0; --i) v += __builtin_convertvector(*reinterpret_cast<const bf16x4*>(p + i * plane), f32x4);
+    return v;
+}
+__device__ __forceinline__ f32x8 joined(f32x4 a, f32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+// a sum's first terms
+template <int W, int P>
+__device__ __forceinline__ Sum<W, 8> first_terms(const Sum<P, 8>& s) {
+    Sum<W, 8> r;
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.term[i] = s.term[i];
+    return r;
+}
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// a state times one + f (Keep): one instruction a value, either way
+template <int B>
+__device__ __forceinline__ void decayed(f32x4 (&z)[B], float one, float f) {
+    if (one != 0.f && f != 0.f) {
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[b][r] = fmaf(f, z[b][r], z[b][r]);
+    } else {
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z[b][r] *= one + f;       // (one of them is 0)
+    }
+}
+constexpr float GONE = -110.f;           // a log decay whose factor is 0 in float32
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// ------------------------------------------------------------------------------------------------ T, P and the factors
+// A workgroup a chunk and head.  K K^T and Q K^T on the matrix cores; N in float32 in LDS; T by blocks of 16: those on the diagonal by
+// forward substitution, a lane a column, then T_ij = -T_ii sum_k N_ik T_kj down each column of blocks, in float32 products
+// whose second operand stays in registers.  G is summed in 64 bits and kept in two floats: a difference of two of them is
+// exact to its own last bits however much has been forgotten before.  BWD: the operands of the transposes.
+// A moment whose key, decay or rate is not finite spoils all from there on (k_delta_scan): here its chunk ends before it.
+template <class T, int KT, bool BWD>
+__global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
+    using F = DeltaForm<T>;
+    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, XC = KW / VN;
+    constexpr int NP = CH + 4;                            // a row of N and T, padded
+    __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP];
+    __shared__ __align__(16) float sn[CH * NP], st[CH * NP];
+    __shared__ float hi[CH], lo[CH], sb[CH];
+    __shared__ int bad;
+    const unsigned block = (unsigned)block_number();
+    const int place_in = (int)(block / a.heads), h = (int)(block - (unsigned)place_in * a.heads);
+    if (place_in >= a.slots) return;
+    int n, seg, slot;
+    long long first, count;
+    if (!segment_of(a, place_in, n, seg, slot, first, count)) return;
+    const long long from = (long long)seg * CH, left = count - from;
+    const int rows = (int)(left < CH ? left : CH);
+    if (rows <= 0) return;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const long long moment = first + from;
+    char* const prep = a.prep + ((size_t)slot * a.heads + h) * F::PREP;
+    if (tid == 0) bad = rows;
+    __syncthreads();
+    {
+        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
+        for (int i = tid; i < CH * XC; i += 256) {
+            const int row = i / XC, col = i % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
+            const uint4 kr = k(row, col);
+            store_terms<T>(q(row, col), sq + to, XP);
+            store_terms<T>(kr, sk + to, XP);
+            if (odd16<T>(kr)) atomicMin(&bad, row);
+        }
+    }
+    float ld = 0.f, be = 0.f;
+    if (tid < rows) {
+        ld = a.log_decay[(a.starts ? 0 : n * a.ld_seq) + (moment + tid) * a.ld_moment + h * a.ld_head];
+        be = a.beta[(a.starts ? 0 : n * a.be_seq) + (moment + tid) * a.be_moment + h * a.be_head];
+        if (!(ld < INFINITY) || !(fabsf(be) < INFINITY)) atomicMin(&bad, tid);
+    }
+    __syncthreads();
+    const int stop = bad;                                 // rows from here on: nothing
+    if (stop < rows)
+        for (int i = tid; i < CH * XC; i += 256)
+            if (i / XC >= stop) store_terms<T>(make_uint4(0, 0, 0, 0), sk + place<KW>(i / XC, i % XC * VN >> 3) + (i % XC * VN & 7), XP);
+    if (wave == 0) {
+        double s = lane < stop ? (double)fmaxf(ld, GONE) : 0.0;
+        for (int m = 1; m < 64; m <<= 1) {
+            const double t = __shfl_up(s, m);
+            if (lane >= m) s += t;
+        }
+        const double end = __shfl(s, CH - 1);             // (rows past the last add nothing)
+        const float b = lane < stop ? be : 0.f, high = (float)s;
+        float* const f = const_cast<float*>(factors_of<T>(prep));
+        if (lane < CH) {
+            hi[lane] = high;
+            lo[lane] = (float)(s - (double)high);
+            sb[lane] = b;
+            const float e = exp_of((float)s), left_over = exp_of((float)(end - s));
+            f[F_E + lane] = e;
+            f[F_E + CH + lane] = left_over * b;
+            f[F_E + 2 * CH + lane] = left_over;
+            f[F_E + 3 * CH + lane] = b;
+            f[F_E + 4 * CH + lane] = hi[lane];
+            f[F_E + 5 * CH + lane] = lo[lane];
+        }
+        if (lane == 0) {
+            const Keep keep((float)end);
+            f[0] = keep.one;
+            f[1] = keep.f;
+            f[2] = __int_as_float(stop < rows ? stop : CH);
+            f[3] = 0.f;
+        }
+    }
+    __syncthreads();
+
+    bf16x8* const units = reinterpret_cast<bf16x8*>(prep);
+    auto apart = [&](int i, int j) { return exp_of(fminf((hi[i] - hi[j]) + (lo[i] - lo[j]), 88.f)); };
+    auto store_half = [&](int unit, int half, const Sum<W, 4>& s) {
+#pragma unroll
+        for (int t = 0; t < W; ++t) reinterpret_cast<bf16x4*>(&units[(unit * W + t) * 64 + lane])[half] = s.term[t];
+    };
+    constexpr int BLOCKS = JB * (JB + 1) / 2;
+    for (int task = wave; task < 2 * BLOCKS; task += 4) {
+        const bool of_q = task >= BLOCKS;
+        int i, j;
+        block_of(of_q ? task - BLOCKS : task, i, j);
+        // of_q forwards: rows j, columns i; else rows i, columns j
+        const bool turned = of_q && !BWD;
+        const bf16* const ra = turned ? sk + 16 * j * KW : (of_q ? sq : sk) + 16 * i * KW;
+        const bf16* const rb = turned ? sq + 16 * i * KW : sk + 16 * j * KW;
+        f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < KT; ++b) {
+            const int at = place<KW>(c, g) ^ 32 * b;
+            p = mfma(across<X>(ra + at, XP), across<X>(rb + at, XP), p);
+        }
+        if (!of_q) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * i + 4 * g + r, col = 16 * j + c;
+                sn[row * NP + col] = row > col ? apart(row, col) * sb[col] * p[r] : 0.f;
+            }
+            continue;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = turned ? 16 * i + c : 16 * i + 4 * g + r, col = turned ? 16 * j + 4 * g + r : 16 * j + c;
+            p[r] = row >= col ? a.c * apart(row, col) * sb[col] * p[r] : 0.f;
+        }
+        Sum<W, 4> s;
+        s.of_summed(p);
+        if (BWD) {
+            store_half(tpiece_of(i >> 1, j), i & 1, s);
+            if ((i & 1) && i == j) store_half(tpiece_of(i >> 1, j), 0, Sum<W, 4>{});
+        } else {
+            store_half(piece_of(j >> 1, i), j & 1, s);
+            if (!(j & 1) && i == j) store_half(piece_of(j >> 1, i), 1, Sum<W, 4>{});
+        }
+    }
+    __syncthreads();
+    if (tid < CH) {                                       // the diagonal blocks: column c of block tid / 16
+        const int b0 = tid & ~15, col = tid & 15;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s = i == col ? 1.f : 0.f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) s = fmaf(-sn[(b0 + i) * NP + b0 + j], x[j], s);
+            x[i] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[(b0 + i) * NP + b0 + col] = x[i];
+    }
+    __syncthreads();
+    if (wave < JB - 1) {                                  // column `wave` of the blocks below the diagonal
+        const int j = wave;
+        f32x4 t[JB];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[0][r] = st[(16 * j + 4 * g + r) * NP + 16 * j + c];
+#pragma unroll
+        for (int d = 1; d < JB; ++d) {                    // block (j + d, j)
+            const int i = j + d;
+            if (i >= JB) break;
+            f32x4 s = {0.f, 0.f, 0.f, 0.f}, o = s;
+#pragma unroll
+            for (int k = 0; k < JB - 1; ++k) {
+                if (k >= d) break;
+                const f32x4 na = *reinterpret_cast<const f32x4*>(&sn[(16 * i + c) * NP + 16 * (j + k) + 4 * g]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s = mfma4(na[r], t[k][r], s);
+            }
+            const f32x4 ta = *reinterpret_cast<const f32x4*>(&st[(16 * i + c) * NP + 16 * i + 4 * g]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o = mfma4(-ta[r], s[r], o);
+            t[d] = o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st[(16 * i + 4 * g + r) * NP + 16 * j + c] = o[r];
+        }
+    }
+    __syncthreads();
+    for (int task = wave; task < F::PIECES; task += 4) {
+        f32x4 half[2];
+        if (BWD) {                                        // rows j, summed over i
+            const int ii = task >= 2, j = ii ? task - 2 : task;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    half[e][r] = 2 * ii + e >= j ? st[(16 * (2 * ii + e) + 4 * g + r) * NP + 16 * j + c] : 0.f;
+        } else {                                          // rows i, summed over j
+            const int jj = task >= 4, i = jj ? task - 2 : task;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int j = 2 * jj + e;
+                half[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (j <= i) half[e] = *reinterpret_cast<const f32x4*>(&st[(16 * i + c) * NP + 16 * j + 4 * g]);
+            }
+        }
+        Sum<T_TERMS, 8> s;
+        s.of_summed(joined(half[0], half[1]));
+#pragma unroll
+        for (int t = 0; t < T_TERMS; ++t) units[(F::P_UNITS + task * T_TERMS + t) * 64 + lane] = s.term[t];
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ the walk forwards
+// A workgroup of 4 waves walks one head's chunks for 64 columns of its state, a wave 16: columns never meet, so waves share only
+// what they read.  A chunk's rows and operands go through LDS, the next chunk's on their way in registers meanwhile.  An
+// accumulator block of 16 x 16 (lane (c, g): column c, rows 4g .. 4g + 3) is the operand of the product that sums over its
+// rows, so S, v - E K S and e pass between products in registers; outputs are formed transposed, so that a lane stores a row's
+// values side by side.
+// A value of v that is not finite makes its column NaN from its moment on; a key, decay or rate that is not, all columns:
+// such moments are left out of the products (0 times them would not be 0) and marked in what is stored.
+template <class T, int KT, bool SAVE>
+__global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
+    using F = DeltaForm<T>;
+    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
+    constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
+    constexpr int UV = (F::UNITS * 64 + 255) / 256;       // a thread's units of operands
+    static_assert(XV * XR == CH && VV * VR == CH, "");
+    __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP], sv[X * VP];
+    __shared__ __align__(16) bf16x8 su[F::UNITS * 64];
+    __shared__ __align__(16) float sf[4 + 2 * CH];
+    const int blocks_v = (a.V + NW - 1) / NW;
+    const unsigned block = (unsigned)block_number(), chain = block / blocks_v;
+    const int vb = (int)(block - chain * blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
+    if (n >= a.n_seq) return;
+    long long first, count;
+    stretch_of(a, n, first, count);
+    first = shared_by_all(first);
+    count = shared_by_all(count);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int v0 = NW * vb, col = v0 + 16 * wave + c, VW = NW * blocks_v;
+    const size_t at_state = ((size_t)n * a.heads + h) * a.K * a.V;
+    auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    f32x4 z[2 * KT];
+#pragma unroll
+    for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = row_of(b, r);
+            z[b][r] = a.init && k < a.K && col < a.V ? a.init[at_state + (size_t)k * a.V + col] : 0.f;
+        }
+    const int slot0 = first_slot(a, n, first);
+    const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
+    uint4 rq[XV], rk[XV], rv[VV], ru[UV], rf = make_uint4(0, 0, 0, 0);
+    auto fetch = [&](long long i0) {
+        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
+        const Chunk<T> v = chunk_of<T>(a, a.v, n, h / a.share, first + i0, rows, a.V);
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+            rq[i] = q(xrow + i * XR, xcol);
+            rk[i] = k(xrow + i * XR, xcol);
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) rv[i] = v(vrow + i * VR, v0 + vcol);
+        const char* const prep = a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
+        const uint4* const u = reinterpret_cast<const uint4*>(prep);
+#pragma unroll
+        for (int i = 0; i < UV; ++i)
+            if (i * 256 + tid < F::UNITS * 64) ru[i] = u[i * 256 + tid];
+        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<T>(prep))[tid];
+    };
+    if (count > 0) fetch(0);
+    const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
+    const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
+    const bf16* const vdown = sv + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+    const bf16x8* const sp = su + lane;
+    const bf16x8* const stt = su + F::P_UNITS * 64 + lane;
+    for (long long i0 = 0; i0 < count; i0 += CH) {
+        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+        __syncthreads();                                  // (the chunk before is read)
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+            const int to = XR % 16 ? place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7) : xto + i * XR * KW;
+            store_terms<T>(rq[i], sq + to, XP);
+            store_terms<T>(rk[i], sk + to, XP);
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) {
+            const int to = VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW;
+            store_terms<T>(rv[i], sv + to, VP);
+        }
+#pragma unroll
+        for (int i = 0; i < UV; ++i)
+            if (i * 256 + tid < F::UNITS * 64) reinterpret_cast<uint4*>(su)[i * 256 + tid] = ru[i];
+        if (tid < 1 + CH / 2) reinterpret_cast<uint4*>(sf)[tid] = rf;
+        __syncthreads();
+        const int bad = __builtin_amdgcn_readfirstlane(__float_as_int(sf[2]));
+        if (bad < CH) {                                   // keys from there on: nothing
+            for (int i = tid; i < CH * XC; i += 256)
+                if (i / XC >= bad) store_terms<T>(make_uint4(0, 0, 0, 0), sk + place<KW>(i / XC, i % XC * VN >> 3) + (i % XC * VN & 7), XP);
+            __syncthreads();
+        }
+        const long long next = i0 + CH;
+        const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
+        if (SAVE) {
+            float* const to = a.states + mine * KW * VW + col;
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[row_of(b, r) * VW] = z[b][r];
+        }
+        f32x4 e[JB], o[JB];
+#pragma unroll
+        for (int i = 0; i < JB; ++i) e[i] = o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < KT; ++b) {
+            Sum<T_TERMS, 8> zf;
+            zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
+            const Sum<W, 8> zo = first_terms<W>(zf);
+            const int at = here(xat) ^ 32 * b;
+#pragma unroll
+            for (int i = 0; i < JB; ++i) {
+                e[i] = mfma(across<X>(sk + 16 * i * KW + at, XP), zf, e[i]);
+                o[i] = mfma(zo, across<X>(sq + 16 * i * KW + at, XP), o[i]);
+            }
+        }
+        if (next < count) fetch(next);
+        int since = CH;                                   // the column's first moment that is not finite
+        {
+            f32x4 d[JB];
+#pragma unroll
+            for (int jj = 0; jj < JB / 2; ++jj) {
+                f32x8 v = widened(down<X>(vdown + 32 * jj * NW, 16 * NW, VP));
+                float s = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) s = fmaf(v[r], 0.f, s);
+                if (__ballot(!(s == 0.f)))
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (!(fabsf(v[r]) < INFINITY)) {
+                            since = min(since, 32 * jj + 16 * (r >> 2) + 4 * g + (r & 3));
+                            v[r] = 0.f;
+                        }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int i = 2 * jj + half;
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + 16 * i + 4 * g]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) d[i][r] = fmaf(-f[r], e[i][r], v[4 * half + r]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < JB; ++i) e[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int jj = 0; jj < JB / 2; ++jj) {
+                Sum<T_TERMS, 8> df;
+                df.of_summed(joined(d[2 * jj], d[2 * jj + 1]));
+#pragma unroll
+                for (int i = 2 * jj; i < JB; ++i) {
+                    Sum<T_TERMS, 8> t;
+#pragma unroll
+                    for (int p = 0; p < T_TERMS; ++p) t.term[p] = stt[(piece_of(jj, i) * T_TERMS + p) * 64];
+                    e[i] = mfma(t, df, e[i]);
+                }
+            }
+        }
+        if (__ballot(since < CH)) {
+            since = min(since, __shfl_xor(since, 16));
+            since = min(since, __shfl_xor(since, 32));
+        }
+        since = min(since, bad);
+        const bool spoiled = __ballot(since < CH) != 0;
+        if (SAVE) {
+            float* const to = a.errors + mine * CH * VW + col;
+#pragma unroll
+            for (int i = 0; i < JB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * i + 4 * g + r;
+                    to[row * VW] = row < since ? e[i][r] : row < rows ? NAN : 0.f;
+                }
+        }
+        // the state after the chunk
+        decayed<2 * KT>(z, sf[0], sf[1]);
+#pragma unroll
+        for (int jj = 0; jj < JB / 2; ++jj) {
+            f32x8 u = joined(e[2 * jj], e[2 * jj + 1]);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 32 * jj + 16 * half + 4 * g]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[4 * half + r] *= f[r];
+            }
+            Sum<T_TERMS, 8> uf;
+            uf.of_summed(u);
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) {
+                const bf16* p = sk + 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
+                z[b] = mfma(down<X>(p, 16 * KW, XP), uf, z[b]);
+            }
+        }
+        if (spoiled && since < CH)
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z[b][r] = NAN;
+        // outputs
+#pragma unroll
+        for (int i = 0; i < JB; ++i) {
+            const float f = a.c * sf[F_E + 16 * i + c];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][r] *= f;
+        }
+#pragma unroll
+        for (int jj = 0; jj < JB / 2; ++jj) {
+            Sum<W, 8> ef;
+            ef.of_summed(joined(e[2 * jj], e[2 * jj + 1]));
+#pragma unroll
+            for (int i = 2 * jj; i < JB; ++i) {
+                Sum<W, 8> p;
+#pragma unroll
+                for (int t = 0; t < W; ++t) p.term[t] = sp[(piece_of(jj, i) * W + t) * 64];
+                o[i] = mfma(ef, p, o[i]);
+            }
+        }
+        if (spoiled)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int f = __shfl(since, 4 * g + r);
+#pragma unroll
+                for (int i = 0; i < JB; ++i)
+                    if (16 * i + c >= f) o[i][r] = NAN;
+            }
+        {
+            const int oc = v0 + 16 * wave + 4 * g;
+            T* const po = (T*)a.o + (((a.starts ? 0 : n * a.n_moments) + first + i0) * a.heads + h) * a.V;
+            typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int i = 0; i < JB; ++i) {
+                const int row = 16 * i + c;
+                if (row >= rows || oc >= a.V) continue;
+                T* const to = po + (long long)row * a.heads * a.V + oc;
+                if (a.vec) *reinterpret_cast<vec4*>(to) = __builtin_convertvector(o[i], vec4);
+                else
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (oc + r < a.V) to[r] = narrow<T>(o[i][r]);
+            }
+        }
+    }
+    if (a.fin && col < a.V)
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = row_of(b, r);
+                if (k < a.K) a.fin[at_state + (size_t)k * a.V + col] = z[b][r];
+            }
+}
+
+// ------------------------------------------------------------------------------------------------ the walk backwards
+// The same of X, the gradient of the state after a chunk: y = T^T (P^T g + F beta K X), X' = E_end X + Q^T (c E g) - K^T (E y).
+template <class T, int KT>
+__global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
+    using F = DeltaForm<T>;
+    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
+    constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
+    constexpr int UV = (F::UNITS * 64 + 255) / 256;
+    __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP], sg[X * VP];
+    __shared__ __align__(16) bf16x8 su[F::UNITS * 64];
+    __shared__ __align__(16) float sf[4 + 2 * CH];
+    const int blocks_v = (a.V + NW - 1) / NW;
+    const unsigned block = (unsigned)block_number(), chain = block / blocks_v;
+    const int vb = (int)(block - chain * blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
+    if (n >= a.n_seq) return;
+    long long first, count;
+    stretch_of(a, n, first, count);
+    first = shared_by_all(first);
+    count = shared_by_all(count);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const int v0 = NW * vb, col = v0 + 16 * wave + c, VW = NW * blocks_v;
+    const size_t at_state = ((size_t)n * a.heads + h) * a.K * a.V;
+    auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    f32x4 z[2 * KT];
+#pragma unroll
+    for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int k = row_of(b, r);
+            z[b][r] = a.gfin && k < a.K && col < a.V ? a.gfin[at_state + (size_t)k * a.V + col] : 0.f;
+        }
+    const int slot0 = first_slot(a, n, first);
+    const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
+    uint4 rq[XV], rk[XV], rg[VV], ru[UV], rf = make_uint4(0, 0, 0, 0);
+    auto fetch = [&](long long i0) {
+        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
+        const Chunk<T> go = chunk_of<T>(a, a.go, n, h, first + i0, rows, a.V);
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+            rq[i] = q(xrow + i * XR, xcol);
+            rk[i] = k(xrow + i * XR, xcol);
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) rg[i] = go(vrow + i * VR, v0 + vcol);
+        const char* const prep = a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
+        const uint4* const u = reinterpret_cast<const uint4*>(prep);
+#pragma unroll
+        for (int i = 0; i < UV; ++i)
+            if (i * 256 + tid < F::UNITS * 64) ru[i] = u[i * 256 + tid];
+        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<T>(prep))[tid];
+    };
+    const long long last = count > 0 ? (count - 1) / CH * CH : -1;
+    if (last >= 0) fetch(last);
+    const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
+    const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
+    const bf16* const gdown = sg + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+    const bf16x8* const sp = su + lane;
+    const bf16x8* const stt = su + F::P_UNITS * 64 + lane;
+    for (long long i0 = last; i0 >= 0; i0 -= CH) {
+        __syncthreads();                                  // (the chunk before is read)
+#pragma unroll
+        for (int i = 0; i < XV; ++i) {
+            const int to = XR % 16 ? place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7) : xto + i * XR * KW;
+            store_terms<T>(rq[i], sq + to, XP);
+            store_terms<T>(rk[i], sk + to, XP);
+        }
+#pragma unroll
+        for (int i = 0; i < VV; ++i) {
+            const int to = VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW;
+            store_terms<T>(rg[i], sg + to, VP);
+        }
+#pragma unroll
+        for (int i = 0; i < UV; ++i)
+            if (i * 256 + tid < F::UNITS * 64) reinterpret_cast<uint4*>(su)[i * 256 + tid] = ru[i];
+        if (tid < 1 + CH / 2) reinterpret_cast<uint4*>(sf)[tid] = rf;
+        __syncthreads();
+        const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
+        {
+            float* const to = a.grads + mine * KW * VW + col;
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[row_of(b, r) * VW] = z[b][r];
+        }
+        f32x4 d[JB], y[JB];
+#pragma unroll
+        for (int i = 0; i < JB; ++i) d[i] = y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < KT; ++b) {
+            Sum<T_TERMS, 8> zf;
+            zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
+            const int at = here(xat) ^ 32 * b;
+#pragma unroll
+            for (int i = 0; i < JB; ++i) d[i] = mfma(across<X>(sk + 16 * i * KW + at, XP), zf, d[i]);
+        }
+        if (i0) fetch(i0 - CH);
+#pragma unroll
+        for (int i = 0; i < JB; ++i) {
+            const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 16 * i + 4 * g]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[i][r] *= f[r];
+        }
+        Sum<X, 8> gf[JB / 2];
+#pragma unroll
+        for (int ii = 0; ii < JB / 2; ++ii) {
+            gf[ii] = down<X>(gdown + 32 * ii * NW, 16 * NW, VP);
+#pragma unroll
+            for (int j = 0; j < 2 * ii + 2; ++j) {
+                Sum<W, 8> p;
+#pragma unroll
+                for (int t = 0; t < W; ++t) p.term[t] = sp[(tpiece_of(ii, j) * W + t) * 64];
+                d[j] = mfma(p, gf[ii], d[j]);
+            }
+        }
+#pragma unroll
+        for (int ii = 0; ii < JB / 2; ++ii) {
+            Sum<T_TERMS, 8> df;
+            df.of_summed(joined(d[2 * ii], d[2 * ii + 1]));
+#pragma unroll
+            for (int j = 0; j < 2 * ii + 2; ++j) {
+                Sum<T_TERMS, 8> t;
+#pragma unroll
+                for (int p = 0; p < T_TERMS; ++p) t.term[p] = stt[(tpiece_of(ii, j) * T_TERMS + p) * 64];
+                y[j] = mfma(t, df, y[j]);
+            }
+        }
+        {
+            float* const to = a.ys + mine * CH * VW + col;
+#pragma unroll
+            for (int i = 0; i < JB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) to[(16 * i + 4 * g + r) * VW] = y[i][r];
+        }
+        decayed<2 * KT>(z, sf[0], sf[1]);
+#pragma unroll
+        for (int jj = 0; jj < JB / 2; ++jj) {
+            f32x8 wg = widened(gf[jj]), wy = joined(y[2 * jj], y[2 * jj + 1]);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + 32 * jj + 16 * half + 4 * g]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    wg[4 * half + r] *= a.c * f[r];
+                    wy[4 * half + r] *= -f[r];
+                }
+            }
+            Sum<T_TERMS, 8> gt, yt;
+            gt.of_summed(wg);
+            yt.of_summed(wy);
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) {
+                const int at = 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
+                z[b] = mfma(down<X>(sq + at, 16 * KW, XP), gt, z[b]);
+                z[b] = mfma(down<X>(sk + at, 16 * KW, XP), yt, z[b]);
+            }
+        }
+    }
+    if (a.ginit && col < a.V)
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int k = row_of(b, r);
+                if (k < a.K) a.ginit[at_state + (size_t)k * a.V + col] = z[b][r];
+            }
+}
+
+// ------------------------------------------------------------------------------------------------ the gradients
+// A workgroup a chunk and head; a wave 16 of the keys' values.  First what sums over the values' columns (g S^T, y S^T, e X^T
+// transposed, and g e^T, y e^T in both orders), with g, y and e in LDS and a wave's rows of S and X straight from memory; then
+// q and k take their place, and the 16 x 16 blocks of H and Z, as products' operands, the rest.
+template <class T, int KT, int VT>
+__global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
+    using F = DeltaForm<T>;
+    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, VW = 64 * VT, XP = CH * KW, VP = CH * VW, VN = Vec<T>::N;
+    constexpr int WAVES_ = 2 * KT, THREADS = 64 * WAVES_, XC = KW / VN, VC = VW / VN, PIECES = F::PIECES;
+    constexpr int FIRST = (X + 2 * W) * VP, PIECE = W * 512, SECOND = 2 * X * XP + 4 * PIECES * PIECE;
+    __shared__ __align__(16) bf16 room[FIRST > SECOND ? FIRST : SECOND];
+    __shared__ float hi[CH], lo[CH], sb[CH], se[CH], sw[CH], red[WAVES_][4][CH], red_state[WAVES_];
+    bf16 *const sg = room, *const sy = sg + X * VP, *const ser = sy + W * VP;
+    bf16 *const sq = room, *const sk = sq + X * XP;
+    bf16x8* const sp = reinterpret_cast<bf16x8*>(sk + X * XP);            // [4][PIECES][W][64]
+    const unsigned block = (unsigned)block_number();
+    const int place_in = (int)(block / a.heads), h = (int)(block - (unsigned)place_in * a.heads);
+    if (place_in >= a.slots) return;
+    int n, seg, slot;
+    long long first, count;
+    if (!segment_of(a, place_in, n, seg, slot, first, count)) return;
+    const long long from = (long long)seg * CH, left = count - from;
+    const int rows = (int)(left < CH ? left : CH);
+    if (rows <= 0) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
+    const long long moment = first + from, out_row = (a.starts ? 0 : n * a.n_moments) + moment;
+    const size_t mine = (size_t)slot * a.heads + h;
+    const float* const f = factors_of<T>(a.prep + mine * F::PREP);
+    for (int i = tid; i < CH; i += THREADS) {
+        se[i] = f[F_E + i];
+        sw[i] = f[F_E + 2 * CH + i];
+        sb[i] = f[F_E + 3 * CH + i];
+        hi[i] = f[F_E + 4 * CH + i];
+        lo[i] = f[F_E + 5 * CH + i];
+    }
+    {
+        const Chunk<T> go = chunk_of<T>(a, a.go, n, h, moment, rows, a.V);
+        for (int i = tid; i < CH * VC; i += THREADS) {
+            const int row = i / VC, col = i % VC * VN;
+            store_terms<T>(go(row, col), sg + place<VW>(row, col >> 3) + (col & 7), VP);
+        }
+        const float *const ys = a.ys + mine * CH * VW, *const es = a.errors + mine * CH * VW;
+        for (int i = tid; i < CH * VW / 8; i += THREADS) {
+            const int row = i / (VW / 8), col = i % (VW / 8) * 8, to = place<VW>(row, col >> 3);
+            f32x8 y = joined(reinterpret_cast<const f32x4*>(ys)[2 * i], reinterpret_cast<const f32x4*>(ys)[2 * i + 1]);
+            f32x8 e = joined(reinterpret_cast<const f32x4*>(es)[2 * i], reinterpret_cast<const f32x4*>(es)[2 * i + 1]);
+            if (a.gv && row < rows) {
+                const long long at = ((out_row + row) * a.heads + h) * a.V + col;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (col + r < a.V) {
+                        if (a.share > 1) ((float*)a.gv)[at + r] = y[r];
+                        else ((T*)a.gv)[at + r] = narrow<T>(y[r]);
+                    }
+            }
+            Sum<W, 8> ts, us;
+            ts.of(y);
+            us.of(e);
+#pragma unroll
+            for (int p = 0; p < W; ++p) {
+                *reinterpret_cast<bf16x8*>(sy + to + p * VP) = ts.term[p];
+                *reinterpret_cast<bf16x8*>(ser + to + p * VP) = us.term[p];
+            }
+        }
+    }
+    __syncthreads();
+    f32x4 x1[JB], x2[JB], x3[JB];
+    float dot = 0.f;                                      // <S, X>
+#pragma unroll
+    for (int i = 0; i < JB; ++i) x1[i] = x2[i] = x3[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    {
+        const size_t row = mine * KW * VW + (size_t)(16 * wave + c) * VW + 8 * g;
+#pragma unroll
+        for (int b = 0; b < VW / 32; ++b) {
+            const f32x4* const ps = reinterpret_cast<const f32x4*>(a.states + row + 32 * b);
+            const f32x4* const pg = reinterpret_cast<const f32x4*>(a.grads + row + 32 * b);
+            const f32x8 s = joined(ps[0], ps[1]), x = joined(pg[0], pg[1]);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) dot = fmaf(s[r], x[r], dot);
+            Sum<W, 8> st, xt;
+            st.of_summed(s);
+            xt.of_summed(x);
+#pragma unroll
+            for (int i = 0; i < JB; ++i) {
+                const int at = 16 * i * VW + (place<VW>(c, g) ^ 32 * b);
+                x1[i] = mfma(st, across<X>(sg + at, VP), x1[i]);
+                x2[i] = mfma(st, across<W>(sy + at, VP), x2[i]);
+                x3[i] = mfma(xt, across<W>(ser + at, VP), x3[i]);
+            }
+        }
+    }
+    // blocks of H beta (rows j, columns i), H^T's (rows i, columns j), Z beta, Z^T's
+    constexpr int BLOCKS = JB * (JB + 1) / 2, TASKS = 4 * BLOCKS, MOST = (TASKS + WAVES_ - 1) / WAVES_;
+    f32x4 p[MOST];
+#pragma unroll
+    for (int m = 0; m < MOST; ++m) {
+        const int task = m * WAVES_ + wave;
+        if (task >= TASKS) break;
+        const int set = task / BLOCKS;
+        int i, j;
+        block_of(task - set * BLOCKS, i, j);
+        const int ri = 16 * i * VW, rj = 16 * j * VW;
+        p[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < VW / 32; ++b) {
+            const int at = place<VW>(c, g) ^ 32 * b;
+            if (set == 0) p[m] = mfma(across<W>(ser + rj + at, VP), across<X>(sg + ri + at, VP), p[m]);
+            else if (set == 1) p[m] = mfma(across<X>(sg + ri + at, VP), across<W>(ser + rj + at, VP), p[m]);
+            else if (set == 2) p[m] = mfma(across<W>(ser + rj + at, VP), across<W>(sy + ri + at, VP), p[m]);
+            else p[m] = mfma(across<W>(sy + ri + at, VP), across<W>(ser + rj + at, VP), p[m]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool by_row = set & 1;                  // rows i, columns j
+            const int row = 16 * i + (by_row ? 4 * g + r : c), col = 16 * j + (by_row ? c : 4 * g + r);
+            const float d = exp_of(fminf((hi[row] - hi[col]) + (lo[row] - lo[col]), 88.f)) * (by_row ? 1.f : sb[col]);
+            p[m][r] = set < 2 ? (row >= col ? a.c * d * p[m][r] : 0.f) : (row > col ? -d * p[m][r] : 0.f);
+        }
+    }
+    __syncthreads();                                      // (g, y and e are read)
+#pragma unroll
+    for (int m = 0; m < MOST; ++m) {
+        const int task = m * WAVES_ + wave;
+        if (task >= TASKS) break;
+        const int set = task / BLOCKS;
+        int i, j;
+        block_of(task - set * BLOCKS, i, j);
+        const bool by_row = set & 1;
+        const int piece = by_row ? tpiece_of(i >> 1, j) : piece_of(j >> 1, i), half = by_row ? i & 1 : j & 1;
+        const bool alone = i == j && (by_row ? half == 1 : half == 0);    // (the other half lies above the diagonal)
+        Sum<W, 4> s;
+        s.of_summed(p[m]);
+#pragma unroll
+        for (int t = 0; t < W; ++t) {
+            bf16x4* const to = reinterpret_cast<bf16x4*>(&sp[((set * PIECES + piece) * W + t) * 64 + lane]);
+            to[half] = s.term[t];
+            if (alone) to[1 - half] = bf16x4{};
+        }
+    }
+    {
+        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
+        for (int i = tid; i < CH * XC; i += THREADS) {
+            const int row = i / XC, col = i % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
+            store_terms<T>(q(row, col), sq + to, XP);
+            store_terms<T>(k(row, col), sk + to, XP);
+        }
+    }
+    __syncthreads();
+    const int kd = place<KW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+    const int krow = place<KW>(c, 2 * wave + (g >> 1)) + 4 * (g & 1);     // 4 values of row c, from 16 wave + 4 g
+    float dots[4][JB];
+#pragma unroll
+    for (int i = 0; i < JB; ++i) {
+        const f32x4 k4 = widened<X>(sk + 16 * i * KW + krow, XP);
+        const float e = se[16 * i + c], w = sw[16 * i + c];
+        float s = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s = fmaf(k4[r], x3[i][r], s);
+            x1[i][r] *= a.c * e;
+            x2[i][r] *= -e;
+            x3[i][r] *= w;
+        }
+        dots[3][i] = s;
+    }
+    const bf16x8* const spl = sp + lane;
+    auto piece = [&](int set, int number) {
+        Sum<W, 8> s;
+#pragma unroll
+        for (int t = 0; t < W; ++t) s.term[t] = spl[((set * PIECES + number) * W + t) * 64];
+        return s;
+    };
+#pragma unroll
+    for (int jj = 0; jj < JB / 2; ++jj) {
+        const Sum<X, 8> kt = down<X>(sk + 32 * jj * KW + kd, 16 * KW, XP), qt = down<X>(sq + 32 * jj * KW + kd, 16 * KW, XP);
+#pragma unroll
+        for (int i = 2 * jj; i < JB; ++i) {
+            x1[i] = mfma(kt, piece(0, piece_of(jj, i)), x1[i]);
+            x2[i] = mfma(kt, piece(2, piece_of(jj, i)), x2[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2 * jj + 2; ++j) {
+            x3[j] = mfma(qt, piece(1, tpiece_of(jj, j)), x3[j]);
+            x3[j] = mfma(kt, piece(3, tpiece_of(jj, j)), x3[j]);
+        }
+    }
+    const int kc = 16 * wave + 4 * g;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < JB; ++i) {
+        const f32x4 k4 = widened<X>(sk + 16 * i * KW + krow, XP), q4 = widened<X>(sq + 16 * i * KW + krow, XP);
+        const int row = 16 * i + c;
+        dots[0][i] = dots[1][i] = dots[2][i] = 0.f;
+        f32x4 gk;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            dots[0][i] = fmaf(q4[r], x1[i][r], dots[0][i]);
+            dots[1][i] = fmaf(k4[r], x2[i][r], dots[1][i]);
+            dots[2][i] = fmaf(k4[r], x3[i][r], dots[2][i]);
+            gk[r] = fmaf(sb[row], x3[i][r], x2[i][r]);
+        }
+        if (row >= rows || kc >= a.K) continue;
+        const long long at = ((out_row + row) * a.heads + h) * a.K + kc;
+        if (a.vec) {
+            if (a.gq) *reinterpret_cast<vec4*>((T*)a.gq + at) = __builtin_convertvector(x1[i], vec4);
+            if (a.gk && a.share > 1) *reinterpret_cast<f32x4*>((float*)a.gk + at) = gk;
+            else if (a.gk) *reinterpret_cast<vec4*>((T*)a.gk + at) = __builtin_convertvector(gk, vec4);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (kc + r >= a.K) continue;
+                if (a.gq) ((T*)a.gq)[at + r] = narrow<T>(x1[i][r]);
+                if (a.gk && a.share > 1) ((float*)a.gk)[at + r] = gk[r];
+                else if (a.gk) ((T*)a.gk)[at + r] = narrow<T>(gk[r]);
+            }
+        }
+    }
+    if (!a.glog_decay && !a.gbeta) return;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < JB; ++i) {
+            float s = dots[d][i];
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (g == 0) red[wave][d][16 * i + c] = s;
+        }
+    dot = wave_sum(dot, 64);
+    if (lane == 0) red_state[wave] = dot;
+    __syncthreads();
+    if (wave == 0) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, sx = 0.f;
+        for (int w = 0; w < WAVES_; ++w) {
+            sx += red_state[w];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) s[d] += lane < CH ? red[w][d][lane] : 0.f;
+        }
+        const float b = lane < CH ? sb[lane] : 0.f;
+        float gg = s[0] + s[1] - b * s[2], end = lane < CH ? sw[lane] * b * s[3] : 0.f;
+        end = wave_sum(end, 64) + (f[0] + f[1]) * sx;
+        for (int m = 1; m < 64; m <<= 1) {
+            const float t = __shfl_down(gg, m);
+            if (lane + m < 64) gg += t;
+        }
+        const long long at = (out_row + lane) * a.heads + h;
+        if (lane < rows && a.glog_decay) a.glog_decay[at] = gg + end;
+        if (lane < rows && a.gbeta) a.gbeta[at] = s[2];
+    }
+}
+
+// gradients of shared heads: out[m][j][d] = the sum over a key head's query heads of part[m][share j + i][d]; the first `first`
+// workgroups those of k, the rest those of v
+template <class T>
+__global__ __launch_bounds__(256) void k_delta_share(const float* part_k, T* out_k, int K, long long nk, long long first,
+                                                     const float* part_v, T* out_v, int V, long long nv, int share) {
+    const long long block = block_number();
+    const bool of_v = block >= first;
+    const float* part = of_v ? part_v : part_k;
+    T* out = of_v ? out_v : out_k;
+    const int D = of_v ? V : K;
+    const long long i = (block - (of_v ? first : 0)) * 256 + threadIdx.x, row = i / D;
+    if (i >= (of_v ? nv : nk)) return;
+    const int d = (int)(i - row * D);
+    float s = 0.f;
+    for (int j = 0; j < share; ++j) s += part[(row * share + j) * D + d];
+    out[i] = narrow<T>(s);
+}
+
+// Packed moments before the first stretch and after the last one: zeros in each output.  grid (workgroups, outputs)
+struct Outside {
+    char* out[8];
+    long long row[8];                    // bytes a moment
+};
+__global__ __launch_bounds__(256) void k_delta_outside(Delta a, Outside z) {
+    long long first = 0, rest = a.n_moments, before = 0;
+    if (a.n_seq) {
+        leaf_of(a, a.n_seq, first, rest);
+        before = bound_of(a, 0);
+    }
+    const long long row = z.row[blockIdx.y];
+    auto clear = [&](uintptr_t from, uintptr_t to) {      // (4-byte words, or 2-byte values at the ends)
+        for (uintptr_t p = from + 4 * ((uintptr_t)blockIdx.x * 256 + threadIdx.x); p < to; p += 4 * 256 * (uintptr_t)gridDim.x) {
+            if (!(from & 3) && p + 4 <= to) *(unsigned*)p = 0;
+            else {
+                *(unsigned short*)p = 0;
+                if (p + 2 < to) *(unsigned short*)(p + 2) = 0;
+            }
+        }
+    };
+    const uintptr_t out = (uintptr_t)z.out[blockIdx.y];
+    clear(out, out + before * row);
+    clear(out + first * row, out + (first + rest) * row);
+}
+
+// ------------------------------------------------------------------------------------------------ one moment
+// A workgroup takes CB columns of a row's state of one head, CB / 4 lanes a row of it, every (1024 / CB)th row a lane, all a
+// lane's loads under way at once.  What the state holds under the key, S^T k, and what the query reads of it, S^T q, are joined over
+// rows in one go, as o = c (S^T q + (q . k) beta e) needs no second pass.
+// VEC: 16-byte loads and stores of the states (v_dim a multiple of 4, states aligned).  grid (blocks of columns, heads, rows)
+template <class T, int CB, bool VEC>
+__global__ __launch_bounds__(256) void k_delta_step(fm_delta_step_args a) {
+    constexpr int LR = CB / 4, RG = 256 / LR, PER = DELTA_MAX / RG;
+    __shared__ float part[4][2 * CB + 1];
+    const int tid = threadIdx.x, cg = tid % LR, rg = tid / LR, h = blockIdx.y, K = (int)a.k_dim, N = (int)a.v_dim;
+    const int c0 = blockIdx.x * CB + 4 * cg;
+    const long long n = blockIdx.z, slot = a.slots ? a.slots[n] : n;
+    T* o = (T*)a.o + (n * a.q_heads + h) * N + blockIdx.x * CB;
+    const int cols = min(CB, N - (int)blockIdx.x * CB);
+    if (slot < 0 || slot >= a.n_states) {
+        if (tid < cols) o[tid] = narrow<T>(slot < 0 ? 0.f : NAN);
+        return;
+    }
+    const int hk = h / (int)(a.q_heads / a.k_heads);
+    const T* q = (const T*)a.q.data + n * a.q.seq + h * a.q.head;
+    const T* k = (const T*)a.k.data + n * a.k.seq + hk * a.k.head;
+    const T* v = (const T*)a.v.data + n * a.v.seq + hk * a.v.head;
+    const size_t at = ((size_t)slot * a.q_heads + h) * K * N;
+    float4 s[PER];
+    float kr[PER], qr[PER], vv[4];
+    auto load = [&](const float* p) {
+        if (VEC) return c0 < N ? *reinterpret_cast<const float4*>(p + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
+        return make_float4(c0 < N ? p[c0] : 0.f, c0 + 1 < N ? p[c0 + 1] : 0.f, c0 + 2 < N ? p[c0 + 2] : 0.f,
+                           c0 + 3 < N ? p[c0 + 3] : 0.f);
+    };
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int r = rg + i * RG;
+        s[i] = r < K ? load(a.state + at + (size_t)r * N) : make_float4(0.f, 0.f, 0.f, 0.f);
+        kr[i] = r < K ? widen(k[r]) : 0.f;
+        qr[i] = r < K ? widen(q[r]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = c0 + j < N ? widen(v[c0 + j]) : 0.f;
+    const Keep keep(a.log_decay[n * a.ld_row + h * a.ld_head]);
+    const float beta = a.beta[n * a.be_row + h * a.be_head];
+    float sum[9] = {};                                    // S^T k, S^T q of 4 columns; q . k
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if (rg + i * RG >= K) break;
+        s[i] = make_float4(keep(s[i].x), keep(s[i].y), keep(s[i].z), keep(s[i].w));
+        const float x[4] = {s[i].x, s[i].y, s[i].z, s[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            sum[j] = fmaf(kr[i], x[j], sum[j]);
+            sum[4 + j] = fmaf(qr[i], x[j], sum[4 + j]);
+        }
+        sum[8] = fmaf(qr[i], kr[i], sum[8]);
+    }
+#pragma unroll
+    for (int m = LR; m < 64; m <<= 1)
+#pragma unroll
+        for (int j = 0; j < 9; ++j) sum[j] += __shfl_xor(sum[j], m);
+    if ((tid & 63) < LR) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            part[tid >> 6][4 * cg + j] = sum[j];
+            part[tid >> 6][CB + 4 * cg + j] = sum[4 + j];
+        }
+        if (cg == 0) part[tid >> 6][2 * CB] = sum[8];
+    }
+    __syncthreads();
+    auto joined_at = [&](int i) { return part[0][i] + part[1][i] + part[2][i] + part[3][i]; };
+    float u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = beta * (vv[j] - joined_at(4 * cg + j));
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int r = rg + i * RG;
+        if (r >= K) break;
+        s[i] = make_float4(fmaf(kr[i], u[0], s[i].x), fmaf(kr[i], u[1], s[i].y), fmaf(kr[i], u[2], s[i].z), fmaf(kr[i], u[3], s[i].w));
+        float* p = a.next + at + (size_t)r * N + c0;
+        if (VEC) {
+            if (c0 < N) *reinterpret_cast<float4*>(p) = s[i];
+        } else {
+            if (c0 < N) p[0] = s[i].x;
+            if (c0 + 1 < N) p[1] = s[i].y;
+            if (c0 + 2 < N) p[2] = s[i].z;
+            if (c0 + 3 < N) p[3] = s[i].w;
+        }
+    }
+    if (rg == 0) {
+        const float qk = joined_at(2 * CB);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (4 * cg + j < cols) o[4 * cg + j] = narrow<T>((float)a.scale * fmaf(qk, u[j], joined_at(CB + 4 * cg + j)));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+const char* delta_heads_wrong(long long dtype, long long qh, long long kh, long long kd, long long vd) {
+    if (dtype < FM_F32 || dtype > FM_F16) return "values of an unknown type";
+    if (qh < 1 || kh < 1 || qh % kh || qh > 65535) return "query heads must be a multiple of key heads, at most 65535";
+    if (kd < 1 || kd > DELTA_MAX || vd < 1 || vd > DELTA_MAX) return "heads of other than 1 to 128 values";
+    return nullptr;
+}
+bool share_memory(const float* a, const float* b, long long n) {
+    return a && b && (uintptr_t)a < (uintptr_t)b + 4 * n && (uintptr_t)b < (uintptr_t)a + 4 * n;
+}
+const char* delta_wrong(const fm_delta_args& a, bool bwd, bool sizes_only = false) {
+    if (const char* e = delta_heads_wrong(a.dtype, a.q_heads, a.k_heads, a.k_dim, a.v_dim)) return e;
+    if (a.n_seq < 0 || a.n_seq > 16384) return "other than 0 to 16384 stretches";
+    if (a.n_moments < 0 || a.n_moments > 1LL << 31) return "other than 0 to 2^31 moments";
+    if ((double)a.n_moments * (a.starts ? 1 : (double)a.n_seq) * (double)a.q_heads > 8e9) return "more than 8e9 heads of moments";
+    if (sizes_only) return nullptr;
+    const bool any = a.n_seq && a.n_moments;
+    if (any && (!a.q.data || !a.k.data || !a.v.data || !a.log_decay || !a.beta)) return "a null tensor";
+    if (!bwd && a.n_moments && (a.n_seq || a.starts) && !a.o) return "a null tensor";
+    if (!bwd && share_memory(a.state, a.state_out, a.n_seq * a.q_heads * a.k_dim * a.v_dim)) return "state_out must not be state";
+    if (bwd && any && (!a.go.data || !a.saved)) return "a null tensor";
+    return nullptr;
+}
+
+int chunk_length(long long dtype) { return dtype == FM_BF16 ? Form<bf16>::CHUNK : Form<float>::CHUNK; }
+long long prep_bytes(long long dtype) {
+    return dtype == FM_BF16 ? DeltaForm<bf16>::PREP : dtype == FM_F16 ? DeltaForm<f16>::PREP : DeltaForm<float>::PREP;
+}
+long long chunk_slots(const fm_delta_args& a) {
+    const long long C = chunk_length(a.dtype), most = (a.n_moments + C - 1) / C;
+    if (!a.n_seq || !a.n_moments) return 0;
+    return a.starts && most > 1 ? a.n_moments / C + a.n_seq : a.n_seq * most;
+}
+// floats of a state or of a chunk's rows, padded as the kernels hold them
+long long state_floats(const fm_delta_args& a) { return (a.k_dim <= 64 ? 64 : 128) * (a.v_dim <= 64 ? 64LL : 128); }
+long long row_floats(const fm_delta_args& a) { return chunk_length(a.dtype) * (a.v_dim <= 64 ? 64LL : 128); }
+long long delta_saved_bytes(const fm_delta_args& a) { return 4 * chunk_slots(a) * a.q_heads * (state_floats(a) + row_floats(a)); }
+// float32 parts of shared key / value heads' gradients
+long long delta_part_floats(const fm_delta_args& a, bool of_v) {
+    const long long moments = a.n_moments * (a.starts ? 1 : a.n_seq);
+    return a.q_heads > a.k_heads ? (moments * a.q_heads * (of_v ? a.v_dim : a.k_dim) + 3) / 4 * 4 : 0;
+}
+long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
+    const long long prep = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype);
+    return bwd ? prep + delta_saved_bytes(a) + 4 * (delta_part_floats(a, false) + delta_part_floats(a, true)) : prep;
+}
+
+// 16-byte loads, whole stores: heads of a multiple of 16 bytes, everything aligned, a chunk's rows within 2^30 bytes
+bool delta_wide_rows(const fm_delta_args& p, bool bwd) {
+    const int size = p.dtype == FM_F32 ? 4 : 2;
+    if (p.k_dim * size % 16 || p.v_dim * size % 16) return false;
+    if (!aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
+    auto near = [](long long s) { return s >= 0 && s < STRIDE_MOST; };
+    if (!near(p.q.moment) || !near(p.k.moment) || !near(p.v.moment)) return false;
+    if (!bwd) return !((uintptr_t)p.o & 15);
+    return near(p.go.moment) && aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv) & 15);
+}
+
+Delta delta_of(const fm_delta_args& p, bool bwd) {
+    Delta a{};
+    a.q = p.q;
+    a.k = p.k;
+    a.v = p.v;
+    a.go = p.go;
+    a.log_decay = p.log_decay;
+    a.beta = p.beta;
+    a.ld_seq = p.ld_seq;
+    a.ld_moment = p.ld_moment;
+    a.ld_head = p.ld_head;
+    a.be_seq = p.be_seq;
+    a.be_moment = p.be_moment;
+    a.be_head = p.be_head;
+    a.starts = p.starts;
+    a.n_moments = p.n_moments;
+    a.L = a.L0 = chunk_length(p.dtype);
+    a.nseg = (int)((p.n_moments + a.L - 1) / a.L);
+    if (a.nseg < 1) a.nseg = 1;
+    a.slots = (int)chunk_slots(p);
+    a.wide = (int)p.wide;
+    a.heads = (int)p.q_heads;
+    a.share = (int)(p.q_heads / p.k_heads);
+    a.n_seq = (int)p.n_seq;
+    a.K = (int)p.k_dim;
+    a.V = (int)p.v_dim;
+    a.c = (float)p.scale;
+    a.vec = delta_wide_rows(p, bwd);
+    a.prep = (char*)p.workspace;
+    const long long states = chunk_slots(p) * p.q_heads * state_floats(p);
+    a.states = (float*)p.saved;
+    a.errors = a.states ? a.states + states : nullptr;
+    if (bwd) {
+        a.grads = (float*)(a.prep + chunk_slots(p) * p.q_heads * prep_bytes(p.dtype));
+        a.ys = a.grads + states;
+    }
+    a.init = p.state;
+    a.fin = p.state_out;
+    a.o = p.o;
+    a.gfin = p.gstate_out;
+    a.ginit = p.gstate;
+    a.gq = p.gq;
+    a.gk = p.gk;
+    a.gv = p.gv;
+    a.glog_decay = p.glog_decay;
+    a.gbeta = p.gbeta;
+    return a;
+}
+
+template <class T, int KT>
+void delta_fwd(const Delta& a, hipStream_t st) {
+    if (a.slots) k_delta_prep<T, KT, false><<<blocks_of((long long)a.slots * a.heads), 256, 0, st>>>(a);
+    const dim3 grid = blocks_of((long long)a.n_seq * a.heads * ((a.V + 63) / 64));
+    if (a.states) k_delta_scan<T, KT, true><<<grid, 256, 0, st>>>(a);
+    else k_delta_scan<T, KT, false><<<grid, 256, 0, st>>>(a);
+}
+template <class T, int KT>
+void delta_bwd(const Delta& a, hipStream_t st) {
+    if (a.slots) k_delta_prep<T, KT, true><<<blocks_of((long long)a.slots * a.heads), 256, 0, st>>>(a);
+    k_delta_back<T, KT><<<blocks_of((long long)a.n_seq * a.heads * ((a.V + 63) / 64)), 256, 0, st>>>(a);
+    if (!a.slots || !(a.gq || a.gk || a.gv || a.glog_decay || a.gbeta)) return;
+    const dim3 chunks = blocks_of((long long)a.slots * a.heads);
+    if (a.V <= 64) k_delta_grads<T, KT, 1><<<chunks, 128 * KT, 0, st>>>(a);
+    else k_delta_grads<T, KT, 2><<<chunks, 128 * KT, 0, st>>>(a);
+}
+
+template <class T>
+void delta_of_type(const fm_delta_args& p, bool bwd, hipStream_t st) {
+    Delta a = delta_of(p, bwd);
+    if (p.starts && p.n_moments) {
+        const int size = sizeof(T);
+        Outside z{};
+        int n = 0;
+        auto add = [&](void* out, long long row) {
+            if (!out) return;
+            z.out[n] = (char*)out;
+            z.row[n++] = row;
+        };
+        if (!bwd) add(p.o, p.q_heads * p.v_dim * size);
+        else {
+            const int ks = a.share > 1 && p.n_seq ? 0 : size;             // (shared heads: their parts, below)
+            add(p.gq, p.q_heads * p.k_dim * size);
+            if (ks) add(p.gk, p.k_heads * p.k_dim * size);
+            if (ks) add(p.gv, p.k_heads * p.v_dim * size);
+            add(p.glog_decay, p.q_heads * 4);
+            add(p.gbeta, p.q_heads * 4);
+        }
+        if (bwd && a.share > 1 && p.n_seq) {
+            float* part = a.grads + chunk_slots(p) * p.q_heads * (state_floats(p) + row_floats(p));
+            if (p.gk) add(part, p.q_heads * p.k_dim * 4);
+            if (p.gv) add(part + delta_part_floats(p, false), p.q_heads * p.v_dim * 4);
+        }
+        if (n) k_delta_outside<<<dim3(256, n), 256, 0, st>>>(a, z);
+    }
+    if (!p.n_seq) return;
+    float *part_k = nullptr, *part_v = nullptr;
+    if (bwd && a.share > 1) {
+        part_k = a.grads + chunk_slots(p) * p.q_heads * (state_floats(p) + row_floats(p));
+        part_v = part_k + delta_part_floats(p, false);
+        a.gk = p.gk ? part_k : nullptr;
+        a.gv = p.gv ? part_v : nullptr;
+    }
+    if (bwd) p.k_dim <= 64 ? delta_bwd<T, 2>(a, st) : delta_bwd<T, 4>(a, st);
+    else p.k_dim <= 64 ? delta_fwd<T, 2>(a, st) : delta_fwd<T, 4>(a, st);
+    if (!part_k) return;
+    const long long rows = p.n_moments * (p.starts ? 1 : p.n_seq) * p.k_heads;
+    const long long nk = p.gk ? rows * p.k_dim : 0, nv = p.gv ? rows * p.v_dim : 0;
+    const long long bk = (nk + 255) / 256, bv = (nv + 255) / 256;
+    if (bk + bv)
+        k_delta_share<T><<<blocks_of(bk + bv), 256, 0, st>>>(part_k, (T*)p.gk, (int)p.k_dim, nk, bk, part_v, (T*)p.gv,
+                                                             (int)p.v_dim, nv, a.share);
+}
+
+int delta(const fm_delta_args* args, bool bwd, void* stream) {
+    const std::string name = bwd ? "fm_delta_bwd: " : "fm_delta: ";
+    clear_error();
+    if (!args) return fail((name + "no arguments").c_str());
+    if (const char* e = delta_wrong(*args, bwd)) return fail((name + e).c_str());
+    const long long need = delta_workspace_bytes(*args, bwd);
+    if (need && (!args->workspace || args->workspace_bytes < need)) return fail((name + "the workspace is too small").c_str());
+    const long long kept = delta_saved_bytes(*args);
+    if (kept && args->saved && args->saved_bytes < kept) return fail((name + "saved is too small").c_str());
+    hipStream_t st = (hipStream_t)stream;
+    if (args->dtype == FM_F32) delta_of_type<float>(*args, bwd, st);
+    else if (args->dtype == FM_BF16) delta_of_type<bf16>(*args, bwd, st);
+    else delta_of_type<f16>(*args, bwd, st);
+    FG_CHECK(hipGetLastError(), -1);
+    return 0;
+}
+
+// 32 columns a workgroup, as for the memory that only adds (k_step)
+template <class T>
+void delta_step_of_type(const fm_delta_step_args& a, hipStream_t st) {
+    constexpr int CB = 32;
+    const dim3 grid((unsigned)((a.v_dim + CB - 1) / CB), (unsigned)a.q_heads, (unsigned)a.n);
+    if (a.v_dim % 4 || (((uintptr_t)a.state | (uintptr_t)a.next) & 15)) k_delta_step<T, CB, false><<<grid, 256, 0, st>>>(a);
+    else k_delta_step<T, CB, true><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace fg
+
+using namespace fg;
+
+extern "C" {
+
+long long fm_delta_workspace(const fm_delta_args* a, int backward) {
+    return a && !delta_wrong(*a, false, true) ? delta_workspace_bytes(*a, backward) : 0;
+}
+long long fm_delta_saved(const fm_delta_args* a) { return a && !delta_wrong(*a, false, true) ? delta_saved_bytes(*a) : 0; }
+int fm_delta(const fm_delta_args* a, void* stream) { return delta(a, false, stream); }
+int fm_delta_bwd(const fm_delta_args* a, void* stream) { return delta(a, true, stream); }
+
+int fm_delta_step(const fm_delta_step_args* a, void* stream) {
+    clear_error();
+    if (!a) return fail("fm_delta_step: no arguments");
+    if (const char* e = delta_heads_wrong(a->dtype, a->q_heads, a->k_heads, a->k_dim, a->v_dim))
+        return fail((std::string("fm_delta_step: ") + e).c_str());
+    if (a->n < 0 || a->n > 65535 || a->n_states < 0) return fail("fm_delta_step: other than 0 to 65535 rows");
+    if (!a->n) return 0;
+    if (!a->q.data || !a->k.data || !a->v.data || !a->log_decay || !a->beta || !a->state || !a->next || !a->o)
+        return fail("fm_delta_step: a null tensor");
+    if (!a->slots && a->n_states < a->n) return fail("fm_delta_step: fewer states than rows");
+    if (a->next != a->state && share_memory(a->state, a->next, a->n_states * a->q_heads * a->k_dim * a->v_dim))
+        return fail("fm_delta_step: next must be state or lie outside it");
+    if (a->dtype == FM_F32) delta_step_of_type<float>(*a, (hipStream_t)stream);
+    else if (a->dtype == FM_BF16) delta_step_of_type<bf16>(*a, (hipStream_t)stream);
+    else delta_step_of_type<f16>(*a, (hipStream_t)stream);
+    FG_CHECK(hipGetLastError(), -1);
+    return 0;
+}
+
+}  // extern "C"

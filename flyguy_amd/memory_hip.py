@@ -1,15 +1,18 @@
-"""A memory over decisions on the MI355X library: rotary positions, per-head norms with the rotation, and linear attention
-with a decay for each head (include/flyguy_memory.h).  An addition: the reference remembers nothing from one decision to
+"""A memory over decisions on the MI355X library: rotary positions, per-head norms with the rotation, linear attention
+with a decay for each head, and the gated delta rule (include/flyguy_memory.h).  An addition: the reference remembers nothing from one decision to
 the next (flyguy/fly.py:286-305 decides each moment alone).
 
     q, k = rotary(q, k, table, positions)                       # turned by their positions
     q, k = norm_rotary(q, k, wq, wk, table, positions)          # each head's norm and the turn, in one pass
     o, state = decay_attention(q, k, v, log_decay, state)       # whole stretches, from a state and to a state
     o = decay_step(q, k, v, log_decay, state)                   # one new moment, the state updated in place
+    o, state = delta_attention(q, k, v, log_decay, beta, state) # a memory that corrects what it holds: the gated delta rule
+    o = delta_step(q, k, v, log_decay, beta, state)
 
 Queries and keys are [stretches, moments, heads, values] (decay_step: [rows, heads, values]), float32, bfloat16 or
 binary16, on the GPU, with any strides whose last is 1 (another last stride costs a copy); query heads share key / value
-heads in consecutive groups.  The first three have gradients (backwards, of the first order; tables and decays are fixed).
+heads in consecutive groups.  All but the steps have gradients (backwards, of the first order; tables and decay_attention's
+decays are fixed).
 Work goes to the current stream; nothing synchronises.
 """
 from __future__ import annotations
@@ -27,6 +30,8 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TURN = struct.Struct("=44qd")
 _ATTENTION = struct.Struct("=36qd")
 _STEP = struct.Struct("=24qd")
+_DELTA = struct.Struct("=47qd")
+_DELTA_STEP = struct.Struct("=29qd")
 _PARTIAL_ROWS = 2 * 1024                # fm_turn_partial's most, in rows of a head's values
 
 
@@ -368,6 +373,26 @@ def decay_attention(q, k, v, log_decay, state=None, starts=None, scale: float | 
     return _attend(p, q, k, v, state)
 
 
+def _states(what, state, into, slots, n: int, heads: tuple, dev):
+    """A step's states and slots checked: (where the new states go, slots)."""
+    into = state if into is None else into
+    for name, x in (("state", state), ("into", into)):
+        if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != dev or x.dim() != 4 or \
+                tuple(x.shape[1:]) != heads or not x.is_contiguous():
+            raise ValueError(f"{what}: {name} must be dense float32 [states, {heads[0]}, {heads[1]}, {heads[2]}] on the same GPU")
+    if into.shape != state.shape:
+        raise ValueError(f"{what}: into must hold as many states")
+    if slots is None:
+        if state.shape[0] != n:
+            raise ValueError(f"{what}: one state per row, or slots")
+    elif not isinstance(slots, torch.Tensor) or slots.dtype != torch.int32 or slots.device != dev or \
+            tuple(slots.shape) != (n,):
+        raise ValueError(f"{what}: slots must be int32 [rows] on the same GPU")
+    else:
+        slots = slots.contiguous()
+    return into, slots
+
+
 def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None, into=None):
     """One new moment of decay_attention for each row: q [rows, q heads, values], k, v -> o [rows, q heads, v values].
     state (float32 [states, q heads, values, v values], dense) is updated in place, or the new states are written to
@@ -382,21 +407,7 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
         raise ValueError(f"{what}: has no gradients; decay_attention has")
     n, Hq, K = q.shape
     V, dev = v.shape[2], q.device
-    into = state if into is None else into
-    for name, x in (("state", state), ("into", into)):
-        if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != dev or x.dim() != 4 or \
-                tuple(x.shape[1:]) != (Hq, K, V) or not x.is_contiguous():
-            raise ValueError(f"{what}: {name} must be dense float32 [states, {Hq}, {K}, {V}] on the same GPU")
-    if into.shape != state.shape:
-        raise ValueError(f"{what}: into must hold as many states")
-    if slots is None:
-        if state.shape[0] != n:
-            raise ValueError(f"{what}: one state per row, or slots")
-    elif not isinstance(slots, torch.Tensor) or slots.dtype != torch.int32 or slots.device != dev or \
-            tuple(slots.shape) != (n,):
-        raise ValueError(f"{what}: slots must be int32 [rows] on the same GPU")
-    else:
-        slots = slots.contiguous()
+    into, slots = _states(what, state, into, slots, n, (Hq, K, V), dev)
     log_decay = _decays(what, log_decay, Hq, dev)
     q, k, v = _rows(q), _rows(k), _rows(v)
     o = q.new_empty((n, Hq, V))
@@ -404,6 +415,139 @@ def decay_step(q, k, v, log_decay, state, slots=None, scale: float | None = None
     _call("fm_step", q, _STEP.pack(*views, log_decay.data_ptr(), state.data_ptr(), into.data_ptr(), _ptr(slots),
                                     o.data_ptr(), n, state.shape[0], Hq, k.shape[1], K, V, _TYPES[q.dtype],
                                     float(K ** -0.5 if scale is None else scale)))
+    if not into.is_inference():
+        increment_version(into)               # (autograd does not see the library's write)
+    return o
+
+
+# ------------------------------------------------------------------------------------------------ the gated delta rule
+class _Corrections:
+    """What a delta_attention shares with its gradient."""
+    __slots__ = ("starts", "sizes", "state", "V", "scale")
+
+    def pack(self, q, k, v, log_decay, beta, go=None, state=None, o=None, state_out=None, saved=None, gstate_out=None, gq=None,
+             gk=None, gv=None, glog_decay=None, gbeta=None, gstate=None, work=None) -> bytes:
+        packed = self.starts is not None
+        view = _view3 if packed else _view4
+        gates = (log_decay.data_ptr(), beta.data_ptr(), *((0,) if packed else ()), *log_decay.stride(),
+                 *((0,) if packed else ()), *beta.stride())
+        return _DELTA.pack(*view(q), *view(k), *view(v), *view(go), *gates, _ptr(state), _ptr(self.starts), _ptr(o),
+                           _ptr(state_out), _ptr(saved), 0 if saved is None else saved.numel(), _ptr(gstate_out), _ptr(gq),
+                           _ptr(gk), _ptr(gv), _ptr(glog_decay), _ptr(gbeta), _ptr(gstate), _ptr(work),
+                           0 if work is None else work.numel(), *self.sizes, self.scale)
+
+    def room(self, which: str, *tensors) -> torch.Tensor | None:
+        """A workspace of the forward or the gradient, or what the one leaves for the other."""
+        sizes = (which, self.starts is None, *self.sizes)
+        n = _workspaces.get(sizes)
+        if n is None:
+            if len(_workspaces) >= 4096:
+                _workspaces.clear()
+            args = self.pack(*tensors)
+            n = lib().fm_delta_saved(args) if which == "saved" else lib().fm_delta_workspace(args, int(which == "gradient"))
+            _workspaces[sizes] = n
+        return tensors[0].new_empty(n, dtype=torch.uint8) if n else None
+
+
+def _correct(p: _Corrections, tensors, state, saved=None):
+    q, k, v = map(_rows, tensors[:3])
+    o, state_out = q.new_empty((*q.shape[:-1], p.V)), tensors[3].new_empty(p.state)
+    tensors = (q, k, v, *tensors[3:])
+    _call("fm_delta", q, p.pack(*tensors, state=state, o=o, state_out=state_out, saved=saved, work=p.room("forward", *tensors)))
+    return o, state_out
+
+
+class DeltaHip(torch.autograd.Function):
+    """delta_attention with gradients: apply(q, k, v, log_decay, beta, state, corrections) (state may be None)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, beta, state, p):
+        ctx.p = p
+        ctx.set_materialize_grads(False)
+        tensors = (q, k, v, log_decay, beta)
+        saved = p.room("saved", *tensors)
+        ctx.save_for_backward(*tensors, p.starts, saved)
+        return _correct(p, tensors, state, saved)
+
+    @staticmethod
+    def backward(ctx, go, gstate_out):
+        _once("delta_attention")
+        p = ctx.p
+        q, k, v, log_decay, beta, _, saved = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        go = q.new_zeros((*q.shape[:-1], p.V)) if go is None else _rows(go)
+        gstate_out = None if gstate_out is None else gstate_out.contiguous()
+        gq, gk, gv, gl, gb = (x.new_empty(x.shape) if w else None for x, w in zip((q, k, v, log_decay, beta), want))
+        gstate = log_decay.new_empty(p.state) if want[5] else None
+        tensors = (q, k, v, log_decay, beta)
+        _call("fm_delta_bwd", q, p.pack(*tensors, go=go, saved=saved, gstate_out=gstate_out, gq=gq, gk=gk, gv=gv, glog_decay=gl,
+                                        gbeta=gb, gstate=gstate, work=p.room("gradient", *tensors)))
+        return gq, gk, gv, gl, gb, gstate, None
+
+
+def _gates(what, q, log_decay, beta) -> None:
+    for name, x in (("log_decay", log_decay), ("beta", beta)):
+        if not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.device != q.device or x.shape != q.shape[:-1]:
+            raise ValueError(f"{what}: {name} must be float32 {list(q.shape[:-1])} on the same GPU")
+
+
+def delta_attention(q, k, v, log_decay, beta, state=None, starts=None, scale: float | None = None):
+    """The gated delta rule, a memory that moves what it holds under a key towards the key's new value: with a = exp(log_decay),
+        e_t = v_t - (a_t S_{t-1})^T k_t,   S_t = a_t S_{t-1} + beta_t k_t e_t^T,   o_t = scale S_t^T q_t.
+    q, k, v, state, starts and scale as for decay_attention; log_decay (at most 1; -inf forgets all) and beta are float32, one
+    number for each moment and query head (q's shape without its values), with any strides.  Meant for keys with beta |k|^2 at
+    most 2, as keys of length 1 and rates in (0, 1) have; beyond that a state may grow from moment to moment.
+    Returns (o in q's type, the state after each stretch).  Gradients of q, k, v, log_decay, beta and state; for them the forward
+    keeps each chunk's state and errors (1.5 KB a moment and head of 128 values)."""
+    what = "delta_attention"
+    _no_tangents(what, q, k, v, log_decay, beta, state)
+    dims = 4 if starts is None else 3
+    _heads(what, dims, q, k, v)
+    _shared(what, q, k, v, dims - 2)
+    _gates(what, q, log_decay, beta)
+    p = _Corrections()
+    p.starts, wide = None, 0
+    if starts is None:
+        n, moments = q.shape[:2]
+    else:
+        if not isinstance(starts, torch.Tensor) or starts.dtype not in (torch.int32, torch.int64) or starts.dim() != 1 or \
+                starts.numel() < 1 or starts.device != q.device:
+            raise ValueError(f"{what}: starts must be int32 or int64 [stretches + 1] on the same GPU")
+        p.starts, wide = starts.contiguous(), int(starts.dtype == torch.int64)
+        n, moments = starts.numel() - 1, q.shape[0]
+    H, K = q.shape[-2:]
+    p.V = v.shape[-1]
+    p.state = (n, H, K, p.V)
+    p.sizes = (wide, n, moments, H, k.shape[-2], K, p.V, _TYPES[q.dtype])
+    p.scale = float(K ** -0.5 if scale is None else scale)
+    if state is not None:
+        state = _floats(what, "state", state, p.state, q.device)
+    if _wants_grad(q, k, v, log_decay, beta, state):
+        return DeltaHip.apply(q, k, v, log_decay, beta, state, p)
+    return _correct(p, (q, k, v, log_decay, beta), state)
+
+
+def delta_step(q, k, v, log_decay, beta, state, slots=None, scale: float | None = None, into=None):
+    """One new moment of delta_attention for each row: q [rows, q heads, values], k, v, log_decay and beta float32 [rows, q heads]
+    -> o [rows, q heads, v values].  state, slots and into as for decay_step: the states are updated in place, or the new ones
+    written to `into`.  At most 65535 rows.  No gradients."""
+    what = "delta_step"
+    _no_tangents(what, q, k, v, log_decay, beta, state, into)
+    _heads(what, 3, q, k, v)
+    _shared(what, q, k, v, 1)
+    _gates(what, q, log_decay, beta)
+    if _wants_grad(q, k, v, log_decay, beta, state, into):
+        raise ValueError(f"{what}: has no gradients; delta_attention has")
+    n, Hq, K = q.shape
+    into, slots = _states(what, state, into, slots, n, (Hq, K, v.shape[2]), q.device)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    o = q.new_empty((n, Hq, v.shape[2]))
+    views = [f for x in (q, k, v) for f in (x.data_ptr(), x.stride(0), 0, x.stride(1))]
+    _call("fm_delta_step", q, _DELTA_STEP.pack(*views, log_decay.data_ptr(), beta.data_ptr(), *log_decay.stride(), *beta.stride(),
+                                               state.data_ptr(), into.data_ptr(), _ptr(slots), o.data_ptr(), n, state.shape[0],
+                                               Hq, k.shape[1], K, v.shape[2], _TYPES[q.dtype],
+                                               float(K ** -0.5 if scale is None else scale)))
     if not into.is_inference():
         increment_version(into)               # (autograd does not see the library's write)
     return o

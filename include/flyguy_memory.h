@@ -99,6 +99,55 @@ typedef struct fm_step_args {
 } fm_step_args;
 int fm_step(const fm_step_args* a, void* stream);
 
+/* The gated delta rule: a memory that moves what it holds under a key towards the key's new value.  Each query head has a state,
+ * and each moment a decay a = exp(log_decay) (0 keeps everything, -inf forgets everything, above 0, at most 1, states grow) and a
+ * rate beta of its own; query head h reads key / value head h / (q_heads / k_heads):
+ *   e_t = v_t - (a_t S_{t-1})^T k_t,   S_t = a_t S_{t-1} + beta_t k_t e_t^T,   o_t = scale S_t^T q_t,   S_{-1} = state (0: zeros)
+ * Meant for keys with beta |k|^2 <= 2 (beyond, a state may grow from moment to moment).  Sizes, stretches, packed stretches, o,
+ * state and state_out as for fm_attention; also at most 8e9 heads of moments.  log_decay, beta: float32, strides in values.
+ * A query that is not finite reaches its own output only.  A value of v that is not finite makes its column of outputs and of
+ * the state NaN from its moment on; a key, decay (NaN or +inf) or rate that is not, all of the head's; no earlier moment, other
+ * head or stretch (gradients: no other head or stretch).
+ * saved: fm_delta_saved(a) bytes that the gradient reads (0: no gradient is wanted), workspace: fm_delta_workspace(a, backward)
+ * bytes.  Gradients (fm_delta_bwd): inputs and saved as the forward left them; go of o, gstate_out of state_out (0: zeros); gq, gk,
+ * gv dense like their tensors, glog_decay, gbeta float32 [moments][q_heads], gstate float32; each 0 where not wanted. */
+typedef struct fm_delta_args {
+    fm_view q, k, v, go;
+    const float *log_decay, *beta;
+    long long ld_seq, ld_moment, ld_head, be_seq, be_moment, be_head;
+    const float* state;
+    const void* starts;
+    void* o;
+    float* state_out;
+    void* saved;
+    long long saved_bytes;
+    const float* gstate_out;
+    void *gq, *gk, *gv;
+    float *glog_decay, *gbeta, *gstate;
+    void* workspace;
+    long long workspace_bytes;
+    long long wide, n_seq, n_moments, q_heads, k_heads, k_dim, v_dim, dtype;
+    double scale;
+} fm_delta_args;
+int fm_delta(const fm_delta_args* a, void* stream);
+int fm_delta_bwd(const fm_delta_args* a, void* stream);
+long long fm_delta_workspace(const fm_delta_args* a, int backward);
+long long fm_delta_saved(const fm_delta_args* a);
+
+/* One moment of it for n <= 65535 rows, as fm_step: log_decay and beta of row i and head h at i row + h head. */
+typedef struct fm_delta_step_args {
+    fm_view q, k, v;
+    const float *log_decay, *beta;
+    long long ld_row, ld_head, be_row, be_head;
+    const float* state;
+    float* next;
+    const int* slots;
+    void* o;
+    long long n, n_states, q_heads, k_heads, k_dim, v_dim, dtype;
+    double scale;
+} fm_delta_step_args;
+int fm_delta_step(const fm_delta_step_args* a, void* stream);
+
 /* Layer norm of rows of `width` values (1 to 2^24), row i at x + i x_row (strides in values):
  *   m = mean(x), r = (mean((x - m)^2) + eps)^-1/2, xh = (x - m) r, y = xh weight + bias   (weight 0: 1; bias 0: 0)
  * stats: float32 [rows][2], (m, r) of each row, written if not 0.  Gradients (fm_norm_bwd): x, weight and stats the forward's,
