@@ -53,9 +53,12 @@ struct Delta {
     float *glog_decay, *gbeta;
 };
 
-template <class T>
+// Terms (memory_chunk.h: Form): X hold an input exactly; W what makes an output in the values' type alone, 3 all that a float32 result
+// depends on (the state, and a decay's and rate's gradients: with 2 of them these were off by 3.6e-6 and 6.4e-6 of their
+// size, by 4e-7 in float32's own products).
+template <class T, bool BWD = false>
 struct DeltaForm {
-    static constexpr int X = Form<T>::X, W = Form<T>::W, CH = Form<T>::CHUNK, JB = CH / 16, PIECES = JB == 4 ? 6 : 2;
+    static constexpr int X = Form<T>::X, W = BWD ? T_TERMS : Form<T>::W, CH = Form<T>::CHUNK, JB = CH / 16, PIECES = JB == 4 ? 6 : 2;
     // operands in units of 64 lanes x 16 bytes: P's terms, then T's
     static constexpr int P_UNITS = PIECES * W, T_UNITS = PIECES * T_TERMS, UNITS = P_UNITS + T_UNITS;
     // factors: E_end as 1 + x or x (Keep), the first moment that is not finite (as int), 0; then E, F beta, F, beta and G (high
@@ -64,9 +67,9 @@ struct DeltaForm {
     static constexpr int PREP = UNITS * 1024 + FACTORS * 4;
 };
 enum { F_E = 4 };
-template <class T>
+template <class F>
 __device__ __forceinline__ const float* factors_of(const char* prep) {
-    return reinterpret_cast<const float*>(prep + DeltaForm<T>::UNITS * 1024);
+    return reinterpret_cast<const float*>(prep + F::UNITS * 1024);
 }
 
 // piece of rows' block i and the pair jj of summed blocks 2jj, 2jj + 1 of a lower triangular matrix (JB 4: (0,0) (0,1) (0,2)
@@ -135,6 +138,12 @@ __device__ __forceinline__ Sum<W, 8> first_terms(const Sum<P, 8>& s) {
     for (int i = 0; i < W; ++i) r.term[i] = s.term[i];
     return r;
 }
+// a product of two inputs: all pairs of terms where these are two (binary16: the last is 2^-18 of the product), else mfma's
+template <int P>
+__device__ __forceinline__ f32x4 mfma_whole(const Sum<P, 8>& a, const Sum<P, 8>& b, f32x4 c) {
+    if constexpr (P == 2) c = mfma(a.term[1], b.term[1], c);
+    return mfma(a, b, c);
+}
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // a state times one + f (Keep): one instruction a value, either way
 template <int B>
@@ -162,7 +171,7 @@ __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f
 // A moment whose key, decay or rate is not finite spoils all from there on (k_delta_scan): here its chunk ends before it.
 template <class T, int KT, bool BWD>
 __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
-    using F = DeltaForm<T>;
+    using F = DeltaForm<T, BWD>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, XC = KW / VN;
     constexpr int NP = CH + 4;                            // a row of N and T, padded
     __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP];
@@ -212,7 +221,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
         }
         const double end = __shfl(s, CH - 1);             // (rows past the last add nothing)
         const float b = lane < stop ? be : 0.f, high = (float)s;
-        float* const f = const_cast<float*>(factors_of<T>(prep));
+        float* const f = const_cast<float*>(factors_of<F>(prep));
         if (lane < CH) {
             hi[lane] = high;
             lo[lane] = (float)(s - (double)high);
@@ -254,7 +263,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
 #pragma unroll
         for (int b = 0; b < KT; ++b) {
             const int at = place<KW>(c, g) ^ 32 * b;
-            p = mfma(across<X>(ra + at, XP), across<X>(rb + at, XP), p);
+            p = mfma_whole(across<X>(ra + at, XP), across<X>(rb + at, XP), p);
         }
         if (!of_q) {
 #pragma unroll
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
 #pragma unroll
         for (int i = 0; i < UV; ++i)
             if (i * 256 + tid < F::UNITS * 64) ru[i] = u[i * 256 + tid];
-        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<T>(prep))[tid];
+        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<F>(prep))[tid];
     };
     if (count > 0) fetch(0);
     const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
@@ -597,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
 // The same of X, the gradient of the state after a chunk: y = T^T (P^T g + F beta K X), X' = E_end X + Q^T (c E g) - K^T (E y).
 template <class T, int KT>
 __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
-    using F = DeltaForm<T>;
+    using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
     constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
     constexpr int UV = (F::UNITS * 64 + 255) / 256;
@@ -643,7 +652,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
 #pragma unroll
         for (int i = 0; i < UV; ++i)
             if (i * 256 + tid < F::UNITS * 64) ru[i] = u[i * 256 + tid];
-        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<T>(prep))[tid];
+        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<F>(prep))[tid];
     };
     const long long last = count > 0 ? (count - 1) / CH * CH : -1;
     if (last >= 0) fetch(last);
@@ -767,7 +776,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
 // q and k take their place, and the 16 x 16 blocks of H and Z, as products' operands, the rest.
 template <class T, int KT, int VT>
 __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
-    using F = DeltaForm<T>;
+    using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, VW = 64 * VT, XP = CH * KW, VP = CH * VW, VN = Vec<T>::N;
     constexpr int WAVES_ = 2 * KT, THREADS = 64 * WAVES_, XC = KW / VN, VC = VW / VN, PIECES = F::PIECES;
     constexpr int FIRST = (X + 2 * W) * VP, PIECE = W * 512, SECOND = 2 * X * XP + 4 * PIECES * PIECE;
@@ -788,7 +797,7 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const long long moment = first + from, out_row = (a.starts ? 0 : n * a.n_moments) + moment;
     const size_t mine = (size_t)slot * a.heads + h;
-    const float* const f = factors_of<T>(a.prep + mine * F::PREP);
+    const float* const f = factors_of<F>(a.prep + mine * F::PREP);
     for (int i = tid; i < CH; i += THREADS) {
         se[i] = f[F_E + i];
         sw[i] = f[F_E + 2 * CH + i];
@@ -1174,9 +1183,11 @@ const char* delta_wrong(const fm_delta_args& a, bool bwd, bool sizes_only = fals
 }
 
 int chunk_length(long long dtype) { return dtype == FM_BF16 ? Form<bf16>::CHUNK : Form<float>::CHUNK; }
-long long prep_bytes(long long dtype) {
-    return dtype == FM_BF16 ? DeltaForm<bf16>::PREP : dtype == FM_F16 ? DeltaForm<f16>::PREP : DeltaForm<float>::PREP;
+template <bool BWD>
+long long prep_bytes_of(long long dtype) {
+    return dtype == FM_BF16 ? DeltaForm<bf16, BWD>::PREP : dtype == FM_F16 ? DeltaForm<f16, BWD>::PREP : DeltaForm<float, BWD>::PREP;
 }
+long long prep_bytes(long long dtype, bool bwd) { return bwd ? prep_bytes_of<true>(dtype) : prep_bytes_of<false>(dtype); }
 long long chunk_slots(const fm_delta_args& a) {
     const long long C = chunk_length(a.dtype), most = (a.n_moments + C - 1) / C;
     if (!a.n_seq || !a.n_moments) return 0;
@@ -1192,7 +1203,7 @@ long long delta_part_floats(const fm_delta_args& a, bool of_v) {
     return a.q_heads > a.k_heads ? (moments * a.q_heads * (of_v ? a.v_dim : a.k_dim) + 3) / 4 * 4 : 0;
 }
 long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
-    const long long prep = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype);
+    const long long prep = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, bwd);
     return bwd ? prep + delta_saved_bytes(a) + 4 * (delta_part_floats(a, false) + delta_part_floats(a, true)) : prep;
 }
 
@@ -1240,7 +1251,7 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
     a.states = (float*)p.saved;
     a.errors = a.states ? a.states + states : nullptr;
     if (bwd) {
-        a.grads = (float*)(a.prep + chunk_slots(p) * p.q_heads * prep_bytes(p.dtype));
+        a.grads = (float*)(a.prep + chunk_slots(p) * p.q_heads * prep_bytes(p.dtype, true));
         a.ys = a.grads + states;
     }
     a.init = p.state;
