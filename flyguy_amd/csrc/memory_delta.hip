@@ -38,7 +38,7 @@ struct Delta {
     long long n_moments, L, L0;
     int wide, heads, share, n_seq, nseg, slots, K, V;
     float c;
-    int vec;                             // 16-byte loads
+    int vec;                             // whole stores: heads of a multiple of 16 bytes, outputs aligned
     // workspace, by chunk slot and head
     char* prep;                          // T and P as the products' operands, then the chunk's factors
     float *states, *errors;              // S before each chunk [KW][VW], e [CH][VW] (0: not kept)
@@ -59,8 +59,8 @@ struct Delta {
 template <class T, bool BWD = false>
 struct DeltaForm {
     static constexpr int X = Form<T>::X, W = BWD ? T_TERMS : Form<T>::W, CH = Form<T>::CHUNK, JB = CH / 16, PIECES = JB == 4 ? 6 : 2;
-    // operands in units of 64 lanes x 16 bytes: P's terms, then T's
-    static constexpr int P_UNITS = PIECES * W, T_UNITS = PIECES * T_TERMS, UNITS = P_UNITS + T_UNITS;
+    // operands in units of 64 lanes x 16 bytes: P's terms, then T's, up to whole loads of a workgroup
+    static constexpr int P_UNITS = PIECES * W, T_UNITS = PIECES * T_TERMS, UNITS = (P_UNITS + T_UNITS + 3) / 4 * 4;
     // factors: E_end as 1 + x or x (Keep), the first moment that is not finite (as int), 0; then E, F beta, F, beta and G (high
     // and low part) of each moment
     static constexpr int FACTORS = 4 + 6 * CH;
@@ -83,28 +83,22 @@ __device__ __forceinline__ void block_of(int n, int& i, int& j) {
 }
 
 // ------------------------------------------------------------------------------------------------ a chunk's rows
-// rows of a chunk in memory: 16 bytes of row `row` from value `col`; zeros past the rows and columns
+// rows of a chunk in memory: 16 bytes of row `row` from value `col`; zeros past the rows and columns (whole units: k_delta_pack)
 template <class T>
 struct Chunk {
-    const T* p;
-    int rows, width, vec;
-    long long step;
+    int rows, width, step;
     __amdgpu_buffer_rsrc_t rsrc;
-    __device__ __forceinline__ Chunk(const T* data, int rows, long long step, int width, int vec)
-        : p(data), rows(rows), width(width), vec(vec), step(step),
-          rsrc(rows_at(data, rows, vec ? step * (int)sizeof(T) : 0, width * (int)sizeof(T))) {}
+    __device__ __forceinline__ Chunk(const T* data, int rows, long long step, int width)
+        : rows(rows), width(width), step((int)step * (int)sizeof(T)),
+          rsrc(rows_at(data, rows, step * (int)sizeof(T), (width + Vec<T>::N - 1) / Vec<T>::N * 16)) {}
     __device__ __forceinline__ uint4 operator()(int row, int col) const {
-        const bool there = row < rows && col < width;
-        if (vec) {
-            const unsigned at = there ? row * (int)step * (int)sizeof(T) + col * (int)sizeof(T) : NOWHERE;
-            return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
-        }
-        return load16(p + row * step, col, width, there);
+        const unsigned at = row < rows && col < width ? row * step + col * (int)sizeof(T) : NOWHERE;
+        return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0));
     }
 };
 template <class T>
 __device__ __forceinline__ Chunk<T> chunk_of(const Delta& a, const fm_view& v, int n, int head, long long moment, int rows, int width) {
-    return Chunk<T>((const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + moment * v.moment, rows, v.moment, width, a.vec);
+    return Chunk<T>((const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + moment * v.moment, rows, v.moment, width);
 }
 // a value that is not finite among 16 bytes
 template <class T>
@@ -162,6 +156,28 @@ __device__ __forceinline__ void decayed(f32x4 (&z)[B], float one, float f) {
 }
 constexpr float GONE = -110.f;           // a log decay whose factor is 0 in float32
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// Tensors whose heads are not whole, aligned 16-byte units, or whose moments lie far apart, are copied so that they are, with
+// zeros at a head's end: all other kernels load units.  grid (workgroups, tensors)
+struct Packs {
+    fm_view from[3];
+    void* to[3];
+    int heads[3], width[3];
+    long long moments, n_moments;        // all; of a stretch
+};
+template <class T>
+__global__ __launch_bounds__(256) void k_delta_pack(Packs p) {
+    constexpr int VN = Vec<T>::N;
+    const int t = blockIdx.y, H = p.heads[t], D = p.width[t], units = (D + VN - 1) / VN;
+    const fm_view& v = p.from[t];
+    const long long all = p.moments * H * units;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += 256LL * gridDim.x) {
+        const long long row = i / units, m = row / H, n = m / p.n_moments;
+        const int col = (int)(i - row * units) * VN, h = (int)(row - m * H);
+        const T* from = (const T*)v.data + n * v.seq + (m - n * p.n_moments) * v.moment + h * v.head;
+        reinterpret_cast<uint4*>(p.to[t])[i] = load16(from, col, D, true);
+    }
+}
 
 // ------------------------------------------------------------------------------------------------ T, P and the factors
 // A workgroup a chunk and head.  K K^T and Q K^T on the matrix cores; N in float32 in LDS; T by blocks of 16: those on the diagonal by
@@ -367,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
     using F = DeltaForm<T>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
     constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
-    constexpr int UV = (F::UNITS * 64 + 255) / 256;       // a thread's units of operands
+    constexpr int UV = F::UNITS / 4;                      // a thread's share of the operands
     static_assert(XV * XR == CH && VV * VR == CH, "");
     __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP], sv[X * VP];
     __shared__ __align__(16) bf16x8 su[F::UNITS * 64];
@@ -394,7 +410,8 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
         }
     const int slot0 = first_slot(a, n, first);
     const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
-    uint4 rq[XV], rk[XV], rv[VV], ru[UV], rf = make_uint4(0, 0, 0, 0);
+    uint4 rq[XV], rk[XV], rv[VV];
+    u32x4 ru[UV], rf;
     auto fetch = [&](long long i0) {
         const int rows = (int)(count - i0 < CH ? count - i0 : CH);
         const Chunk<T> q = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
@@ -407,11 +424,10 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
 #pragma unroll
         for (int i = 0; i < VV; ++i) rv[i] = v(vrow + i * VR, v0 + vcol);
         const char* const prep = a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
-        const uint4* const u = reinterpret_cast<const uint4*>(prep);
+        const u32x4* const u = reinterpret_cast<const u32x4*>(prep);
 #pragma unroll
-        for (int i = 0; i < UV; ++i)
-            if (i * 256 + tid < F::UNITS * 64) ru[i] = u[i * 256 + tid];
-        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<F>(prep))[tid];
+        for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];
+        rf = reinterpret_cast<const u32x4*>(factors_of<F>(prep))[min(tid, CH / 2)];
     };
     if (count > 0) fetch(0);
     const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
@@ -434,9 +450,8 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
             store_terms<T>(rv[i], sv + to, VP);
         }
 #pragma unroll
-        for (int i = 0; i < UV; ++i)
-            if (i * 256 + tid < F::UNITS * 64) reinterpret_cast<uint4*>(su)[i * 256 + tid] = ru[i];
-        if (tid < 1 + CH / 2) reinterpret_cast<uint4*>(sf)[tid] = rf;
+        for (int i = 0; i < UV; ++i) reinterpret_cast<u32x4*>(su)[i * 256 + tid] = ru[i];
+        if (tid < 1 + CH / 2) reinterpret_cast<u32x4*>(sf)[tid] = rf;
         __syncthreads();
         const int bad = __builtin_amdgcn_readfirstlane(__float_as_int(sf[2]));
         if (bad < CH) {                                   // keys from there on: nothing
@@ -609,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
     using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
     constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
-    constexpr int UV = (F::UNITS * 64 + 255) / 256;
+    constexpr int UV = F::UNITS / 4;
     __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP], sg[X * VP];
     __shared__ __align__(16) bf16x8 su[F::UNITS * 64];
     __shared__ __align__(16) float sf[4 + 2 * CH];
@@ -635,7 +650,8 @@ __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
         }
     const int slot0 = first_slot(a, n, first);
     const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
-    uint4 rq[XV], rk[XV], rg[VV], ru[UV], rf = make_uint4(0, 0, 0, 0);
+    uint4 rq[XV], rk[XV], rg[VV];
+    u32x4 ru[UV], rf;
     auto fetch = [&](long long i0) {
         const int rows = (int)(count - i0 < CH ? count - i0 : CH);
         const Chunk<T> q = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
@@ -648,11 +664,10 @@ __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
 #pragma unroll
         for (int i = 0; i < VV; ++i) rg[i] = go(vrow + i * VR, v0 + vcol);
         const char* const prep = a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
-        const uint4* const u = reinterpret_cast<const uint4*>(prep);
+        const u32x4* const u = reinterpret_cast<const u32x4*>(prep);
 #pragma unroll
-        for (int i = 0; i < UV; ++i)
-            if (i * 256 + tid < F::UNITS * 64) ru[i] = u[i * 256 + tid];
-        if (tid < 1 + CH / 2) rf = reinterpret_cast<const uint4*>(factors_of<F>(prep))[tid];
+        for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];
+        rf = reinterpret_cast<const u32x4*>(factors_of<F>(prep))[min(tid, CH / 2)];
     };
     const long long last = count > 0 ? (count - 1) / CH * CH : -1;
     if (last >= 0) fetch(last);
@@ -675,9 +690,8 @@ __global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
             store_terms<T>(rg[i], sg + to, VP);
         }
 #pragma unroll
-        for (int i = 0; i < UV; ++i)
-            if (i * 256 + tid < F::UNITS * 64) reinterpret_cast<uint4*>(su)[i * 256 + tid] = ru[i];
-        if (tid < 1 + CH / 2) reinterpret_cast<uint4*>(sf)[tid] = rf;
+        for (int i = 0; i < UV; ++i) reinterpret_cast<u32x4*>(su)[i * 256 + tid] = ru[i];
+        if (tid < 1 + CH / 2) reinterpret_cast<u32x4*>(sf)[tid] = rf;
         __syncthreads();
         const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
         {
@@ -1202,21 +1216,34 @@ long long delta_part_floats(const fm_delta_args& a, bool of_v) {
     const long long moments = a.n_moments * (a.starts ? 1 : a.n_seq);
     return a.q_heads > a.k_heads ? (moments * a.q_heads * (of_v ? a.v_dim : a.k_dim) + 3) / 4 * 4 : 0;
 }
-long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
-    const long long prep = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, bwd);
-    return bwd ? prep + delta_saved_bytes(a) + 4 * (delta_part_floats(a, false) + delta_part_floats(a, true)) : prep;
-}
-
-// 16-byte loads, whole stores: heads of a multiple of 16 bytes, everything aligned, a chunk's rows within 2^30 bytes
-bool delta_wide_rows(const fm_delta_args& p, bool bwd) {
+// whether the kernels can load these tensors as they are: heads of whole 16-byte units, aligned, a chunk's rows within 2^30 bytes
+bool in_whole_units(const fm_delta_args& p, bool bwd) {
     const int size = p.dtype == FM_F32 ? 4 : 2;
     if (p.k_dim * size % 16 || p.v_dim * size % 16) return false;
-    if (!aligned16(p.q, size) || !aligned16(p.k, size) || !aligned16(p.v, size)) return false;
-    auto near = [](long long s) { return s >= 0 && s < STRIDE_MOST; };
-    if (!near(p.q.moment) || !near(p.k.moment) || !near(p.v.moment)) return false;
-    if (!bwd) return !((uintptr_t)p.o & 15);
-    return near(p.go.moment) && aligned16(p.go, size) && !(((uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv) & 15);
+    for (const fm_view* v : {&p.q, &p.k, bwd ? &p.go : &p.v})
+        if (!aligned16(*v, size) || v->moment < 0 || v->moment >= STRIDE_MOST) return false;
+    return true;
 }
+// bytes of their copies: queries, keys, and values or (gradient) the output's gradient
+long long pack_bytes(const fm_delta_args& p, bool bwd, int which) {
+    const int size = p.dtype == FM_F32 ? 4 : 2;
+    const long long moments = p.n_moments * (p.starts ? 1 : p.n_seq), K = (p.k_dim * size + 15) / 16, V = (p.v_dim * size + 15) / 16;
+    return 16 * moments * (which == 0 ? p.q_heads * K : which == 1 ? p.k_heads * K : (bwd ? p.q_heads : p.k_heads) * V);
+}
+bool whole_stores(const fm_delta_args& p) {
+    const int size = p.dtype == FM_F32 ? 4 : 2;
+    return p.k_dim * size % 16 == 0 && p.v_dim * size % 16 == 0 &&
+           !(((uintptr_t)p.o | (uintptr_t)p.gq | (uintptr_t)p.gk | (uintptr_t)p.gv) & 15);
+}
+
+long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
+    long long n = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, bwd);
+    if (bwd) n += delta_saved_bytes(a) + 4 * (delta_part_floats(a, false) + delta_part_floats(a, true));
+    if (chunk_slots(a) && !in_whole_units(a, bwd))
+        for (int i = 0; i < 3; ++i) n += pack_bytes(a, bwd, i);
+    return n;
+}
+
 
 Delta delta_of(const fm_delta_args& p, bool bwd) {
     Delta a{};
@@ -1245,7 +1272,7 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
     a.K = (int)p.k_dim;
     a.V = (int)p.v_dim;
     a.c = (float)p.scale;
-    a.vec = delta_wide_rows(p, bwd);
+    a.vec = whole_stores(p);
     a.prep = (char*)p.workspace;
     const long long states = chunk_slots(p) * p.q_heads * state_floats(p);
     a.states = (float*)p.saved;
@@ -1313,6 +1340,23 @@ void delta_of_type(const fm_delta_args& p, bool bwd, hipStream_t st) {
         if (n) k_delta_outside<<<dim3(256, n), 256, 0, st>>>(a, z);
     }
     if (!p.n_seq) return;
+    if (a.slots && !in_whole_units(p, bwd)) {
+        Packs k{};
+        char* to = a.prep + delta_workspace_bytes(p, bwd);
+        fm_view* const views[3] = {&a.q, &a.k, bwd ? &a.go : &a.v};
+        k.n_moments = p.n_moments;
+        k.moments = p.n_moments * (p.starts ? 1 : p.n_seq);
+        for (int i = 2; i >= 0; --i) {
+            to -= pack_bytes(p, bwd, i);
+            k.from[i] = *views[i];
+            k.to[i] = to;
+            k.heads[i] = i == 0 || (i == 2 && bwd) ? a.heads : (int)p.k_heads;
+            k.width[i] = i == 2 ? a.V : a.K;
+            const long long row = (k.width[i] + Vec<T>::N - 1) / Vec<T>::N * Vec<T>::N;
+            *views[i] = fm_view{to, p.n_moments * k.heads[i] * row, k.heads[i] * row, row};
+        }
+        k_delta_pack<T><<<dim3(2048, 3), 256, 0, st>>>(k);
+    }
     float *part_k = nullptr, *part_v = nullptr;
     if (bwd && a.share > 1) {
         part_k = a.grads + chunk_slots(p) * p.q_heads * (state_floats(p) + row_floats(p));

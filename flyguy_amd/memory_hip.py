@@ -449,8 +449,19 @@ class _Corrections:
         return tensors[0].new_empty(n, dtype=torch.uint8) if n else None
 
 
+def _units(x: torch.Tensor) -> torch.Tensor:
+    """x with its heads' values side by side, and in aligned 16-byte units where they are a multiple of that (the library copies
+    others, in room that goes by sizes alone)."""
+    s, size = x.stride(), x.element_size()
+    if s[-1] != 1 and x.shape[-1] != 1:
+        return x.contiguous()
+    if x.shape[-1] * size % 16 or not (x.data_ptr() % 16 or any(d * size % 16 for d in s[:-1]) or s[-3] >= 1 << 22):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 def _correct(p: _Corrections, tensors, state, saved=None):
-    q, k, v = map(_rows, tensors[:3])
+    q, k, v = map(_units, tensors[:3])
     o, state_out = q.new_empty((*q.shape[:-1], p.V)), tensors[3].new_empty(p.state)
     tensors = (q, k, v, *tensors[3:])
     _call("fm_delta", q, p.pack(*tensors, state=state, o=o, state_out=state_out, saved=saved, work=p.room("forward", *tensors)))
@@ -475,8 +486,8 @@ class DeltaHip(torch.autograd.Function):
         p = ctx.p
         q, k, v, log_decay, beta, _, saved = ctx.saved_tensors
         want = ctx.needs_input_grad
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        go = q.new_zeros((*q.shape[:-1], p.V)) if go is None else _rows(go)
+        q, k, v = _units(q), _units(k), _units(v)
+        go = q.new_zeros((*q.shape[:-1], p.V)) if go is None else _units(go)
         gstate_out = None if gstate_out is None else gstate_out.contiguous()
         gq, gk, gv, gl, gb = (x.new_empty(x.shape) if w else None for x, w in zip((q, k, v, log_decay, beta), want))
         gstate = log_decay.new_empty(p.state) if want[5] else None
