@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
 // A value of v that is not finite makes its column NaN from its moment on; a key, decay or rate that is not, all columns:
 // such moments are left out of the products (0 times them would not be 0) and marked in what is stored.
 template <class T, int KT, bool SAVE>
-__global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
+__global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
     using F = DeltaForm<T>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
     constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_scan(Delta a) {
 // ------------------------------------------------------------------------------------------------ the walk backwards
 // The same of X, the gradient of the state after a chunk: y = T^T (P^T g + F beta K X), X' = E_end X + Q^T (c E g) - K^T (E y).
 template <class T, int KT>
-__global__ __launch_bounds__(256, 2) void k_delta_back(Delta a) {
+__global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
     using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
     constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
