@@ -154,6 +154,8 @@ __device__ __forceinline__ void decayed(f32x4 (&z)[B], float one, float f) {
             for (int r = 0; r < 4; ++r) z[b][r] *= one + f;       // (one of them is 0)
     }
 }
+// (before a loop that uses what was loaded: its first iteration's wait would be every iteration's, for its stores)
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 constexpr float GONE = -110.f;           // a log decay whose factor is 0 in float32
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
             lo[lane] = (float)(s - (double)high);
             sb[lane] = b;
             const float e = exp_of((float)s), left_over = exp_of((float)(end - s));
-            f[F_E + lane] = e;
+            f[F_E + lane] = lane < rows ? e : 0.f;         // (a row past the last adds nothing to a gradient)
             f[F_E + CH + lane] = left_over * b;
             f[F_E + 2 * CH + lane] = left_over;
             f[F_E + 3 * CH + lane] = b;
@@ -370,6 +372,120 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     }
 }
 
+// A chunk's inputs in LDS: rows of q, k and of 64 columns of a third tensor (as terms, swizzled: place), the operands that
+// k_delta_prep left and its first factors.
+// Inputs of one term go there straight from memory (a wave 1 KB at a time), a chunk ahead into the other of two rooms; others
+// pass through registers, where they become terms, a chunk ahead too.
+template <class T, class F, int KT>
+struct Stage {
+    static constexpr int X = F::X, CH = F::CH, KW = 32 * KT, NW = 64, XP = CH * KW, VP = CH * NW, VN = Vec<T>::N;
+    static constexpr bool STRAIGHT = X == 1;
+    static constexpr int K_AT = 2 * X * XP, W_AT = 2 * K_AT, U_AT = W_AT + 2 * X * VP, F_AT = U_AT + F::UNITS * 1024;   // bytes
+    static constexpr int BYTES = F_AT + (STRAIGHT ? 1024 : (16 + 8 * CH)), ROOMS = STRAIGHT ? 2 : 1;
+    static constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR, UV = F::UNITS / 4;
+    static_assert(XV * XR == CH && VV * VR == CH && F::FACTORS * 4 >= (STRAIGHT ? 1024 : 16 + 8 * CH), "");
+    uint4 rq[STRAIGHT ? 1 : XV], rk[STRAIGHT ? 1 : XV], rw[STRAIGHT ? 1 : VV];
+    u32x4 ru[STRAIGHT ? 1 : UV], rf;
+    char* room;
+    int tid, wave, lane;
+    const Delta& a;
+    const fm_view& w;
+    int n, h, hw, c0, slot0;
+    long long first, count;
+
+    __device__ __forceinline__ Stage(char* room, const Delta& a, const fm_view& w, int n, int h, int hw, int c0, int slot0,
+                                     long long first, long long count)
+        : room(room), tid(threadIdx.x), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lane(threadIdx.x & 63), a(a), w(w),
+          n(n), h(h), hw(hw), c0(c0), slot0(slot0), first(first), count(count) {
+        if constexpr (STRAIGHT) {                         // columns past a head's end: zeros for good
+            for (int i = tid; i < ROOMS * BYTES / 16; i += 256) reinterpret_cast<uint4*>(room)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
+    }
+    __device__ __forceinline__ const bf16* q(int which) const { return reinterpret_cast<const bf16*>(room + which * BYTES); }
+    __device__ __forceinline__ bf16* k(int which) const { return reinterpret_cast<bf16*>(room + which * BYTES + K_AT); }
+    __device__ __forceinline__ const bf16* third(int which) const { return reinterpret_cast<const bf16*>(room + which * BYTES + W_AT); }
+    __device__ __forceinline__ const bf16x8* units(int which) const { return reinterpret_cast<const bf16x8*>(room + which * BYTES + U_AT); }
+    __device__ __forceinline__ const float* factors(int which) const { return reinterpret_cast<const float*>(room + which * BYTES + F_AT); }
+
+    __device__ __forceinline__ const char* prepared(long long i0) const {
+        return a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
+    }
+    // 1 KB: a lane's 16 bytes from `from` to 16 bytes times the lane's number behind `to`
+    __device__ __forceinline__ static void straight(const void* from, const char* to) {
+        const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)to);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+    }
+    // rows of a tensor; one past the chunk's last is the last once more (k_delta_prep's factors leave it out)
+    template <int WIDTH, int PER_WAVE>
+    __device__ __forceinline__ void rows_straight(const fm_view& v, int head, long long i0, int rows, int col0, int width, char* to) const {
+        const T* const p = (const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + (first + i0) * v.moment;
+#pragma unroll
+        for (int i = 0; i < PER_WAVE; ++i) {
+            const int unit = 4 * i + wave, at = unit * 512 + lane * 8, row = at / WIDTH;
+            const int col = col0 + (place<WIDTH>(row, at % WIDTH >> 3) - row * WIDTH);
+            if (col < width) straight(p + min(row, rows - 1) * v.moment + col, to + unit * 1024);
+        }
+    }
+    // the chunk from moment i0 on its way into room `which`
+    __device__ __forceinline__ void fetch(long long i0, int which) {
+        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+        const char* const prep = prepared(i0);
+        if constexpr (STRAIGHT) {
+            char* const to = room + which * BYTES;
+            rows_straight<KW, CH * KW / 2048>(a.q, h, i0, rows, 0, a.K, to);
+            rows_straight<KW, CH * KW / 2048>(a.k, h / a.share, i0, rows, 0, a.K, to + K_AT);
+            rows_straight<NW, CH * NW / 2048>(w, hw, i0, rows, c0, a.V, to + W_AT);
+#pragma unroll
+            for (int i = 0; i < UV; ++i) straight(prep + (4 * i + wave) * 1024 + lane * 16, to + U_AT + (4 * i + wave) * 1024);
+            if (wave == 0) straight(prep + F::UNITS * 1024 + lane * 16, to + F_AT);
+        } else {
+            const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
+            const Chunk<T> cw = chunk_of<T>(a, w, n, hw, first + i0, rows, a.V);
+#pragma unroll
+            for (int i = 0; i < XV; ++i) {
+                rq[i] = cq(tid / XC + i * XR, tid % XC * VN);
+                rk[i] = ck(tid / XC + i * XR, tid % XC * VN);
+            }
+#pragma unroll
+            for (int i = 0; i < VV; ++i) rw[i] = cw(tid / VC + i * VR, c0 + tid % VC * VN);
+            const u32x4* const u = reinterpret_cast<const u32x4*>(prep);
+#pragma unroll
+            for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];
+            rf = reinterpret_cast<const u32x4*>(prep + F::UNITS * 1024)[min(tid, CH / 2)];
+        }
+    }
+    // what this wave has on its way is there (before its stores: they are not waited for)
+    __device__ __forceinline__ void landed() const {
+        if constexpr (STRAIGHT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    // what has landed is there for all waves, and what was there before is read by all
+    __device__ __forceinline__ void arrive() {
+        if constexpr (STRAIGHT) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        } else {
+            __syncthreads();
+            bf16 *const sq = const_cast<bf16*>(q(0)), *const sk = k(0), *const sw = const_cast<bf16*>(third(0));
+            const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
+#pragma unroll
+            for (int i = 0; i < XV; ++i) {
+                const int to = place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7);
+                store_terms<T>(rq[i], sq + to, XP);
+                store_terms<T>(rk[i], sk + to, XP);
+            }
+#pragma unroll
+            for (int i = 0; i < VV; ++i)
+                store_terms<T>(rw[i], sw + place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7), VP);
+#pragma unroll
+            for (int i = 0; i < UV; ++i) reinterpret_cast<u32x4*>(room + U_AT)[i * 256 + tid] = ru[i];
+            if (tid < 1 + CH / 2) reinterpret_cast<u32x4*>(room + F_AT)[tid] = rf;
+            __syncthreads();
+        }
+    }
+};
+
 // ------------------------------------------------------------------------------------------------ the walk forwards
 // A workgroup of 4 waves walks one head's chunks for 64 columns of its state, a wave 16: columns never meet, so waves share only
 // what they read.  A chunk's rows and operands go through LDS, the next chunk's on their way in registers meanwhile.  An
@@ -381,13 +497,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
 template <class T, int KT, bool SAVE>
 __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
     using F = DeltaForm<T>;
-    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
-    constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
-    constexpr int UV = F::UNITS / 4;                      // a thread's share of the operands
-    static_assert(XV * XR == CH && VV * VR == CH, "");
-    __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP], sv[X * VP];
-    __shared__ __align__(16) bf16x8 su[F::UNITS * 64];
-    __shared__ __align__(16) float sf[4 + 2 * CH];
+    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, NW = 64, VP = CH * NW;
+    using In = Stage<T, F, KT>;
+    __shared__ __align__(16) char room[In::ROOMS * In::BYTES];
     const int blocks_v = (a.V + NW - 1) / NW;
     const unsigned block = (unsigned)block_number(), chain = block / blocks_v;
     const int vb = (int)(block - chain * blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
@@ -409,57 +521,29 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             z[b][r] = a.init && k < a.K && col < a.V ? a.init[at_state + (size_t)k * a.V + col] : 0.f;
         }
     const int slot0 = first_slot(a, n, first);
-    const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
-    uint4 rq[XV], rk[XV], rv[VV];
-    u32x4 ru[UV], rf;
-    auto fetch = [&](long long i0) {
-        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
-        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
-        const Chunk<T> v = chunk_of<T>(a, a.v, n, h / a.share, first + i0, rows, a.V);
-#pragma unroll
-        for (int i = 0; i < XV; ++i) {
-            rq[i] = q(xrow + i * XR, xcol);
-            rk[i] = k(xrow + i * XR, xcol);
-        }
-#pragma unroll
-        for (int i = 0; i < VV; ++i) rv[i] = v(vrow + i * VR, v0 + vcol);
-        const char* const prep = a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
-        const u32x4* const u = reinterpret_cast<const u32x4*>(prep);
-#pragma unroll
-        for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];
-        rf = reinterpret_cast<const u32x4*>(factors_of<F>(prep))[min(tid, CH / 2)];
-    };
-    if (count > 0) fetch(0);
-    const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
+    In in(room, a, a.v, n, h, h / a.share, v0, slot0, first, count);
+    int which = 0;
+    if (count > 0) in.fetch(0, 0);
+    loads_done();
     const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
-    const bf16* const vdown = sv + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
-    const bf16x8* const sp = su + lane;
-    const bf16x8* const stt = su + F::P_UNITS * 64 + lane;
-    for (long long i0 = 0; i0 < count; i0 += CH) {
+    const int vat = place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+    for (long long i0 = 0; i0 < count; i0 += CH, which ^= In::ROOMS - 1) {
         const int rows = (int)(count - i0 < CH ? count - i0 : CH);
-        __syncthreads();                                  // (the chunk before is read)
-#pragma unroll
-        for (int i = 0; i < XV; ++i) {
-            const int to = XR % 16 ? place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7) : xto + i * XR * KW;
-            store_terms<T>(rq[i], sq + to, XP);
-            store_terms<T>(rk[i], sk + to, XP);
-        }
-#pragma unroll
-        for (int i = 0; i < VV; ++i) {
-            const int to = VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW;
-            store_terms<T>(rv[i], sv + to, VP);
-        }
-#pragma unroll
-        for (int i = 0; i < UV; ++i) reinterpret_cast<u32x4*>(su)[i * 256 + tid] = ru[i];
-        if (tid < 1 + CH / 2) reinterpret_cast<u32x4*>(sf)[tid] = rf;
-        __syncthreads();
+        const long long next = i0 + CH;
+        in.arrive();
+        if (In::STRAIGHT && next < count) in.fetch(next, which ^ 1);
+        const bf16 *const sq = in.q(which), *const vdown = in.third(which) + vat;
+        bf16* const sk = in.k(which);
+        const bf16x8 *const sp = in.units(which) + lane, *const stt = sp + F::P_UNITS * 64;
+        const float* const sf = in.factors(which);
         const int bad = __builtin_amdgcn_readfirstlane(__float_as_int(sf[2]));
         if (bad < CH) {                                   // keys from there on: nothing
-            for (int i = tid; i < CH * XC; i += 256)
-                if (i / XC >= bad) store_terms<T>(make_uint4(0, 0, 0, 0), sk + place<KW>(i / XC, i % XC * VN >> 3) + (i % XC * VN & 7), XP);
-            __syncthreads();
+            for (int i = tid; i < X * CH * KW / 8; i += 256)
+                if (i % (CH * KW / 8) / (KW / 8) >= bad) reinterpret_cast<uint4*>(sk)[i] = make_uint4(0, 0, 0, 0);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
         }
-        const long long next = i0 + CH;
         const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
         if (SAVE) {
             float* const to = a.states + mine * KW * VW + col;
@@ -476,14 +560,14 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
             const Sum<W, 8> zo = first_terms<W>(zf);
-            const int at = here(xat) ^ 32 * b;
+            const int at = xat ^ 32 * b;
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
                 e[i] = mfma(across<X>(sk + 16 * i * KW + at, XP), zf, e[i]);
                 o[i] = mfma(zo, across<X>(sq + 16 * i * KW + at, XP), o[i]);
             }
         }
-        if (next < count) fetch(next);
+        if (!In::STRAIGHT && next < count) in.fetch(next, 0);
         int since = CH;                                   // the column's first moment that is not finite
         {
             f32x4 d[JB];
@@ -554,7 +638,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             uf.of_summed(u);
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
-                const bf16* p = sk + 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
+                const bf16* p = sk + 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1);
                 z[b] = mfma(down<X>(p, 16 * KW, XP), uf, z[b]);
             }
         }
@@ -590,6 +674,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
                 for (int i = 0; i < JB; ++i)
                     if (16 * i + c >= f) o[i][r] = NAN;
             }
+        in.landed();
         {
             const int oc = v0 + 16 * wave + 4 * g;
             T* const po = (T*)a.o + (((a.starts ? 0 : n * a.n_moments) + first + i0) * a.heads + h) * a.V;
@@ -622,12 +707,9 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 template <class T, int KT>
 __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
     using F = DeltaForm<T, true>;
-    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, NW = 64, VP = CH * NW;
-    constexpr int XC = KW / VN, VC = NW / VN, XR = 256 / XC, VR = 256 / VC, XV = CH / XR, VV = CH / VR;
-    constexpr int UV = F::UNITS / 4;
-    __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP], sg[X * VP];
-    __shared__ __align__(16) bf16x8 su[F::UNITS * 64];
-    __shared__ __align__(16) float sf[4 + 2 * CH];
+    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, NW = 64, VP = CH * NW;
+    using In = Stage<T, F, KT>;
+    __shared__ __align__(16) char room[In::ROOMS * In::BYTES];
     const int blocks_v = (a.V + NW - 1) / NW;
     const unsigned block = (unsigned)block_number(), chain = block / blocks_v;
     const int vb = (int)(block - chain * blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
@@ -649,50 +731,19 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
             z[b][r] = a.gfin && k < a.K && col < a.V ? a.gfin[at_state + (size_t)k * a.V + col] : 0.f;
         }
     const int slot0 = first_slot(a, n, first);
-    const int xrow = tid / XC, xcol = tid % XC * VN, vrow = tid / VC, vcol = tid % VC * VN;
-    uint4 rq[XV], rk[XV], rg[VV];
-    u32x4 ru[UV], rf;
-    auto fetch = [&](long long i0) {
-        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
-        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
-        const Chunk<T> go = chunk_of<T>(a, a.go, n, h, first + i0, rows, a.V);
-#pragma unroll
-        for (int i = 0; i < XV; ++i) {
-            rq[i] = q(xrow + i * XR, xcol);
-            rk[i] = k(xrow + i * XR, xcol);
-        }
-#pragma unroll
-        for (int i = 0; i < VV; ++i) rg[i] = go(vrow + i * VR, v0 + vcol);
-        const char* const prep = a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
-        const u32x4* const u = reinterpret_cast<const u32x4*>(prep);
-#pragma unroll
-        for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];
-        rf = reinterpret_cast<const u32x4*>(factors_of<F>(prep))[min(tid, CH / 2)];
-    };
+    In in(room, a, a.go, n, h, h, v0, slot0, first, count);
+    int which = 0;
     const long long last = count > 0 ? (count - 1) / CH * CH : -1;
-    if (last >= 0) fetch(last);
-    const int xto = place<KW>(xrow, xcol >> 3) + (xcol & 7), vto = place<NW>(vrow, vcol >> 3) + (vcol & 7);
+    if (last >= 0) in.fetch(last, 0);
+    loads_done();
     const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
-    const bf16* const gdown = sg + place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
-    const bf16x8* const sp = su + lane;
-    const bf16x8* const stt = su + F::P_UNITS * 64 + lane;
-    for (long long i0 = last; i0 >= 0; i0 -= CH) {
-        __syncthreads();                                  // (the chunk before is read)
-#pragma unroll
-        for (int i = 0; i < XV; ++i) {
-            const int to = XR % 16 ? place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7) : xto + i * XR * KW;
-            store_terms<T>(rq[i], sq + to, XP);
-            store_terms<T>(rk[i], sk + to, XP);
-        }
-#pragma unroll
-        for (int i = 0; i < VV; ++i) {
-            const int to = VR % 16 ? place<NW>(vrow + i * VR, vcol >> 3) + (vcol & 7) : vto + i * VR * NW;
-            store_terms<T>(rg[i], sg + to, VP);
-        }
-#pragma unroll
-        for (int i = 0; i < UV; ++i) reinterpret_cast<u32x4*>(su)[i * 256 + tid] = ru[i];
-        if (tid < 1 + CH / 2) reinterpret_cast<u32x4*>(sf)[tid] = rf;
-        __syncthreads();
+    const int gat = place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+    for (long long i0 = last; i0 >= 0; i0 -= CH, which ^= In::ROOMS - 1) {
+        in.arrive();
+        if (In::STRAIGHT && i0) in.fetch(i0 - CH, which ^ 1);
+        const bf16 *const sq = in.q(which), *const sk = in.k(which), *const gdown = in.third(which) + gat;
+        const bf16x8 *const sp = in.units(which) + lane, *const stt = sp + F::P_UNITS * 64;
+        const float* const sf = in.factors(which);
         const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
         {
             float* const to = a.grads + mine * KW * VW + col;
@@ -708,11 +759,11 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
         for (int b = 0; b < KT; ++b) {
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
-            const int at = here(xat) ^ 32 * b;
+            const int at = xat ^ 32 * b;
 #pragma unroll
             for (int i = 0; i < JB; ++i) d[i] = mfma(across<X>(sk + 16 * i * KW + at, XP), zf, d[i]);
         }
-        if (i0) fetch(i0 - CH);
+        if (!In::STRAIGHT && i0) in.fetch(i0 - CH, 0);
 #pragma unroll
         for (int i = 0; i < JB; ++i) {
             const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 16 * i + 4 * g]);
@@ -768,11 +819,12 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
             yt.of_summed(wy);
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
-                const int at = 32 * jj * KW + (here(yat) ^ 32 * (b >> 1)) + 4 * (b & 1);
+                const int at = 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1);
                 z[b] = mfma(down<X>(sq + at, 16 * KW, XP), gt, z[b]);
                 z[b] = mfma(down<X>(sk + at, 16 * KW, XP), yt, z[b]);
             }
         }
+        in.landed();
     }
     if (a.ginit && col < a.V)
 #pragma unroll
