@@ -154,6 +154,10 @@ __device__ __forceinline__ void decayed(f32x4 (&z)[B], float one, float f) {
             for (int r = 0; r < 4; ++r) z[b][r] *= one + f;       // (one of them is 0)
     }
 }
+// What stands before it is issued before what follows, vector instructions aside.  A SIMD has one wave here: each part of a chunk
+// reads the next part's operands from LDS before its own products, or their wait would be in the open (the compiler reads an
+// operand right before its product).
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0x6); }
 // (before a loop that uses what was loaded: its first iteration's wait would be every iteration's, for its stores)
 __device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 constexpr float GONE = -110.f;           // a log decay whose factor is 0 in float32
@@ -386,6 +390,9 @@ struct Stage {
     static_assert(XV * XR == CH && VV * VR == CH && F::FACTORS * 4 >= (STRAIGHT ? 1024 : 16 + 8 * CH), "");
     uint4 rq[STRAIGHT ? 1 : XV], rk[STRAIGHT ? 1 : XV], rw[STRAIGHT ? 1 : VV];
     u32x4 ru[STRAIGHT ? 1 : UV], rf;
+    static constexpr int QV = CH * KW / 2048, WV = CH * NW / 2048;        // units of 1 KB a wave
+    unsigned oq[QV], ok[QV], ow[WV];                      // a lane's places in them
+    int placed = -1;                                      // ... for chunks of so many rows
     char* room;
     int tid, wave, lane;
     const Delta& a;
@@ -411,34 +418,51 @@ struct Stage {
     __device__ __forceinline__ const char* prepared(long long i0) const {
         return a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
     }
-    // 1 KB: a lane's 16 bytes from `from` to 16 bytes times the lane's number behind `to`
-    __device__ __forceinline__ static void straight(const void* from, const char* to) {
+    // 1 KB: a lane's 16 bytes from `offset` bytes past `base` to 16 bytes times the lane's number behind `to`
+    __device__ __forceinline__ static void straight(const void* base, unsigned offset, const char* to) {
         const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)to);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base) : "memory");
     }
-    // rows of a tensor; one past the chunk's last is the last once more (k_delta_prep's factors leave it out)
-    template <int WIDTH, int PER_WAVE>
-    __device__ __forceinline__ void rows_straight(const fm_view& v, int head, long long i0, int rows, int col0, int width, char* to) const {
-        const T* const p = (const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + (first + i0) * v.moment;
+    // a lane's place in unit 4 i + wave of rows of WIDTH values: value at..; 0xffffffff: past the head's end
+    template <int WIDTH>
+    __device__ __forceinline__ unsigned place_of(int i, int rows, long long step, int col0, int width) const {
+        const int at = (4 * i + wave) * 512 + lane * 8, row = at / WIDTH;
+        const int col = col0 + (place<WIDTH>(row, at % WIDTH >> 3) - row * WIDTH);
+        return col < width ? (unsigned)(min(row, rows - 1) * (int)step + col) * (unsigned)sizeof(T) : ~0u;
+    }
+    __device__ __forceinline__ void places_of(int rows) {
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const int unit = 4 * i + wave, at = unit * 512 + lane * 8, row = at / WIDTH;
-            const int col = col0 + (place<WIDTH>(row, at % WIDTH >> 3) - row * WIDTH);
-            if (col < width) straight(p + min(row, rows - 1) * v.moment + col, to + unit * 1024);
+        for (int i = 0; i < QV; ++i) {
+            oq[i] = place_of<KW>(i, rows, a.q.moment, 0, a.K);
+            ok[i] = place_of<KW>(i, rows, a.k.moment, 0, a.K);
         }
+#pragma unroll
+        for (int i = 0; i < WV; ++i) ow[i] = place_of<NW>(i, rows, w.moment, c0, a.V);
+    }
+    __device__ __forceinline__ const T* base(const fm_view& v, int head, long long i0) const {
+        return (const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + (first + i0) * v.moment;
     }
     // the chunk from moment i0 on its way into room `which`
     __device__ __forceinline__ void fetch(long long i0, int which) {
         const int rows = (int)(count - i0 < CH ? count - i0 : CH);
         const char* const prep = prepared(i0);
         if constexpr (STRAIGHT) {
-            char* const to = room + which * BYTES;
-            rows_straight<KW, CH * KW / 2048>(a.q, h, i0, rows, 0, a.K, to);
-            rows_straight<KW, CH * KW / 2048>(a.k, h / a.share, i0, rows, 0, a.K, to + K_AT);
-            rows_straight<NW, CH * NW / 2048>(w, hw, i0, rows, c0, a.V, to + W_AT);
+            // (rows past the chunk's last are the last once more: k_delta_prep's factors leave them out)
+            if (rows != placed) places_of(placed = rows);
+            char* const to = room + which * BYTES + wave * 1024;
+            const T *const bq = base(a.q, h, i0), *const bk = base(a.k, h / a.share, i0), *const bw = base(w, hw, i0);
 #pragma unroll
-            for (int i = 0; i < UV; ++i) straight(prep + (4 * i + wave) * 1024 + lane * 16, to + U_AT + (4 * i + wave) * 1024);
-            if (wave == 0) straight(prep + F::UNITS * 1024 + lane * 16, to + F_AT);
+            for (int i = 0; i < QV; ++i)
+                if (oq[i] != ~0u) straight(bq, oq[i], to + i * 4096);
+#pragma unroll
+            for (int i = 0; i < QV; ++i)
+                if (ok[i] != ~0u) straight(bk, ok[i], to + K_AT + i * 4096);
+#pragma unroll
+            for (int i = 0; i < WV; ++i)
+                if (ow[i] != ~0u) straight(bw, ow[i], to + W_AT + i * 4096);
+#pragma unroll
+            for (int i = 0; i < UV; ++i) straight(prep + (4 * i + wave) * 1024, lane * 16, to + U_AT + i * 4096);
+            if (wave == 0) straight(prep + F::UNITS * 1024, lane * 16, to + F_AT);
         } else {
             const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
             const Chunk<T> cw = chunk_of<T>(a, w, n, hw, first + i0, rows, a.V);
@@ -501,8 +525,9 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
     using In = Stage<T, F, KT>;
     __shared__ __align__(16) char room[In::ROOMS * In::BYTES];
     const int blocks_v = (a.V + NW - 1) / NW;
-    const unsigned block = (unsigned)block_number(), chain = block / blocks_v;
-    const int vb = (int)(block - chain * blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
+    // (a chain's blocks of columns 8 workgroups apart: on one XCD, whose L2 then holds what they both read)
+    const unsigned block = (unsigned)block_number(), chain = block / (8 * blocks_v) * 8 + (block & 7);
+    const int vb = (int)(block / 8 % blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
     if (n >= a.n_seq) return;
     long long first, count;
     stretch_of(a, n, first, count);
@@ -555,25 +580,50 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
         f32x4 e[JB], o[JB];
 #pragma unroll
         for (int i = 0; i < JB; ++i) e[i] = o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        Sum<X, 8> kf[2][JB], qf[2][JB], vf[JB / 2];
+        Sum<T_TERMS, 8> tf[F::PIECES];
+        auto read_rows = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < JB; ++i) {
+                kf[b & 1][i] = across<X>(sk + 16 * i * KW + (xat ^ 32 * b), XP);
+                qf[b & 1][i] = across<X>(sq + 16 * i * KW + (xat ^ 32 * b), XP);
+            }
+        };
+        read_rows(0);
 #pragma unroll
         for (int b = 0; b < KT; ++b) {
+            if (b + 1 < KT) read_rows(b + 1);
+            else {
+#pragma unroll
+                for (int jj = 0; jj < JB / 2; ++jj) vf[jj] = down<X>(vdown + 32 * jj * NW, 16 * NW, VP);
+#pragma unroll
+                for (int m = 0; m < JB; ++m)
+#pragma unroll
+                    for (int t = 0; t < T_TERMS; ++t) tf[m].term[t] = stt[(m * T_TERMS + t) * 64];
+            }
+            in_order();
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
             const Sum<W, 8> zo = first_terms<W>(zf);
-            const int at = xat ^ 32 * b;
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
-                e[i] = mfma(across<X>(sk + 16 * i * KW + at, XP), zf, e[i]);
-                o[i] = mfma(zo, across<X>(sq + 16 * i * KW + at, XP), o[i]);
+                e[i] = mfma(kf[b & 1][i], zf, e[i]);
+                o[i] = mfma(zo, qf[b & 1][i], o[i]);
             }
+            in_order();
         }
         if (!In::STRAIGHT && next < count) in.fetch(next, 0);
+        Sum<X, 8> kt[2 * KT];                             // (of the first 32 moments; then of the others)
+        auto read_columns = [&](int jj) {
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) kt[b] = down<X>(sk + 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1), 16 * KW, XP);
+        };
         int since = CH;                                   // the column's first moment that is not finite
         {
             f32x4 d[JB];
 #pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
-                f32x8 v = widened(down<X>(vdown + 32 * jj * NW, 16 * NW, VP));
+                f32x8 v = widened(vf[jj]);
                 float s = 0.f;
 #pragma unroll
                 for (int r = 0; r < 8; ++r) s = fmaf(v[r], 0.f, s);
@@ -595,17 +645,19 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 #pragma unroll
             for (int i = 0; i < JB; ++i) e[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
+            for (int m = JB; m < F::PIECES; ++m)
+#pragma unroll
+                for (int t = 0; t < T_TERMS; ++t) tf[m].term[t] = stt[(m * T_TERMS + t) * 64];
+            read_columns(0);
+            in_order();
+#pragma unroll
             for (int jj = 0; jj < JB / 2; ++jj) {
                 Sum<T_TERMS, 8> df;
                 df.of_summed(joined(d[2 * jj], d[2 * jj + 1]));
 #pragma unroll
-                for (int i = 2 * jj; i < JB; ++i) {
-                    Sum<T_TERMS, 8> t;
-#pragma unroll
-                    for (int p = 0; p < T_TERMS; ++p) t.term[p] = stt[(piece_of(jj, i) * T_TERMS + p) * 64];
-                    e[i] = mfma(t, df, e[i]);
-                }
+                for (int i = 2 * jj; i < JB; ++i) e[i] = mfma(tf[piece_of(jj, i)], df, e[i]);
             }
+            in_order();
         }
         if (__ballot(since < CH)) {
             since = min(since, __shfl_xor(since, 16));
@@ -613,34 +665,31 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
         }
         since = min(since, bad);
         const bool spoiled = __ballot(since < CH) != 0;
-        if (SAVE) {
-            float* const to = a.errors + mine * CH * VW + col;
-#pragma unroll
-            for (int i = 0; i < JB; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * i + 4 * g + r;
-                    to[row * VW] = row < since ? e[i][r] : row < rows ? NAN : 0.f;
-                }
-        }
         // the state after the chunk
+        Sum<W, 8> pf[F::PIECES];
+        f32x4 fb[JB];
+        float fo[JB];
+#pragma unroll
+        for (int i = 0; i < JB; ++i) {
+            fb[i] = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 16 * i + 4 * g]);
+            fo[i] = a.c * sf[F_E + 16 * i + c];
+        }
         decayed<2 * KT>(z, sf[0], sf[1]);
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
-            f32x8 u = joined(e[2 * jj], e[2 * jj + 1]);
+            if (jj == JB / 2 - 1) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 32 * jj + 16 * half + 4 * g]);
+                for (int m = 0; m < F::PIECES; ++m)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) u[4 * half + r] *= f[r];
+                    for (int t = 0; t < W; ++t) pf[m].term[t] = sp[(m * W + t) * 64];
             }
+            in_order();
             Sum<T_TERMS, 8> uf;
-            uf.of_summed(u);
+            uf.of_summed(joined(e[2 * jj] * fb[2 * jj], e[2 * jj + 1] * fb[2 * jj + 1]));
 #pragma unroll
-            for (int b = 0; b < 2 * KT; ++b) {
-                const bf16* p = sk + 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1);
-                z[b] = mfma(down<X>(p, 16 * KW, XP), uf, z[b]);
-            }
+            for (int b = 0; b < 2 * KT; ++b) z[b] = mfma(kt[b], uf, z[b]);
+            in_order();
+            if (jj + 1 < JB / 2) read_columns(jj + 1);
         }
         if (spoiled && since < CH)
 #pragma unroll
@@ -649,22 +698,13 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
                 for (int r = 0; r < 4; ++r) z[b][r] = NAN;
         // outputs
 #pragma unroll
-        for (int i = 0; i < JB; ++i) {
-            const float f = a.c * sf[F_E + 16 * i + c];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[i][r] *= f;
-        }
+        for (int i = 0; i < JB; ++i) o[i] *= fo[i];
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
             Sum<W, 8> ef;
             ef.of_summed(joined(e[2 * jj], e[2 * jj + 1]));
 #pragma unroll
-            for (int i = 2 * jj; i < JB; ++i) {
-                Sum<W, 8> p;
-#pragma unroll
-                for (int t = 0; t < W; ++t) p.term[t] = sp[(piece_of(jj, i) * W + t) * 64];
-                o[i] = mfma(ef, p, o[i]);
-            }
+            for (int i = 2 * jj; i < JB; ++i) o[i] = mfma(ef, pf[piece_of(jj, i)], o[i]);
         }
         if (spoiled)
 #pragma unroll
@@ -675,6 +715,16 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
                     if (16 * i + c >= f) o[i][r] = NAN;
             }
         in.landed();
+        if (SAVE) {
+            float* const to = a.errors + mine * CH * VW + col;
+#pragma unroll
+            for (int i = 0; i < JB; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * i + 4 * g + r;
+                    to[row * VW] = row < since ? e[i][r] : row < rows ? NAN : 0.f;
+                }
+        }
         {
             const int oc = v0 + 16 * wave + 4 * g;
             T* const po = (T*)a.o + (((a.starts ? 0 : n * a.n_moments) + first + i0) * a.heads + h) * a.V;
@@ -711,8 +761,9 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
     using In = Stage<T, F, KT>;
     __shared__ __align__(16) char room[In::ROOMS * In::BYTES];
     const int blocks_v = (a.V + NW - 1) / NW;
-    const unsigned block = (unsigned)block_number(), chain = block / blocks_v;
-    const int vb = (int)(block - chain * blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
+    // (a chain's blocks of columns 8 workgroups apart: on one XCD, whose L2 then holds what they both read)
+    const unsigned block = (unsigned)block_number(), chain = block / (8 * blocks_v) * 8 + (block & 7);
+    const int vb = (int)(block / 8 % blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
     if (n >= a.n_seq) return;
     long long first, count;
     stretch_of(a, n, first, count);
@@ -755,45 +806,70 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
         f32x4 d[JB], y[JB];
 #pragma unroll
         for (int i = 0; i < JB; ++i) d[i] = y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        Sum<X, 8> kf[2][JB], gf[JB / 2];
+        Sum<W, 8> pf[F::PIECES];
+        Sum<T_TERMS, 8> tf[F::PIECES];
+        f32x4 fb[JB], fe[JB];
+        auto read_rows = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < JB; ++i) kf[b & 1][i] = across<X>(sk + 16 * i * KW + (xat ^ 32 * b), XP);
+        };
+        read_rows(0);
 #pragma unroll
         for (int b = 0; b < KT; ++b) {
+            if (b + 1 < KT) read_rows(b + 1);
+            else {
+#pragma unroll
+                for (int ii = 0; ii < JB / 2; ++ii) gf[ii] = down<X>(gdown + 32 * ii * NW, 16 * NW, VP);
+#pragma unroll
+                for (int m = 0; m < F::PIECES; ++m)
+#pragma unroll
+                    for (int t = 0; t < W; ++t) pf[m].term[t] = sp[(m * W + t) * 64];
+#pragma unroll
+                for (int i = 0; i < JB; ++i) {
+                    fe[i] = *reinterpret_cast<const f32x4*>(&sf[F_E + 16 * i + 4 * g]);
+                    fb[i] = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 16 * i + 4 * g]);
+                }
+            }
+            in_order();
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
-            const int at = xat ^ 32 * b;
 #pragma unroll
-            for (int i = 0; i < JB; ++i) d[i] = mfma(across<X>(sk + 16 * i * KW + at, XP), zf, d[i]);
+            for (int i = 0; i < JB; ++i) d[i] = mfma(kf[b & 1][i], zf, d[i]);
+            in_order();
         }
         if (!In::STRAIGHT && i0) in.fetch(i0 - CH, 0);
 #pragma unroll
-        for (int i = 0; i < JB; ++i) {
-            const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 16 * i + 4 * g]);
+        for (int m = 0; m < F::PIECES; ++m)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d[i][r] *= f[r];
-        }
-        Sum<X, 8> gf[JB / 2];
+            for (int t = 0; t < T_TERMS; ++t) tf[m].term[t] = stt[(m * T_TERMS + t) * 64];
+        in_order();
 #pragma unroll
-        for (int ii = 0; ii < JB / 2; ++ii) {
-            gf[ii] = down<X>(gdown + 32 * ii * NW, 16 * NW, VP);
+        for (int i = 0; i < JB; ++i) d[i] *= fb[i];
 #pragma unroll
-            for (int j = 0; j < 2 * ii + 2; ++j) {
-                Sum<W, 8> p;
+        for (int ii = 0; ii < JB / 2; ++ii)
 #pragma unroll
-                for (int t = 0; t < W; ++t) p.term[t] = sp[(tpiece_of(ii, j) * W + t) * 64];
-                d[j] = mfma(p, gf[ii], d[j]);
+            for (int j = 0; j < 2 * ii + 2; ++j) d[j] = mfma(pf[tpiece_of(ii, j)], gf[ii], d[j]);
+        in_order();
+        Sum<X, 8> qt[2 * KT], kt[2 * KT];                 // (of the first 32 moments; then of the others)
+        auto read_columns = [&](int jj) {
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) {
+                const int at = 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1);
+                qt[b] = down<X>(sq + at, 16 * KW, XP);
+                kt[b] = down<X>(sk + at, 16 * KW, XP);
             }
-        }
+        };
+        read_columns(0);
+        in_order();
 #pragma unroll
         for (int ii = 0; ii < JB / 2; ++ii) {
             Sum<T_TERMS, 8> df;
             df.of_summed(joined(d[2 * ii], d[2 * ii + 1]));
 #pragma unroll
-            for (int j = 0; j < 2 * ii + 2; ++j) {
-                Sum<T_TERMS, 8> t;
-#pragma unroll
-                for (int p = 0; p < T_TERMS; ++p) t.term[p] = stt[(tpiece_of(ii, j) * T_TERMS + p) * 64];
-                y[j] = mfma(t, df, y[j]);
-            }
+            for (int j = 0; j < 2 * ii + 2; ++j) y[j] = mfma(tf[tpiece_of(ii, j)], df, y[j]);
         }
+        in_order();
         {
             float* const to = a.ys + mine * CH * VW + col;
 #pragma unroll
@@ -804,25 +880,17 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
         decayed<2 * KT>(z, sf[0], sf[1]);
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
-            f32x8 wg = widened(gf[jj]), wy = joined(y[2 * jj], y[2 * jj + 1]);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const f32x4 f = *reinterpret_cast<const f32x4*>(&sf[F_E + 32 * jj + 16 * half + 4 * g]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    wg[4 * half + r] *= a.c * f[r];
-                    wy[4 * half + r] *= -f[r];
-                }
-            }
+            const f32x8 f = joined(fe[2 * jj], fe[2 * jj + 1]);
             Sum<T_TERMS, 8> gt, yt;
-            gt.of_summed(wg);
-            yt.of_summed(wy);
+            gt.of_summed(widened(gf[jj]) * (f * a.c));
+            yt.of_summed(-joined(y[2 * jj], y[2 * jj + 1]) * f);
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
-                const int at = 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1);
-                z[b] = mfma(down<X>(sq + at, 16 * KW, XP), gt, z[b]);
-                z[b] = mfma(down<X>(sk + at, 16 * KW, XP), yt, z[b]);
+                z[b] = mfma(qt[b], gt, z[b]);
+                z[b] = mfma(kt[b], yt, z[b]);
             }
+            in_order();
+            if (jj + 1 < JB / 2) read_columns(jj + 1);
         }
         in.landed();
     }
@@ -1349,14 +1417,14 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
 template <class T, int KT>
 void delta_fwd(const Delta& a, hipStream_t st) {
     if (a.slots) k_delta_prep<T, KT, false><<<blocks_of((long long)a.slots * a.heads), 256, 0, st>>>(a);
-    const dim3 grid = blocks_of((long long)a.n_seq * a.heads * ((a.V + 63) / 64));
+    const dim3 grid = blocks_of(((long long)a.n_seq * a.heads + 7) / 8 * 8 * ((a.V + 63) / 64));
     if (a.states) k_delta_scan<T, KT, true><<<grid, 256, 0, st>>>(a);
     else k_delta_scan<T, KT, false><<<grid, 256, 0, st>>>(a);
 }
 template <class T, int KT>
 void delta_bwd(const Delta& a, hipStream_t st) {
     if (a.slots) k_delta_prep<T, KT, true><<<blocks_of((long long)a.slots * a.heads), 256, 0, st>>>(a);
-    k_delta_back<T, KT><<<blocks_of((long long)a.n_seq * a.heads * ((a.V + 63) / 64)), 256, 0, st>>>(a);
+    k_delta_back<T, KT><<<blocks_of(((long long)a.n_seq * a.heads + 7) / 8 * 8 * ((a.V + 63) / 64)), 256, 0, st>>>(a);
     if (!a.slots || !(a.gq || a.gk || a.gv || a.glog_decay || a.gbeta)) return;
     const dim3 chunks = blocks_of((long long)a.slots * a.heads);
     if (a.V <= 64) k_delta_grads<T, KT, 1><<<chunks, 128 * KT, 0, st>>>(a);
