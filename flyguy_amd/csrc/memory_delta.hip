@@ -939,34 +939,68 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
         hi[i] = f[F_E + 4 * CH + i];
         lo[i] = f[F_E + 5 * CH + i];
     }
+    // all loads at once, in the order that they are used in
+    constexpr int GN = CH * VC, EN = CH * VW / 8, QN = CH * XC;
+    constexpr int GV = (GN + THREADS - 1) / THREADS, EV = (EN + THREADS - 1) / THREADS, QV = (QN + THREADS - 1) / THREADS;
+    auto nth = [&](int i, int most) { return min(i * THREADS + tid, most - 1); };     // (a share past the last: it once more)
+    uint4 rg[GV], rq[QV], rk[QV];
+    f32x4 ry[EV][2], re[EV][2], rs[VW / 32][2], rx[VW / 32][2];
+    const Chunk<T> go = chunk_of<T>(a, a.go, n, h, moment, rows, a.V);
+    const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
     {
-        const Chunk<T> go = chunk_of<T>(a, a.go, n, h, moment, rows, a.V);
-        for (int i = tid; i < CH * VC; i += THREADS) {
-            const int row = i / VC, col = i % VC * VN;
-            store_terms<T>(go(row, col), sg + place<VW>(row, col >> 3) + (col & 7), VP);
+        const f32x4 *const ys = reinterpret_cast<const f32x4*>(a.ys + mine * CH * VW), *const es = reinterpret_cast<const f32x4*>(a.errors + mine * CH * VW);
+        const size_t row = mine * KW * VW + (size_t)(16 * wave + c) * VW + 8 * g;
+#pragma unroll
+        for (int i = 0; i < GV; ++i) rg[i] = go(nth(i, GN) / VC, nth(i, GN) % VC * VN);
+#pragma unroll
+        for (int i = 0; i < EV; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                ry[i][half] = ys[2 * nth(i, EN) + half];
+                re[i][half] = es[2 * nth(i, EN) + half];
+            }
+#pragma unroll
+        for (int b = 0; b < VW / 32; ++b)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                rs[b][half] = *reinterpret_cast<const f32x4*>(a.states + row + 32 * b + 4 * half);
+                rx[b][half] = *reinterpret_cast<const f32x4*>(a.grads + row + 32 * b + 4 * half);
+            }
+#pragma unroll
+        for (int i = 0; i < QV; ++i) {
+            rq[i] = cq(nth(i, QN) / XC, nth(i, QN) % XC * VN);
+            rk[i] = ck(nth(i, QN) / XC, nth(i, QN) % XC * VN);
         }
-        const float *const ys = a.ys + mine * CH * VW, *const es = a.errors + mine * CH * VW;
-        for (int i = tid; i < CH * VW / 8; i += THREADS) {
-            const int row = i / (VW / 8), col = i % (VW / 8) * 8, to = place<VW>(row, col >> 3);
-            f32x8 y = joined(reinterpret_cast<const f32x4*>(ys)[2 * i], reinterpret_cast<const f32x4*>(ys)[2 * i + 1]);
-            f32x8 e = joined(reinterpret_cast<const f32x4*>(es)[2 * i], reinterpret_cast<const f32x4*>(es)[2 * i + 1]);
-            if (a.gv && row < rows) {
-                const long long at = ((out_row + row) * a.heads + h) * a.V + col;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < GV; ++i) {
+        const int row = nth(i, GN) / VC, col = nth(i, GN) % VC * VN;
+        store_terms<T>(rg[i], sg + place<VW>(row, col >> 3) + (col & 7), VP);
+    }
+#pragma unroll
+    for (int i = 0; i < EV; ++i) {
+        const int at = nth(i, EN), row = at / (VW / 8), col = at % (VW / 8) * 8, to = place<VW>(row, col >> 3);
+        const f32x8 y = joined(ry[i][0], ry[i][1]);
+        if (a.gv && row < rows && col < a.V) {
+            const long long to_v = ((out_row + row) * a.heads + h) * a.V + col;
+            typedef T vec8 __attribute__((ext_vector_type(8)));
+            if (a.vec && a.share == 1 && sizeof(T) == 2) *reinterpret_cast<vec8*>((T*)a.gv + to_v) = __builtin_convertvector(y, vec8);
+            else
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
                     if (col + r < a.V) {
-                        if (a.share > 1) ((float*)a.gv)[at + r] = y[r];
-                        else ((T*)a.gv)[at + r] = narrow<T>(y[r]);
+                        if (a.share > 1) ((float*)a.gv)[to_v + r] = y[r];
+                        else ((T*)a.gv)[to_v + r] = narrow<T>(y[r]);
                     }
-            }
-            Sum<W, 8> ts, us;
-            ts.of(y);
-            us.of(e);
+        }
+        Sum<W, 8> ts, us;
+        ts.of(y);
+        us.of(joined(re[i][0], re[i][1]));
 #pragma unroll
-            for (int p = 0; p < W; ++p) {
-                *reinterpret_cast<bf16x8*>(sy + to + p * VP) = ts.term[p];
-                *reinterpret_cast<bf16x8*>(ser + to + p * VP) = us.term[p];
-            }
+        for (int p = 0; p < W; ++p) {
+            *reinterpret_cast<bf16x8*>(sy + to + p * VP) = ts.term[p];
+            *reinterpret_cast<bf16x8*>(ser + to + p * VP) = us.term[p];
         }
     }
     __syncthreads();
@@ -975,12 +1009,9 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
 #pragma unroll
     for (int i = 0; i < JB; ++i) x1[i] = x2[i] = x3[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     {
-        const size_t row = mine * KW * VW + (size_t)(16 * wave + c) * VW + 8 * g;
 #pragma unroll
         for (int b = 0; b < VW / 32; ++b) {
-            const f32x4* const ps = reinterpret_cast<const f32x4*>(a.states + row + 32 * b);
-            const f32x4* const pg = reinterpret_cast<const f32x4*>(a.grads + row + 32 * b);
-            const f32x8 s = joined(ps[0], ps[1]), x = joined(pg[0], pg[1]);
+            const f32x8 s = joined(rs[b][0], rs[b][1]), x = joined(rx[b][0], rx[b][1]);
 #pragma unroll
             for (int r = 0; r < 8; ++r) dot = fmaf(s[r], x[r], dot);
             Sum<W, 8> st, xt;
@@ -1043,13 +1074,11 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
             if (alone) to[1 - half] = bf16x4{};
         }
     }
-    {
-        const Chunk<T> q = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
-        for (int i = tid; i < CH * XC; i += THREADS) {
-            const int row = i / XC, col = i % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
-            store_terms<T>(q(row, col), sq + to, XP);
-            store_terms<T>(k(row, col), sk + to, XP);
-        }
+#pragma unroll
+    for (int i = 0; i < QV; ++i) {
+        const int at = nth(i, QN), row = at / XC, col = at % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
+        store_terms<T>(rq[i], sq + to, XP);
+        store_terms<T>(rk[i], sk + to, XP);
     }
     __syncthreads();
     const int kd = place<KW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
