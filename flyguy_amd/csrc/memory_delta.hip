@@ -29,20 +29,27 @@ namespace fg {
 constexpr int DELTA_MAX = 128;           // values of a head
 constexpr int T_TERMS = 3;               // terms of T, of what it multiplies and of the state: the state is a float32 result
 
-// A launch's view of its stretches, cut into chunks (memory_chunk.h: L is a chunk).
+// How stretches are cut (memory_chunk.h): into chunks, and into segments of whole chunks.
+struct Cuts {
+    const void* starts;
+    long long n_moments, L, L0;
+    int wide, n_seq, nseg, slots;
+};
 struct Delta {
     fm_view q, k, v, go;
     const float *log_decay, *beta;
     long long ld_seq, ld_moment, ld_head, be_seq, be_moment, be_head;
-    const void* starts;
-    long long n_moments, L, L0;
-    int wide, heads, share, n_seq, nseg, slots, K, V;
+    Cuts chunks, segs;
+    int heads, share, K, V;
     float c;
     int vec;                             // whole stores: heads of a multiple of 16 bytes, outputs aligned
     // workspace, by chunk slot and head
     char* prep;                          // T and P as the products' operands, then the chunk's factors
     float *states, *errors;              // S before each chunk [KW][VW], e [CH][VW] (0: not kept)
     float *grads, *ys;                   // X after each chunk, y, the same way
+    // by segment slot and head: a segment's own end state, then its joined one (backwards: X before it) [KW][VW]; what it makes of the
+    // state before it, M with S' = M S + own, and M^T [KW][KW]
+    float *own, *trans, *trans_t;
     // whole tensors
     const float* init;
     float* fin;
@@ -98,7 +105,7 @@ struct Chunk {
 };
 template <class T>
 __device__ __forceinline__ Chunk<T> chunk_of(const Delta& a, const fm_view& v, int n, int head, long long moment, int rows, int width) {
-    return Chunk<T>((const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + moment * v.moment, rows, v.moment, width);
+    return Chunk<T>((const T*)v.data + (a.chunks.starts ? 0 : n * v.seq) + head * v.head + moment * v.moment, rows, v.moment, width);
 }
 // a value that is not finite among 16 bytes
 template <class T>
@@ -202,10 +209,10 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     __shared__ int bad;
     const unsigned block = (unsigned)block_number();
     const int place_in = (int)(block / a.heads), h = (int)(block - (unsigned)place_in * a.heads);
-    if (place_in >= a.slots) return;
+    if (place_in >= a.chunks.slots) return;
     int n, seg, slot;
     long long first, count;
-    if (!segment_of(a, place_in, n, seg, slot, first, count)) return;
+    if (!segment_of(a.chunks, place_in, n, seg, slot, first, count)) return;
     const long long from = (long long)seg * CH, left = count - from;
     const int rows = (int)(left < CH ? left : CH);
     if (rows <= 0) return;
@@ -226,8 +233,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     }
     float ld = 0.f, be = 0.f;
     if (tid < rows) {
-        ld = a.log_decay[(a.starts ? 0 : n * a.ld_seq) + (moment + tid) * a.ld_moment + h * a.ld_head];
-        be = a.beta[(a.starts ? 0 : n * a.be_seq) + (moment + tid) * a.be_moment + h * a.be_head];
+        ld = a.log_decay[(a.chunks.starts ? 0 : n * a.ld_seq) + (moment + tid) * a.ld_moment + h * a.ld_head];
+        be = a.beta[(a.chunks.starts ? 0 : n * a.be_seq) + (moment + tid) * a.be_moment + h * a.be_head];
         if (!(ld < INFINITY) || !(fabsf(be) < INFINITY)) atomicMin(&bad, tid);
     }
     __syncthreads();
@@ -399,11 +406,12 @@ struct Stage {
     const fm_view& w;
     int n, h, hw, c0, slot0;
     long long first, count;
+    bool with_q, with_w;                 // whether q and P, and the third tensor, are wanted
 
     __device__ __forceinline__ Stage(char* room, const Delta& a, const fm_view& w, int n, int h, int hw, int c0, int slot0,
-                                     long long first, long long count)
+                                     long long first, long long count, bool with_q = true, bool with_w = true)
         : room(room), tid(threadIdx.x), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), lane(threadIdx.x & 63), a(a), w(w),
-          n(n), h(h), hw(hw), c0(c0), slot0(slot0), first(first), count(count) {
+          n(n), h(h), hw(hw), c0(c0), slot0(slot0), first(first), count(count), with_q(with_q), with_w(with_w) {
         if constexpr (STRAIGHT) {                         // columns past a head's end: zeros for good
             for (int i = tid; i < ROOMS * BYTES / 16; i += 256) reinterpret_cast<uint4*>(room)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
@@ -440,7 +448,7 @@ struct Stage {
         for (int i = 0; i < WV; ++i) ow[i] = place_of<NW>(i, rows, w.moment, c0, a.V);
     }
     __device__ __forceinline__ const T* base(const fm_view& v, int head, long long i0) const {
-        return (const T*)v.data + (a.starts ? 0 : n * v.seq) + head * v.head + (first + i0) * v.moment;
+        return (const T*)v.data + (a.chunks.starts ? 0 : n * v.seq) + head * v.head + (first + i0) * v.moment;
     }
     // the chunk from moment i0 on its way into room `which`
     __device__ __forceinline__ void fetch(long long i0, int which) {
@@ -453,29 +461,30 @@ struct Stage {
             const T *const bq = base(a.q, h, i0), *const bk = base(a.k, h / a.share, i0), *const bw = base(w, hw, i0);
 #pragma unroll
             for (int i = 0; i < QV; ++i)
-                if (oq[i] != ~0u) straight(bq, oq[i], to + i * 4096);
+                if (with_q && oq[i] != ~0u) straight(bq, oq[i], to + i * 4096);
 #pragma unroll
             for (int i = 0; i < QV; ++i)
                 if (ok[i] != ~0u) straight(bk, ok[i], to + K_AT + i * 4096);
 #pragma unroll
             for (int i = 0; i < WV; ++i)
-                if (ow[i] != ~0u) straight(bw, ow[i], to + W_AT + i * 4096);
+                if (with_w && ow[i] != ~0u) straight(bw, ow[i], to + W_AT + i * 4096);
 #pragma unroll
-            for (int i = 0; i < UV; ++i) straight(prep + (4 * i + wave) * 1024, lane * 16, to + U_AT + i * 4096);
+            for (int i = 0; i < UV; ++i)
+                if (with_q || 4 * i + wave >= F::P_UNITS) straight(prep + (4 * i + wave) * 1024, lane * 16, to + U_AT + i * 4096);
             if (wave == 0) straight(prep + F::UNITS * 1024, lane * 16, to + F_AT);
         } else {
             const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
             const Chunk<T> cw = chunk_of<T>(a, w, n, hw, first + i0, rows, a.V);
 #pragma unroll
             for (int i = 0; i < XV; ++i) {
-                rq[i] = cq(tid / XC + i * XR, tid % XC * VN);
+                if (with_q) rq[i] = cq(tid / XC + i * XR, tid % XC * VN);
                 rk[i] = ck(tid / XC + i * XR, tid % XC * VN);
             }
 #pragma unroll
-            for (int i = 0; i < VV; ++i) rw[i] = cw(tid / VC + i * VR, c0 + tid % VC * VN);
+            for (int i = 0; i < VV; ++i) rw[i] = with_w ? cw(tid / VC + i * VR, c0 + tid % VC * VN) : make_uint4(0, 0, 0, 0);
             const u32x4* const u = reinterpret_cast<const u32x4*>(prep);
 #pragma unroll
-            for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];
+            for (int i = 0; i < UV; ++i) ru[i] = u[i * 256 + tid];        // (P too, where it is not wanted)
             rf = reinterpret_cast<const u32x4*>(prep + F::UNITS * 1024)[min(tid, CH / 2)];
         }
     }
@@ -496,7 +505,7 @@ struct Stage {
 #pragma unroll
             for (int i = 0; i < XV; ++i) {
                 const int to = place<KW>(xrow + i * XR, xcol >> 3) + (xcol & 7);
-                store_terms<T>(rq[i], sq + to, XP);
+                if (with_q) store_terms<T>(rq[i], sq + to, XP);
                 store_terms<T>(rk[i], sk + to, XP);
             }
 #pragma unroll
@@ -518,45 +527,57 @@ struct Stage {
 // values side by side.
 // A value of v that is not finite makes its column NaN from its moment on; a key, decay or rate that is not, all columns:
 // such moments are left out of the products (0 times them would not be 0) and marked in what is stored.
-template <class T, int KT, bool SAVE>
+enum Walk { PLAY, KEEP, OWN };            // outputs; outputs, states and errors kept; a segment's own end state alone
+template <class T, int KT, Walk WALK>
 __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
     using F = DeltaForm<T>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, NW = 64, VP = CH * NW;
     using In = Stage<T, F, KT>;
     __shared__ __align__(16) char room[In::ROOMS * In::BYTES];
-    const int blocks_v = (a.V + NW - 1) / NW;
-    // (a chain's blocks of columns 8 workgroups apart: on one XCD, whose L2 then holds what they both read)
-    const unsigned block = (unsigned)block_number(), chain = block / (8 * blocks_v) * 8 + (block & 7);
-    const int vb = (int)(block / 8 % blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
-    if (n >= a.n_seq) return;
+    const int blocks_v = (a.V + NW - 1) / NW, blocks = WALK == OWN ? blocks_v + KT / 2 : blocks_v;
+    // (a segment's blocks of columns 8 workgroups apart: on one XCD, whose L2 then holds what they all read)
+    const unsigned block = (unsigned)block_number(), unit = block / (8 * blocks) * 8 + (block & 7), place_in = unit / a.heads;
+    const int vb = (int)(block / 8 % blocks), h = (int)(unit - place_in * a.heads);
+    if (place_in >= (unsigned)a.segs.slots) return;
+    int n, seg, slot;
     long long first, count;
-    stretch_of(a, n, first, count);
-    first = shared_by_all(first);
-    count = shared_by_all(count);
+    if (!segment_of(a.segs, (int)place_in, n, seg, slot, first, count)) return;
+    n = __builtin_amdgcn_readfirstlane(n);
+    seg = __builtin_amdgcn_readfirstlane(seg);
+    slot = __builtin_amdgcn_readfirstlane(slot);
+    const int slot0 = first_slot(a.chunks, n, shared_by_all(first)) + (int)(seg * (a.segs.L / CH));
+    const long long from = start_of(a.segs, seg), left = shared_by_all(count - from < a.segs.L ? count - from : a.segs.L);
+    const bool last = shared_by_all(count) == from + left;
+    first = shared_by_all(first) + from;
+    // a segment's own state: none is needed of the last one; the first one's is the true one, which needs no M
+    const bool moves = WALK == OWN && vb >= blocks_v;     // columns of M
+    if (WALK == OWN && (last || (moves && seg == 0))) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int v0 = NW * vb, col = v0 + 16 * wave + c, VW = NW * blocks_v;
     const size_t at_state = ((size_t)n * a.heads + h) * a.K * a.V;
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    const size_t seg_state = (size_t)a.heads * KW * VW, at_seg = (size_t)slot * seg_state + (size_t)h * KW * VW;
     f32x4 z[2 * KT];
 #pragma unroll
     for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = row_of(b, r);
-            z[b][r] = a.init && k < a.K && col < a.V ? a.init[at_state + (size_t)k * a.V + col] : 0.f;
+            if (moves) z[b][r] = k == col - NW * blocks_v ? 1.f : 0.f;
+            else if (seg) z[b][r] = WALK == OWN ? 0.f : a.own[at_seg - seg_state + (size_t)k * VW + col];
+            else z[b][r] = a.init && k < a.K && col < a.V ? a.init[at_state + (size_t)k * a.V + col] : 0.f;
         }
-    const int slot0 = first_slot(a, n, first);
-    In in(room, a, a.v, n, h, h / a.share, v0, slot0, first, count);
+    In in(room, a, a.v, n, h, h / a.share, v0, slot0, first, left, WALK != OWN, !moves);
     int which = 0;
-    if (count > 0) in.fetch(0, 0);
+    if (left > 0) in.fetch(0, 0);
     loads_done();
     const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
     const int vat = place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
-    for (long long i0 = 0; i0 < count; i0 += CH, which ^= In::ROOMS - 1) {
-        const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+    for (long long i0 = 0; i0 < left; i0 += CH, which ^= In::ROOMS - 1) {
+        const int rows = (int)(left - i0 < CH ? left - i0 : CH);
         const long long next = i0 + CH;
         in.arrive();
-        if (In::STRAIGHT && next < count) in.fetch(next, which ^ 1);
+        if (In::STRAIGHT && next < left) in.fetch(next, which ^ 1);
         const bf16 *const sq = in.q(which), *const vdown = in.third(which) + vat;
         bf16* const sk = in.k(which);
         const bf16x8 *const sp = in.units(which) + lane, *const stt = sp + F::P_UNITS * 64;
@@ -570,7 +591,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             asm volatile("" ::: "memory");
         }
         const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
-        if (SAVE) {
+        if (WALK == KEEP) {
             float* const to = a.states + mine * KW * VW + col;
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
@@ -586,7 +607,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
                 kf[b & 1][i] = across<X>(sk + 16 * i * KW + (xat ^ 32 * b), XP);
-                qf[b & 1][i] = across<X>(sq + 16 * i * KW + (xat ^ 32 * b), XP);
+                if (WALK != OWN) qf[b & 1][i] = across<X>(sq + 16 * i * KW + (xat ^ 32 * b), XP);
             }
         };
         read_rows(0);
@@ -608,11 +629,11 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
                 e[i] = mfma(kf[b & 1][i], zf, e[i]);
-                o[i] = mfma(zo, qf[b & 1][i], o[i]);
+                if (WALK != OWN) o[i] = mfma(zo, qf[b & 1][i], o[i]);
             }
             in_order();
         }
-        if (!In::STRAIGHT && next < count) in.fetch(next, 0);
+        if (!In::STRAIGHT && next < left) in.fetch(next, 0);
         Sum<X, 8> kt[2 * KT];                             // (of the first 32 moments; then of the others)
         auto read_columns = [&](int jj) {
 #pragma unroll
@@ -677,7 +698,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
         decayed<2 * KT>(z, sf[0], sf[1]);
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
-            if (jj == JB / 2 - 1) {
+            if (WALK != OWN && jj == JB / 2 - 1) {
 #pragma unroll
                 for (int m = 0; m < F::PIECES; ++m)
 #pragma unroll
@@ -696,6 +717,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) z[b][r] = NAN;
+        if constexpr (WALK != OWN) {
         // outputs
 #pragma unroll
         for (int i = 0; i < JB; ++i) o[i] *= fo[i];
@@ -714,8 +736,9 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
                 for (int i = 0; i < JB; ++i)
                     if (16 * i + c >= f) o[i][r] = NAN;
             }
+        }
         in.landed();
-        if (SAVE) {
+        if (WALK == KEEP) {
             float* const to = a.errors + mine * CH * VW + col;
 #pragma unroll
             for (int i = 0; i < JB; ++i)
@@ -725,9 +748,9 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
                     to[row * VW] = row < since ? e[i][r] : row < rows ? NAN : 0.f;
                 }
         }
-        {
+        if constexpr (WALK != OWN) {
             const int oc = v0 + 16 * wave + 4 * g;
-            T* const po = (T*)a.o + (((a.starts ? 0 : n * a.n_moments) + first + i0) * a.heads + h) * a.V;
+            T* const po = (T*)a.o + (((a.chunks.starts ? 0 : n * a.chunks.n_moments) + first + i0) * a.heads + h) * a.V;
             typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
@@ -742,7 +765,21 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             }
         }
     }
-    if (a.fin && col < a.V)
+    if (WALK == OWN) {
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b) {
+            const int at = col - NW * blocks_v;
+            if (moves && a.trans_t)
+                *reinterpret_cast<f32x4*>(a.trans_t + (((size_t)slot * a.heads + h) * KW + at) * KW + row_of(b, 0)) = z[b];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (moves) a.trans[(((size_t)slot * a.heads + h) * KW + row_of(b, r)) * KW + at] = z[b][r];
+                else a.own[at_seg + (size_t)row_of(b, r) * VW + col] = z[b][r];
+            }
+        }
+        return;
+    }
+    if (last && a.fin && col < a.V)
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
@@ -754,49 +791,57 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 
 // ------------------------------------------------------------------------------------------------ the walk backwards
 // The same of X, the gradient of the state after a chunk: y = T^T (P^T g + F beta K X), X' = E_end X + Q^T (c E g) - K^T (E y).
-template <class T, int KT>
+template <class T, int KT, Walk WALK>
 __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
     using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, NW = 64, VP = CH * NW;
     using In = Stage<T, F, KT>;
     __shared__ __align__(16) char room[In::ROOMS * In::BYTES];
-    const int blocks_v = (a.V + NW - 1) / NW;
-    // (a chain's blocks of columns 8 workgroups apart: on one XCD, whose L2 then holds what they both read)
-    const unsigned block = (unsigned)block_number(), chain = block / (8 * blocks_v) * 8 + (block & 7);
-    const int vb = (int)(block / 8 % blocks_v), n = (int)(chain / a.heads), h = (int)(chain - (unsigned)n * a.heads);
-    if (n >= a.n_seq) return;
+    const int blocks_v = (a.V + NW - 1) / NW, blocks = blocks_v;
+    // (a segment's blocks of columns 8 workgroups apart: on one XCD, whose L2 then holds what they all read)
+    const unsigned block = (unsigned)block_number(), unit = block / (8 * blocks) * 8 + (block & 7), place_in = unit / a.heads;
+    const int vb = (int)(block / 8 % blocks), h = (int)(unit - place_in * a.heads);
+    if (place_in >= (unsigned)a.segs.slots) return;
+    int n, seg, slot;
     long long first, count;
-    stretch_of(a, n, first, count);
-    first = shared_by_all(first);
-    count = shared_by_all(count);
+    if (!segment_of(a.segs, (int)place_in, n, seg, slot, first, count)) return;
+    n = __builtin_amdgcn_readfirstlane(n);
+    seg = __builtin_amdgcn_readfirstlane(seg);
+    slot = __builtin_amdgcn_readfirstlane(slot);
+    const int slot0 = first_slot(a.chunks, n, shared_by_all(first)) + (int)(seg * (a.segs.L / CH));
+    const long long from = start_of(a.segs, seg), left = shared_by_all(count - from < a.segs.L ? count - from : a.segs.L);
+    const bool last = shared_by_all(count) == from + left;
+    first = shared_by_all(first) + from;
+    if (WALK == OWN && seg == 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const int v0 = NW * vb, col = v0 + 16 * wave + c, VW = NW * blocks_v;
     const size_t at_state = ((size_t)n * a.heads + h) * a.K * a.V;
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    const size_t seg_state = (size_t)a.heads * KW * VW, at_seg = (size_t)slot * seg_state + (size_t)h * KW * VW;
     f32x4 z[2 * KT];
 #pragma unroll
     for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int k = row_of(b, r);
-            z[b][r] = a.gfin && k < a.K && col < a.V ? a.gfin[at_state + (size_t)k * a.V + col] : 0.f;
+            if (!last) z[b][r] = WALK == OWN ? 0.f : a.own[at_seg + seg_state + (size_t)k * VW + col];
+            else z[b][r] = a.gfin && k < a.K && col < a.V ? a.gfin[at_state + (size_t)k * a.V + col] : 0.f;
         }
-    const int slot0 = first_slot(a, n, first);
-    In in(room, a, a.go, n, h, h, v0, slot0, first, count);
+    In in(room, a, a.go, n, h, h, v0, slot0, first, left);
     int which = 0;
-    const long long last = count > 0 ? (count - 1) / CH * CH : -1;
-    if (last >= 0) in.fetch(last, 0);
+    const long long end = left > 0 ? (left - 1) / CH * CH : -1;
+    if (end >= 0) in.fetch(end, 0);
     loads_done();
     const int xat = place<KW>(c, g), yat = place<KW>(4 * g + (c >> 2), c & 3);
     const int gat = place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
-    for (long long i0 = last; i0 >= 0; i0 -= CH, which ^= In::ROOMS - 1) {
+    for (long long i0 = end; i0 >= 0; i0 -= CH, which ^= In::ROOMS - 1) {
         in.arrive();
         if (In::STRAIGHT && i0) in.fetch(i0 - CH, which ^ 1);
         const bf16 *const sq = in.q(which), *const sk = in.k(which), *const gdown = in.third(which) + gat;
         const bf16x8 *const sp = in.units(which) + lane, *const stt = sp + F::P_UNITS * 64;
         const float* const sf = in.factors(which);
         const size_t mine = (size_t)(slot0 + i0 / CH) * a.heads + h;
-        {
+        if (WALK != OWN) {
             float* const to = a.grads + mine * KW * VW + col;
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b)
@@ -870,7 +915,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
             for (int j = 0; j < 2 * ii + 2; ++j) y[j] = mfma(tf[tpiece_of(ii, j)], df, y[j]);
         }
         in_order();
-        {
+        if (WALK != OWN) {
             float* const to = a.ys + mine * CH * VW + col;
 #pragma unroll
             for (int i = 0; i < JB; ++i)
@@ -894,7 +939,14 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
         }
         in.landed();
     }
-    if (a.ginit && col < a.V)
+    if (WALK == OWN) {
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a.own[at_seg + (size_t)row_of(b, r) * VW + col] = z[b][r];
+        return;
+    }
+    if (seg == 0 && a.ginit && col < a.V)
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
@@ -902,6 +954,58 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
                 const int k = row_of(b, r);
                 if (k < a.K) a.ginit[at_state + (size_t)k * a.V + col] = z[b][r];
             }
+}
+
+// Segments' end states from their own: S_0 = own_0, S_s = M_s S_{s-1} + own_s, in place; backwards X_s = M_s^T X_{s+1} + own_s
+// from the last segment's.  A wave 16 columns, as in the walks; M's rows straight from memory.  The last segment's end state
+// (backwards: the first one's X) is left to the walk.  grid (blocks of 64 columns x heads, stretches)
+template <int KT, bool BACK>
+__global__ __launch_bounds__(256) void k_delta_join(Delta a) {
+    constexpr int KW = 32 * KT;
+    const int blocks_v = (a.V + 63) / 64, VW = 64 * blocks_v, h = blockIdx.x / blocks_v, n = blockIdx.y;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int col = 64 * (blockIdx.x % blocks_v) + 16 * wave + c;
+    long long first, count;
+    stretch_of(a.segs, n, first, count);
+    const int segments = (int)((count + a.segs.L - 1) / a.segs.L), slot = first_slot(a.segs, n, first);
+    if (segments < 3) return;                             // (one end state, and it is the true one)
+    auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
+    const size_t step = (size_t)a.heads * KW * VW, mstep = (size_t)a.heads * KW * KW;
+    const int s0 = BACK ? segments - 1 : 0;
+    float* own = a.own + (slot + s0) * step + (size_t)h * KW * VW + col;
+    const float* m = (BACK ? a.trans_t : a.trans) + (slot + s0) * mstep + (size_t)h * KW * KW + (size_t)(8 * (c >> 2) + (c & 3)) * KW + 8 * g;
+    f32x4 z[2 * KT];
+#pragma unroll
+    for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[b][r] = own[row_of(b, r) * VW];
+    for (int i = 1; i < segments - 1; ++i) {
+        own += BACK ? -(ptrdiff_t)step : (ptrdiff_t)step;
+        m += BACK ? -(ptrdiff_t)mstep : (ptrdiff_t)mstep;
+        f32x4 y[2 * KT];
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[b][r] = own[row_of(b, r) * VW];
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+            Sum<T_TERMS, 8> zf;
+            zf.of_summed(joined(z[2 * k], z[2 * k + 1]));
+#pragma unroll
+            for (int b = 0; b < 2 * KT; ++b) {
+                const f32x4* const row = reinterpret_cast<const f32x4*>(m + (32 * (b >> 1) + 4 * (b & 1)) * KW + 32 * k);
+                Sum<T_TERMS, 8> mf;
+                mf.of_summed(joined(row[0], row[1]));
+                y[b] = mfma(mf, zf, y[b]);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b) {
+            z[b] = y[b];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) own[row_of(b, r) * VW] = z[b][r];
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ the gradients
@@ -921,15 +1025,15 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
     bf16x8* const sp = reinterpret_cast<bf16x8*>(sk + X * XP);            // [4][PIECES][W][64]
     const unsigned block = (unsigned)block_number();
     const int place_in = (int)(block / a.heads), h = (int)(block - (unsigned)place_in * a.heads);
-    if (place_in >= a.slots) return;
+    if (place_in >= a.chunks.slots) return;
     int n, seg, slot;
     long long first, count;
-    if (!segment_of(a, place_in, n, seg, slot, first, count)) return;
+    if (!segment_of(a.chunks, place_in, n, seg, slot, first, count)) return;
     const long long from = (long long)seg * CH, left = count - from;
     const int rows = (int)(left < CH ? left : CH);
     if (rows <= 0) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
-    const long long moment = first + from, out_row = (a.starts ? 0 : n * a.n_moments) + moment;
+    const long long moment = first + from, out_row = (a.chunks.starts ? 0 : n * a.chunks.n_moments) + moment;
     const size_t mine = (size_t)slot * a.heads + h;
     const float* const f = factors_of<F>(a.prep + mine * F::PREP);
     for (int i = tid; i < CH; i += THREADS) {
@@ -1206,7 +1310,7 @@ struct Outside {
     char* out[8];
     long long row[8];                    // bytes a moment
 };
-__global__ __launch_bounds__(256) void k_delta_outside(Delta a, Outside z) {
+__global__ __launch_bounds__(256) void k_delta_outside(Cuts a, Outside z) {
     long long first = 0, rest = a.n_moments, before = 0;
     if (a.n_seq) {
         leaf_of(a, a.n_seq, first, rest);
@@ -1356,10 +1460,58 @@ long long chunk_slots(const fm_delta_args& a) {
     if (!a.n_seq || !a.n_moments) return 0;
     return a.starts && most > 1 ? a.n_moments / C + a.n_seq : a.n_seq * most;
 }
+// Segments: a walk takes a workgroup for 64 columns and a CU for itself, so that few chains leave most CUs without work.  Cut
+// into segments of L moments, these are walked at the same time, for more work: their own end states, with M (K more columns) but
+// for the first, then those joined one after another, then the walk.  By the following estimate (us): a chunk takes a walk
+// `chunk`, four fifths of it where only the own state is wanted, a join `join`, the launches 12.
+// Packed stretches, whose lengths only the device knows, are taken to be of any length up to twice the middle one.
+long long segment_length(const fm_delta_args& p) {
+    const long long C = chunk_length(p.dtype), whole = (p.n_moments + C - 1) / C * C;
+    if (!p.n_seq || whole <= C) return whole ? whole : C;
+    const bool packed = p.starts && p.n_seq > 1, deep = p.k_dim > 64;
+    const double chunk = p.dtype == FM_BF16 ? (deep ? 4.5 : 3.6) : p.dtype == FM_F16 ? (deep ? 4.0 : 2.8) : (deep ? 7.0 : 4.0);
+    const double join = deep ? 4.0 : 1.5, BV = p.v_dim <= 64 ? 1 : 2, BK = deep ? 2 : 1;
+    const double middle = (double)p.n_moments / (packed ? p.n_seq : 1), longest = packed ? fmin(2 * middle, (double)p.n_moments) : middle;
+    const double chains = (double)p.n_seq * p.q_heads;
+    auto rounds = [](double groups) { return fmax(1.0, groups / 256); };
+    const double chunks = ceil(longest / C);
+    double best = 0.95 * fmax(chunks * chunk, chains * BV * ceil(middle / C) / 256 * chunk);
+    long long L = whole;
+    for (int nseg = 2; nseg <= 256; nseg += nseg < 8 ? 1 : nseg / 4) {
+        const double each = ceil(chunks / nseg);
+        if (each < 1 || each >= chunks) continue;
+        const double mean = packed ? middle / (each * C) + 0.5 : ceil(chunks / each);            // segments a chain
+        const double t = rounds(chains * BV * mean) * each * chunk +
+                         rounds(chains * (BV * fmax(0.0, mean - 1) + BK * fmax(0.0, mean - 2))) * each * 0.8 * chunk +
+                         fmax(0.0, ceil(chunks / each) - 2) * join + 12;
+        if (t < best) {
+            best = t;
+            L = (long long)each * C;
+        }
+        if (each == 1) break;
+    }
+    return L;
+}
+long long segment_slots(const fm_delta_args& p) {
+    const long long L = segment_length(p), most = (p.n_moments + L - 1) / L;
+    return p.starts && most > 1 ? p.n_moments / L + p.n_seq : p.n_seq * (most > 1 ? most : 1);
+}
+bool in_segments(const fm_delta_args& p) { return p.n_seq && p.n_moments > segment_length(p); }
+Cuts cuts_of(const fm_delta_args& p, long long L, int slots) {
+    const long long most = (p.n_moments + L - 1) / L;
+    return Cuts{p.starts, p.n_moments, L, L, (int)p.wide, (int)p.n_seq, (int)(most > 1 ? most : 1), slots};
+}
 // floats of a state or of a chunk's rows, padded as the kernels hold them
 long long state_floats(const fm_delta_args& a) { return (a.k_dim <= 64 ? 64 : 128) * (a.v_dim <= 64 ? 64LL : 128); }
 long long row_floats(const fm_delta_args& a) { return chunk_length(a.dtype) * (a.v_dim <= 64 ? 64LL : 128); }
-long long delta_saved_bytes(const fm_delta_args& a) { return 4 * chunk_slots(a) * a.q_heads * (state_floats(a) + row_floats(a)); }
+// floats of segments' states, of their M
+long long cut_floats(const fm_delta_args& a) { return in_segments(a) ? segment_slots(a) * a.q_heads * state_floats(a) : 0; }
+long long move_floats(const fm_delta_args& a) {
+    const long long KW = a.k_dim <= 64 ? 64 : 128;
+    return in_segments(a) ? segment_slots(a) * a.q_heads * KW * KW : 0;
+}
+long long kept_floats(const fm_delta_args& a) { return chunk_slots(a) * a.q_heads * (state_floats(a) + row_floats(a)); }
+long long delta_saved_bytes(const fm_delta_args& a) { return 4 * (kept_floats(a) + move_floats(a)); }
 // float32 parts of shared key / value heads' gradients
 long long delta_part_floats(const fm_delta_args& a, bool of_v) {
     const long long moments = a.n_moments * (a.starts ? 1 : a.n_seq);
@@ -1386,8 +1538,8 @@ bool whole_stores(const fm_delta_args& p) {
 }
 
 long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
-    long long n = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, bwd);
-    if (bwd) n += delta_saved_bytes(a) + 4 * (delta_part_floats(a, false) + delta_part_floats(a, true));
+    long long n = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, bwd) + 4 * cut_floats(a);
+    n += 4 * (bwd ? kept_floats(a) + delta_part_floats(a, false) + delta_part_floats(a, true) : move_floats(a));
     if (chunk_slots(a) && !in_whole_units(a, bwd))
         for (int i = 0; i < 3; ++i) n += pack_bytes(a, bwd, i);
     return n;
@@ -1408,16 +1560,12 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
     a.be_seq = p.be_seq;
     a.be_moment = p.be_moment;
     a.be_head = p.be_head;
-    a.starts = p.starts;
-    a.n_moments = p.n_moments;
-    a.L = a.L0 = chunk_length(p.dtype);
-    a.nseg = (int)((p.n_moments + a.L - 1) / a.L);
-    if (a.nseg < 1) a.nseg = 1;
-    a.slots = (int)chunk_slots(p);
-    a.wide = (int)p.wide;
+    const long long C = chunk_length(p.dtype);
+    a.chunks = cuts_of(p, C, (int)chunk_slots(p));
+    const long long L = segment_length(p);
+    a.segs = cuts_of(p, L, (int)segment_slots(p));
     a.heads = (int)p.q_heads;
     a.share = (int)(p.q_heads / p.k_heads);
-    a.n_seq = (int)p.n_seq;
     a.K = (int)p.k_dim;
     a.V = (int)p.v_dim;
     a.c = (float)p.scale;
@@ -1426,9 +1574,15 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
     const long long states = chunk_slots(p) * p.q_heads * state_floats(p);
     a.states = (float*)p.saved;
     a.errors = a.states ? a.states + states : nullptr;
+    float* room = (float*)(a.prep + chunk_slots(p) * p.q_heads * prep_bytes(p.dtype, bwd));
+    a.own = room;
+    room += cut_floats(p);
+    a.trans_t = a.errors ? a.errors + chunk_slots(p) * p.q_heads * row_floats(p) : nullptr;
     if (bwd) {
-        a.grads = (float*)(a.prep + chunk_slots(p) * p.q_heads * prep_bytes(p.dtype, true));
+        a.grads = room;
         a.ys = a.grads + states;
+    } else {
+        a.trans = room;
     }
     a.init = p.state;
     a.fin = p.state_out;
@@ -1443,19 +1597,30 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
     return a;
 }
 
+// a launch of the walks: 8 segments' blocks of columns at a time
+dim3 walks_of(const Delta& a, int blocks) { return blocks_of(((long long)a.segs.slots * a.heads + 7) / 8 * 8 * blocks); }
 template <class T, int KT>
 void delta_fwd(const Delta& a, hipStream_t st) {
-    if (a.slots) k_delta_prep<T, KT, false><<<blocks_of((long long)a.slots * a.heads), 256, 0, st>>>(a);
-    const dim3 grid = blocks_of(((long long)a.n_seq * a.heads + 7) / 8 * 8 * ((a.V + 63) / 64));
-    if (a.states) k_delta_scan<T, KT, true><<<grid, 256, 0, st>>>(a);
-    else k_delta_scan<T, KT, false><<<grid, 256, 0, st>>>(a);
+    const int BV = (a.V + 63) / 64;
+    if (a.chunks.slots) k_delta_prep<T, KT, false><<<blocks_of((long long)a.chunks.slots * a.heads), 256, 0, st>>>(a);
+    if (a.segs.nseg > 1) {
+        k_delta_scan<T, KT, OWN><<<walks_of(a, BV + KT / 2), 256, 0, st>>>(a);
+        if (a.segs.nseg > 2) k_delta_join<KT, false><<<dim3(BV * a.heads, a.segs.n_seq), 256, 0, st>>>(a);
+    }
+    if (a.states) k_delta_scan<T, KT, KEEP><<<walks_of(a, BV), 256, 0, st>>>(a);
+    else k_delta_scan<T, KT, PLAY><<<walks_of(a, BV), 256, 0, st>>>(a);
 }
 template <class T, int KT>
 void delta_bwd(const Delta& a, hipStream_t st) {
-    if (a.slots) k_delta_prep<T, KT, true><<<blocks_of((long long)a.slots * a.heads), 256, 0, st>>>(a);
-    k_delta_back<T, KT><<<blocks_of(((long long)a.n_seq * a.heads + 7) / 8 * 8 * ((a.V + 63) / 64)), 256, 0, st>>>(a);
-    if (!a.slots || !(a.gq || a.gk || a.gv || a.glog_decay || a.gbeta)) return;
-    const dim3 chunks = blocks_of((long long)a.slots * a.heads);
+    const int BV = (a.V + 63) / 64;
+    if (a.chunks.slots) k_delta_prep<T, KT, true><<<blocks_of((long long)a.chunks.slots * a.heads), 256, 0, st>>>(a);
+    if (a.segs.nseg > 1) {
+        k_delta_back<T, KT, OWN><<<walks_of(a, BV), 256, 0, st>>>(a);
+        if (a.segs.nseg > 2) k_delta_join<KT, true><<<dim3(BV * a.heads, a.segs.n_seq), 256, 0, st>>>(a);
+    }
+    k_delta_back<T, KT, KEEP><<<walks_of(a, BV), 256, 0, st>>>(a);
+    if (!a.chunks.slots || !(a.gq || a.gk || a.gv || a.glog_decay || a.gbeta)) return;
+    const dim3 chunks = blocks_of((long long)a.chunks.slots * a.heads);
     if (a.V <= 64) k_delta_grads<T, KT, 1><<<chunks, 128 * KT, 0, st>>>(a);
     else k_delta_grads<T, KT, 2><<<chunks, 128 * KT, 0, st>>>(a);
 }
@@ -1486,10 +1651,10 @@ void delta_of_type(const fm_delta_args& p, bool bwd, hipStream_t st) {
             if (p.gk) add(part, p.q_heads * p.k_dim * 4);
             if (p.gv) add(part + delta_part_floats(p, false), p.q_heads * p.v_dim * 4);
         }
-        if (n) k_delta_outside<<<dim3(256, n), 256, 0, st>>>(a, z);
+        if (n) k_delta_outside<<<dim3(256, n), 256, 0, st>>>(a.chunks, z);
     }
     if (!p.n_seq) return;
-    if (a.slots && !in_whole_units(p, bwd)) {
+    if (a.chunks.slots && !in_whole_units(p, bwd)) {
         Packs k{};
         char* to = a.prep + delta_workspace_bytes(p, bwd);
         fm_view* const views[3] = {&a.q, &a.k, bwd ? &a.go : &a.v};

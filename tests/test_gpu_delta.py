@@ -99,6 +99,55 @@ def test_delta_attention_and_its_gradients(gpu_lib, case):
     check(inputs(gen, (N, T), H, Hk, K, V, dt, how, N if start else None), None, dt, gen=gen)
 
 
+LONG = [  # few chains of many chunks: walked in segments
+    (1, 2100, 2, 1, 64, 64, F32, "dense", True),
+    (1, 3001, 2, 2, 128, 128, BF16, "packed", True),
+    (2, 1500, 3, 1, 40, 56, F16, "dense", True),
+    (1, 2500, 1, 1, 128, 64, F32, "dense", False),
+    (1, 2300, 1, 1, 64, 128, BF16, "dense", True),
+    (1, 1800, 2, 2, 100, 36, F16, "packed", True),
+    (3, 1024, 1, 1, 16, 16, BF16, "dense", False),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(str(v).replace("torch.", "") for v in c))
+def test_long_stretches_of_few_heads(gpu_lib, case):
+    N, T, H, Hk, K, V, dt, how, start = case
+    say(f"long {case}")
+    gen = torch.Generator().manual_seed(N + T + K + V)
+    check(inputs(gen, (N, T), H, Hk, K, V, dt, how, N if start else None), None, dt, gen=gen)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_long_packed_stretches(gpu_lib, dt):
+    say(f"long packed {dt}")
+    gen = torch.Generator().manual_seed(31)
+    starts = [5]
+    for x in [1900, 0, 700, 3, 2500, 64, 130]:
+        starts.append(starts[-1] + x)
+    check(inputs(gen, (starts[-1] + 7,), 2, 1, 48, 80, dt, "packed", 7), starts, dt, gen=gen)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("where", [0, 700, 2599])
+def test_odd_moments_in_segments(gpu_lib, dt, where):
+    """What is not finite reaches the same in a stretch that is walked in segments."""
+    from flyguy_amd.memory_hip import delta_attention
+    say(f"odd in segments {dt} {where}")
+    gen = torch.Generator().manual_seed(32)
+    ins = inputs(gen, (1, 2600), 2, 2, 48, 40, dt, "dense", 1)
+    want_o, want_e = delta_attention(*ins)
+    for what in (1, 2, 4):
+        given = [x.clone() for x in ins]
+        given[what][(0, where, 1) + ((7,) if what < 3 else ())] = math.nan
+        o, e = delta_attention(*given)
+        columns = slice(7, 8) if what == 2 else slice(None)
+        t, te = torch.zeros_like(o, dtype=torch.bool), torch.zeros_like(e, dtype=torch.bool)
+        t[0, where:, 1, columns], te[0, 1, :, columns] = True, True
+        assert torch.equal(o[~t], want_o[~t]) and torch.equal(e[~te], want_e[~te]), what
+        assert torch.isnan(o[t]).all() and torch.isnan(e[te]).all(), what
+
+
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
 @pytest.mark.parametrize("lengths", [[1], [7, 64, 65, 1], [0, 130, 0, 3, 64, 0], [200, 1, 1, 90, 33, 31]])
 def test_packed_stretches(gpu_lib, dt, lengths):
