@@ -203,8 +203,11 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     using F = DeltaForm<T, BWD>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, XC = KW / VN;
     constexpr int NP = CH + 4;                            // a row of N and T, padded
-    __shared__ __align__(16) bf16 sq[X * XP], sk[X * XP];
-    __shared__ __align__(16) float sn[CH * NP], st[CH * NP];
+    // q and k; then, when their products are made, N and T (4 workgroups a CU)
+    constexpr int ROWS_BYTES = 2 * X * XP * 2, NT_BYTES = 2 * CH * NP * 4;
+    __shared__ __align__(16) char room[ROWS_BYTES > NT_BYTES ? ROWS_BYTES : NT_BYTES];
+    bf16 *const sq = reinterpret_cast<bf16*>(room), *const sk = sq + X * XP;
+    float *const sn = reinterpret_cast<float*>(room), *const st = sn + CH * NP;
     __shared__ float hi[CH], lo[CH], sb[CH];
     __shared__ int bad;
     const unsigned block = (unsigned)block_number();
@@ -279,8 +282,12 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
 #pragma unroll
         for (int t = 0; t < W; ++t) reinterpret_cast<bf16x4*>(&units[(unit * W + t) * 64 + lane])[half] = s.term[t];
     };
-    constexpr int BLOCKS = JB * (JB + 1) / 2;
-    for (int task = wave; task < 2 * BLOCKS; task += 4) {
+    constexpr int BLOCKS = JB * (JB + 1) / 2, MINE = (2 * BLOCKS + 3) / 4, NS = (BLOCKS + 3) / 4;
+    f32x4 own_n[NS];                                      // this wave's blocks of N
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+        const int task = 4 * m + wave;
+        if (task >= 2 * BLOCKS) break;
         const bool of_q = task >= BLOCKS;
         int i, j;
         block_of(of_q ? task - BLOCKS : task, i, j);
@@ -298,8 +305,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = 16 * i + 4 * g + r, col = 16 * j + c;
-                sn[row * NP + col] = row > col ? apart(row, col) * sb[col] * p[r] : 0.f;
+                p[r] = row > col ? apart(row, col) * sb[col] * p[r] : 0.f;
             }
+            if (m < NS) own_n[m < NS ? m : 0] = p;
             continue;
         }
 #pragma unroll
@@ -317,16 +325,30 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
             if (!(j & 1) && i == j) store_half(piece_of(j >> 1, i), 1, Sum<W, 4>{});
         }
     }
+    __syncthreads();                                      // (q and k are read)
+#pragma unroll
+    for (int m = 0; m < NS; ++m) {
+        int i, j;
+        block_of(4 * m + wave, i, j);
+        if (4 * m + wave < BLOCKS)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sn[(16 * i + 4 * g + r) * NP + 16 * j + c] = own_n[m][r];
+    }
     __syncthreads();
     if (tid < CH) {                                       // the diagonal blocks: column c of block tid / 16
         const int b0 = tid & ~15, col = tid & 15;
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float s = i == col ? 1.f : 0.f;
+            float s[4] = {i == col ? 1.f : 0.f, 0.f, 0.f, 0.f};           // (four sums: a chain of dependent products a quarter as long)
 #pragma unroll
-            for (int j = 0; j < i; ++j) s = fmaf(-sn[(b0 + i) * NP + b0 + j], x[j], s);
-            x[i] = s;
+            for (int j = 0; j < i; j += 4) {
+                const f32x4 row = *reinterpret_cast<const f32x4*>(&sn[(b0 + i) * NP + b0 + j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (j + e < i) s[e] = fmaf(-row[e], x[j + e], s[e]);
+            }
+            x[i] = (s[0] + s[1]) + (s[2] + s[3]);
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) st[(b0 + i) * NP + b0 + col] = x[i];
@@ -957,53 +979,78 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
 }
 
 // Segments' end states from their own: S_0 = own_0, S_s = M_s S_{s-1} + own_s, in place; backwards X_s = M_s^T X_{s+1} + own_s
-// from the last segment's.  A wave 16 columns, as in the walks; M's rows straight from memory.  The last segment's end state
-// (backwards: the first one's X) is left to the walk.  grid (blocks of 64 columns x heads, stretches)
+// from the last segment's.  A wave 16 columns, as in the walks; the workgroup's waves share the work of M's terms, and the next M
+// is on its way meanwhile (10 -> 2 us a segment of 128 x 128).  The last segment's end state (backwards: the first one's X) is left to the walk.
+// grid (blocks of 64 columns x heads, stretches)
 template <int KT, bool BACK>
 __global__ __launch_bounds__(256) void k_delta_join(Delta a) {
-    constexpr int KW = 32 * KT;
+    constexpr int KW = 32 * KT, MINE = 2 * KT * KT / 4;   // a wave's operands of M
+    __shared__ __align__(16) bf16x8 sm[2 * KT * KT][T_TERMS][64];
     const int blocks_v = (a.V + 63) / 64, VW = 64 * blocks_v, h = blockIdx.x / blocks_v, n = blockIdx.y;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int col = 64 * (blockIdx.x % blocks_v) + 16 * wave + c;
     long long first, count;
     stretch_of(a.segs, n, first, count);
     const int segments = (int)((count + a.segs.L - 1) / a.segs.L), slot = first_slot(a.segs, n, first);
     if (segments < 3) return;                             // (one end state, and it is the true one)
     auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
-    const size_t step = (size_t)a.heads * KW * VW, mstep = (size_t)a.heads * KW * KW;
+    const ptrdiff_t step = (ptrdiff_t)a.heads * KW * VW * (BACK ? -1 : 1), mstep = (ptrdiff_t)a.heads * KW * KW * (BACK ? -1 : 1);
     const int s0 = BACK ? segments - 1 : 0;
-    float* own = a.own + (slot + s0) * step + (size_t)h * KW * VW + col;
-    const float* m = (BACK ? a.trans_t : a.trans) + (slot + s0) * mstep + (size_t)h * KW * KW + (size_t)(8 * (c >> 2) + (c & 3)) * KW + 8 * g;
-    f32x4 z[2 * KT];
+    float* own = a.own + ((size_t)(slot + s0) * a.heads + h) * KW * VW + col;
+    const float* m = (BACK ? a.trans_t : a.trans) + ((size_t)(slot + s0) * a.heads + h) * KW * KW + (size_t)(8 * (c >> 2) + (c & 3)) * KW + 8 * g;
+    f32x4 z[2 * KT], y[2 * KT], rm[MINE][2];
+    auto fetch = [&]() {                                  // the next segment's
+        own += step;
+        m += mstep;
 #pragma unroll
-    for (int b = 0; b < 2 * KT; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z[b][r] = own[row_of(b, r) * VW];
-    for (int i = 1; i < segments - 1; ++i) {
-        own += BACK ? -(ptrdiff_t)step : (ptrdiff_t)step;
-        m += BACK ? -(ptrdiff_t)mstep : (ptrdiff_t)mstep;
-        f32x4 y[2 * KT];
+        for (int i = 0; i < MINE; ++i) {
+            const int b = (4 * i + wave) / KT, k = (4 * i + wave) % KT;
+            const f32x4* const row = reinterpret_cast<const f32x4*>(m + (32 * (b >> 1) + 4 * (b & 1)) * KW + 32 * k);
+            rm[i][0] = row[0];
+            rm[i][1] = row[1];
+        }
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[b][r] = own[row_of(b, r) * VW];
+    };
+#pragma unroll
+    for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) z[b][r] = own[row_of(b, r) * VW];
+    fetch();
+    for (int i = 1; i < segments - 1; ++i) {
+        __syncthreads();                                  // (the M before is read)
+#pragma unroll
+        for (int j = 0; j < MINE; ++j) {
+            Sum<T_TERMS, 8> mf;
+            mf.of_summed(joined(rm[j][0], rm[j][1]));
+#pragma unroll
+            for (int t = 0; t < T_TERMS; ++t) sm[4 * j + wave][t][lane] = mf.term[t];
+        }
+        __syncthreads();
+        float* const to = own;
+        f32x4 x[2 * KT];
+#pragma unroll
+        for (int b = 0; b < 2 * KT; ++b) x[b] = y[b];
+        if (i + 1 < segments - 1) fetch();
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * k], z[2 * k + 1]));
 #pragma unroll
             for (int b = 0; b < 2 * KT; ++b) {
-                const f32x4* const row = reinterpret_cast<const f32x4*>(m + (32 * (b >> 1) + 4 * (b & 1)) * KW + 32 * k);
                 Sum<T_TERMS, 8> mf;
-                mf.of_summed(joined(row[0], row[1]));
-                y[b] = mfma(mf, zf, y[b]);
+#pragma unroll
+                for (int t = 0; t < T_TERMS; ++t) mf.term[t] = sm[b * KT + k][t][lane];
+                x[b] = mfma(mf, zf, x[b]);
             }
         }
 #pragma unroll
         for (int b = 0; b < 2 * KT; ++b) {
-            z[b] = y[b];
+            z[b] = x[b];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) own[row_of(b, r) * VW] = z[b][r];
+            for (int r = 0; r < 4; ++r) to[row_of(b, r) * VW] = z[b][r];
         }
     }
 }
@@ -1470,7 +1517,7 @@ long long segment_length(const fm_delta_args& p) {
     if (!p.n_seq || whole <= C) return whole ? whole : C;
     const bool packed = p.starts && p.n_seq > 1, deep = p.k_dim > 64;
     const double chunk = p.dtype == FM_BF16 ? (deep ? 4.5 : 3.6) : p.dtype == FM_F16 ? (deep ? 4.0 : 2.8) : (deep ? 7.0 : 4.0);
-    const double join = deep ? 4.0 : 1.5, BV = p.v_dim <= 64 ? 1 : 2, BK = deep ? 2 : 1;
+    const double join = deep ? 3.0 : 1.0, BV = p.v_dim <= 64 ? 1 : 2, BK = deep ? 2 : 1;
     const double middle = (double)p.n_moments / (packed ? p.n_seq : 1), longest = packed ? fmin(2 * middle, (double)p.n_moments) : middle;
     const double chains = (double)p.n_seq * p.q_heads;
     auto rounds = [](double groups) { return fmax(1.0, groups / 256); };
