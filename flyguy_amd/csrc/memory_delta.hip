@@ -1056,20 +1056,21 @@ __global__ __launch_bounds__(256) void k_delta_join(Delta a) {
 }
 
 // ------------------------------------------------------------------------------------------------ the gradients
-// A workgroup a chunk and head; a wave 16 of the keys' values.  First what sums over the values' columns (g S^T, y S^T, e X^T
-// transposed, and g e^T, y e^T in both orders), with g, y and e in LDS and a wave's rows of S and X straight from memory; then
-// q and k take their place, and the 16 x 16 blocks of H and Z, as products' operands, the rest.
+// A workgroup a chunk and head; a wave 16 of the keys' values.  First what sums over the values' columns: g S^T, y S^T and e X^T
+// (transposed), with g, y and e in LDS and a wave's rows of S and X straight from memory, and the 16 x 16 blocks of g e^T and y e^T.
+// Then q and k take their place, and H and Z as blocks of terms, which are read by rows for what sums over j and through the
+// transposing read for what sums over i.
 template <class T, int KT, int VT>
 __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
     using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, VW = 64 * VT, XP = CH * KW, VP = CH * VW, VN = Vec<T>::N;
-    constexpr int WAVES_ = 2 * KT, THREADS = 64 * WAVES_, XC = KW / VN, VC = VW / VN, PIECES = F::PIECES;
-    constexpr int FIRST = (X + 2 * W) * VP, PIECE = W * 512, SECOND = 2 * X * XP + 4 * PIECES * PIECE;
+    constexpr int WAVES_ = 2 * KT, THREADS = 64 * WAVES_, XC = KW / VN, VC = VW / VN, BLOCKS = JB * (JB + 1) / 2;
+    constexpr int FIRST = (X + 2 * W) * VP, BLOCK = W * 256, SECOND = 2 * X * XP + 2 * BLOCKS * BLOCK;
     __shared__ __align__(16) bf16 room[FIRST > SECOND ? FIRST : SECOND];
-    __shared__ float hi[CH], lo[CH], sb[CH], se[CH], sw[CH], red[WAVES_][4][CH], red_state[WAVES_];
+    __shared__ __align__(16) float hi[CH], lo[CH], sb[CH], se[CH], sw[CH], red[WAVES_][4][CH], red_state[WAVES_];
     bf16 *const sg = room, *const sy = sg + X * VP, *const ser = sy + W * VP;
-    bf16 *const sq = room, *const sk = sq + X * XP;
-    bf16x8* const sp = reinterpret_cast<bf16x8*>(sk + X * XP);            // [4][PIECES][W][64]
+    bf16 *const sq = room, *const sk = sq + X * XP, *const sh = sk + X * XP;   // sh: [H, Z][block][W][16 i][16 j]
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const unsigned block = (unsigned)block_number();
     const int place_in = (int)(block / a.heads), h = (int)(block - (unsigned)place_in * a.heads);
     if (place_in >= a.chunks.slots) return;
@@ -1079,30 +1080,19 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
     const long long from = (long long)seg * CH, left = count - from;
     const int rows = (int)(left < CH ? left : CH);
     if (rows <= 0) return;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
     const long long moment = first + from, out_row = (a.chunks.starts ? 0 : n * a.chunks.n_moments) + moment;
     const size_t mine = (size_t)slot * a.heads + h;
     const float* const f = factors_of<F>(a.prep + mine * F::PREP);
-    for (int i = tid; i < CH; i += THREADS) {
-        se[i] = f[F_E + i];
-        sw[i] = f[F_E + 2 * CH + i];
-        sb[i] = f[F_E + 3 * CH + i];
-        hi[i] = f[F_E + 4 * CH + i];
-        lo[i] = f[F_E + 5 * CH + i];
-    }
-    // all loads at once, in the order that they are used in
     constexpr int GN = CH * VC, EN = CH * VW / 8, QN = CH * XC;
     constexpr int GV = (GN + THREADS - 1) / THREADS, EV = (EN + THREADS - 1) / THREADS, QV = (QN + THREADS - 1) / THREADS;
     auto nth = [&](int i, int most) { return min(i * THREADS + tid, most - 1); };     // (a share past the last: it once more)
-    uint4 rg[GV], rq[QV], rk[QV];
+    u32x4 rg[GV], rq[QV], rk[QV];
     f32x4 ry[EV][2], re[EV][2], rs[VW / 32][2], rx[VW / 32][2];
-    const Chunk<T> go = chunk_of<T>(a, a.go, n, h, moment, rows, a.V);
-    const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
-    {
-        const f32x4 *const ys = reinterpret_cast<const f32x4*>(a.ys + mine * CH * VW), *const es = reinterpret_cast<const f32x4*>(a.errors + mine * CH * VW);
-        const size_t row = mine * KW * VW + (size_t)(16 * wave + c) * VW + 8 * g;
+    {                                                     // all at once, in the order that it is used in
+        const Chunk<T> go = chunk_of<T>(a, a.go, n, h, moment, rows, a.V);
 #pragma unroll
-        for (int i = 0; i < GV; ++i) rg[i] = go(nth(i, GN) / VC, nth(i, GN) % VC * VN);
+        for (int i = 0; i < GV; ++i) rg[i] = __builtin_bit_cast(u32x4, go(nth(i, GN) / VC, nth(i, GN) % VC * VN));
+        const f32x4 *const ys = reinterpret_cast<const f32x4*>(a.ys + mine * CH * VW), *const es = reinterpret_cast<const f32x4*>(a.errors + mine * CH * VW);
 #pragma unroll
         for (int i = 0; i < EV; ++i)
 #pragma unroll
@@ -1110,6 +1100,7 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
                 ry[i][half] = ys[2 * nth(i, EN) + half];
                 re[i][half] = es[2 * nth(i, EN) + half];
             }
+        const size_t row = mine * KW * VW + (16 * wave + c) * VW + 8 * g;
 #pragma unroll
         for (int b = 0; b < VW / 32; ++b)
 #pragma unroll
@@ -1117,49 +1108,62 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
                 rs[b][half] = *reinterpret_cast<const f32x4*>(a.states + row + 32 * b + 4 * half);
                 rx[b][half] = *reinterpret_cast<const f32x4*>(a.grads + row + 32 * b + 4 * half);
             }
-#pragma unroll
-        for (int i = 0; i < QV; ++i) {
-            rq[i] = cq(nth(i, QN) / XC, nth(i, QN) % XC * VN);
-            rk[i] = ck(nth(i, QN) / XC, nth(i, QN) % XC * VN);
-        }
-        __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int i = 0; i < GV; ++i) {
-        const int row = nth(i, GN) / VC, col = nth(i, GN) % VC * VN;
-        store_terms<T>(rg[i], sg + place<VW>(row, col >> 3) + (col & 7), VP);
+    if (tid < CH) {
+        se[tid] = f[F_E + tid];
+        sw[tid] = f[F_E + 2 * CH + tid];
+        sb[tid] = f[F_E + 3 * CH + tid];
+        hi[tid] = f[F_E + 4 * CH + tid];
+        lo[tid] = f[F_E + 5 * CH + tid];
     }
-#pragma unroll
-    for (int i = 0; i < EV; ++i) {
-        const int at = nth(i, EN), row = at / (VW / 8), col = at % (VW / 8) * 8, to = place<VW>(row, col >> 3);
-        const f32x8 y = joined(ry[i][0], ry[i][1]);
-        if (a.gv && row < rows && col < a.V) {
-            const long long to_v = ((out_row + row) * a.heads + h) * a.V + col;
-            typedef T vec8 __attribute__((ext_vector_type(8)));
-            if (a.vec && a.share == 1 && sizeof(T) == 2) *reinterpret_cast<vec8*>((T*)a.gv + to_v) = __builtin_convertvector(y, vec8);
-            else
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (col + r < a.V) {
-                        if (a.share > 1) ((float*)a.gv)[to_v + r] = y[r];
-                        else ((T*)a.gv)[to_v + r] = narrow<T>(y[r]);
-                    }
-        }
-        Sum<W, 8> ts, us;
-        ts.of(y);
-        us.of(joined(re[i][0], re[i][1]));
-#pragma unroll
-        for (int p = 0; p < W; ++p) {
-            *reinterpret_cast<bf16x8*>(sy + to + p * VP) = ts.term[p];
-            *reinterpret_cast<bf16x8*>(ser + to + p * VP) = us.term[p];
-        }
-    }
-    __syncthreads();
     f32x4 x1[JB], x2[JB], x3[JB];
     float dot = 0.f;                                      // <S, X>
+    constexpr int TASKS = 2 * BLOCKS, MOST = (TASKS + WAVES_ - 1) / WAVES_;
+    f32x4 p[MOST];                                        // this wave's blocks of g e^T (task < BLOCKS) and y e^T: rows j, columns i
 #pragma unroll
     for (int i = 0; i < JB; ++i) x1[i] = x2[i] = x3[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < MOST; ++m) p[m] = f32x4{0.f, 0.f, 0.f, 0.f};
     {
+#pragma unroll
+        for (int i = 0; i < GV; ++i) {
+            const int row = nth(i, GN) / VC, col = nth(i, GN) % VC * VN;
+            store_terms<T>(__builtin_bit_cast(uint4, rg[i]), sg + place<VW>(row, col >> 3) + (col & 7), VP);
+        }
+#pragma unroll
+        for (int i = 0; i < EV; ++i) {
+            const int at = nth(i, EN), row = at / (VW / 8), col = at % (VW / 8) * 8, to = place<VW>(row, col >> 3);
+            const f32x8 y = joined(ry[i][0], ry[i][1]);
+            if (a.gv && row < rows && col < a.V) {
+                const long long to_v = ((out_row + row) * a.heads + h) * a.V + col;
+                typedef T vec8 __attribute__((ext_vector_type(8)));
+                if (a.vec && a.share == 1 && sizeof(T) == 2) *reinterpret_cast<vec8*>((T*)a.gv + to_v) = __builtin_convertvector(y, vec8);
+                else
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (col + r < a.V) {
+                            if (a.share > 1) ((float*)a.gv)[to_v + r] = y[r];
+                            else ((T*)a.gv)[to_v + r] = narrow<T>(y[r]);
+                        }
+            }
+            Sum<W, 8> ts, us;
+            ts.of(y);
+            us.of(joined(re[i][0], re[i][1]));
+#pragma unroll
+            for (int t = 0; t < W; ++t) {
+                *reinterpret_cast<bf16x8*>(sy + to + t * VP) = ts.term[t];
+                *reinterpret_cast<bf16x8*>(ser + to + t * VP) = us.term[t];
+            }
+        }
+        __syncthreads();
+        {
+            const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
+#pragma unroll
+            for (int i = 0; i < QV; ++i) {
+                rq[i] = __builtin_bit_cast(u32x4, cq(nth(i, QN) / XC, nth(i, QN) % XC * VN));
+                rk[i] = __builtin_bit_cast(u32x4, ck(nth(i, QN) / XC, nth(i, QN) % XC * VN));
+            }
+        }
 #pragma unroll
         for (int b = 0; b < VW / 32; ++b) {
             const f32x8 s = joined(rs[b][0], rs[b][1]), x = joined(rx[b][0], rx[b][1]);
@@ -1168,115 +1172,133 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
             Sum<W, 8> st, xt;
             st.of_summed(s);
             xt.of_summed(x);
+            const int at = place<VW>(c, g) ^ 32 * b;
 #pragma unroll
             for (int i = 0; i < JB; ++i) {
-                const int at = 16 * i * VW + (place<VW>(c, g) ^ 32 * b);
-                x1[i] = mfma(st, across<X>(sg + at, VP), x1[i]);
-                x2[i] = mfma(st, across<W>(sy + at, VP), x2[i]);
-                x3[i] = mfma(xt, across<W>(ser + at, VP), x3[i]);
+                x1[i] = mfma(st, across<X>(sg + 16 * i * VW + at, VP), x1[i]);
+                x2[i] = mfma(st, across<W>(sy + 16 * i * VW + at, VP), x2[i]);
+                x3[i] = mfma(xt, across<W>(ser + 16 * i * VW + at, VP), x3[i]);
             }
         }
-    }
-    // blocks of H beta (rows j, columns i), H^T's (rows i, columns j), Z beta, Z^T's
-    constexpr int BLOCKS = JB * (JB + 1) / 2, TASKS = 4 * BLOCKS, MOST = (TASKS + WAVES_ - 1) / WAVES_;
-    f32x4 p[MOST];
 #pragma unroll
-    for (int m = 0; m < MOST; ++m) {
-        const int task = m * WAVES_ + wave;
-        if (task >= TASKS) break;
-        const int set = task / BLOCKS;
-        int i, j;
-        block_of(task - set * BLOCKS, i, j);
-        const int ri = 16 * i * VW, rj = 16 * j * VW;
-        p[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int m = 0; m < MOST; ++m) {
+            const int task = WAVES_ * m + wave;
+            if (task >= TASKS) break;
+            int i, j;
+            block_of(task < BLOCKS ? task : task - BLOCKS, i, j);
+            const bf16 *const pe = ser + 16 * j * VW, *const pg = sg + 16 * i * VW, *const py = sy + 16 * i * VW;
+            if (task < BLOCKS) {
 #pragma unroll
-        for (int b = 0; b < VW / 32; ++b) {
-            const int at = place<VW>(c, g) ^ 32 * b;
-            if (set == 0) p[m] = mfma(across<W>(ser + rj + at, VP), across<X>(sg + ri + at, VP), p[m]);
-            else if (set == 1) p[m] = mfma(across<X>(sg + ri + at, VP), across<W>(ser + rj + at, VP), p[m]);
-            else if (set == 2) p[m] = mfma(across<W>(ser + rj + at, VP), across<W>(sy + ri + at, VP), p[m]);
-            else p[m] = mfma(across<W>(sy + ri + at, VP), across<W>(ser + rj + at, VP), p[m]);
-        }
+                for (int b = 0; b < VW / 32; ++b) {
+                    const int at = place<VW>(c, g) ^ 32 * b;
+                    p[m] = mfma(across<W>(pe + at, VP), across<X>(pg + at, VP), p[m]);
+                }
+            } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const bool by_row = set & 1;                  // rows i, columns j
-            const int row = 16 * i + (by_row ? 4 * g + r : c), col = 16 * j + (by_row ? c : 4 * g + r);
-            const float d = exp_of(fminf((hi[row] - hi[col]) + (lo[row] - lo[col]), 88.f)) * (by_row ? 1.f : sb[col]);
-            p[m][r] = set < 2 ? (row >= col ? a.c * d * p[m][r] : 0.f) : (row > col ? -d * p[m][r] : 0.f);
+                for (int b = 0; b < VW / 32; ++b) {
+                    const int at = place<VW>(c, g) ^ 32 * b;
+                    p[m] = mfma(across<W>(pe + at, VP), across<W>(py + at, VP), p[m]);
+                }
+            }
         }
     }
     __syncthreads();                                      // (g, y and e are read)
 #pragma unroll
     for (int m = 0; m < MOST; ++m) {
-        const int task = m * WAVES_ + wave;
+        const int task = WAVES_ * m + wave;
         if (task >= TASKS) break;
-        const int set = task / BLOCKS;
+        const bool of_z = task >= BLOCKS;
         int i, j;
-        block_of(task - set * BLOCKS, i, j);
-        const bool by_row = set & 1;
-        const int piece = by_row ? tpiece_of(i >> 1, j) : piece_of(j >> 1, i), half = by_row ? i & 1 : j & 1;
-        const bool alone = i == j && (by_row ? half == 1 : half == 0);    // (the other half lies above the diagonal)
-        Sum<W, 4> s;
-        s.of_summed(p[m]);
+        block_of(of_z ? task - BLOCKS : task, i, j);
+        const int row = 16 * i + c;
+        const f32x4 hj = *reinterpret_cast<const f32x4*>(&hi[16 * j + 4 * g]), lj = *reinterpret_cast<const f32x4*>(&lo[16 * j + 4 * g]);
 #pragma unroll
-        for (int t = 0; t < W; ++t) {
-            bf16x4* const to = reinterpret_cast<bf16x4*>(&sp[((set * PIECES + piece) * W + t) * 64 + lane]);
-            to[half] = s.term[t];
-            if (alone) to[1 - half] = bf16x4{};
+        for (int r = 0; r < 4; ++r) {
+            const int col = 16 * j + 4 * g + r;
+            const float d = exp_of(fminf((hi[row] - hj[r]) + (lo[row] - lj[r]), 88.f));
+            p[m][r] = of_z ? (row > col ? -d * p[m][r] : 0.f) : (row >= col ? a.c * d * p[m][r] : 0.f);
         }
+        Sum<W, 4> t4;
+        t4.of_summed(p[m]);
+#pragma unroll
+        for (int t = 0; t < W; ++t) *reinterpret_cast<bf16x4*>(sh + task * BLOCK + t * 256 + c * 16 + 4 * g) = t4.term[t];
     }
 #pragma unroll
     for (int i = 0; i < QV; ++i) {
         const int at = nth(i, QN), row = at / XC, col = at % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
-        store_terms<T>(rq[i], sq + to, XP);
-        store_terms<T>(rk[i], sk + to, XP);
+        store_terms<T>(__builtin_bit_cast(uint4, rq[i]), sq + to, XP);
+        store_terms<T>(__builtin_bit_cast(uint4, rk[i]), sk + to, XP);
     }
     __syncthreads();
-    const int kd = place<KW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
-    const int krow = place<KW>(c, 2 * wave + (g >> 1)) + 4 * (g & 1);     // 4 values of row c, from 16 wave + 4 g
-    float dots[4][JB];
+    typedef __attribute__((address_space(3))) s16x4* at_lds;
+    const bf16* const by_row = sh + c * 16 + 4 * g;       // this lane's 4 values of row c; of the transposing read
+    const bf16* const turned = sh + (4 * g + (c >> 2)) * 16 + 4 * (c & 3);
+    auto number = [](int i, int j) { return i * (i + 1) / 2 + j; };
+    // columns i of H (set 0) or Z, summed over moments j of blocks 2jj, 2jj + 1
+    auto rows_of = [&](int set, int jj, int i) {
+        Sum<W, 8> s;
+#pragma unroll
+        for (int t = 0; t < W; ++t) {
+            bf16x4 v[2] = {};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (2 * jj + e <= i) v[e] = *reinterpret_cast<const bf16x4*>(by_row + (set * BLOCKS + number(i, 2 * jj + e)) * BLOCK + t * 256);
+            s.term[t] = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return s;
+    };
+    // columns j of the transpose, summed over moments i of blocks 2ii, 2ii + 1
+    auto columns_of = [&](int set, int ii, int j) {
+        Sum<W, 8> s;
+#pragma unroll
+        for (int t = 0; t < W; ++t) {
+            bf16x4 v[2] = {};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (2 * ii + e >= j)
+                    v[e] = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (at_lds)(turned + (set * BLOCKS + number(2 * ii + e, j)) * BLOCK + t * 256)));
+            s.term[t] = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return s;
+    };
+    float dots[4][JB] = {};
+    const int krow = place<KW>(c, 2 * wave + (g >> 1)) + 4 * (g & 1), kc = 16 * wave + 4 * g;        // 4 values of row c, from there
 #pragma unroll
     for (int i = 0; i < JB; ++i) {
-        const f32x4 k4 = widened<X>(sk + 16 * i * KW + krow, XP);
         const float e = se[16 * i + c], w = sw[16 * i + c];
-        float s = 0.f;
+        const f32x4 k4 = widened<X>(sk + 16 * i * KW + krow, XP);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            s = fmaf(k4[r], x3[i][r], s);
+            dots[3][i] = fmaf(k4[r], x3[i][r], dots[3][i]);
             x1[i][r] *= a.c * e;
             x2[i][r] *= -e;
             x3[i][r] *= w;
         }
-        dots[3][i] = s;
     }
-    const bf16x8* const spl = sp + lane;
-    auto piece = [&](int set, int number) {
-        Sum<W, 8> s;
-#pragma unroll
-        for (int t = 0; t < W; ++t) s.term[t] = spl[((set * PIECES + number) * W + t) * 64];
-        return s;
-    };
 #pragma unroll
     for (int jj = 0; jj < JB / 2; ++jj) {
-        const Sum<X, 8> kt = down<X>(sk + 32 * jj * KW + kd, 16 * KW, XP), qt = down<X>(sq + 32 * jj * KW + kd, 16 * KW, XP);
+        const int at = 32 * jj * KW + place<KW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
+        const Sum<X, 8> kt = down<X>(sk + at, 16 * KW, XP), qt = down<X>(sq + at, 16 * KW, XP);
+        Sum<W, 8> kb;                                     // k times its rate
+        kb.of_summed(widened(kt) * joined(*reinterpret_cast<const f32x4*>(&sb[32 * jj + 4 * g]),
+                                          *reinterpret_cast<const f32x4*>(&sb[32 * jj + 16 + 4 * g])));
 #pragma unroll
         for (int i = 2 * jj; i < JB; ++i) {
-            x1[i] = mfma(kt, piece(0, piece_of(jj, i)), x1[i]);
-            x2[i] = mfma(kt, piece(2, piece_of(jj, i)), x2[i]);
+            x1[i] = mfma(kb, rows_of(0, jj, i), x1[i]);
+            x2[i] = mfma(kb, rows_of(1, jj, i), x2[i]);
         }
 #pragma unroll
         for (int j = 0; j < 2 * jj + 2; ++j) {
-            x3[j] = mfma(qt, piece(1, tpiece_of(jj, j)), x3[j]);
-            x3[j] = mfma(kt, piece(3, tpiece_of(jj, j)), x3[j]);
+            x3[j] = mfma(qt, columns_of(0, jj, j), x3[j]);
+            x3[j] = mfma(kt, columns_of(1, jj, j), x3[j]);
         }
     }
-    const int kc = 16 * wave + 4 * g;
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int i = 0; i < JB; ++i) {
         const f32x4 k4 = widened<X>(sk + 16 * i * KW + krow, XP), q4 = widened<X>(sq + 16 * i * KW + krow, XP);
         const int row = 16 * i + c;
-        dots[0][i] = dots[1][i] = dots[2][i] = 0.f;
         f32x4 gk;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
