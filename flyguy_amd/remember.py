@@ -2,7 +2,7 @@
 
     python -m flyguy_amd.remember --data GAME.bin [MORE.bin ...] --graph GRAPH.npz [--start CKPT.pt] [--hops 3]
         [--teacher T.pt] [--stretch 256] [--cars 16] [--steps 500] [--lr 1e-3] [--temp 0.5] [--heads 8] [--dim 64]
-        [--out runs/remember/memory.pt] [--device cuda] [--kernel hip|torch] [--seed 0]
+        [--rule decay|delta] [--norm] [--dropout 0] [--out runs/remember/memory.pt] [--device cuda] [--kernel hip|torch] [--seed 0]
 
 DATA: FLYD files or FLYR recordings of the bot as flyguy_amd.teach reads them, their moments in the order they were played;
 the answers are those in the files, or a fly-actor --teacher's.  The actor itself (--start, or a fresh one) stays as it is:
@@ -49,6 +49,9 @@ def main(argv=None) -> int:
     ap.add_argument("--temp", type=float, default=0.5)
     ap.add_argument("--heads", type=int, default=8)
     ap.add_argument("--dim", type=int, default=64)
+    ap.add_argument("--rule", default="decay", choices=["decay", "delta"], help="a memory that adds, or one that corrects")
+    ap.add_argument("--norm", action="store_true", help="a layer norm of the firing before the memory")
+    ap.add_argument("--dropout", type=float, default=0.0, help="the share of the memory's read-out dropped while teaching")
     ap.add_argument("--out", type=Path, default=Path("runs") / "remember" / "memory.pt")
     ap.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
     ap.add_argument("--kernel", default="hip", choices=["hip", "torch"])
@@ -56,6 +59,8 @@ def main(argv=None) -> int:
     args = ap.parse_args(argv)
     if min(args.steps, args.cars, args.stretch) < 1:
         raise SystemExit("--steps, --cars and --stretch are at least 1")
+    if not 0 <= args.dropout <= 1:
+        raise SystemExit("--dropout is a share from 0 to 1")
     dev = torch.device(args.device)
     torch.manual_seed(args.seed)
     rng = np.random.default_rng(args.seed)
@@ -68,7 +73,7 @@ def main(argv=None) -> int:
         raise SystemExit(f"no file holds {args.stretch} moments")
     teacher = None if args.teacher is None else _actor(args.graph, args.teacher, args.hops, args.kernel).to(dev)
     net = MemoryActor(_actor(args.graph, args.start, args.hops, args.kernel), heads=args.heads, dim=args.dim,
-                      positions=max(args.stretch, 65536)).to(dev)
+                      positions=max(args.stretch, 65536), rule=args.rule, norm=args.norm, dropout=args.dropout).to(dev)
     learns = [p for p in net.parameters() if p.requires_grad]
     opt = torch.optim.Adam(learns, lr=args.lr)
 
@@ -102,6 +107,7 @@ def main(argv=None) -> int:
     torch.save({**net.checkpoint(args.graph), "taught_steps": args.steps}, args.out)
 
     x, _ = draw()
+    net.eval()                                # (nothing is dropped in play)
     with torch.no_grad():
         at_once, _ = net(x)
         live = net.state(x.shape[0])

@@ -522,3 +522,55 @@ def test_far_strides(gpu_lib):
     view.copy_(k)
     for x, y in zip(delta_attention(q, view, v, g, b, s), delta_attention(q, k, v, g, b, s)):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("kw", [dict(rule="delta", norm=True, dropout=0.25), dict(rule="delta"), dict(norm=True, dropout=0.1)])
+def test_memory_actor_on_the_gpu(gpu_lib, kw):
+    """The layer norm, the projections, the rotation, the delta rule and the dropout together: MemoryActor against its CPU form,
+    the same numbers dropped; logits, state and every gradient to 1e-4 of the largest entry, as its other tests; then played."""
+    import copy
+
+    from conftest import lively, toy
+    from flyguy_amd.fly import FlyActor
+    from flyguy_amd.memory import MemoryActor
+    from gpu_helpers import rel
+    say(f"actor {kw}")
+    torch.manual_seed(3)
+    f = lively(FlyActor(toy("b"), 517, 90, hops=3), 3)
+    f.kernel = "hip"
+    m = MemoryActor(f, heads=4, k_heads=2, dim=24, positions=128, **kw)
+    with torch.no_grad():
+        m.back.weight.normal_(0, 0.3)
+        if m.rule == "delta":
+            m.gates.weight.normal_(0, 0.05)
+            m.gates.bias.normal_(0, 1)
+    x, R = torch.randn(3, 75, 517), torch.randn(3, 75, 90)
+    g = copy.deepcopy(m).cuda()
+    for _ in range(2):                                      # (the second pass drops others)
+        out, (mem, _) = g(x.cuda())
+        (out * R.cuda()).sum().backward()
+        want, (want_mem, _) = m(x)
+        (want * R).sum().backward()
+        assert rel(out.detach().cpu(), want.detach()) <= 1e-4 and rel(mem.detach().cpu(), want_mem.detach()) <= 1e-4
+    for (name, p), (_, q) in zip(g.named_parameters(), m.named_parameters()):
+        assert p.grad is not None and rel(p.grad.cpu(), q.grad) <= 1e-4, name
+    g.eval()
+    with torch.no_grad():
+        want, _ = g(x.cuda())
+        live = g.state(3)
+        played = torch.stack([g.step(x[:, t].cuda(), live) for t in range(75)], 1)
+    assert rel(played.cpu(), want.cpu()) <= 1e-4 and live[1].tolist() == [75] * 3
+
+
+def test_the_teaching_command_on_the_gpu(gpu_lib, tmp_path, capsys):
+    import numpy as np
+
+    from conftest import GOLDEN
+    from flyguy_amd.remember import main
+    from oracle import trainer as ot
+    rng = np.random.default_rng(4)
+    ot.write_chunk(tmp_path / "game.bin", rng.standard_normal((300, 517)).astype(np.float16),
+                   (3 * rng.standard_normal((300, 90))).astype(np.float16))
+    assert main(["--data", str(tmp_path / "game.bin"), "--graph", str(GOLDEN / "toy_a.npz"), "--stretch", "100", "--cars", "8",
+                 "--steps", "20", "--rule", "delta", "--norm", "--dropout", "0.1", "--out", str(tmp_path / "m.pt")]) == 0
+    assert float(capsys.readouterr().out.split("logits off by ")[1].split()[0]) < 1e-4
