@@ -139,6 +139,20 @@ __device__ __forceinline__ Sum<W, 8> first_terms(const Sum<P, 8>& s) {
     for (int i = 0; i < W; ++i) r.term[i] = s.term[i];
     return r;
 }
+// Products of several accumulators with a shared operand, a pair of terms of all of them at a time: an accumulator's next product
+// waits for its last one, so that these stand apart.  ROWS: the shared one is the second.
+template <bool ROWS, int N, int PA, int PB>
+__device__ __forceinline__ void mfmas(f32x4* c, const Sum<PA, 8>* a, const Sum<PB, 8>& b) {
+    constexpr int most = PA > PB ? PA : PB;
+#pragma unroll
+    for (int o = most - 1; o >= 0; --o)
+#pragma unroll
+        for (int i = 0; i < PA; ++i)
+            if (o - i >= 0 && o - i < PB)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    c[n] = ROWS ? mfma(a[n].term[i], b.term[o - i], c[n]) : mfma(b.term[o - i], a[n].term[i], c[n]);
+}
 // a product of two inputs: all pairs of terms where these are two (binary16: the last is 2^-18 of the product), else mfma's
 template <int P>
 __device__ __forceinline__ f32x4 mfma_whole(const Sum<P, 8>& a, const Sum<P, 8>& b, f32x4 c) {
@@ -421,6 +435,7 @@ struct Stage {
     u32x4 ru[STRAIGHT ? 1 : UV], rf;
     static constexpr int QV = CH * KW / 2048, WV = CH * NW / 2048;        // units of 1 KB a wave
     unsigned oq[QV], ok[QV], ow[WV];                      // a lane's places in them
+    unsigned long long mq[QV], mw[WV];                    // the lanes that have one
     int placed = -1;                                      // ... for chunks of so many rows
     char* room;
     int tid, wave, lane;
@@ -448,53 +463,70 @@ struct Stage {
     __device__ __forceinline__ const char* prepared(long long i0) const {
         return a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
     }
-    // 1 KB: a lane's 16 bytes from `offset` bytes past `base` to 16 bytes times the lane's number behind `to`
-    __device__ __forceinline__ static void straight(const void* base, unsigned offset, const char* to) {
+    // 1 KB: a lane's 16 bytes from `offset` bytes past `base` to 16 bytes times the lane's number behind `to`, of the lanes in `mask`
+    __device__ __forceinline__ static void straight(const void* base, unsigned offset, unsigned long long mask, const char* to) {
         const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)to);
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(base) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(at), "v"(offset),
+                     "s"(base), "s"(mask) : "memory");
     }
-    // a lane's place in unit 4 i + wave of rows of WIDTH values: value at..; 0xffffffff: past the head's end
+    // a lane's place in unit 4 i + wave of rows of WIDTH values, and the lanes whose columns are the head's
     template <int WIDTH>
-    __device__ __forceinline__ unsigned place_of(int i, int rows, long long step, int col0, int width) const {
+    __device__ __forceinline__ unsigned place_of(int i, int rows, long long step, int col0, int width, unsigned long long& mask) const {
         const int at = (4 * i + wave) * 512 + lane * 8, row = at / WIDTH;
         const int col = col0 + (place<WIDTH>(row, at % WIDTH >> 3) - row * WIDTH);
-        return col < width ? (unsigned)(min(row, rows - 1) * (int)step + col) * (unsigned)sizeof(T) : ~0u;
+        mask = __ballot(col < width);
+        return (unsigned)(min(row, rows - 1) * (int)step + (col < width ? col : 0)) * (unsigned)sizeof(T);
     }
     __device__ __forceinline__ void places_of(int rows) {
 #pragma unroll
         for (int i = 0; i < QV; ++i) {
-            oq[i] = place_of<KW>(i, rows, a.q.moment, 0, a.K);
-            ok[i] = place_of<KW>(i, rows, a.k.moment, 0, a.K);
+            oq[i] = place_of<KW>(i, rows, a.q.moment, 0, a.K, mq[i]);
+            ok[i] = place_of<KW>(i, rows, a.k.moment, 0, a.K, mq[i]);
         }
 #pragma unroll
-        for (int i = 0; i < WV; ++i) ow[i] = place_of<NW>(i, rows, w.moment, c0, a.V);
+        for (int i = 0; i < WV; ++i) ow[i] = place_of<NW>(i, rows, w.moment, c0, a.V, mw[i]);
     }
     __device__ __forceinline__ const T* base(const fm_view& v, int head, long long i0) const {
         return (const T*)v.data + (a.chunks.starts ? 0 : n * v.seq) + head * v.head + (first + i0) * v.moment;
     }
-    // the chunk from moment i0 on its way into room `which`
-    __device__ __forceinline__ void fetch(long long i0, int which) {
+    // A quarter of it: issued all at once, the loads' wave waits for their queue (2,000 cycles a chunk).
+    __device__ __forceinline__ void fetch_part(long long i0, int which, int part) {
+        // (rows past the chunk's last are the last once more: k_delta_prep's factors leave them out)
         const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+        if (part == 0 && rows != placed) places_of(placed = rows);
+        char* const to = room + which * BYTES + wave * 1024;
         const char* const prep = prepared(i0);
-        if constexpr (STRAIGHT) {
-            // (rows past the chunk's last are the last once more: k_delta_prep's factors leave them out)
-            if (rows != placed) places_of(placed = rows);
-            char* const to = room + which * BYTES + wave * 1024;
-            const T *const bq = base(a.q, h, i0), *const bk = base(a.k, h / a.share, i0), *const bw = base(w, hw, i0);
+        if (part == 0 && with_q) {
+            const T* const from = base(a.q, h, i0);
 #pragma unroll
-            for (int i = 0; i < QV; ++i)
-                if (with_q && oq[i] != ~0u) straight(bq, oq[i], to + i * 4096);
+            for (int i = 0; i < QV; ++i) straight(from, oq[i], mq[i], to + i * 4096);
+        }
+        if (part == 1) {
+            const T* const from = base(a.k, h / a.share, i0);
 #pragma unroll
-            for (int i = 0; i < QV; ++i)
-                if (ok[i] != ~0u) straight(bk, ok[i], to + K_AT + i * 4096);
+            for (int i = 0; i < QV; ++i) straight(from, ok[i], mq[i], to + K_AT + i * 4096);
+        }
+        if (part == 2) {
+            const T* const from = base(w, hw, i0);
 #pragma unroll
             for (int i = 0; i < WV; ++i)
-                if (with_w && ow[i] != ~0u) straight(bw, ow[i], to + W_AT + i * 4096);
+                if (with_w) straight(from, ow[i], mw[i], to + W_AT + i * 4096);
+            straight(prep + F::UNITS * 1024, lane * 16, ~0ull, room + which * BYTES + F_AT);      // (all waves the same)
+        }
 #pragma unroll
-            for (int i = 0; i < UV; ++i)
-                if (with_q || 4 * i + wave >= F::P_UNITS) straight(prep + (4 * i + wave) * 1024, lane * 16, to + U_AT + i * 4096);
-            if (wave == 0) straight(prep + F::UNITS * 1024, lane * 16, to + F_AT);
+        for (int i = 0; i < UV; ++i) {
+            if (part != 2 + (i >= UV / 2)) continue;
+            if (with_q || 4 * i + wave >= F::P_UNITS) straight(prep + (4 * i + wave) * 1024, lane * 16, ~0ull, to + U_AT + i * 4096);
+        }
+    }
+    // the chunk from moment i0 on its way into room `which`
+    __device__ __forceinline__ void fetch(long long i0, int which) {
+        if constexpr (STRAIGHT) {
+#pragma unroll
+            for (int part = 0; part < 4; ++part) fetch_part(i0, which, part);
         } else {
+            const int rows = (int)(count - i0 < CH ? count - i0 : CH);
+            const char* const prep = prepared(i0);
             const Chunk<T> cq = chunk_of<T>(a, a.q, n, h, first + i0, rows, a.K), ck = chunk_of<T>(a, a.k, n, h / a.share, first + i0, rows, a.K);
             const Chunk<T> cw = chunk_of<T>(a, w, n, hw, first + i0, rows, a.V);
 #pragma unroll
@@ -599,7 +631,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
         const int rows = (int)(left - i0 < CH ? left - i0 : CH);
         const long long next = i0 + CH;
         in.arrive();
-        if (In::STRAIGHT && next < left) in.fetch(next, which ^ 1);
+        const long long coming = next < left ? next : i0;    // (after the last chunk it once more, for nothing: no branch)
         const bf16 *const sq = in.q(which), *const vdown = in.third(which) + vat;
         bf16* const sk = in.k(which);
         const bf16x8 *const sp = in.units(which) + lane, *const stt = sp + F::P_UNITS * 64;
@@ -644,22 +676,22 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 #pragma unroll
                     for (int t = 0; t < T_TERMS; ++t) tf[m].term[t] = stt[(m * T_TERMS + t) * 64];
             }
+            if (In::STRAIGHT) {
+#pragma unroll
+                for (int part = 4 / KT * b; part < 4 / KT * (b + 1); ++part) in.fetch_part(coming, which ^ 1, part);
+            }
             in_order();
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
-            const Sum<W, 8> zo = first_terms<W>(zf);
-#pragma unroll
-            for (int i = 0; i < JB; ++i) {
-                e[i] = mfma(kf[b & 1][i], zf, e[i]);
-                if (WALK != OWN) o[i] = mfma(zo, qf[b & 1][i], o[i]);
-            }
+            mfmas<true, JB>(e, kf[b & 1], zf);
+            if (WALK != OWN) mfmas<false, JB>(o, qf[b & 1], first_terms<W>(zf));
             in_order();
         }
         if (!In::STRAIGHT && next < left) in.fetch(next, 0);
-        Sum<X, 8> kt[2 * KT];                             // (of the first 32 moments; then of the others)
+        Sum<X, 8> kt[JB / 2][2 * KT];
         auto read_columns = [&](int jj) {
 #pragma unroll
-            for (int b = 0; b < 2 * KT; ++b) kt[b] = down<X>(sk + 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1), 16 * KW, XP);
+            for (int b = 0; b < 2 * KT; ++b) kt[jj][b] = down<X>(sk + 32 * jj * KW + (yat ^ 32 * (b >> 1)) + 4 * (b & 1), 16 * KW, XP);
         };
         int since = CH;                                   // the column's first moment that is not finite
         {
@@ -697,8 +729,8 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             for (int jj = 0; jj < JB / 2; ++jj) {
                 Sum<T_TERMS, 8> df;
                 df.of_summed(joined(d[2 * jj], d[2 * jj + 1]));
-#pragma unroll
-                for (int i = 2 * jj; i < JB; ++i) e[i] = mfma(tf[piece_of(jj, i)], df, e[i]);
+                if (jj) mfmas<true, JB - 2>(e + 2, tf + JB, df);
+                else mfmas<true, JB>(e, tf, df);
             }
             in_order();
         }
@@ -720,6 +752,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
         decayed<2 * KT>(z, sf[0], sf[1]);
 #pragma unroll
         for (int jj = 0; jj < JB / 2; ++jj) {
+            if (jj + 1 < JB / 2) read_columns(jj + 1);
             if (WALK != OWN && jj == JB / 2 - 1) {
 #pragma unroll
                 for (int m = 0; m < F::PIECES; ++m)
@@ -729,10 +762,8 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
             in_order();
             Sum<T_TERMS, 8> uf;
             uf.of_summed(joined(e[2 * jj] * fb[2 * jj], e[2 * jj + 1] * fb[2 * jj + 1]));
-#pragma unroll
-            for (int b = 0; b < 2 * KT; ++b) z[b] = mfma(kt[b], uf, z[b]);
+            mfmas<true, 2 * KT>(z, kt[jj], uf);
             in_order();
-            if (jj + 1 < JB / 2) read_columns(jj + 1);
         }
         if (spoiled && since < CH)
 #pragma unroll
@@ -747,8 +778,8 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
         for (int jj = 0; jj < JB / 2; ++jj) {
             Sum<W, 8> ef;
             ef.of_summed(joined(e[2 * jj], e[2 * jj + 1]));
-#pragma unroll
-            for (int i = 2 * jj; i < JB; ++i) o[i] = mfma(ef, pf[piece_of(jj, i)], o[i]);
+            if (jj) mfmas<false, JB - 2>(o + 2, pf + JB, ef);
+            else mfmas<false, JB>(o, pf, ef);
         }
         if (spoiled)
 #pragma unroll
@@ -771,19 +802,25 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
                 }
         }
         if constexpr (WALK != OWN) {
-            const int oc = v0 + 16 * wave + 4 * g;
+            const int oc = v0 + 16 * wave + 4 * g, step = a.heads * a.V * (int)sizeof(T);
             T* const po = (T*)a.o + (((a.chunks.starts ? 0 : n * a.chunks.n_moments) + first + i0) * a.heads + h) * a.V;
             typedef T vec4 __attribute__((ext_vector_type(4)));
+            if (a.vec) {                                  // (what lies outside is dropped)
+                const auto to = rows_at(po, rows, step, a.V * (int)sizeof(T));
+                const unsigned at = oc < a.V ? c * step + oc * (int)sizeof(T) : NOWHERE;
 #pragma unroll
-            for (int i = 0; i < JB; ++i) {
-                const int row = 16 * i + c;
-                if (row >= rows || oc >= a.V) continue;
-                T* const to = po + (long long)row * a.heads * a.V + oc;
-                if (a.vec) *reinterpret_cast<vec4*>(to) = __builtin_convertvector(o[i], vec4);
-                else
+                for (int i = 0; i < JB; ++i) {
+                    const vec4 v = __builtin_convertvector(o[i], vec4);
+                    const unsigned there = 16 * i + c < rows ? at + 16 * i * step : NOWHERE;
+                    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, there, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), to, there, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < JB; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (oc + r < a.V) to[r] = narrow<T>(o[i][r]);
+                        if (16 * i + c < rows && oc + r < a.V) po[(long long)(16 * i + c) * a.heads * a.V + oc + r] = narrow<T>(o[i][r]);
             }
         }
     }
@@ -858,7 +895,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
     const int gat = place<NW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
     for (long long i0 = end; i0 >= 0; i0 -= CH, which ^= In::ROOMS - 1) {
         in.arrive();
-        if (In::STRAIGHT && i0) in.fetch(i0 - CH, which ^ 1);
+        const long long coming = i0 ? i0 - CH : i0;       // (after the last chunk it once more, for nothing: no branch)
         const bf16 *const sq = in.q(which), *const sk = in.k(which), *const gdown = in.third(which) + gat;
         const bf16x8 *const sp = in.units(which) + lane, *const stt = sp + F::P_UNITS * 64;
         const float* const sf = in.factors(which);
@@ -898,11 +935,14 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
                     fb[i] = *reinterpret_cast<const f32x4*>(&sf[F_E + CH + 16 * i + 4 * g]);
                 }
             }
+            if (In::STRAIGHT) {
+#pragma unroll
+                for (int part = 4 / KT * b; part < 4 / KT * (b + 1); ++part) in.fetch_part(coming, which ^ 1, part);
+            }
             in_order();
             Sum<T_TERMS, 8> zf;
             zf.of_summed(joined(z[2 * b], z[2 * b + 1]));
-#pragma unroll
-            for (int i = 0; i < JB; ++i) d[i] = mfma(kf[b & 1][i], zf, d[i]);
+            mfmas<true, JB>(d, kf[b & 1], zf);
             in_order();
         }
         if (!In::STRAIGHT && i0) in.fetch(i0 - CH, 0);
@@ -914,9 +954,10 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
 #pragma unroll
         for (int i = 0; i < JB; ++i) d[i] *= fb[i];
 #pragma unroll
-        for (int ii = 0; ii < JB / 2; ++ii)
-#pragma unroll
-            for (int j = 0; j < 2 * ii + 2; ++j) d[j] = mfma(pf[tpiece_of(ii, j)], gf[ii], d[j]);
+        for (int ii = 0; ii < JB / 2; ++ii) {
+            if (ii) mfmas<true, JB>(d, pf + 2, gf[ii]);
+            else mfmas<true, 2>(d, pf, gf[ii]);
+        }
         in_order();
         Sum<X, 8> qt[2 * KT], kt[2 * KT];                 // (of the first 32 moments; then of the others)
         auto read_columns = [&](int jj) {
@@ -933,8 +974,8 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
         for (int ii = 0; ii < JB / 2; ++ii) {
             Sum<T_TERMS, 8> df;
             df.of_summed(joined(d[2 * ii], d[2 * ii + 1]));
-#pragma unroll
-            for (int j = 0; j < 2 * ii + 2; ++j) y[j] = mfma(tf[tpiece_of(ii, j)], df, y[j]);
+            if (ii) mfmas<true, JB>(y, tf + 2, df);
+            else mfmas<true, 2>(y, tf, df);
         }
         in_order();
         if (WALK != OWN) {
@@ -951,11 +992,8 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
             Sum<T_TERMS, 8> gt, yt;
             gt.of_summed(widened(gf[jj]) * (f * a.c));
             yt.of_summed(-joined(y[2 * jj], y[2 * jj + 1]) * f);
-#pragma unroll
-            for (int b = 0; b < 2 * KT; ++b) {
-                z[b] = mfma(qt[b], gt, z[b]);
-                z[b] = mfma(kt[b], yt, z[b]);
-            }
+            mfmas<true, 2 * KT>(z, qt, gt);
+            mfmas<true, 2 * KT>(z, kt, yt);
             in_order();
             if (jj + 1 < JB / 2) read_columns(jj + 1);
         }
