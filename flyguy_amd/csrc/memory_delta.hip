@@ -45,6 +45,7 @@ struct Delta {
     int vec;                             // whole stores: heads of a multiple of 16 bytes, outputs aligned
     // workspace, by chunk slot and head
     char* prep;                          // T and P as the products' operands, then the chunk's factors
+    char* turned;                        // the same of their transposes, kept for the gradient (0: not wanted)
     float *states, *errors;              // S before each chunk [KW][VW], e [CH][VW] (0: not kept)
     float *grads, *ys;                   // X after each chunk, y, the same way
     // by segment slot and head: a segment's own end state, then its joined one (backwards: X before it) [KW][VW]; what it makes of the
@@ -210,12 +211,13 @@ __global__ __launch_bounds__(256) void k_delta_pack(Packs p) {
 // A workgroup a chunk and head.  K K^T and Q K^T on the matrix cores; N in float32 in LDS; T by blocks of 16: those on the diagonal by
 // forward substitution, a lane a column, then T_ij = -T_ii sum_k N_ik T_kj down each column of blocks, in float32 products
 // whose second operand stays in registers.  G is summed in 64 bits and kept in two floats: a difference of two of them is
-// exact to its own last bits however much has been forgotten before.  BWD: the operands of the transposes.
+// exact to its own last bits however much has been forgotten before.  BOTH: the operands of the transposes too, for the gradient.
 // A moment whose key, decay or rate is not finite spoils all from there on (k_delta_scan): here its chunk ends before it.
-template <class T, int KT, bool BWD>
+template <class T, int KT, bool BOTH>
 __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
-    using F = DeltaForm<T, BWD>;
-    constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, XC = KW / VN;
+    using F = DeltaForm<T>;
+    using B = DeltaForm<T, true>;
+    constexpr int X = F::X, CH = F::CH, JB = F::JB, KW = 32 * KT, XP = CH * KW, VN = Vec<T>::N, XC = KW / VN;
     constexpr int NP = CH + 4;                            // a row of N and T, padded
     // q and k; then, when their products are made, N and T (4 workgroups a CU)
     constexpr int ROWS_BYTES = 2 * X * XP * 2, NT_BYTES = 2 * CH * NP * 4;
@@ -236,23 +238,32 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, c = lane & 15;
     const long long moment = first + from;
     char* const prep = a.prep + ((size_t)slot * a.heads + h) * F::PREP;
-    if (tid == 0) bad = rows;
-    __syncthreads();
+    char* const turned_prep = BOTH ? a.turned + ((size_t)slot * a.heads + h) * B::PREP : nullptr;
+    float ld = 0.f, be = 0.f;
     {
         const Chunk<T> q = chunk_of<T>(a, a.q, n, h, moment, rows, a.K), k = chunk_of<T>(a, a.k, n, h / a.share, moment, rows, a.K);
-        for (int i = tid; i < CH * XC; i += 256) {
-            const int row = i / XC, col = i % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
-            const uint4 kr = k(row, col);
-            store_terms<T>(q(row, col), sq + to, XP);
-            store_terms<T>(kr, sk + to, XP);
-            if (odd16<T>(kr)) atomicMin(&bad, row);
+        constexpr int N = CH * XC / 256;
+        static_assert(N * 256 == CH * XC, "");
+        u32x4 rq[N], rk[N];                               // (all on their way at once)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            rq[i] = __builtin_bit_cast(u32x4, q((i * 256 + tid) / XC, (i * 256 + tid) % XC * VN));
+            rk[i] = __builtin_bit_cast(u32x4, k((i * 256 + tid) / XC, (i * 256 + tid) % XC * VN));
         }
-    }
-    float ld = 0.f, be = 0.f;
-    if (tid < rows) {
-        ld = a.log_decay[(a.chunks.starts ? 0 : n * a.ld_seq) + (moment + tid) * a.ld_moment + h * a.ld_head];
-        be = a.beta[(a.chunks.starts ? 0 : n * a.be_seq) + (moment + tid) * a.be_moment + h * a.be_head];
-        if (!(ld < INFINITY) || !(fabsf(be) < INFINITY)) atomicMin(&bad, tid);
+        if (tid < rows) {
+            ld = a.log_decay[(a.chunks.starts ? 0 : n * a.ld_seq) + (moment + tid) * a.ld_moment + h * a.ld_head];
+            be = a.beta[(a.chunks.starts ? 0 : n * a.be_seq) + (moment + tid) * a.be_moment + h * a.be_head];
+        }
+        if (tid == 0) bad = rows;
+        __syncthreads();
+        if (tid < rows && (!(ld < INFINITY) || !(fabsf(be) < INFINITY))) atomicMin(&bad, tid);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = (i * 256 + tid) / XC, col = (i * 256 + tid) % XC * VN, to = place<KW>(row, col >> 3) + (col & 7);
+            store_terms<T>(__builtin_bit_cast(uint4, rq[i]), sq + to, XP);
+            store_terms<T>(__builtin_bit_cast(uint4, rk[i]), sk + to, XP);
+            if (odd16<T>(__builtin_bit_cast(uint4, rk[i]))) atomicMin(&bad, row);
+        }
     }
     __syncthreads();
     const int stop = bad;                                 // rows from here on: nothing
@@ -267,46 +278,60 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
         }
         const double end = __shfl(s, CH - 1);             // (rows past the last add nothing)
         const float b = lane < stop ? be : 0.f, high = (float)s;
-        float* const f = const_cast<float*>(factors_of<F>(prep));
         if (lane < CH) {
             hi[lane] = high;
             lo[lane] = (float)(s - (double)high);
             sb[lane] = b;
-            const float e = exp_of((float)s), left_over = exp_of((float)(end - s));
-            f[F_E + lane] = lane < rows ? e : 0.f;         // (a row past the last adds nothing to a gradient)
-            f[F_E + CH + lane] = left_over * b;
-            f[F_E + 2 * CH + lane] = left_over;
-            f[F_E + 3 * CH + lane] = b;
-            f[F_E + 4 * CH + lane] = hi[lane];
-            f[F_E + 5 * CH + lane] = lo[lane];
         }
-        if (lane == 0) {
-            const Keep keep((float)end);
-            f[0] = keep.one;
-            f[1] = keep.f;
-            f[2] = __int_as_float(stop < rows ? stop : CH);
-            f[3] = 0.f;
-        }
+        const float e = lane < rows ? exp_of((float)s) : 0.f;              // (a row past the last adds nothing to a gradient)
+        const float left_over = exp_of((float)(end - s));
+        const Keep keep((float)end);
+        auto write = [&](float* f) {
+            if (lane < CH) {
+                f[F_E + lane] = e;
+                f[F_E + CH + lane] = left_over * b;
+                f[F_E + 2 * CH + lane] = left_over;
+                f[F_E + 3 * CH + lane] = b;
+                f[F_E + 4 * CH + lane] = high;
+                f[F_E + 5 * CH + lane] = (float)(s - (double)high);
+            }
+            if (lane == 0) {
+                f[0] = keep.one;
+                f[1] = keep.f;
+                f[2] = __int_as_float(stop < rows ? stop : CH);
+                f[3] = 0.f;
+            }
+        };
+        write(const_cast<float*>(factors_of<F>(prep)));
+        if (BOTH) write(const_cast<float*>(factors_of<B>(turned_prep)));
     }
     __syncthreads();
 
-    bf16x8* const units = reinterpret_cast<bf16x8*>(prep);
+    bf16x8 *const units = reinterpret_cast<bf16x8*>(prep), *const turned_units = reinterpret_cast<bf16x8*>(turned_prep);
     auto apart = [&](int i, int j) { return exp_of(fminf((hi[i] - hi[j]) + (lo[i] - lo[j]), 88.f)); };
-    auto store_half = [&](int unit, int half, const Sum<W, 4>& s) {
+    // a block of P as half an operand, and the half above the diagonal beside it
+    auto store_halves = [&](auto form, bf16x8* to, int unit, int half, bool alone, f32x4 p) {
+        constexpr int W = decltype(form)::W;
+        Sum<W, 4> s;
+        s.of_summed(p);
 #pragma unroll
-        for (int t = 0; t < W; ++t) reinterpret_cast<bf16x4*>(&units[(unit * W + t) * 64 + lane])[half] = s.term[t];
+        for (int t = 0; t < W; ++t) {
+            bf16x4* const at = reinterpret_cast<bf16x4*>(&to[(unit * W + t) * 64 + lane]);
+            at[half] = s.term[t];
+            if (alone) at[1 - half] = bf16x4{};
+        }
     };
-    constexpr int BLOCKS = JB * (JB + 1) / 2, MINE = (2 * BLOCKS + 3) / 4, NS = (BLOCKS + 3) / 4;
+    constexpr int BLOCKS = JB * (JB + 1) / 2, TASKS = (BOTH ? 3 : 2) * BLOCKS, MINE = (TASKS + 3) / 4, NS = (BLOCKS + 3) / 4;
     f32x4 own_n[NS];                                      // this wave's blocks of N
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
         const int task = 4 * m + wave;
-        if (task >= 2 * BLOCKS) break;
+        if (task >= TASKS) break;
         const bool of_q = task >= BLOCKS;
         int i, j;
-        block_of(of_q ? task - BLOCKS : task, i, j);
-        // of_q forwards: rows j, columns i; else rows i, columns j
-        const bool turned = of_q && !BWD;
+        block_of(task - task / BLOCKS * BLOCKS, i, j);
+        // P forwards: rows j, columns i; else rows i, columns j
+        const bool turned = task / BLOCKS == 1;
         const bf16* const ra = turned ? sk + 16 * j * KW : (of_q ? sq : sk) + 16 * i * KW;
         const bf16* const rb = turned ? sq + 16 * i * KW : sk + 16 * j * KW;
         f32x4 p = {0.f, 0.f, 0.f, 0.f};
@@ -329,15 +354,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
             const int row = turned ? 16 * i + c : 16 * i + 4 * g + r, col = turned ? 16 * j + 4 * g + r : 16 * j + c;
             p[r] = row >= col ? a.c * apart(row, col) * sb[col] * p[r] : 0.f;
         }
-        Sum<W, 4> s;
-        s.of_summed(p);
-        if (BWD) {
-            store_half(tpiece_of(i >> 1, j), i & 1, s);
-            if ((i & 1) && i == j) store_half(tpiece_of(i >> 1, j), 0, Sum<W, 4>{});
-        } else {
-            store_half(piece_of(j >> 1, i), j & 1, s);
-            if (!(j & 1) && i == j) store_half(piece_of(j >> 1, i), 1, Sum<W, 4>{});
-        }
+        if (turned) store_halves(F{}, units, piece_of(j >> 1, i), j & 1, !(j & 1) && i == j, p);
+        else if (BOTH) store_halves(B{}, turned_units, tpiece_of(i >> 1, j), i & 1, (i & 1) && i == j, p);
     }
     __syncthreads();                                      // (q and k are read)
 #pragma unroll
@@ -394,10 +412,10 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
         }
     }
     __syncthreads();
-    for (int task = wave; task < F::PIECES; task += 4) {
+    for (int task = wave; task < (BOTH ? 2 : 1) * F::PIECES; task += 4) {
         f32x4 half[2];
-        if (BWD) {                                        // rows j, summed over i
-            const int ii = task >= 2, j = ii ? task - 2 : task;
+        if (task >= F::PIECES) {                          // rows j, summed over i
+            const int m = task - F::PIECES, ii = m >= 2, j = ii ? m - 2 : m;
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -414,8 +432,9 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
         }
         Sum<T_TERMS, 8> s;
         s.of_summed(joined(half[0], half[1]));
+        bf16x8* const to = task < F::PIECES ? units + (F::P_UNITS + task * T_TERMS) * 64 : turned_units + (B::P_UNITS + (task - F::PIECES) * T_TERMS) * 64;
 #pragma unroll
-        for (int t = 0; t < T_TERMS; ++t) units[(F::P_UNITS + task * T_TERMS + t) * 64 + lane] = s.term[t];
+        for (int t = 0; t < T_TERMS; ++t) to[t * 64 + lane] = s.term[t];
     }
 }
 
@@ -1618,7 +1637,8 @@ long long move_floats(const fm_delta_args& a) {
     return in_segments(a) ? segment_slots(a) * a.q_heads * KW * KW : 0;
 }
 long long kept_floats(const fm_delta_args& a) { return chunk_slots(a) * a.q_heads * (state_floats(a) + row_floats(a)); }
-long long delta_saved_bytes(const fm_delta_args& a) { return 4 * (kept_floats(a) + move_floats(a)); }
+long long turned_bytes(const fm_delta_args& a) { return chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, true); }
+long long delta_saved_bytes(const fm_delta_args& a) { return 4 * (kept_floats(a) + move_floats(a)) + turned_bytes(a); }
 // float32 parts of shared key / value heads' gradients
 long long delta_part_floats(const fm_delta_args& a, bool of_v) {
     const long long moments = a.n_moments * (a.starts ? 1 : a.n_seq);
@@ -1645,7 +1665,7 @@ bool whole_stores(const fm_delta_args& p) {
 }
 
 long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
-    long long n = chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, bwd) + 4 * cut_floats(a);
+    long long n = (bwd ? 0 : chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, false)) + 4 * cut_floats(a);
     n += 4 * (bwd ? kept_floats(a) + delta_part_floats(a, false) + delta_part_floats(a, true) : move_floats(a));
     if (chunk_slots(a) && !in_whole_units(a, bwd))
         for (int i = 0; i < 3; ++i) n += pack_bytes(a, bwd, i);
@@ -1677,11 +1697,12 @@ Delta delta_of(const fm_delta_args& p, bool bwd) {
     a.V = (int)p.v_dim;
     a.c = (float)p.scale;
     a.vec = whole_stores(p);
-    a.prep = (char*)p.workspace;
     const long long states = chunk_slots(p) * p.q_heads * state_floats(p);
     a.states = (float*)p.saved;
     a.errors = a.states ? a.states + states : nullptr;
-    float* room = (float*)(a.prep + chunk_slots(p) * p.q_heads * prep_bytes(p.dtype, bwd));
+    a.turned = a.errors ? (char*)(a.errors + chunk_slots(p) * p.q_heads * row_floats(p) + move_floats(p)) : nullptr;
+    a.prep = bwd ? a.turned : (char*)p.workspace;
+    float* room = (float*)((char*)p.workspace + (bwd ? 0 : chunk_slots(p) * p.q_heads * prep_bytes(p.dtype, false)));
     a.own = room;
     room += cut_floats(p);
     a.trans_t = a.errors ? a.errors + chunk_slots(p) * p.q_heads * row_floats(p) : nullptr;
@@ -1709,7 +1730,9 @@ dim3 walks_of(const Delta& a, int blocks) { return blocks_of(((long long)a.segs.
 template <class T, int KT>
 void delta_fwd(const Delta& a, hipStream_t st) {
     const int BV = (a.V + 63) / 64;
-    if (a.chunks.slots) k_delta_prep<T, KT, false><<<blocks_of((long long)a.chunks.slots * a.heads), 256, 0, st>>>(a);
+    const dim3 chunks = a.chunks.slots ? blocks_of((long long)a.chunks.slots * a.heads) : dim3(1);
+    if (a.chunks.slots && a.turned) k_delta_prep<T, KT, true><<<chunks, 256, 0, st>>>(a);
+    else if (a.chunks.slots) k_delta_prep<T, KT, false><<<chunks, 256, 0, st>>>(a);
     if (a.segs.nseg > 1) {
         k_delta_scan<T, KT, OWN><<<walks_of(a, BV + KT / 2), 256, 0, st>>>(a);
         if (a.segs.nseg > 2) k_delta_join<KT, false><<<dim3(BV * a.heads, a.segs.n_seq), 256, 0, st>>>(a);
@@ -1720,7 +1743,6 @@ void delta_fwd(const Delta& a, hipStream_t st) {
 template <class T, int KT>
 void delta_bwd(const Delta& a, hipStream_t st) {
     const int BV = (a.V + 63) / 64;
-    if (a.chunks.slots) k_delta_prep<T, KT, true><<<blocks_of((long long)a.chunks.slots * a.heads), 256, 0, st>>>(a);
     if (a.segs.nseg > 1) {
         k_delta_back<T, KT, OWN><<<walks_of(a, BV), 256, 0, st>>>(a);
         if (a.segs.nseg > 2) k_delta_join<KT, true><<<dim3(BV * a.heads, a.segs.n_seq), 256, 0, st>>>(a);
@@ -1763,7 +1785,7 @@ void delta_of_type(const fm_delta_args& p, bool bwd, hipStream_t st) {
     if (!p.n_seq) return;
     if (a.chunks.slots && !in_whole_units(p, bwd)) {
         Packs k{};
-        char* to = a.prep + delta_workspace_bytes(p, bwd);
+        char* to = (char*)p.workspace + delta_workspace_bytes(p, bwd);
         fm_view* const views[3] = {&a.q, &a.k, bwd ? &a.go : &a.v};
         k.n_moments = p.n_moments;
         k.moments = p.n_moments * (p.starts ? 1 : p.n_seq);
