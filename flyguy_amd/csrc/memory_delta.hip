@@ -224,7 +224,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     __shared__ __align__(16) char room[ROWS_BYTES > NT_BYTES ? ROWS_BYTES : NT_BYTES];
     bf16 *const sq = reinterpret_cast<bf16*>(room), *const sk = sq + X * XP;
     float *const sn = reinterpret_cast<float*>(room), *const st = sn + CH * NP;
-    __shared__ float hi[CH], lo[CH], sb[CH];
+    __shared__ __align__(16) float hi[CH], lo[CH], sb[CH];
     __shared__ int bad;
     const unsigned block = (unsigned)block_number();
     const int place_in = (int)(block / a.heads), h = (int)(block - (unsigned)place_in * a.heads);
@@ -308,7 +308,6 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
     __syncthreads();
 
     bf16x8 *const units = reinterpret_cast<bf16x8*>(prep), *const turned_units = reinterpret_cast<bf16x8*>(turned_prep);
-    auto apart = [&](int i, int j) { return exp_of(fminf((hi[i] - hi[j]) + (lo[i] - lo[j]), 88.f)); };
     // a block of P as half an operand, and the half above the diagonal beside it
     auto store_halves = [&](auto form, bf16x8* to, int unit, int half, bool alone, f32x4 p) {
         constexpr int W = decltype(form)::W;
@@ -322,40 +321,42 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
         }
     };
     constexpr int BLOCKS = JB * (JB + 1) / 2, TASKS = (BOTH ? 3 : 2) * BLOCKS, MINE = (TASKS + 3) / 4, NS = (BLOCKS + 3) / 4;
-    f32x4 own_n[NS];                                      // this wave's blocks of N
+    f32x4 p[MINE];                                        // this wave's blocks: of N (task < BLOCKS), P, and P by rows
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) p[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < KT; ++b) {
+        const int at = place<KW>(c, g) ^ 32 * b;
+#pragma unroll
+        for (int m = 0; m < MINE; ++m) {                  // (past the last: some block once more)
+            const int task = min(4 * m + wave, TASKS - 1), kind = task / BLOCKS;
+            int i, j;
+            block_of(task - kind * BLOCKS, i, j);
+            // P forwards: rows j, columns i; else rows i, columns j
+            const bf16* const ra = kind == 1 ? sk + 16 * j * KW : (kind ? sq : sk) + 16 * i * KW;
+            const bf16* const rb = kind == 1 ? sq + 16 * i * KW : sk + 16 * j * KW;
+            p[m] = mfma_whole(across<X>(ra + at, XP), across<X>(rb + at, XP), p[m]);
+        }
+    }
 #pragma unroll
     for (int m = 0; m < MINE; ++m) {
-        const int task = 4 * m + wave;
+        const int task = 4 * m + wave, kind = task / BLOCKS;
         if (task >= TASKS) break;
-        const bool of_q = task >= BLOCKS;
         int i, j;
-        block_of(task - task / BLOCKS * BLOCKS, i, j);
-        // P forwards: rows j, columns i; else rows i, columns j
-        const bool turned = task / BLOCKS == 1;
-        const bf16* const ra = turned ? sk + 16 * j * KW : (of_q ? sq : sk) + 16 * i * KW;
-        const bf16* const rb = turned ? sq + 16 * i * KW : sk + 16 * j * KW;
-        f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int b = 0; b < KT; ++b) {
-            const int at = place<KW>(c, g) ^ 32 * b;
-            p = mfma_whole(across<X>(ra + at, XP), across<X>(rb + at, XP), p);
-        }
-        if (!of_q) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * i + 4 * g + r, col = 16 * j + c;
-                p[r] = row > col ? apart(row, col) * sb[col] * p[r] : 0.f;
-            }
-            if (m < NS) own_n[m < NS ? m : 0] = p;
-            continue;
-        }
+        block_of(task - kind * BLOCKS, i, j);
+        const int ri = 16 * i + (kind == 1 ? c : 4 * g), cj = 16 * j + (kind == 1 ? 4 * g : c);     // a lane's first
+        const f32x4 h4 = *reinterpret_cast<const f32x4*>(&hi[kind == 1 ? cj : ri]), l4 = *reinterpret_cast<const f32x4*>(&lo[kind == 1 ? cj : ri]);
+        const f32x4 b4 = *reinterpret_cast<const f32x4*>(&sb[kind == 1 ? cj : ri]);
+        const float h1 = hi[kind == 1 ? ri : cj], l1 = lo[kind == 1 ? ri : cj], b1 = sb[cj];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = turned ? 16 * i + c : 16 * i + 4 * g + r, col = turned ? 16 * j + 4 * g + r : 16 * j + c;
-            p[r] = row >= col ? a.c * apart(row, col) * sb[col] * p[r] : 0.f;
+            const int row = kind == 1 ? ri : ri + r, col = kind == 1 ? cj + r : cj;
+            const float apart = kind == 1 ? (h1 - h4[r]) + (l1 - l4[r]) : (h4[r] - h1) + (l4[r] - l1);
+            const float d = exp_of(fminf(apart, 88.f)) * (kind == 1 ? b4[r] : b1);
+            p[m][r] = kind ? (row >= col ? a.c * d * p[m][r] : 0.f) : (row > col ? d * p[m][r] : 0.f);
         }
-        if (turned) store_halves(F{}, units, piece_of(j >> 1, i), j & 1, !(j & 1) && i == j, p);
-        else if (BOTH) store_halves(B{}, turned_units, tpiece_of(i >> 1, j), i & 1, (i & 1) && i == j, p);
+        if (kind == 1) store_halves(F{}, units, piece_of(j >> 1, i), j & 1, !(j & 1) && i == j, p[m]);
+        else if (BOTH && kind == 2) store_halves(B{}, turned_units, tpiece_of(i >> 1, j), i & 1, (i & 1) && i == j, p[m]);
     }
     __syncthreads();                                      // (q and k are read)
 #pragma unroll
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(Delta a) {
         block_of(4 * m + wave, i, j);
         if (4 * m + wave < BLOCKS)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sn[(16 * i + 4 * g + r) * NP + 16 * j + c] = own_n[m][r];
+            for (int r = 0; r < 4; ++r) sn[(16 * i + 4 * g + r) * NP + 16 * j + c] = p[m][r];
     }
     __syncthreads();
     if (tid < CH) {                                       // the diagonal blocks: column c of block tid / 16
@@ -1118,13 +1119,27 @@ __global__ __launch_bounds__(256) void k_delta_join(Delta a) {
 // Then q and k take their place, and H and Z as blocks of terms, which are read by rows for what sums over j and through the
 // transposing read for what sums over i.
 template <class T, int KT, int VT>
-__global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
+constexpr int grads_room() {                              // 16-bit values of LDS
+    using F = DeltaForm<T, true>;
+    constexpr int first = (F::X + 2 * F::W) * F::CH * 64 * VT, second = 2 * F::X * F::CH * 32 * KT + F::JB * (F::JB + 1) * F::W * 256;
+    constexpr int third = 64 * KT * F::CH, most = first > second ? first : second;
+    return most > third ? most : third;
+}
+// workgroups a CU that LDS lets in, and that registers are left for (waves a SIMD)
+template <class T, int KT, int VT>
+constexpr int grads_waves() {
+    constexpr int fit = 78 * 1024 / grads_room<T, KT, VT>();
+    constexpr int most = Form<T>::X == 3 ? 2 : 3;
+    return KT == 4 ? 2 : fit < 1 ? 1 : fit > most ? most : fit;
+}
+template <class T, int KT, int VT>
+__global__ __launch_bounds__(128 * KT, (grads_waves<T, KT, VT>())) void k_delta_grads(Delta a) {
     using F = DeltaForm<T, true>;
     constexpr int X = F::X, W = F::W, CH = F::CH, JB = F::JB, KW = 32 * KT, VW = 64 * VT, XP = CH * KW, VP = CH * VW, VN = Vec<T>::N;
     constexpr int WAVES_ = 2 * KT, THREADS = 64 * WAVES_, XC = KW / VN, VC = VW / VN, BLOCKS = JB * (JB + 1) / 2;
-    constexpr int FIRST = (X + 2 * W) * VP, BLOCK = W * 256, SECOND = 2 * X * XP + 2 * BLOCKS * BLOCK;
-    __shared__ __align__(16) bf16 room[FIRST > SECOND ? FIRST : SECOND];
-    __shared__ __align__(16) float hi[CH], lo[CH], sb[CH], se[CH], sw[CH], red[WAVES_][4][CH], red_state[WAVES_];
+    constexpr int BLOCK = W * 256;
+    __shared__ __align__(16) bf16 room[grads_room<T, KT, VT>()];
+    __shared__ __align__(16) float hi[CH], lo[CH], sb[CH], se[CH], sw[CH], sums[4][CH], red_state[WAVES_];
     bf16 *const sg = room, *const sy = sg + X * VP, *const ser = sy + W * VP;
     bf16 *const sq = room, *const sk = sq + X * XP, *const sh = sk + X * XP;   // sh: [H, Z][block][W][16 i][16 j]
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, c = lane & 15;
@@ -1333,23 +1348,50 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
             x3[i][r] *= w;
         }
     }
+    // (a step's operands are read before the products of the step before)
+    Sum<X, 8> kt[JB / 2], qt[JB / 2];
+    Sum<W, 8> kb[JB / 2];                                 // k times its rate
 #pragma unroll
     for (int jj = 0; jj < JB / 2; ++jj) {
         const int at = 32 * jj * KW + place<KW>(4 * g + (c >> 2), 2 * wave + (c >> 1 & 1)) + 4 * (c & 1);
-        const Sum<X, 8> kt = down<X>(sk + at, 16 * KW, XP), qt = down<X>(sq + at, 16 * KW, XP);
-        Sum<W, 8> kb;                                     // k times its rate
-        kb.of_summed(widened(kt) * joined(*reinterpret_cast<const f32x4*>(&sb[32 * jj + 4 * g]),
-                                          *reinterpret_cast<const f32x4*>(&sb[32 * jj + 16 + 4 * g])));
+        kt[jj] = down<X>(sk + at, 16 * KW, XP);
+        qt[jj] = down<X>(sq + at, 16 * KW, XP);
+    }
+    constexpr int STEPS = 2 * F::PIECES;                  // each piece by rows, then each of the transposes
+    Sum<W, 8> hz[2][2];
+    auto read_step = [&](int step) {
+        const int m = step % F::PIECES, jj = m >= JB, i = jj ? m - JB + 2 : m, ii = m >= 2, j = ii ? m - 2 : m;
+        hz[step & 1][0] = step < F::PIECES ? rows_of(0, jj, i) : columns_of(0, ii, j);
+        hz[step & 1][1] = step < F::PIECES ? rows_of(1, jj, i) : columns_of(1, ii, j);
+    };
+    read_step(0);
 #pragma unroll
-        for (int i = 2 * jj; i < JB; ++i) {
-            x1[i] = mfma(kb, rows_of(0, jj, i), x1[i]);
-            x2[i] = mfma(kb, rows_of(1, jj, i), x2[i]);
-        }
+    for (int jj = 0; jj < JB / 2; ++jj)
+        kb[jj].of_summed(widened(kt[jj]) * joined(*reinterpret_cast<const f32x4*>(&sb[32 * jj + 4 * g]),
+                                                  *reinterpret_cast<const f32x4*>(&sb[32 * jj + 16 + 4 * g])));
 #pragma unroll
-        for (int j = 0; j < 2 * jj + 2; ++j) {
-            x3[j] = mfma(qt, columns_of(0, jj, j), x3[j]);
-            x3[j] = mfma(kt, columns_of(1, jj, j), x3[j]);
+    for (int step = 0; step < STEPS; ++step) {
+        const int m = step % F::PIECES, jj = m >= JB, i = jj ? m - JB + 2 : m, ii = m >= 2, j = ii ? m - 2 : m;
+        if (step + 1 < STEPS) read_step(step + 1);
+        in_order();
+        if (step < F::PIECES) {
+            f32x4 two[2] = {x1[i], x2[i]};
+            mfmas<false, 2>(two, hz[step & 1], kb[jj]);   // (two sums at a time: no product waits for the one before it)
+            x1[i] = two[0];
+            x2[i] = two[1];
+        } else {
+            f32x4 two[2] = {x3[j], f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int t = W - 1; t >= 0; --t)
+#pragma unroll
+                for (int u = 0; u < X; ++u)
+                    if (t + u < W) {
+                        two[0] = mfma(qt[ii].term[u], hz[step & 1][0].term[t], two[0]);
+                        two[1] = mfma(kt[ii].term[u], hz[step & 1][1].term[t], two[1]);
+                    }
+            x3[j] = two[0] + two[1];
         }
+        in_order();
     }
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -1381,25 +1423,28 @@ __global__ __launch_bounds__(128 * KT) void k_delta_grads(Delta a) {
         }
     }
     if (!a.glog_decay && !a.gbeta) return;
+    __syncthreads();                                      // (q, k, H and Z are read)
+    float* const red = reinterpret_cast<float*>(room);    // [wave][g][4][CH]
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int i = 0; i < JB; ++i) {
-            float s = dots[d][i];
-            s += __shfl_xor(s, 16);
-            s += __shfl_xor(s, 32);
-            if (g == 0) red[wave][d][16 * i + c] = s;
-        }
+        for (int i = 0; i < JB; ++i) red[((wave * 4 + g) * 4 + d) * CH + 16 * i + c] = dots[d][i];
     dot = wave_sum(dot, 64);
     if (lane == 0) red_state[wave] = dot;
     __syncthreads();
-    if (wave == 0) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, sx = 0.f;
-        for (int w = 0; w < WAVES_; ++w) {
-            sx += red_state[w];
+    if (tid < 4 * CH) {
+        float s = 0.f;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) s[d] += lane < CH ? red[w][d][lane] : 0.f;
-        }
+        for (int w = 0; w < 4 * WAVES_; ++w) s += red[w * 4 * CH + tid];
+        sums[tid / CH][tid % CH] = s;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        float s[4], sx = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES_; ++w) sx += red_state[w];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) s[d] = lane < CH ? sums[d][lane] : 0.f;
         const float b = lane < CH ? sb[lane] : 0.f;
         float gg = s[0] + s[1] - b * s[2], end = lane < CH ? sw[lane] * b * s[3] : 0.f;
         end = wave_sum(end, 64) + (f[0] + f[1]) * sx;
