@@ -273,7 +273,10 @@ __global__ __launch_bounds__(256) void k_norm_sums(fm_norm_args a, int blocks) {
     }
 }
 
-// widest rows of a wave, of a workgroup (single values take more registers for their addresses)
+// widest rows of a wave, of a workgroup (single values take more registers for their addresses).  A wave's rows need no barrier,
+// a workgroup's keep fewer values a lane.  8,192 rows, us forward and with gradients: of 768 values in bfloat16 9.4 and 28 by waves,
+// 14.6 and 37 by workgroups; of 1,024 in float32 13.7 and 43, 15.1 and 41; of 2,048 in float32 55 and 157 by waves, 23 and 68 by
+// workgroups, in bfloat16 16.9 and 49, 17.2 and 45.
 constexpr int NORM_WAVE = 64 * 16, NORM_MOST = 256 * 32, NORM_MOST_SINGLE = 256 * 16;
 
 // a wave's rows: the fewest lanes, a power of two, that hold a row `held` values each
@@ -288,7 +291,8 @@ inline Group group_of(long long width, int held) {
 inline int norm_rows_per_block(const fm_norm_args& a) {
     return a.width <= NORM_WAVE ? 256 >> group_of(a.width, 16).shift : 1;
 }
-// Workgroups of a gradient: 4 rows a group or more, at most 4 a CU.
+// Workgroups of a gradient: 4 rows a group or more, at most 4 a CU.  (Each leaves its sums to be joined: 8,192 rows of 4,096 values
+// of float32 with gradients 178 us by at most 512 workgroups, 151 by 1,024, 170 by 2,048.)
 inline int norm_blocks(const fm_norm_args& a) {
     const long long at_once = 4LL * norm_rows_per_block(a), b = (a.rows + at_once - 1) / at_once;
     return (int)(b < 1 ? 1 : b > 1024 ? 1024 : b);
