@@ -512,6 +512,82 @@ def test_another_stream_and_a_graph(gpu_lib):
             assert torch.equal(a, b), i
 
 
+def test_a_gradient_taken_twice(gpu_lib):
+    """What the forward leaves for its gradient stays as it was: a second pass gives the same numbers."""
+    from flyguy_amd.memory_hip import delta_attention
+    gen = torch.Generator().manual_seed(41)
+    for dt, shape in ((BF16, (2, 150)), (F32, (1, 2100))):
+        leaves = [x.detach().requires_grad_() for x in inputs(gen, shape, 2, 1, 64, 64, dt, "dense", shape[0])]
+        outs = delta_attention(*leaves)
+        given = [torch.randn_like(x) for x in outs]
+        first = torch.autograd.grad(outs, leaves, given, retain_graph=True)
+        for a, b in zip(first, torch.autograd.grad(outs, leaves, given)):
+            assert torch.equal(a, b)
+
+
+def test_two_at_once_and_two_graphs(gpu_lib):
+    """Calls of the same sizes on two streams at the same time, and two graphs of them replayed in turn and side by side, each
+    with its own inputs, give what they give alone."""
+    from flyguy_amd.memory_hip import delta_attention
+    gen = torch.Generator().manual_seed(42)
+    both = [inputs(gen, (1, 2100), 2, 1, 64, 64, BF16, "dense", 1) for _ in range(2)]
+    go = draw(gen, 1, 2100, 2, 64, dtype=BF16)
+
+    def work(given):
+        leaves = [x.detach().requires_grad_() for x in given]
+        o, e = delta_attention(*leaves)
+        return (o.detach(), e.detach(), *torch.autograd.grad((o, e), leaves, (go, torch.ones_like(e))))
+
+    want = [work(x) for x in both]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for i in range(3):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[n].append(work(both[n]))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for run in got[n]:
+            for a, b in zip(want[n], run):
+                assert torch.equal(a, b), n
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for n, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            outs.append(work(both[n]))
+    for i in range(4):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st if i >= 2 else streams[0]):
+                graphs[n].replay()
+        torch.cuda.synchronize()
+        for n in range(2):
+            for a, b in zip(want[n], outs[n]):
+                assert torch.equal(a, b), (i, n)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_tensors_at_odd_places(gpu_lib, dt):
+    """States and values that begin inside other memory, at no multiple of 16 bytes, and one tensor given as two of the three."""
+    from flyguy_amd.memory_hip import delta_attention, delta_step
+    gen = torch.Generator().manual_seed(43)
+
+    def moved(x):
+        room = torch.full((x.numel() + 3,), math.nan, dtype=x.dtype, device="cuda")
+        return room[3:].view(x.shape).copy_(x)
+
+    q, k, v, g, b, s = inputs(gen, (2, 70), 2, 2, 64, 64, dt, "dense", 2)
+    for x, y in zip(delta_attention(q, k, v, g, b, s), delta_attention(*map(moved, (q, k, v, g, b, s)))):
+        assert torch.equal(x, y)
+    for x, y in zip(delta_attention(k, k, k, g, b, s), delta_attention(k, k.clone(), moved(k), g, b, s)):
+        assert torch.equal(x, y)
+    one = [x[:, 0] for x in (q, k, v, g, b)]
+    there, odd = s.clone(), moved(s)
+    o, p = delta_step(*one, there), delta_step(*map(moved, one), odd)
+    assert torch.equal(o, p) and torch.equal(there, odd)
+    into = moved(torch.zeros_like(s))
+    assert torch.equal(delta_step(*one, s, into=into), o) and torch.equal(into, there)
+
+
 def test_far_strides(gpu_lib):
     """Moments more than 2^31 bytes apart."""
     from flyguy_amd.memory_hip import delta_attention

@@ -270,3 +270,28 @@ def test_rows_on_another_stream_and_in_a_graph(gpu_lib):
         torch.cuda.synchronize()
         for a, c in zip(want[i], outs):
             assert torch.equal(a, c), i
+
+
+def test_rows_at_odd_places(gpu_lib):
+    """One row for all, every second row, rows and weights at no multiple of 16 bytes, a counter inside other memory."""
+    from flyguy_amd.rows_hip import dropout, layer_norm
+    gen = torch.Generator().manual_seed(19)
+    room = draw(gen, 70, 1333)
+    w, b = room[0, 1:257], room[1, 3:259]
+    for x in (room[2, 5:261].expand(9, 256), room[::2, 1:257], room[4:, 2:258].unflatten(0, (6, 11))):
+        # (bounds as above; not the dense copies' numbers, bit for bit: those are read in units of 16 bytes, these one by one, so
+        # that a row's 256 numbers are summed in another order)
+        leaves, n, D = [t.detach().requires_grad_() for t in (x, w, b)], x.numel() // 256, 256
+        y, g = layer_norm(*leaves), room[5, 7:263].expand(x.shape)
+        f = [t.detach().cpu().double() for t in (x.reshape(-1, D), w, b)]
+        want = rows_ref.layer_norm(*f, 1e-5, g.reshape(-1, D).cpu().double())
+        r = (f[0].var(1, unbiased=False, keepdim=True) + 1e-5).rsqrt()
+        second = float(((D + 2) * ref.U * f[0].abs().mean(1, keepdim=True) * r).square().max())
+        gx, gw, gb = torch.autograd.grad(y, leaves, g)
+        ref.within(y.view(-1, D), *want[0], D + 20, "y", second)
+        ref.within(gx.reshape(-1, D), *want[1], 3 * D + 60, "gx", 3 * second)
+        ref.within(gw, *want[2], n + D + 40, "gweight", second)
+        ref.within(gb, *want[3], n + 5, "gbias")
+        counts = torch.tensor([9, 5, 9, 3], device="cuda")
+        assert torch.equal(dropout(x, 0.5, counts[::2]), dropout(x.clone(), 0.5, torch.tensor([9, 9], device="cuda")))
+        assert torch.equal(dropout(x, 0.5, counts[2:]), dropout(x.clone(), 0.5, torch.tensor([9, 3], device="cuda")))
