@@ -1037,79 +1037,83 @@ __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
 }
 
 // Segments' end states from their own: S_0 = own_0, S_s = M_s S_{s-1} + own_s, in place; backwards X_s = M_s^T X_{s+1} + own_s
-// from the last segment's.  A wave 16 columns, as in the walks; the workgroup's waves share the work of M's terms, and the next M
-// is on its way meanwhile (10 -> 2 us a segment of 128 x 128).  The last segment's end state (backwards: the first one's X) is left to the walk.
-// grid (blocks of 64 columns x heads, stretches)
+// from the last segment's.  This is the one part that no other chain fills the machine beside: a workgroup takes 16 columns, a
+// wave 32 rows of M, whose terms stay its own; S passes between waves through LDS, in two rooms for one barrier a segment.  A segment
+// of 128 x 128 takes 2.6 us (64 columns a workgroup, M's terms in LDS: 5.5, with 96 KB read from LDS by each wave), most of it
+// for M's terms; a second M on its way changes nothing.  The last segment's end state (backwards: the first one's X) is left to
+// the walk.  grid (blocks of 16 columns x heads, a head's on one XCD where their number is a multiple of 8; stretches)
 template <int KT, bool BACK>
-__global__ __launch_bounds__(256) void k_delta_join(Delta a) {
-    constexpr int KW = 32 * KT, MINE = 2 * KT * KT / 4;   // a wave's operands of M
-    __shared__ __align__(16) bf16x8 sm[2 * KT * KT][T_TERMS][64];
-    const int blocks_v = (a.V + 63) / 64, VW = 64 * blocks_v, h = blockIdx.x / blocks_v, n = blockIdx.y;
+__global__ __launch_bounds__(64 * KT) void k_delta_join(Delta a) {
+    constexpr int KW = 32 * KT;
+    __shared__ __align__(16) bf16x8 sz[2][KT][T_TERMS][64];
+    const int VW = 64 * ((a.V + 63) / 64), h = blockIdx.x % a.heads, n = blockIdx.y;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int col = 64 * (blockIdx.x % blocks_v) + 16 * wave + c;
+    const int col = 16 * (blockIdx.x / a.heads) + c;
     long long first, count;
     stretch_of(a.segs, n, first, count);
     const int segments = (int)((count + a.segs.L - 1) / a.segs.L), slot = first_slot(a.segs, n, first);
     if (segments < 3) return;                             // (one end state, and it is the true one)
-    auto row_of = [&](int b, int r) { return 32 * (b >> 1) + 8 * g + 4 * (b & 1) + r; };
     const ptrdiff_t step = (ptrdiff_t)a.heads * KW * VW * (BACK ? -1 : 1), mstep = (ptrdiff_t)a.heads * KW * KW * (BACK ? -1 : 1);
     const int s0 = BACK ? segments - 1 : 0;
-    float* own = a.own + ((size_t)(slot + s0) * a.heads + h) * KW * VW + col;
-    const float* m = (BACK ? a.trans_t : a.trans) + ((size_t)(slot + s0) * a.heads + h) * KW * KW + (size_t)(8 * (c >> 2) + (c & 3)) * KW + 8 * g;
-    f32x4 z[2 * KT], y[2 * KT], rm[MINE][2];
+    float* own = a.own + ((size_t)(slot + s0) * a.heads + h) * KW * VW + (32 * wave + 8 * g) * VW + col;
+    const float* m = (BACK ? a.trans_t : a.trans) + ((size_t)(slot + s0) * a.heads + h) * KW * KW +
+                     (size_t)(32 * wave + 8 * (c >> 2) + (c & 3)) * KW + 8 * g;
+    f32x4 z[2], y[2], rm[KT][2][2];
+    Sum<T_TERMS, 8> mf[KT][2];
+    auto own_of = [&](f32x4 (&v)[2]) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[b][r] = own[(4 * b + r) * VW];
+    };
     auto fetch = [&]() {                                  // the next segment's
-        own += step;
         m += mstep;
 #pragma unroll
-        for (int i = 0; i < MINE; ++i) {
-            const int b = (4 * i + wave) / KT, k = (4 * i + wave) % KT;
-            const f32x4* const row = reinterpret_cast<const f32x4*>(m + (32 * (b >> 1) + 4 * (b & 1)) * KW + 32 * k);
-            rm[i][0] = row[0];
-            rm[i][1] = row[1];
-        }
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int b = 0; b < 2 * KT; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[b][r] = own[row_of(b, r) * VW];
+            for (int b = 0; b < 2; ++b) {
+                const f32x4* const row = reinterpret_cast<const f32x4*>(m + 4 * b * KW + 32 * k);
+                rm[k][b][0] = row[0];
+                rm[k][b][1] = row[1];
+            }
     };
+    auto share = [&](int which) {
+        Sum<T_TERMS, 8> zf;
+        zf.of_summed(joined(z[0], z[1]));
 #pragma unroll
-    for (int b = 0; b < 2 * KT; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) z[b][r] = own[row_of(b, r) * VW];
+        for (int t = 0; t < T_TERMS; ++t) sz[which][wave][t][lane] = zf.term[t];
+    };
+    own_of(z);
+    share(1);
     fetch();
+    own += step;
+    own_of(y);
     for (int i = 1; i < segments - 1; ++i) {
-        __syncthreads();                                  // (the M before is read)
 #pragma unroll
-        for (int j = 0; j < MINE; ++j) {
-            Sum<T_TERMS, 8> mf;
-            mf.of_summed(joined(rm[j][0], rm[j][1]));
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
-            for (int t = 0; t < T_TERMS; ++t) sm[4 * j + wave][t][lane] = mf.term[t];
-        }
-        __syncthreads();
+            for (int b = 0; b < 2; ++b) mf[k][b].of_summed(joined(rm[k][b][0], rm[k][b][1]));
+        z[0] = y[0];
+        z[1] = y[1];
         float* const to = own;
-        f32x4 x[2 * KT];
-#pragma unroll
-        for (int b = 0; b < 2 * KT; ++b) x[b] = y[b];
-        if (i + 1 < segments - 1) fetch();
+        if (i + 1 < segments - 1) {
+            fetch();
+            own += step;
+            own_of(y);
+        }
+        __syncthreads();                                  // (the other room is read: its next writer is behind this)
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
             Sum<T_TERMS, 8> zf;
-            zf.of_summed(joined(z[2 * k], z[2 * k + 1]));
 #pragma unroll
-            for (int b = 0; b < 2 * KT; ++b) {
-                Sum<T_TERMS, 8> mf;
-#pragma unroll
-                for (int t = 0; t < T_TERMS; ++t) mf.term[t] = sm[b * KT + k][t][lane];
-                x[b] = mfma(mf, zf, x[b]);
-            }
+            for (int t = 0; t < T_TERMS; ++t) zf.term[t] = sz[i & 1][k][t][lane];
+            mfmas<true, 2>(z, mf[k], zf);
         }
+        share(~i & 1);
 #pragma unroll
-        for (int b = 0; b < 2 * KT; ++b) {
-            z[b] = x[b];
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) to[row_of(b, r) * VW] = z[b][r];
-        }
+            for (int r = 0; r < 4; ++r) to[(4 * b + r) * VW] = z[b][r];
     }
 }
 
@@ -1634,23 +1638,27 @@ long long chunk_slots(const fm_delta_args& a) {
 // Segments: a walk takes a workgroup for 64 columns and a CU for itself, so that few chains leave most CUs without work.  Cut
 // into segments of L moments, these are walked at the same time, for more work: their own end states, with M (K more columns) but
 // for the first, then those joined one after another, then the walk.  By the following estimate (us): a chunk takes a walk
-// `chunk`, four fifths of it where only the own state is wanted, a join `join`, the launches 12; workgroups go 256 at a time.
+// `chunk`, four fifths of it where only the own state is wanted, a join `join`, the launches 12; workgroups go 256 at a time (narrow heads
+// leave room for some of the next ones beside).
 // Packed stretches, whose lengths only the device knows, are taken to be of any length up to twice the middle one.
 // Measured with 1 to 64 segments, each type, heads of 64 and 128, 1 to 37 stretches of 1,024 to 32,768 moments, with gradients
-// and without (84 calls): the estimate's choice takes 1.02 times the best one's time in the middle, 1.17 at most, walks without
-// segments 2.2 in the middle, 14 at most: 1 x 4 heads of 128 x 16,384 of bfloat16 1,008 us whole and 225 in 16 segments;
-// 16 x 8 x 1,024 109 and 172 in two.
+// and without (84 calls): the estimate's choice takes 1.02 times the best one's time in the middle, 1.18 at most, walks without
+// segments 2.4 in the middle, 18 at most: 1 x 4 heads of 128 x 16,384 of bfloat16 1,012 us whole and 183 in 16 segments;
+// 16 x 8 x 1,024 108 and 172 in two.
 long long segment_length(const fm_delta_args& p) {
     const long long C = chunk_length(p.dtype), whole = (p.n_moments + C - 1) / C * C;
     if (!p.n_seq || whole <= C) return whole ? whole : C;
     const bool packed = p.starts && p.n_seq > 1, deep = p.k_dim > 64;
-    const double chunk = p.dtype == FM_F32 ? 3.4 : 2.4, join = deep ? 4.5 : 1.5, BV = p.v_dim <= 64 ? 1 : 2, BK = deep ? 2 : 1;
+    const double chunk = p.dtype == FM_F32 ? 3.4 : 2.4, join = deep ? 2.5 : 0.8, BV = p.v_dim <= 64 ? 1 : 2, BK = deep ? 2 : 1;
     const double middle = (double)p.n_moments / (packed ? p.n_seq : 1), longest = packed ? fmin(2 * middle, (double)p.n_moments) : middle;
     const double chains = (double)p.n_seq * p.q_heads, chunks = ceil(longest / C);
-    auto rounds = [](double groups) { return fmax(1.0, ceil(groups / 256)); };
-    double best = 0.9 * chunk * fmax(chunks, chains * BV * ceil(middle / C) / 256);
+    auto rounds = [deep](double groups) {
+        const double x = groups / 256;
+        return fmax(1.0, deep ? ceil(x) : (x + ceil(x)) / 2);
+    };
+    double best = chunk * fmax(chunks, chains * BV * ceil(middle / C) / 256);
     long long L = whole;
-    for (int nseg = 2; nseg <= 256; nseg += nseg < 8 ? 1 : nseg / 4) {
+    for (int nseg = 2; nseg <= 256; nseg += nseg < 16 ? 1 : nseg / 8) {
         const double each = ceil(chunks / nseg);
         if (each < 1 || each >= chunks) continue;
         const double mean = packed ? middle / (each * C) + 0.5 : ceil(chunks / each);            // segments a chain
@@ -1782,7 +1790,7 @@ void delta_fwd(const Delta& a, hipStream_t st) {
     else if (a.chunks.slots) k_delta_prep<T, KT, false><<<chunks, 256, 0, st>>>(a);
     if (a.segs.nseg > 1) {
         k_delta_scan<T, KT, OWN><<<walks_of(a, BV + KT / 2), 256, 0, st>>>(a);
-        if (a.segs.nseg > 2) k_delta_join<KT, false><<<dim3(BV * a.heads, a.segs.n_seq), 256, 0, st>>>(a);
+        if (a.segs.nseg > 2) k_delta_join<KT, false><<<dim3(4 * BV * a.heads, a.segs.n_seq), 64 * KT, 0, st>>>(a);
     }
     if (a.states) k_delta_scan<T, KT, KEEP><<<walks_of(a, BV), 256, 0, st>>>(a);
     else k_delta_scan<T, KT, PLAY><<<walks_of(a, BV), 256, 0, st>>>(a);
@@ -1792,7 +1800,7 @@ void delta_bwd(const Delta& a, hipStream_t st) {
     const int BV = (a.V + 63) / 64;
     if (a.segs.nseg > 1) {
         k_delta_back<T, KT, OWN><<<walks_of(a, BV), 256, 0, st>>>(a);
-        if (a.segs.nseg > 2) k_delta_join<KT, true><<<dim3(BV * a.heads, a.segs.n_seq), 256, 0, st>>>(a);
+        if (a.segs.nseg > 2) k_delta_join<KT, true><<<dim3(4 * BV * a.heads, a.segs.n_seq), 64 * KT, 0, st>>>(a);
     }
     k_delta_back<T, KT, KEEP><<<walks_of(a, BV), 256, 0, st>>>(a);
     if (!a.chunks.slots || !(a.gq || a.gk || a.gv || a.glog_decay || a.gbeta)) return;
