@@ -1297,7 +1297,7 @@ __global__ __launch_bounds__(128 * KT, (grads_waves<T, KT, VT>())) void k_delta_
         Sum<W, 4> t4;
         t4.of_summed(p[m]);
 #pragma unroll
-        for (int t = 0; t < W; ++t) *reinterpret_cast<bf16x4*>(sh + task * BLOCK + t * 256 + c * 16 + 4 * g) = t4.term[t];
+        for (int t = 0; t < W; ++t) *reinterpret_cast<bf16x4*>(sh + task * BLOCK + t * 256 + c * 16 + 4 * (g ^ (c >> 2))) = t4.term[t];
     }
 #pragma unroll
     for (int i = 0; i < QV; ++i) {
@@ -1307,8 +1307,9 @@ __global__ __launch_bounds__(128 * KT, (grads_waves<T, KT, VT>())) void k_delta_
     }
     __syncthreads();
     typedef __attribute__((address_space(3))) s16x4* at_lds;
-    const bf16* const by_row = sh + c * 16 + 4 * g;       // this lane's 4 values of row c; of the transposing read
-    const bf16* const turned = sh + (4 * g + (c >> 2)) * 16 + 4 * (c & 3);
+    // this lane's 4 values of row c; of the transposing read (the shares of row 4n + m exchanged by n: rows 4 apart share banks)
+    const bf16* const by_row = sh + c * 16 + 4 * (g ^ (c >> 2));
+    const bf16* const turned = sh + (4 * g + (c >> 2)) * 16 + 4 * ((c & 3) ^ g);
     auto number = [](int i, int j) { return i * (i + 1) / 2 + j; };
     // columns i of H (set 0) or Z, summed over moments j of blocks 2jj, 2jj + 1
     auto rows_of = [&](int set, int jj, int i) {
@@ -1428,18 +1429,18 @@ __global__ __launch_bounds__(128 * KT, (grads_waves<T, KT, VT>())) void k_delta_
     }
     if (!a.glog_decay && !a.gbeta) return;
     __syncthreads();                                      // (q, k, H and Z are read)
-    float* const red = reinterpret_cast<float*>(room);    // [wave][g][4][CH]
+    float* const red = reinterpret_cast<float*>(room);    // [wave][g][4][CH], the 16s of a g exchanged by it
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int i = 0; i < JB; ++i) red[((wave * 4 + g) * 4 + d) * CH + 16 * i + c] = dots[d][i];
+        for (int i = 0; i < JB; ++i) red[(wave * 4 + g) * 4 * CH + ((d * CH + 16 * i + c) ^ (16 * g))] = dots[d][i];
     dot = wave_sum(dot, 64);
     if (lane == 0) red_state[wave] = dot;
     __syncthreads();
     if (tid < 4 * CH) {
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4 * WAVES_; ++w) s += red[w * 4 * CH + tid];
+        for (int w = 0; w < 4 * WAVES_; ++w) s += red[w * 4 * CH + (tid ^ (16 * (w & 3)))];
         sums[tid / CH][tid % CH] = s;
     }
     __syncthreads();
