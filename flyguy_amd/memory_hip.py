@@ -1,6 +1,6 @@
 """A memory over decisions on the MI355X library: rotary positions, per-head norms with the rotation, linear attention
-with a decay for each head, and the gated delta rule (include/flyguy_memory.h).  An addition: the reference remembers nothing from one decision to
-the next (flyguy/fly.py:286-305 decides each moment alone).
+with a decay for each head, and the gated delta rule (include/flyguy_memory.h).  An addition: the reference remembers nothing
+from one decision to the next (flyguy/fly.py:286-305 decides each moment alone).
 
     q, k = rotary(q, k, table, positions)                       # turned by their positions
     q, k = norm_rotary(q, k, wq, wk, table, positions)          # each head's norm and the turn, in one pass
@@ -510,7 +510,8 @@ def delta_attention(q, k, v, log_decay, beta, state=None, starts=None, scale: fl
     number for each moment and query head (q's shape without its values), with any strides.  Meant for keys with beta |k|^2 at
     most 2, as keys of length 1 and rates in (0, 1) have; beyond that a state may grow from moment to moment.
     Returns (o in q's type, the state after each stretch).  Gradients of q, k, v, log_decay, beta and state; for them the forward
-    keeps each chunk's state and errors (1.5 KB a moment and head of 128 values)."""
+    keeps each chunk's state, errors and prepared operands (in bfloat16 2.1 KB a moment and head of 128 values).  log_decay's
+    gradient is what is left of sums that cancel where little was remembered: it is off by the float32 roundings of their terms."""
     what = "delta_attention"
     _no_tangents(what, q, k, v, log_decay, beta, state)
     dims = 4 if starts is None else 3

@@ -122,9 +122,9 @@ class DropoutHip(torch.autograd.Function):
 def dropout(x, share: float, counter):
     """x with a share of its numbers set to 0, the others divided by what is left: number i (in x's order, whatever its strides)
     is dropped where its 16-bit draw is below t = round(65536 share), and multiplied by 65536 / (65536 - t) elsewhere, so that
-    the mean stays exactly; share 1 drops all.  counter: int64 [2] on the same GPU, (seed, offset), read when the work runs: the draws are those of Philox4x32 of
-    10 rounds, of key seed and counter (i // 8, offset).  The same counter gives the same mask; it may not be changed in place before the gradient is
-    taken.  y is dense."""
+    the mean stays exactly; share 1 drops all.  counter: int64 [2] on the same GPU, (seed, offset), read when the work runs: the
+    draws are those of Philox4x32 of 10 rounds, of key seed and counter (i // 8, offset).  The same counter gives the same mask;
+    it may not be changed in place before the gradient is taken.  y is dense."""
     what = "dropout"
     _no_tangents(what, x)
     _of_rows(what, x)

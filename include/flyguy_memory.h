@@ -110,7 +110,8 @@ int fm_step(const fm_step_args* a, void* stream);
  * head or stretch (gradients: no other head or stretch).
  * saved: fm_delta_saved(a) bytes that the gradient reads (0: no gradient is wanted), workspace: fm_delta_workspace(a, backward)
  * bytes.  Gradients (fm_delta_bwd): inputs and saved as the forward left them; go of o, gstate_out of state_out (0: zeros); gq, gk,
- * gv dense like their tensors, glog_decay, gbeta float32 [moments][q_heads], gstate float32; each 0 where not wanted. */
+ * gv dense like their tensors, glog_decay, gbeta float32 [moments][q_heads], gstate float32; each 0 where not wanted.  glog_decay
+ * is what is left of sums that cancel where little was remembered: off by the float32 roundings of their terms. */
 typedef struct fm_delta_args {
     fm_view q, k, v, go;
     const float *log_decay, *beta;
