@@ -525,6 +525,16 @@ def test_a_gradient_taken_twice(gpu_lib):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_states_that_grow(gpu_lib, dt):
+    """Log decays from 0 to 1: what an early moment leaves is 1e17 times larger in the end.  What a moment is off by grows as what
+    it leaves does, so that against the largest number the bound of decaying states holds."""
+    gen = torch.Generator().manual_seed(44)
+    ins = inputs(gen, (2, 40), 2, 1, 64, 64, dt, "dense", 2)
+    ins[3] = 1 - torch.rand(2, 40, 2, generator=gen).cuda() * 0.1
+    check(ins, None, dt, gen=gen)
+
+
 def test_two_at_once_and_two_graphs(gpu_lib):
     """Calls of the same sizes on two streams at the same time, and two graphs of them replayed in turn and side by side, each
     with its own inputs, give what they give alone."""
