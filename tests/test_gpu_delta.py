@@ -610,6 +610,22 @@ def test_far_strides(gpu_lib):
         assert torch.equal(x, y)
 
 
+def test_more_than_2_31_values(gpu_lib):
+    """Two stretches of 1.1e9 values: the one that lies beyond 2^31 bytes, and partly values, gives what it gives as the first."""
+    from flyguy_amd.memory_hip import delta_attention
+    T, H = 140000, 64
+    torch.manual_seed(45)
+    q = torch.randn(2, T, H, 128, dtype=BF16, device="cuda")
+    k, v = (torch.randn(2, T, 1, 128, dtype=BF16, device="cuda") * 0.08 for _ in range(2))
+    g, b = -torch.rand(2, T, H, device="cuda"), torch.rand(2, T, H, device="cuda")
+    o, e = delta_attention(q, k, v, g, b)
+    turned, end = delta_attention(*(x.flip(0) for x in (q, k, v, g, b)))
+    assert torch.isfinite(e).all()
+    for n in range(2):
+        assert torch.equal(o[n], turned[1 - n]) and torch.equal(e[n], end[1 - n])
+        assert float(o[n, -64:].abs().max()) > 0
+
+
 @pytest.mark.parametrize("kw", [dict(rule="delta", norm=True, dropout=0.25), dict(rule="delta"), dict(norm=True, dropout=0.1)])
 def test_memory_actor_on_the_gpu(gpu_lib, kw):
     """The layer norm, the projections, the rotation, the delta rule and the dropout together: MemoryActor against its CPU form,
