@@ -12,10 +12,10 @@ namespace fg {
 // gx = r (u - mean(u) - xh mean(u xh)), gw = sum over rows of g xh, gb = sum over rows of g.
 //
 // A row is held by a group of lanes: a power of two up to a wave's 64, or (WIDE) the whole workgroup, NV units of V values a
-// lane (16 bytes, or single values where rows are not aligned), so that it is read once and its squares are summed about the
+// lane (16 bytes, 8 or single values, as rows are aligned), so that it is read once and its squares are summed about the
 // mean.  A group walks several rows, with the weights (gradient: their gradients' sums) in registers all along.  Bound by the
-// copy rate: 32,768 rows of 4,096 values of bfloat16 take 101 us forward (5.3 TB/s), 155 the gradient (5.2 TB/s), 6.5 the joining
-// of the weights' sums.
+// copy rate: 32,768 rows of 4,096 values of bfloat16 take 98 us forward (5.5 TB/s), 147 the gradient (5.5 TB/s), 4.5 the joining of the
+// weights' sums.
 struct Group {
     int lanes, shift;                    // lanes: 1 << shift (WIDE: 256)
 };
@@ -48,17 +48,16 @@ __device__ __forceinline__ void sum_over(float (&v)[N], const Group& l, float* s
 
 template <class T, int V, int NV>
 __device__ __forceinline__ void read_row(const T* x, int j, int lanes, int D, float (&v)[NV][V]) {
-    typename ValuesOf<T, V>::type u[NV];
+    typename ValuesOf<T, V>::type u[NV];                  // (lanes past the row read its first values: a branch each would wait)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int at = (i * lanes + j) * V;
-        if (at < D) u[i] = *reinterpret_cast<const typename ValuesOf<T, V>::type*>(x + at);
-        else u[i] = (typename ValuesOf<T, V>::type)(T)0.f;
+        u[i] = *reinterpret_cast<const typename ValuesOf<T, V>::type*>(x + (at < D ? at : 0));
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = widen(u[i][e]);
+        for (int e = 0; e < V; ++e) v[i][e] = (i * lanes + j) * V < D ? widen(u[i][e]) : 0.f;
 }
 template <class T, int V, int NV>
 __device__ __forceinline__ void write_row(T* y, int j, int lanes, int D, const float (&v)[NV][V]) {
@@ -78,7 +77,7 @@ __device__ __forceinline__ void read_floats(const float* w, float none, int j, i
     for (int i = 0; i < NV; ++i) {
         const int at = (i * lanes + j) * V;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[i][e] = w && at < D ? w[at + e] : none;
+        for (int e = 0; e < V; ++e) v[i][e] = w ? w[(at < D ? at : 0) + e] : none;
     }
 }
 
@@ -275,11 +274,11 @@ __global__ __launch_bounds__(256) void k_norm_sums(fm_norm_args a, int blocks) {
     }
 }
 
-// widest rows of a wave, of a workgroup (single values take more registers for their addresses).  A wave's rows need no barrier,
-// a workgroup's keep fewer values a lane.  8,192 rows, us forward and with gradients: of 768 values in bfloat16 9.4 and 28 by waves,
-// 14.6 and 37 by workgroups; of 1,024 in float32 13.7 and 43, 15.1 and 41; of 2,048 in float32 55 and 157 by waves, 23 and 68 by
-// workgroups, in bfloat16 16.9 and 49, 17.2 and 45.
-constexpr int NORM_WAVE = 64 * 16, NORM_MOST = 256 * 32, NORM_MOST_SINGLE = 256 * 16;
+// widest rows of a wave, of a workgroup.  A wave's rows need no barrier, a workgroup's keep fewer values a lane.  8,192 rows, us
+// forward and with gradients: of 768 values in bfloat16 9.5 and 28 by waves, 14.3 and 37 by workgroups; of 1,024 in float32 13.4
+// and 39, 15.9 and 41; of 1,332 in float32 18.8 and 51 by waves, 17.0 and 48 by workgroups; of 2,048 in bfloat16 17.0 and 49, 16.5
+// and 45.
+constexpr int NORM_WAVE = 64 * 16, NORM_MOST = 256 * 32;
 
 // a wave's rows: the fewest lanes, a power of two, that hold a row `held` values each
 inline Group group_of(long long width, int held) {
@@ -293,11 +292,13 @@ inline Group group_of(long long width, int held) {
 inline int norm_rows_per_block(const fm_norm_args& a) {
     return a.width <= NORM_WAVE ? 256 >> group_of(a.width, 16).shift : 1;
 }
-// Workgroups of a gradient: 4 rows a group or more, at most 4 a CU.  (Each leaves its sums to be joined: 8,192 rows of 4,096 values
-// of float32 with gradients 178 us by at most 512 workgroups, 151 by 1,024, 170 by 2,048.)
+// Workgroups of a gradient: 4 rows a group or more, at most 4 a CU, 2 where rows are 8 KB or more, whose values leave room for no
+// more at a time; each leaves its sums to be joined.  Forward and gradient with at most 1,024 and 512: 32,768 rows of 4,096 values
+// of bfloat16 287 and 275 us, 8,192 of 4,096 of float32 144 and 131, 32,768 of 2,048 of float32 274 and 258, of bfloat16 141 and 166.
 inline int norm_blocks(const fm_norm_args& a) {
     const long long at_once = 4LL * norm_rows_per_block(a), b = (a.rows + at_once - 1) / at_once;
-    return (int)(b < 1 ? 1 : b > 1024 ? 1024 : b);
+    const long long most = a.width * (a.dtype == FM_F32 ? 4 : 2) >= 8192 ? 512 : 1024;
+    return (int)(b < 1 ? 1 : b > most ? most : b);
 }
 
 template <class T, int V, int HELD>
@@ -320,7 +321,7 @@ void launch_norm(const fm_norm_args& a, bool bwd, hipStream_t st) {
     const long long each = a.width <= NORM_WAVE ? (a.width + 63) / 64 : (a.width + 255) / 256;
     if (each <= 8) launch_held<T, V, 8>(a, bwd, st);
     else if (each <= 16) launch_held<T, V, 16>(a, bwd, st);
-    else if constexpr (V > 1) launch_held<T, V, 32>(a, bwd, st);
+    else launch_held<T, V, 32>(a, bwd, st);
 }
 
 template <class T>
@@ -329,8 +330,10 @@ void norm_of_type(const fm_norm_args& a, bool bwd, hipStream_t st) {
     uintptr_t bits = (uintptr_t)a.x | (uintptr_t)(a.x_row * size) | (uintptr_t)(a.width * size);
     if (bwd) bits |= (uintptr_t)a.g | (uintptr_t)(a.g_row * size) | (uintptr_t)a.gx | (uintptr_t)(a.gx_row * size);
     else bits |= (uintptr_t)a.y | (uintptr_t)(a.y_row * size);
-    const bool units = !(bits & 15);
-    if (a.width > (units ? NORM_MOST : NORM_MOST_SINGLE)) {
+    // (8,192 rows of 1,332 values of bfloat16, forward and with gradients: 16.0 and 41 us in halves of a unit, 17.8 and 47 in single
+    // values; of 6,004: 41 and 136, 55 and 206)
+    const bool units = !(bits & 15), halves = !(bits & 7);
+    if (a.width > NORM_MOST) {
         const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
         if (!bwd) k_norm_any<T><<<blocks, 256, 0, st>>>(a);
         else {
@@ -341,6 +344,7 @@ void norm_of_type(const fm_norm_args& a, bool bwd, hipStream_t st) {
         return;
     }
     if (units) launch_norm<T, Vec<T>::N>(a, bwd, st);
+    else if (halves) launch_norm<T, Vec<T>::N / 2>(a, bwd, st);
     else launch_norm<T, 1>(a, bwd, st);
 }
 

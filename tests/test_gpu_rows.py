@@ -54,6 +54,14 @@ NORMS = [  # rows, width, type, layout, weight, bias
     (2, 8200, F16, "apart", True, True),
     (5, 20001, F32, "dense", True, True),
     (4200, 40, BF16, "dense", True, True),
+    (900, 252, BF16, "dense", True, True),
+    (9, 1002, F32, "dense", True, True),
+    (6, 1332, F16, "dense", True, True),
+    (3, 5001, F32, "dense", True, True),
+    (4, 5002, F32, "dense", True, False),
+    (3, 5002, BF16, "dense", False, True),
+    (3, 6004, BF16, "dense", True, True),
+    (2100, 4096, BF16, "dense", True, True),
 ]
 
 
