@@ -14,7 +14,7 @@ import struct
 import torch
 
 from ._lib import lib
-from .memory_hip import _TYPES, _call, _floats, _no_tangents, _once, _ptr, _wants_grad
+from .memory_hip import _TYPES, _call, _floats, _no_tangents, _once, _ptr, _wants_grad, _workspaces
 
 _NORM = struct.Struct("=17qd")
 _DROP = struct.Struct("=7qd")
@@ -44,6 +44,17 @@ def _pack_norm(x, y, g, gx, weight, bias, gweight, gbias, stats, partial, eps) -
                       _ptr(gweight), _ptr(gbias), _ptr(stats), _ptr(partial), rows, width, _TYPES[x.dtype], eps)
 
 
+def _partial(rows, like) -> torch.Tensor:
+    """Room for the workgroups' sums."""
+    sizes = ("norm", *rows.shape, rows.dtype)
+    n = _workspaces.get(sizes)
+    if n is None:
+        if len(_workspaces) >= 4096:
+            _workspaces.clear()
+        n = _workspaces[sizes] = lib().fm_norm_partial(_pack_norm(rows, *[None] * 9, 0.0))
+    return like.new_empty(n)
+
+
 class LayerNormHip(torch.autograd.Function):
     """layer_norm with gradients: apply(x, weight, bias, eps) (weight and bias may be None)."""
 
@@ -66,10 +77,9 @@ class LayerNormHip(torch.autograd.Function):
         gx = x.new_empty(x.shape) if want_x else None
         gw = torch.empty_like(weight) if want_w else None
         gb = torch.empty_like(bias) if want_b else None
-        pack = lambda partial: _pack_norm(rows, None, g, None if gx is None else gx.view(rows.shape), weight, bias, gw, gb,
-                                          stats, partial, ctx.eps)                                # noqa: E731
-        partial = stats.new_empty(lib().fm_norm_partial(pack(None))) if want_w or want_b else None
-        _call("fm_norm_bwd", x, pack(partial))
+        partial = _partial(rows, stats) if want_w or want_b else None
+        _call("fm_norm_bwd", x, _pack_norm(rows, None, g, None if gx is None else gx.view(rows.shape), weight, bias, gw, gb, stats,
+                                           partial, ctx.eps))
         return gx, gw, gb, None
 
 
