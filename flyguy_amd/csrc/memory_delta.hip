@@ -1543,20 +1543,22 @@ __global__ __launch_bounds__(256) void k_delta_step(fm_delta_step_args a) {
     const size_t at = ((size_t)slot * a.q_heads + h) * K * N;
     float4 s[PER];
     float kr[PER], qr[PER], vv[4];
+    // (lanes past the state's rows and columns load its first ones, which nothing uses: branches would make the loads wait for one
+    // another: 416 rows, 8 heads of 128 x 128 in bfloat16, 94 us instead of 87)
     auto load = [&](const float* p) {
-        if (VEC) return c0 < N ? *reinterpret_cast<const float4*>(p + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
-        return make_float4(c0 < N ? p[c0] : 0.f, c0 + 1 < N ? p[c0 + 1] : 0.f, c0 + 2 < N ? p[c0 + 2] : 0.f,
-                           c0 + 3 < N ? p[c0 + 3] : 0.f);
+        if (VEC) return *reinterpret_cast<const float4*>(p + (c0 < N ? c0 : 0));
+        return make_float4(p[c0 < N ? c0 : 0], p[c0 + 1 < N ? c0 + 1 : 0], p[c0 + 2 < N ? c0 + 2 : 0], p[c0 + 3 < N ? c0 + 3 : 0]);
     };
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = rg + i * RG;
-        s[i] = r < K ? load(a.state + at + (size_t)r * N) : make_float4(0.f, 0.f, 0.f, 0.f);
-        kr[i] = r < K ? widen(k[r]) : 0.f;
-        qr[i] = r < K ? widen(q[r]) : 0.f;
+        const int there = r < K ? r : 0;
+        s[i] = load(a.state + at + (size_t)there * N);
+        kr[i] = widen(k[there]);
+        qr[i] = widen(q[there]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = c0 + j < N ? widen(v[c0 + j]) : 0.f;
+    for (int j = 0; j < 4; ++j) vv[j] = widen(v[c0 + j < N ? c0 + j : 0]);
     const Keep keep(a.log_decay[n * a.ld_row + h * a.ld_head]);
     const float beta = a.beta[n * a.be_row + h * a.be_head];
     float sum[9] = {};                                    // S^T k, S^T q of 4 columns; q . k
@@ -1902,14 +1904,20 @@ int delta(const fm_delta_args* args, bool bwd, void* stream) {
     return 0;
 }
 
-// 32 columns a workgroup, as for the memory that only adds (k_step).  416 rows, 8 heads of 128 x 128: 94.5 us with 32 columns, 129
-// with 16, 99 with 64, 114 with 128; one row: 5.2, 4.5, 6.8, 10.
-template <class T>
-void delta_step_of_type(const fm_delta_step_args& a, hipStream_t st) {
-    constexpr int CB = 32;
+// 32 columns a workgroup, or 64 where that makes two workgroups a CU or more and leaves no half of one idle.  With 32 and 64 columns,
+// us: 416 rows, 8 heads of 128 x 128 in bfloat16 87 and 81, of 64 x 48 in float32 21 and 16, of 64 x 96 28 and 32; 64 rows of 64 x 64
+// 6.1 and 5.5; 16 rows of 128 x 128 5.4 and 6.3, one 4.0 and 5.0.  (16 columns: 117 and 3.8, 128: 88 and 6.3, 416 rows and one.)
+template <class T, int CB>
+void launch_delta_step(const fm_delta_step_args& a, hipStream_t st) {
     const dim3 grid((unsigned)((a.v_dim + CB - 1) / CB), (unsigned)a.q_heads, (unsigned)a.n);
     if (a.v_dim % 4 || (((uintptr_t)a.state | (uintptr_t)a.next) & 15)) k_delta_step<T, CB, false><<<grid, 256, 0, st>>>(a);
     else k_delta_step<T, CB, true><<<grid, 256, 0, st>>>(a);
+}
+template <class T>
+void delta_step_of_type(const fm_delta_step_args& a, hipStream_t st) {
+    const long long blocks = (a.v_dim + 31) / 32;
+    if (blocks % 2 == 0 && a.n * a.q_heads * blocks >= 1024) launch_delta_step<T, 64>(a, st);
+    else launch_delta_step<T, 32>(a, st);
 }
 
 }  // namespace fg

@@ -398,7 +398,7 @@ def test_long_stretches_keep_their_precision(gpu_lib, dt):
 
 
 STEPS = [(1, 8, 8, 64, 64, F32), (3, 4, 2, 40, 56, F16), (5, 2, 1, 128, 128, BF16), (2, 3, 3, 7, 5, F32), (1, 1, 1, 1, 1, BF16),
-         (70, 2, 2, 33, 100, F32)]
+         (70, 2, 2, 33, 100, F32), (70, 8, 4, 64, 64, BF16), (140, 8, 8, 33, 57, F32), (33, 8, 8, 128, 127, F16)]
 
 
 @pytest.mark.parametrize("n,H,Hk,K,V,dt", STEPS)
