@@ -337,9 +337,10 @@ void norm_of_type(const fm_norm_args& a, bool bwd, hipStream_t st) {
         const unsigned blocks = (unsigned)(a.rows < 2048 ? a.rows : 2048);
         if (!bwd) k_norm_any<T><<<blocks, 256, 0, st>>>(a);
         else {
-            if (a.gx) k_norm_any_bwd<T><<<blocks, 256, 0, st>>>(a);
+            // (the weights' sums first: gx may be written over x or g)
             if (a.gweight || a.gbias)
                 k_norm_columns<T><<<dim3((unsigned)((a.width + 255) / 256), norm_blocks(a)), 256, 0, st>>>(a);
+            if (a.gx) k_norm_any_bwd<T><<<blocks, 256, 0, st>>>(a);
         }
         return;
     }
