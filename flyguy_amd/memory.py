@@ -163,7 +163,7 @@ class MemoryActor(nn.Module):
         heads = [x.unflatten(-1, (-1, self.dim)) for x in split]
         if self.rule == "decay":
             return (*heads, self.log_decay, None)
-        forget, rate = self.gates(firing).unflatten(-1, (2, -1)).unbind(-2)
+        forget, rate = self.gates(firing).to(self.log_decay.dtype).unflatten(-1, (2, -1)).unbind(-2)   # (float32 under autocast too)
         return (*heads, self.log_decay * (nn.functional.softplus(forget) / math.log(2)), torch.sigmoid(rate))
 
     def _dropped(self, o: torch.Tensor) -> torch.Tensor:
