@@ -1559,8 +1559,8 @@ __global__ __launch_bounds__(256) void k_delta_step(fm_delta_step_args a) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) vv[j] = widen(v[c0 + j < N ? c0 + j : 0]);
-    const Keep keep(a.log_decay[n * a.ld_row + h * a.ld_head]);
-    const float beta = a.beta[n * a.be_row + h * a.be_head];
+    const float log_decay = a.log_decay[n * a.ld_row + h * a.ld_head], beta = a.beta[n * a.be_row + h * a.be_head];
+    const Keep keep(log_decay);
     float sum[9] = {};                                    // S^T k, S^T q of 4 columns; q . k
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -1590,7 +1590,12 @@ __global__ __launch_bounds__(256) void k_delta_step(fm_delta_step_args a) {
     auto joined_at = [&](int i) { return part[0][i] + part[1][i] + part[2][i] + part[3][i]; };
     float u[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) u[j] = beta * (vv[j] - joined_at(4 * cg + j));
+    for (int j = 0; j < 4; ++j) {
+        // (a value, key, decay or rate that is not finite: NaN in all that it reaches, also where an infinite decay meets a state of 0
+        // or an infinite step a key of any sign)
+        u[j] = beta * (vv[j] - joined_at(4 * cg + j));
+        if (!(fabsf(u[j]) < INFINITY) || !(log_decay < INFINITY)) u[j] = NAN;
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
         const int r = rg + i * RG;

@@ -135,7 +135,8 @@ int fm_delta_bwd(const fm_delta_args* a, void* stream);
 long long fm_delta_workspace(const fm_delta_args* a, int backward);
 long long fm_delta_saved(const fm_delta_args* a);
 
-/* One moment of it for n <= 65535 rows, as fm_step: log_decay and beta of row i and head h at i row + h head. */
+/* One moment of it for n <= 65535 rows, as fm_step: log_decay and beta of row i and head h at i row + h head.  What is not finite
+ * reaches what it reaches there; an update that overflows float32 is NaN. */
 typedef struct fm_delta_step_args {
     fm_view q, k, v;
     const float *log_decay, *beta;
