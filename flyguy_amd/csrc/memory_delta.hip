@@ -1726,6 +1726,13 @@ bool in_whole_units(const fm_delta_args& p, bool bwd) {
         if (!aligned16(*v, size) || v->moment < 0 || v->moment >= STRIDE_MOST) return false;
     return true;
 }
+// Whether dense tensors of these sizes have moments too far apart for that: their copies' room is then counted for any strides, so that
+// what a call takes goes by sizes alone wherever tensors are dense or aligned as in_whole_units wants them (the output's gradient
+// need not be known when room is asked for).
+bool far_apart(const fm_delta_args& p, bool bwd) {
+    const long long third = (bwd ? p.q_heads : p.k_heads) * p.v_dim, row = p.q_heads * p.k_dim;
+    return (row > third ? row : third) >= STRIDE_MOST;
+}
 // bytes of their copies: queries, keys, and values or (gradient) the output's gradient
 long long pack_bytes(const fm_delta_args& p, bool bwd, int which) {
     const int size = p.dtype == FM_F32 ? 4 : 2;
@@ -1741,7 +1748,7 @@ bool whole_stores(const fm_delta_args& p) {
 long long delta_workspace_bytes(const fm_delta_args& a, bool bwd) {
     long long n = (bwd ? 0 : chunk_slots(a) * a.q_heads * prep_bytes(a.dtype, false)) + 4 * cut_floats(a);
     n += 4 * (bwd ? kept_floats(a) + delta_part_floats(a, false) + delta_part_floats(a, true) : move_floats(a));
-    if (chunk_slots(a) && !in_whole_units(a, bwd))
+    if (chunk_slots(a) && (!in_whole_units(a, bwd) || far_apart(a, bwd)))
         for (int i = 0; i < 3; ++i) n += pack_bytes(a, bwd, i);
     return n;
 }

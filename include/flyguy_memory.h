@@ -109,7 +109,8 @@ int fm_step(const fm_step_args* a, void* stream);
  * the state NaN from its moment on; a key, decay (NaN or +inf) or rate that is not, all of the head's; no earlier moment, other
  * head or stretch (gradients: no other head or stretch).
  * saved: fm_delta_saved(a) bytes that the gradient reads (0: no gradient is wanted), workspace: fm_delta_workspace(a, backward)
- * bytes.  Gradients (fm_delta_bwd): inputs and saved as the forward left them; go of o, gstate_out of state_out (0: zeros); gq, gk,
+ * bytes: by sizes alone where the tensors read (backward: q, k, go) have values, strides and starts of multiples of 16 bytes and
+ * strides of moments from 0 to 2^22 - 1 values, or are dense; others are copied, and the room for that is counted by the views given.  Gradients (fm_delta_bwd): inputs and saved as the forward left them; go of o, gstate_out of state_out (0: zeros); gq, gk,
  * gv dense like their tensors, glog_decay, gbeta float32 [moments][q_heads], gstate float32; each 0 where not wanted.  glog_decay
  * is what is left of sums that cancel where little was remembered: off by the float32 roundings of their terms. */
 typedef struct fm_delta_args {
