@@ -82,7 +82,9 @@ class MemoryActor(nn.Module):
     rule: "decay", a memory that adds, each head with its decay, or "delta", one that corrects: keys of length 1, and a rate and
     a decay of each moment and head (the head's own where the firing says nothing).  norm: the firing goes through a layer norm
     first.  dropout: the share of what is read from the memory that is dropped in training mode (nn.Module.train), each pass
-    another."""
+    another: by a seed that each actor draws from torch's generator when it is made or loaded, and the number of the pass.  A
+    copy.deepcopy goes on as its original would.  Under activation checkpointing, whose second pass would drop others, it is
+    refused."""
 
     def __init__(self, actor: FlyActor, heads: int = 8, k_heads: int | None = None, dim: int = 64, longest: float = 2048.0,
                  positions: int = 65536, rule: str = "decay", norm: bool = False, dropout: float = 0.0):
@@ -116,7 +118,8 @@ class MemoryActor(nn.Module):
             nn.init.zeros_(self.gates.bias)
         self.norm_w, self.norm_b = (nn.Parameter(torch.ones(firing)), nn.Parameter(torch.zeros(firing))) if norm else (None, None)
         if self.dropout:
-            self.register_buffer("drops", torch.tensor([torch.initial_seed() % (1 << 63), 0]), persistent=False)
+            # (seed, pass): the seed is drawn, so that no two actors of a process drop the same numbers
+            self.register_buffer("drops", torch.cat([torch.randint(1 << 62, (1,)), torch.zeros(1, dtype=torch.int64)]), persistent=False)
 
     def checkpoint(self, graph: str) -> dict:
         """What MemoryActor.load reads: the memory, and the actor that it was taught on (as flyguy_amd.teach writes actors)."""
@@ -169,6 +172,9 @@ class MemoryActor(nn.Module):
     def _dropped(self, o: torch.Tensor) -> torch.Tensor:
         if not self.dropout:
             return o
+        if torch._C._current_graph_task_id() >= 0:
+            raise RuntimeError("MemoryActor: a pass that is made again while gradients are taken (activation checkpointing) would drop "
+                               "other numbers than the first; checkpoint without dropout, or take the memory out of it")
         now = self.drops.clone()
         self.drops[1:] += 1
         return dropout(o, self.dropout, now) if o.is_cuda else _dropout_cpu(o, self.dropout, now)
