@@ -34,14 +34,18 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found (ROCm is required to build the flyguy library)")
 
 
+def compile_flags() -> list[str]:
+    return ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-result",
+            # packed fp32 instructions are left to nothing: code generation of ordinary float code only
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+            "-I", str(ROOT / "include")]
+
+
 def build(verbose: bool = False) -> Path:
     """Compile every source (always: the build check is that this succeeds) and link the shared library."""
     out_dir = PKG / "_build"
     out_dir.mkdir(exist_ok=True)
-    flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-result",
-             # packed fp32 instructions are left to nothing: code generation of ordinary float code only
-             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-             "-I", str(ROOT / "include")]
+    flags = compile_flags()
     objs = []
     procs = []
     for src in SOURCES:

@@ -485,11 +485,15 @@ struct Stage {
     __device__ __forceinline__ const char* prepared(long long i0) const {
         return a.prep + ((size_t)(slot0 + i0 / CH) * a.heads + h) * F::PREP;
     }
-    // 1 KB: a lane's 16 bytes from `offset` bytes past `base` to 16 bytes times the lane's number behind `to`, of the lanes in `mask`
+    // 1 KB: a lane's 16 bytes from `offset` bytes past `base` to 16 bytes times the lane's number behind `to`, of the lanes in `mask`.
+    // (m0, the place in LDS, is the compiler's to set before each instruction of its own that reads it: it keeps nothing there.  A base
+    // that a vector instruction leaves in scalar registers less than five wait states before would be read too early: `base` and
+    // `prepared` are sums of scalar instructions, and tests/test_delta_loads.py looks at all that stands before these loads.)
     __device__ __forceinline__ static void straight(const void* base, unsigned offset, unsigned long long mask, const char* to) {
         const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)to);
-        asm volatile("s_mov_b32 m0, %0\n\ts_mov_b64 exec, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1" ::"s"(at), "v"(offset),
-                     "s"(base), "s"(mask) : "memory");
+        unsigned long long active;
+        asm volatile("s_mov_b32 m0, %1\n\ts_and_saveexec_b64 %0, %4\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b64 exec, %0" : "=&s"(active)
+                     : "s"(at), "v"(offset), "s"(base), "s"(mask) : "memory", "scc");
     }
     // a lane's place in unit 4 i + wave of rows of WIDTH values, and the lanes whose columns are the head's
     template <int WIDTH>
