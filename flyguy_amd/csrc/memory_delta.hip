@@ -608,9 +608,11 @@ struct Stage {
 // A value of v that is not finite makes its column NaN from its moment on; a key, decay or rate that is not, all columns:
 // such moments are left out of the products (0 times them would not be 0) and marked in what is stored.
 // What bounds it: a chunk depends on the one before it, and its four products on each other, at one wave a SIMD: 8 x 4,096 moments,
-// 16 heads of 128 in bfloat16, one workgroup a CU, take 400 us (KEEP; 6.2 a chunk), matrix instructions 25% of the cycles.  More
-// waves would hold fewer columns each and read the same rows and operands (32 columns a workgroup, two of them a CU: no room in
-// LDS for two chunks each, and without the second room the loads are in the open).  Chunks of 64 moments for binary16 and
+// 16 heads of 128 in bfloat16, one workgroup a CU, take 400 us (KEEP; 6.2 a chunk), matrix instructions 25% of the cycles.  Two
+// workgroups a CU have no room in LDS for two chunks each (116,736 bytes a workgroup at heads of 64, 149,504 at 128, also for a
+// segment's own states, which read neither q nor P), and without the second room the loads are in the open.  8 waves over 128
+// columns could share one chunk (8 KB a room more), in half the registers each: the walks take 239 to 474 of 512 in bfloat16; not
+// tried.  Those of float32 heads over 64 take 322 to 512 (16 x 512 moments, 8 heads of 128, KEEP: 109 us, 6.8 a chunk).  Chunks of 64 moments for binary16 and
 // float32 too, whose terms take two and three times the registers: walks the same, k_delta_prep 20 -> 29 us, k_delta_grads 48 -> 80
 // (16 x 512 moments, 8 heads of 64, float32).
 enum Walk { PLAY, KEEP, OWN };            // outputs; outputs, states and errors kept; a segment's own end state alone
@@ -882,6 +884,7 @@ __global__ __launch_bounds__(256, 1) void k_delta_scan(Delta a) {
 
 // ------------------------------------------------------------------------------------------------ the walk backwards
 // The same of X, the gradient of the state after a chunk: y = T^T (P^T g + F beta K X), X' = E_end X + Q^T (c E g) - K^T (E y).
+// (KEEP of float32 heads over 64 takes all 512 registers and spills 20: 145 us where the walk forwards takes 109.)
 template <class T, int KT, Walk WALK>
 __global__ __launch_bounds__(256, 1) void k_delta_back(Delta a) {
     using F = DeltaForm<T, true>;
@@ -1136,7 +1139,8 @@ __global__ __launch_bounds__(64 * KT) void k_delta_join(Delta a) {
 // transposing read for what sums over i.
 // 8 x 4,096 moments, 16 heads of 128 in bfloat16 take 750 us (880 where the card clocks lower), their 2.4 GB alone 450: one
 // workgroup's 8 waves fill a CU's registers, so that its loads, 112 KB of terms and products follow one another; matrix
-// instructions take 25% of the cycles.  (Two workgroups a CU, or one that walks several chunks, spill: slower.)
+// instructions take 25% of the cycles.  (Two workgroups a CU, or one that walks several chunks, spill: slower.  Keys of up to 64
+// values with values of more, bfloat16: 4 waves of 308 registers and 117 KB of LDS, one workgroup a CU: 626 us at 64 / 128.)
 template <class T, int KT, int VT>
 constexpr int grads_room() {                              // 16-bit values of LDS
     using F = DeltaForm<T, true>;
@@ -1660,14 +1664,17 @@ long long chunk_slots(const fm_delta_args& a) {
 }
 // Segments: a walk takes a workgroup for 64 columns and a CU for itself, so that few chains leave most CUs without work.  Cut
 // into segments of L moments, these are walked at the same time, for more work: their own end states, with M (K more columns) but
-// for the first, then those joined one after another, then the walk.  By the following estimate (us): a chunk takes a walk
-// `chunk`, four fifths of it where only the own state is wanted, a join `join`, the launches 12; workgroups go 256 at a time (narrow heads
-// leave room for some of the next ones beside).
+// for the first, then those joined one after another, then the walk.  The choice is by an estimate whose constants are fitted, in
+// units of about a microsecond: a chunk takes a walk `chunk`, four fifths of it where only the own state is wanted, a join `join`, the
+// launches 12; workgroups go 256 at a time.  (Whole walks of bfloat16 took 3.0 us a chunk at heads of 64, 4.0 at 128, up to 6.2 where
+// chunks are kept and all CUs walk, a join 2.6: the longer the walks, the more joins and launches weigh beside them.  The half in
+// `rounds` for heads of up to 64 is the fit's: registers and LDS let a second workgroup into a CU for some of binary16's walks and
+// float32's own states, for none of bfloat16's.  Whether gradients are wanted is not asked: M serves both, and both are cut alike.)
 // Packed stretches, whose lengths only the device knows, are taken to be of any length up to twice the middle one.
-// Measured with 1 to 64 segments, each type, heads of 64 and 128, 1 to 37 stretches of 1,024 to 32,768 moments, with gradients
-// and without (84 calls): the estimate's choice takes 1.02 times the best one's time in the middle, 1.18 at most, walks without
-// segments 2.4 in the middle, 18 at most: 1 x 4 heads of 128 x 16,384 of bfloat16 1,012 us whole and 183 in 16 segments;
-// 16 x 8 x 1,024 108 and 172 in two.
+// Fitted to 84 calls measured with 1 to 64 segments: each type, heads of 64 and 128, 1 to 37 stretches of 1,024 to 32,768 moments,
+// with gradients and without.  In that same table, interpolated between the counts measured, the choice takes 1.02 times the best
+// one's time in the middle, 1.18 at most, walks without segments 2.4 in the middle, 18 at most: 1 x 4 heads of 128 x 16,384 of bfloat16
+// 1,012 us whole and 183 in 16 segments; 16 x 8 x 1,024 108 and 172 in two.  Calls outside the table were not timed.
 long long segment_length(const fm_delta_args& p) {
     const long long C = chunk_length(p.dtype), whole = (p.n_moments + C - 1) / C * C;
     if (!p.n_seq || whole <= C) return whole ? whole : C;

@@ -85,8 +85,8 @@ class LayerNormHip(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """Each row (the last dimension, 1 to 2^24 values) less its mean, over the root of its mean square deviation plus eps, times
-    weight, plus bias (float32 [width] each, or None).  Means and deviations are taken in float32 about the mean; y is dense,
-    of x's type.  Gradients of x, weight and bias; the weights' are summed in a fixed order."""
+    weight, plus bias (float32 [width] each, or None).  Means and deviations are taken in float32 about the mean (a row whose
+    squares add up past float32's largest number, as two numbers 1e20 apart do, is all bias); y is dense, of x's type.  Gradients of x, weight and bias; the weights' are summed in a fixed order."""
     what = "layer_norm"
     _no_tangents(what, x, weight, bias)
     _of_rows(what, x)

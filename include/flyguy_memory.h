@@ -153,7 +153,7 @@ int fm_delta_step(const fm_delta_step_args* a, void* stream);
 
 /* Layer norm of rows of `width` values (1 to 2^24), row i at x + i x_row (strides in values):
  *   m = mean(x), r = (mean((x - m)^2) + eps)^-1/2, xh = (x - m) r, y = xh weight + bias   (weight 0: 1; bias 0: 0)
- * stats: float32 [rows][2], (m, r) of each row, written if not 0.  Gradients (fm_norm_bwd): x, weight and stats the forward's,
+ * (sums in float32: r is 0 where the squares pass its largest number).  stats: float32 [rows][2], (m, r) of each row, written if not 0.  Gradients (fm_norm_bwd): x, weight and stats the forward's,
  * g the gradient of y; gx, gweight, gbias the gradients, each 0 where not wanted; partial: fm_norm_partial() floats.  weight,
  * bias and their gradients are float32.  y may be x, gx may be x or g, with the same stride, where rows do not overlap; otherwise what is
  * written must lie outside what is read. */
