@@ -46,6 +46,7 @@ def test_nothing_is_written_outside_its_room(gpu_lib, n, D, dt, gap):
         assert torch.equal(t[:, D:].contiguous().view(bits), before[:, D:].contiguous().view(bits))
     # (rows apart may be read in other units than dense ones, whose sums run in another order: a few roundings of sums of D or n numbers)
     for got, w64, count in ((y[:, :D], want_y, D), (gx[:, :D], want[0], 3 * D), (gw, want[1], n + D), (gb, want[2], n)):
+        w64 = w64.detach()
         off = (got.double() - w64.double()).abs()
         step = {F32: 2.0 ** -24, BF16: 2.0 ** -7, F16: 2.0 ** -10}[got.dtype]     # (two roundings of half a step, of values as good as alike)
         scale = float(w64.double().abs().max()) + float(g.double().abs().max())
